@@ -309,6 +309,50 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
                       const int32_t* tables, int max_blocks, const int32_t* ctx_len, const uint64_t* mask, int B,
                       int R, int n_q_heads, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Causal attention of packed prompt rows over the paged pool of one layer
+ * (whole prompts, prompt chunks behind cached tokens, single tokens, in one
+ * call).  Sequence b owns rows row_off[b] .. row_off[b+1]-1 of q and out
+ * (row_off [B+1] int32, device, not decreasing); its row i is the token in
+ * slot ctx_len[b] + i, whose K/V are in the pages already, and sees slots
+ * 0 .. ctx_len[b] + i.  q [T, Hq, hd] and out [T, Hq, hd] fp16 with row
+ * strides ldq / ldo in elements (multiples of 8, so q may lie in the fused
+ * QKV rows); T = rows of the buffers.  A sequence may have no rows; rows
+ * behind row_off[B] are neither read nor written.  Slots a row does not see
+ * may hold anything (NaN and infinities too), pages past the last slot are
+ * not read; slots past max_blocks * 16 do not exist; a table entry outside
+ * the pool reads block 0.  Up to 4096 sequences.  Long key ranges are split
+ * across CTAs and merged through the workspace in a fixed order (the result
+ * is deterministic); calls in flight at the same time, captured graphs
+ * among them, need workspaces of their own.  The first call on a device
+ * comes before any stream capture.  The reference feeds prompts in chunks
+ * (server/chunked_prefill.cpp:4-24) through one row of attention at a time
+ * (server/paged_attention.cpp:16-111). */
+size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
+                                                int max_blocks);
+int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
+                             int head_dim, const int32_t* tables, int max_blocks, const int32_t* ctx_len,
+                             const int32_t* row_off, int B, int T, int n_q_heads, uint16_t* out, int ldo,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* specdec_attention for sequences that share a prefix page by page (prefix
+ * sharing of PagedKVCache::share_prefix, specdec_kv_fork): the prefix's K/V
+ * are read once for all rows of a group instead of once per sequence.  Group
+ * g is the sequences group_off[g] .. group_off[g+1]-1 (group_off
+ * [n_groups+1] int32, device, not decreasing), whose first shared_blocks[g]
+ * table entries are equal (those of the group's first sequence are used;
+ * blocks past any member's ctx_len / 16 are taken as not shared).  Sequences
+ * of no group share nothing.  The other arguments and the result are
+ * specdec_attention's (the result up to the order of the sums); slots no row
+ * sees may hold anything.  Up to 4096 sequences; workspace, capture and
+ * determinism as for specdec_attention_prompt. */
+size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads, int n_kv_heads,
+                                                       int head_dim, int max_blocks);
+int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
+                                    int head_dim, const int32_t* tables, int max_blocks, const int32_t* ctx_len,
+                                    const uint64_t* mask, const int32_t* group_off, const int32_t* shared_blocks,
+                                    int n_groups, int B, int R, int n_q_heads, uint16_t* out, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* ===================================================================== */
 /* 3. Paged KV block manager (device resident).  Mirrors PagedKVCache      */
 /*    (server/paged_kv_cache.h:28-63): lowest-free-index allocation with   */

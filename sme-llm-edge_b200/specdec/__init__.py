@@ -111,6 +111,10 @@ _SIGS = {
     "specdec_w4a16_gemm_simt": (I, [P, I, I, P, I, I, P, I, I, P]),
     "specdec_attention_workspace_bytes": (SZ, [I, I, I, I, I, I]),
     "specdec_attention": (I, [P, P, I, I, I, P, I, P, P, I, I, I, P, P, SZ, P]),
+    "specdec_attention_prompt_workspace_bytes": (SZ, [I, I, I, I, I, I]),
+    "specdec_attention_prompt": (I, [P, I, P, I, I, I, P, I, P, P, I, I, I, P, I, P, SZ, P]),
+    "specdec_attention_shared_prefix_workspace_bytes": (SZ, [I, I, I, I, I, I, I]),
+    "specdec_attention_shared_prefix": (I, [P, P, I, I, I, P, I, P, P, P, P, I, I, I, I, P, P, SZ, P]),
     "specdec_kv_create": (I, [I, I, I, I, C.POINTER(P)]),
     "specdec_kv_destroy": (I, [P]),
     "specdec_kv_append": (I, [P, P, P, I, P, P]),
