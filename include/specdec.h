@@ -320,7 +320,7 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
  * behind row_off[B] are neither read nor written.  Slots a row does not see
  * may hold anything (NaN and infinities too), pages past the last slot are
  * not read; slots past max_blocks * 16 do not exist; a table entry outside
- * the pool reads block 0.  Up to 4096 sequences.  Long key ranges are split
+ * the pool reads block 0.  Up to 1024 sequences.  Long key ranges are split
  * across CTAs and merged through the workspace in a fixed order (the result
  * is deterministic); calls in flight at the same time, captured graphs
  * among them, need workspaces of their own.  The first call on a device
@@ -343,7 +343,7 @@ int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_laye
  * blocks past any member's ctx_len / 16 are taken as not shared).  Sequences
  * of no group share nothing.  The other arguments and the result are
  * specdec_attention's (the result up to the order of the sums); slots no row
- * sees may hold anything.  Up to 4096 sequences; workspace, capture and
+ * sees may hold anything.  Up to 1024 sequences; workspace, capture and
  * determinism as for specdec_attention_prompt. */
 size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads, int n_kv_heads,
                                                        int head_dim, int max_blocks);

@@ -538,7 +538,7 @@ struct AttnPlan {
     size_t smem;
 };
 
-static PFN_cuTensorMapEncodeTiled_v12000 attn_encode() {
+PFN_cuTensorMapEncodeTiled_v12000 attn_encode() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     if (!fn) {
         cudaDriverEntryPointQueryResult q;
@@ -556,9 +556,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 attn_encode() {
 // head, landing in shared memory as [K|V][half][token][64] with 128-byte
 // swizzle -- the same layout as separate 16 x 64 boxes, in one request.
 // `halves` / `kvs` = how many column halves / K|V planes one box spans.
-static int make_kv_tmap(CUtensorMap* map, const __half* kv, int num_blocks, int Hkv, int HD, int halves = -1,
-                        int kvs = 2) {
-    if (halves < 0) halves = HD / 64;
+int make_kv_tmap(CUtensorMap* map, const __half* kv, int num_blocks, int Hkv, int HD, int halves, int kvs) {
     auto enc = attn_encode();
     SD_CHECK(enc, SPECDEC_ENOTSUP, "cuTensorMapEncodeTiled unavailable");
     SD_CHECK((reinterpret_cast<uintptr_t>(kv) & 15) == 0, SPECDEC_EINVAL, "attention: KV pool must be 16-byte aligned");

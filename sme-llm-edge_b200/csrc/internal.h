@@ -5,6 +5,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -79,6 +80,10 @@ int gemv_launch(const __half* X, int ldx, int K, const GemvPlan& p, const void* 
 size_t w4_tiled_bytes(int N, int K);
 
 // ---------------------------------------------------------------- attention
+PFN_cuTensorMapEncodeTiled_v12000 attn_encode();  // null when the driver lacks it
+// The layer's pool as a tensor map whose box is one block of one head:
+// `halves` 64-column halves of `kvs` of the K / V planes.
+int make_kv_tmap(CUtensorMap* map, const __half* kv, int num_blocks, int Hkv, int HD, int halves, int kvs);
 size_t attention_workspace(int B, int R, int Hq, int Hkv, int HD, int max_ctx);
 int launch_attention(const __half* q, const __half* kv_layer, int num_blocks, int Hkv, int HD, const int32_t* tables,
                      int max_blocks, const int32_t* ctx_len, const uint64_t* mask, int B, int R, int Hq, __half* out,

@@ -1,97 +1,1092 @@
 // prompt_attention.cu -- attention of packed prompt rows, and of verify rows
 // whose sequences share a prefix, over paged fp16 KV (sm_100a).
 //
-// First form: one warp per (query row, head); the lanes split the head
-// dimension and walk the visible keys with an online base-2 softmax.
+// Both are the same work: a tile of query rows of one KV head (all G = Hq/Hkv
+// query heads together, row = token * G + g, as many whole tokens as fit into
+// 128 rows) against a range of one block table's slots.  A segment is
+//   a sequence's packed rows, causal             (specdec_attention_prompt)
+//   a group's rows against its shared pages      (specdec_attention_shared_prefix)
+//   a sequence's rows against its own pages,
+//   with the mask of its new rows                (specdec_attention_shared_prefix)
+// An item is two adjacent tiles (one, where no second is left) of a segment and
+// a KV head, and one of the S pieces into which the segment's key range is cut.
+//
+// Mathematics, with x = score * log2(e) / sqrt(hd): in blocks of 128 keys
+//   m' = max(m, rowmax x),  P = 2^(x - m'),  l = l 2^(m - m') + rowsum P,
+//   O = O 2^(m - m') + P V;  out = O / l.
+// m only moves when a row's maximum has grown by more than 8 (P stays below
+// 2^8), so O is rarely rescaled.  P is rounded to fp16 (at most 2^-11 of a
+// weight): the tensor core multiplies fp16 by fp16.  m, l, O are fp32.
+//
+// One persistent CTA per SM, 12 warps:
+//   warps 0-3, 4-7  softmax of tile slot 0 / 1, one thread per query row
+//   warp 8          MMA issuer: S = Q K^T and O += P V, whichever is ready
+//   warp 9          TMA loads: the tiles' queries, 128-key tiles of K and V
+//   warp 10         makes V safe: zeroes the slots behind the range's end in its
+//                   last page, and replaces infinities and NaN in slots that
+//                   not every row sees (0 * NaN would reach rows that do not
+//                   see them); the rows that see them add them at the end
+//   warp 11         scheduler: takes items, decodes them, passes them on
+// Two tiles share each K / V tile, so while the softmax of one works on its
+// scores the tensor cores work for the other.  P overlays S in tensor memory
+// (columns: S0 0, S1 128, O0 256, O1 256 + hd).  Single tiles use slots 0 and 1
+// in turn.
+//
+// Splits of the key range write unnormalised fp32 O with (m, l) into the
+// workspace; rows_merge_kernel joins them in their order.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
 #include "common.cuh"
 #include "internal.h"
+#include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace specdec {
 
-constexpr int kRowsMaxSeqs = 4096;
+constexpr int kRowsMaxSeqs = 1024;   // sequences of a call: the plan's tables live in shared memory
+constexpr int kRowsMaxSplits = 32;   // pieces of one key range
+constexpr int kRowsSorted = 128;     // up to so many segments are taken longest first
+constexpr int kRowsThreads = 384;
+constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
+constexpr int kRowsItems = 3;        // items known ahead in a CTA
+constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte rows, 128B swizzle
+constexpr int kRowsTmemCols = 512;
 
-struct RowAttnArgs {
-    const __half* q;
-    int ldq;
+enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2 };
+
+// Where the partial results of a sequence's rows lie (rows of the partial buffers).
+struct RowsMeta {
+    int n_pre, base_pre, stride_pre;  // pieces of the shared prefix
+    int n_own, base_own, stride_own;  // pieces of the own range; both 0: written by the main kernel
+};
+
+struct RowsArgs {
     const __half* kv;
-    int num_blocks, Hkv, Hq, G;
+    int num_blocks, Hkv, Hq, G, tpt;  // tpt = tokens of a 128-row tile
     const int32_t* tables;
     int max_blocks;
     const int32_t* ctx_len;
-    const int32_t* row_off;  // null: R rows for every sequence
-    const uint64_t* mask;    // null: causal
-    int B, T, R;
+    const int32_t* row_off;  // prompt: [B + 1]; null: R rows for every sequence
+    const uint64_t* mask;
+    const int32_t* group_off;
+    const int32_t* shared_blocks;
+    int n_groups, B, T, R;
+    int tq_small;  // tokens of the small query box
+    int slots_max;  // max_blocks * 16
     __half* out;
     int ldo;
     float scale_log2;
+    // workspace
+    uint32_t* counter;  // null: items go round the CTAs
+    RowsMeta* meta;
+    float2* pml;
+    float* po;
+    int prows;  // rows of the partial buffers
+    DeviceStatus* status;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(128) row_attention_kernel(RowAttnArgs a) {
-    constexpr int E = HD / 32;
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (id >= (long long)a.T * a.Hq) return;
-    const int t = (int)(id / a.Hq), h = (int)(id % a.Hq), kvh = h / a.G;
-    int b, i, n;
+struct RowsSeg {
+    int lo, n;      // token rows
+    int ctx;        // slot of the first row's token (causal, mask)
+    int base, end;  // slots [base, end) are what the segment reads at most
+    int tiles, kt;  // items along the rows; 128-key tiles of the longest
+    int trow, mode;
+};
+
+struct RowsItem {
+    int n_kt;          // 128-key tiles; -1: no more items
+    int slot0, end;    // first slot (a multiple of 16); slots from `end` on are not read
+    int trow, kvh;
+    int tok0, i0;      // first token row; its index within the segment
+    int ntok0, ntok1;  // tokens of the two tiles
+    int ctx, mode;
+    int scan;          // slots >= scan are not seen by every row
+    int prow;          // row of the partial buffers for tok0, -1: the result is final
+    int bad;           // warp 10 found an infinity or NaN past `scan`
+};
+
+// ------------------------------------------------------------------ the plan
+__device__ __forceinline__ int rows_clamp(int v, int lo, int hi) { return max(lo, min(hi, v)); }
+
+__device__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* group_pages, const int* seq_pages) {
+    RowsSeg s;
     if (a.row_off) {
-        int lo = 0, hi = a.B;  // first sequence whose end is past t
+        s.lo = rows_clamp(a.row_off[i], 0, a.T);
+        s.n = rows_clamp(a.row_off[i + 1], s.lo, a.T) - s.lo;
+        s.ctx = rows_clamp(a.ctx_len[i], 0, 1 << 30);
+        s.base = 0;
+        s.end = min(s.ctx + s.n, a.slots_max);
+        s.trow = i;
+        s.mode = kModeCausal;
+    } else if (i < a.n_groups) {
+        const int b0 = rows_clamp(a.group_off[i], 0, a.B), b1 = rows_clamp(a.group_off[i + 1], b0, a.B);
+        s.lo = b0 * a.R;
+        s.n = (b1 - b0) * a.R;
+        s.ctx = 0;
+        s.base = 0;
+        s.end = group_pages[i] * 16;
+        s.trow = min(b0, a.B - 1);
+        s.mode = kModeAll;
+        if (s.end == 0) s.n = 0;
+    } else {
+        const int b = i - a.n_groups;
+        s.lo = b * a.R;
+        s.n = a.R;
+        s.ctx = rows_clamp(a.ctx_len[b], 0, 1 << 30);
+        s.base = seq_pages[b] * 16;
+        s.end = max(s.base, min(s.ctx + a.R, a.slots_max));
+        s.trow = b;
+        s.mode = kModeMask;
+    }
+    s.tiles = (s.n + 2 * a.tpt - 1) / (2 * a.tpt);
+    s.kt = (s.end - s.base + 127) / 128;
+    return s;
+}
+// 128-key tiles of the segment's item p along the rows
+__device__ __forceinline__ int rows_item_end(const RowsArgs& a, const RowsSeg& s, int p) {
+    return s.mode == kModeCausal ? min(s.end, s.ctx + min(s.n, (p + 1) * 2 * a.tpt)) : s.end;
+}
+__device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s, int p) {
+    return (rows_item_end(a, s, p) - s.base + 127) / 128;
+}
+// Pieces of the key range, for pieces of about `fine` tiles where there are few
+// rows (memory-bound: partial results are small) or `coarse`.
+__device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, int fine, int coarse) {
+    const int S = s.n * a.G <= 64 ? (s.kt + fine - 1) / fine : (2 * s.kt + coarse) / (2 * coarse);
+    return rows_clamp(S, 1, max(1, min(kRowsMaxSplits, s.kt)));
+}
+__device__ __forceinline__ bool rows_partial(const RowsSeg& s, int S) { return s.mode == kModeAll || S > 1 || s.base > 0; }
+
+// False only for group bounds that overlap: what would not fit is left out.
+__device__ __forceinline__ bool rows_fit(const RowsArgs& a, const RowsSeg& s, int S, int prow) {
+    return (long long)prow + (long long)s.n * S <= a.prows;
+}
+
+struct RowsPlan {
+    int pre[2 * kRowsMaxSeqs + 1];  // items before position i (without the KV heads)
+    int prow[2 * kRowsMaxSeqs];     // partial rows before position i
+    int group_pages[kRowsMaxSeqs], seq_pages[kRowsMaxSeqs];
+    int order[kRowsSorted];
+    int wsum[2][kRowsThreads / 32];
+    long long wwork[kRowsThreads / 32];
+    int nseg, items, fine, coarse;
+};
+
+// Sums over the CTA; every thread gets them.  before_*: the sums of the threads in front.
+__device__ void rows_scan2(RowsPlan& p, int va, int vb, int* before_a, int* before_b, int* tot_a, int* tot_b) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int xa = va, xb = vb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int ya = __shfl_up_sync(0xffffffffu, xa, o), yb = __shfl_up_sync(0xffffffffu, xb, o);
+        if (lane >= o) {
+            xa += ya;
+            xb += yb;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) {
+        p.wsum[0][w] = xa;
+        p.wsum[1][w] = xb;
+    }
+    __syncthreads();
+    int ba = 0, bb = 0, ta = 0, tb = 0;
+    for (int i = 0; i < kRowsThreads / 32; ++i) {
+        if (i == w) {
+            ba = ta;
+            bb = tb;
+        }
+        ta += p.wsum[0][i];
+        tb += p.wsum[1][i];
+    }
+    *before_a = ba + xa - va;
+    *before_b = bb + xb - vb;
+    *tot_a = ta;
+    *tot_b = tb;
+}
+
+// Every CTA makes the same plan from the lengths in device memory (so a
+// captured call serves other lengths); CTA 0 writes where the partials lie.
+__device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
+    const int tid = threadIdx.x;
+    const int nseg = a.row_off ? a.B : a.n_groups + a.B;
+    if (!a.row_off) {
+        // shared pages of a group: announced, and within every member's context
+        for (int g = tid; g < a.n_groups; g += kRowsThreads)
+            p.group_pages[g] = rows_clamp(a.shared_blocks[g], 0, a.max_blocks);
+        __syncthreads();
+        for (int b = tid; b < a.B; b += kRowsThreads) {
+            int lo = 0, hi = a.n_groups;  // first group whose end is past b
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (a.group_off[mid + 1] > b) hi = mid;
+                else lo = mid + 1;
+            }
+            const int g = lo < a.n_groups && a.group_off[lo] <= b ? lo : -1;
+            p.seq_pages[b] = g;
+            if (g >= 0) {
+                // a group of one shares nothing worth a second pass
+                const bool one = a.group_off[g + 1] - a.group_off[g] < 2;
+                atomicMin(&p.group_pages[g], one ? 0 : rows_clamp(a.ctx_len[b], 0, 1 << 30) / 16);
+            }
+        }
+        __syncthreads();
+        for (int b = tid; b < a.B; b += kRowsThreads) p.seq_pages[b] = p.seq_pages[b] >= 0 ? p.group_pages[p.seq_pages[b]] : 0;
+        __syncthreads();
+    }
+    const int per = (nseg + kRowsThreads - 1) / kRowsThreads;
+    const int s0 = min(nseg, tid * per), s1 = min(nseg, s0 + per);
+    // total work in key tiles, and the longest segments first
+    long long work = 0;
+    int len = 0;
+    for (int i = s0; i < s1; ++i) {
+        const RowsSeg s = rows_seg(a, i, p.group_pages, p.seq_pages);
+        if (s.tiles > 0) work += (long long)s.tiles * (rows_item_kt(a, s, 0) + s.kt) / 2 * a.Hkv;
+        len = s.tiles > 0 ? s.kt : 0;
+        p.pre[i] = len;
+    }
+    work = warp_sum(work);
+    if ((tid & 31) == 0) p.wwork[tid >> 5] = work;
+    __syncthreads();
+    work = 0;
+    for (int i = 0; i < kRowsThreads / 32; ++i) work += p.wwork[i];
+    if (nseg <= kRowsSorted && tid < nseg) {  // here a thread has one segment
+        int rank = 0;
+        for (int j = 0; j < nseg; ++j) rank += p.pre[j] > len || (p.pre[j] == len && j < tid);
+        p.order[rank] = tid;
+    }
+    __syncthreads();
+    int fine = max(4, (int)min((long long)1 << 20, (work + 4 * gridDim.x - 1) / (4 * (long long)gridDim.x)));
+    int coarse = max(8, (int)min((long long)1 << 20, (work + gridDim.x - 1) / (long long)gridDim.x));
+    if (a.prows == 0) fine = coarse = 1 << 26;
+    int items, prows, item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
+    for (int round = 0;; ++round) {
+        items = prows = 0;
+        for (int i = s0; i < s1; ++i) {
+            const RowsSeg s = rows_seg(a, nseg <= kRowsSorted ? p.order[i] : i, p.group_pages, p.seq_pages);
+            const int S = rows_splits(a, s, fine, coarse);
+            items += s.tiles * S;
+            if (rows_partial(s, S)) prows += s.n * S;
+        }
+        rows_scan2(p, items, prows, &item0, &prow0, &tot_items, &tot_prows);
+        if (tot_prows <= a.prows || round >= 8) break;
+        // fewer pieces until their results fit; at last one piece a segment, which always does
+        fine = round == 7 ? 1 << 26 : 2 * fine;
+        coarse = round == 7 ? 1 << 26 : 2 * coarse;
+    }
+    for (int i = s0; i < s1; ++i) {
+        const int id = nseg <= kRowsSorted ? p.order[i] : i;
+        const RowsSeg s = rows_seg(a, id, p.group_pages, p.seq_pages);
+        const int S = rows_splits(a, s, fine, coarse);
+        const bool part = rows_partial(s, S);
+        p.pre[i] = item0;
+        p.prow[i] = prow0;
+        if (blockIdx.x == 0 && a.meta) {
+            if (s.mode == kModeAll) {
+                for (int b = s.lo / a.R; b < (s.lo + s.n) / a.R; ++b) {
+                    a.meta[b].n_pre = rows_fit(a, s, S, prow0) ? S : 0;
+                    a.meta[b].base_pre = prow0 + (b * a.R - s.lo);
+                    a.meta[b].stride_pre = s.n;
+                }
+            } else {
+                RowsMeta& m = a.meta[s.trow];
+                if (s.base == 0) m.n_pre = 0;
+                m.n_own = part && rows_fit(a, s, S, prow0) ? S : 0;
+                m.base_own = prow0;
+                m.stride_own = s.n;
+            }
+        }
+        item0 += s.tiles * S;
+        if (part) prow0 += s.n * S;
+    }
+    if (tid == 0) {
+        p.pre[nseg] = tot_items;
+        p.nseg = nseg;
+        p.items = tot_items * a.Hkv;
+        p.fine = fine;
+        p.coarse = coarse;
+    }
+    __syncthreads();
+}
+
+__device__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
+    RowsItem it;
+    it.n_kt = -1;
+    it.bad = 0;
+    if (idx >= p.items) return it;
+    it.kvh = idx % a.Hkv;
+    const int r = idx / a.Hkv;
+    int lo = 0, hi = p.nseg;  // last position with pre <= r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.pre[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    const RowsSeg s = rows_seg(a, p.nseg <= kRowsSorted ? p.order[lo] : lo, p.group_pages, p.seq_pages);
+    const int S = rows_splits(a, s, p.fine, p.coarse);
+    const int local = r - p.pre[lo];
+    const int tile = s.tiles - 1 - local / S, piece = local % S;  // the longest first
+    const bool part = rows_partial(s, S);
+    if (local < 0 || tile < 0 || (part && !rows_fit(a, s, S, p.prow[lo]))) {  // bounds that overlap: an empty item
+        it.n_kt = it.ntok0 = it.ntok1 = 0;
+        it.prow = -1;
+        return it;
+    }
+    const int kt = rows_item_kt(a, s, tile);
+    const int k0 = (int)((long long)piece * kt / S), k1 = (int)((long long)(piece + 1) * kt / S);
+    it.n_kt = k1 - k0;
+    it.slot0 = s.base + 128 * k0;
+    it.end = min(rows_item_end(a, s, tile), s.base + 128 * k1);
+    it.trow = s.trow;
+    it.i0 = tile * 2 * a.tpt;
+    it.tok0 = s.lo + it.i0;
+    it.ntok0 = min(a.tpt, s.n - it.i0);
+    it.ntok1 = rows_clamp(s.n - it.i0 - a.tpt, 0, a.tpt);
+    it.ctx = s.ctx;
+    it.mode = s.mode;
+    it.scan = s.mode == kModeCausal ? s.ctx + it.i0 + 1 : (s.mode == kModeMask ? s.ctx : it.end);
+    it.prow = part ? p.prow[lo] + piece * s.n + it.i0 : -1;
+    return it;
+}
+
+// ------------------------------------------------------------------ the kernel
+template <int HD>
+struct RowsCfg {
+    static constexpr int NH = HD / 64;                  // 64-column halves
+    static constexpr int TILE = NH * 16384;             // 128 rows x HD fp16
+    static constexpr int RING = HD == 128 ? 2 : 4;      // K tiles and V tiles in flight
+    static constexpr int NBAR = 4 * 2 + 5 * RING + 2 + 2 + 2 * kRowsItems;
+    static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
+                                   NBAR * 8 + 16;
+};
+
+// Four words: bit c = slot key0 + c of a row is seen.
+__device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, uint64_t bits, uint32_t w[4]) {
+    auto below = [](int k) -> uint64_t { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); };
+    const int n = it.end - key0;
+    uint64_t lo, hi;
+    if (it.mode == kModeMask) {
+        const int d = it.ctx - key0;  // column of the first new row
+        lo = below(d);
+        hi = below(d - 64);
+        if (d > -64 && d < 64) lo |= d >= 0 ? bits << d : bits >> -d;
+        const int e = d - 64;
+        if (e > -64 && e < 64) hi |= e >= 0 ? bits << e : bits >> -e;
+        lo &= below(n);
+        hi &= below(n - 64);
+    } else {
+        const int k = it.mode == kModeCausal ? min(n, it.ctx + i + 1 - key0) : n;
+        lo = below(k);
+        hi = below(k - 64);
+    }
+    w[0] = (uint32_t)lo;
+    w[1] = (uint32_t)(lo >> 32);
+    w[2] = (uint32_t)hi;
+    w[3] = (uint32_t)(hi >> 32);
+}
+
+__device__ __forceinline__ float rows_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+    rows_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_small,
+                          const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                          RowsArgs a) {
+    using C = RowsCfg<HD>;
+    constexpr int NH = C::NH, RING = C::RING;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* sQ = base;                       // [2 slots][NH][128 rows][128 B]
+    unsigned char* sK = sQ + 2 * C::TILE;           // [RING][NH][128 keys][128 B]
+    unsigned char* sV = sK + RING * C::TILE;        // [RING][8 pages][NH][16][128 B]
+    RowsPlan& plan = *reinterpret_cast<RowsPlan*>(sV + RING * C::TILE);
+    RowsItem* items = reinterpret_cast<RowsItem*>(&plan + 1);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(
+        (reinterpret_cast<uintptr_t>(items + kRowsItems) + 7) & ~uintptr_t(7));
+    uint64_t* q_full = bars;               // [2] queries of a slot landed
+    uint64_t* q_empty = q_full + 2;        // [2] their last Q.K^T is done
+    uint64_t* s_full = q_empty + 2;        // [2] scores landed
+    uint64_t* p_full = s_full + 2;         // [2] P written (4 warps)
+    uint64_t* pv_done = p_full + 2;        // [2]
+    uint64_t* o_free = pv_done + 2;        // [2] O of an item was read (4 warps)
+    uint64_t* k_full = o_free + 2;         // [RING]
+    uint64_t* k_empty = k_full + RING;     // [RING]
+    uint64_t* v_raw = k_empty + RING;      // [RING] V landed
+    uint64_t* v_full = v_raw + RING;       // [RING] V is safe to multiply
+    uint64_t* v_empty = v_full + RING;     // [RING]
+    uint64_t* i_full = v_empty + RING;     // [kRowsItems]
+    uint64_t* i_empty = i_full + kRowsItems;  // [kRowsItems] 8 softmax warps, MMA, loads, fix
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + kRowsItems);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    pdl_trigger();
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_addr(&q_full[i]), 1);
+            mbar_init(s_addr(&q_empty[i]), 1);
+            mbar_init(s_addr(&s_full[i]), 1);
+            mbar_init(s_addr(&p_full[i]), 4);
+            mbar_init(s_addr(&pv_done[i]), 1);
+            mbar_init(s_addr(&o_free[i]), 4);
+        }
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(s_addr(&k_full[i]), 1);
+            mbar_init(s_addr(&k_empty[i]), 1);
+            mbar_init(s_addr(&v_raw[i]), 1);
+            mbar_init(s_addr(&v_full[i]), 1);
+            mbar_init(s_addr(&v_empty[i]), 1);
+        }
+        for (int i = 0; i < kRowsItems; ++i) {
+            mbar_init(s_addr(&i_full[i]), 1);
+            mbar_init(s_addr(&i_empty[i]), 11);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kRowsMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)),
+                     "r"(kRowsTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
+    rows_plan(a, plan);  // ends with a CTA-wide barrier
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+    auto give_up = [&](int site) {  // a bounded wait ran out: every role leaves at its next wait
+        if (lane == 0) {
+            *abort_flag = 1;
+            record_timeout(a.status, site);
+        }
+    };
+    auto stopped = [&]() { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };
+    auto wait = [&](uint64_t* bar, int parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(s_addr(bar), (uint32_t)parity & 1u)) != 0;
+    };
+    // the k-th item of this CTA; false: none is left, or a wait ran out
+    auto next_item = [&](int k, RowsItem& it) -> bool {
+        const int d = k % kRowsItems;
+        if (!wait(&i_full[d], k / kRowsItems)) {
+            give_up(20);
+            return false;
+        }
+        if (stopped()) return false;
+        it = items[d];
+        return it.n_kt >= 0;
+    };
+    auto done_item = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_addr(&i_empty[k % kRowsItems]));
+    };
+
+    if (warp == kRowsSchedWarp) {
+        // ------------------------------------------------------------ scheduler
+        for (int k = 0;; ++k) {
+            const int d = k % kRowsItems;
+            if (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1)) {
+                give_up(21);
+                break;
+            }
+            if (stopped()) break;
+            int more = 0;
+            if (lane == 0) {
+                const int idx = a.counter ? (int)atomicAdd(a.counter, 1u) : (int)(blockIdx.x + k * gridDim.x);
+                const RowsItem it = rows_item(a, plan, idx);
+                items[d] = it;
+                more = it.n_kt >= 0;
+                mbar_arrive(s_addr(&i_full[d]));
+            }
+            if (!__shfl_sync(0xffffffffu, more, 0)) break;
+        }
+    } else if (warp == kRowsLoadWarp) {
+        // ------------------------------------------------------------ loads
+        int kc = 0, qn[2] = {0, 0};  // K / V tiles loaded; query loads of a slot
+        bool ok = true;
+        RowsItem it;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+            const bool pair = it.ntok1 > 0;
+            const int page0 = it.slot0 >> 4, pages = ((it.end + 15) >> 4) - page0;
+            const int32_t* tab = a.tables + (size_t)it.trow * a.max_blocks + page0;
+            auto page_at = [&](int i) {
+                int x = i < pages ? tab[i] : 0;
+                return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
+            };
+            int pg = it.n_kt > 0 ? page_at(lane) : 0, pg_next = 0;  // pages of four tiles, one a lane
+            for (int j = 0; j < it.n_kt && ok; ++j) {
+                if ((j & 3) == 0) {
+                    if (j) pg = pg_next;
+                    pg_next = page_at(8 * j + 32 + lane);
+                }
+                const int np = min(8, pages - 8 * j), slot = kc % RING, turn = kc / RING;
+                const int mine_k = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + (lane / NH) % 8);
+                const int mine_v = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + lane % 8);
+                if (turn && !(ok = wait(&k_empty[slot], turn - 1))) break;
+                if (lane == 0) mbar_expect_tx(s_addr(&k_full[slot]), (uint32_t)(np * NH * kBlockHalf));
+                __syncwarp();
+                if (lane < np * NH)
+                    tma_load_5d(s_addr(sK + slot * C::TILE + (lane % NH) * 16384 + (lane / NH) * kBlockHalf), &kmap, 0,
+                                it.kvh * 16, lane % NH, 0, mine_k, s_addr(&k_full[slot]));
+                if (j == 0) {  // the queries, behind the first keys
+                    for (int t = 0; t < (pair ? 2 : 1) && ok; ++t) {
+                        const int qs = pair ? t : k & 1;
+                        if (qn[qs] && !(ok = wait(&q_empty[qs], qn[qs] - 1))) break;
+                        ++qn[qs];
+                        const int ntok = t ? it.ntok1 : it.ntok0;
+                        const bool small = ntok <= a.tq_small;
+                        const uint32_t bytes = (uint32_t)((small ? a.tq_small : a.tpt) * a.G * 128);
+                        if (lane == 0) {
+                            mbar_expect_tx(s_addr(&q_full[qs]), bytes * NH);
+                            for (int h = 0; h < NH; ++h)
+                                tma_load_4d(s_addr(sQ + qs * C::TILE + h * 16384), small ? &qmap_small : &qmap, 0, h,
+                                            it.kvh * a.G, it.tok0 + t * a.tpt, s_addr(&q_full[qs]));
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                }
+                if (turn && !(ok = wait(&v_empty[slot], turn - 1))) break;
+                if (lane == 0) mbar_expect_tx(s_addr(&v_raw[slot]), (uint32_t)(np * NH * kBlockHalf));
+                __syncwarp();
+                if (lane < np)
+                    tma_load_5d(s_addr(sV + slot * C::TILE + lane * NH * kBlockHalf), &vmap, 0, it.kvh * 16, 0, 1,
+                                mine_v, s_addr(&v_raw[slot]));
+                ++kc;
+                if (stopped()) break;
+            }
+            if (!ok) give_up(22);
+            if (!ok || stopped()) break;
+            done_item(k);
+        }
+        if (stopped()) {  // the copies in flight land before the CTA leaves
+            for (int s = 0; s < 2; ++s)
+                if (qn[s]) (void)wait(&q_full[s], qn[s] - 1);
+            for (int c = max(0, kc - RING); c < kc; ++c) {
+                (void)wait(&k_full[c % RING], c / RING);
+                (void)wait(&v_raw[c % RING], c / RING);
+            }
+            if (!ok || kc == 0) (void)wait(&k_full[kc % RING], kc / RING);
+        }
+    } else if (warp == kRowsFixWarp) {
+        // ------------------------------------------------------------ V made safe
+        int vc = 0;
+        bool ok = true;
+        RowsItem it;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+            for (int j = 0; j < it.n_kt; ++j, ++vc) {
+                const int slot = vc % RING, key0 = it.slot0 + 128 * j;
+                if (!(ok = wait(&v_raw[slot], vc / RING)) || stopped()) break;
+                unsigned char* v = sV + slot * C::TILE;
+                const int n = min(128, it.end - key0);           // slots that exist
+                const int np = (n + 15) >> 4;
+                const int lo = rows_clamp(it.scan - key0, 0, n);  // from here not every row sees them
+                bool touched = false;
+                if (n < 16 * np) {
+                    for (int i = n * NH * 8 + lane; i < 16 * np * NH * 8; i += 32) {
+                        const int row = i / (NH * 8), h = i / 8 % NH;
+                        *reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
+                                                  (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    touched = true;
+                }
+                bool found = false;
+                for (int i = lo * NH * 8 + lane; i < n * NH * 8; i += 32) {
+                    const int row = i / (NH * 8), h = i / 8 % NH;
+                    uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
+                                                         (i & 7) * 16);
+                    uint4 x = *at;
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+                    bool mine = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
+                        if (l16) xs[e] &= 0xFFFF0000u;
+                        if (h16) xs[e] &= 0x0000FFFFu;
+                        mine |= l16 || h16;
+                    }
+                    if (mine) *at = x;
+                    found |= mine;
+                }
+                found = __any_sync(0xffffffffu, found);
+                if (found && lane == 0) items[k % kRowsItems].bad = 1;
+                if (touched || found) fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_addr(&v_full[slot]));
+            }
+            if (!ok) give_up(23);
+            if (!ok || stopped()) break;
+            done_item(k);
+        }
+    } else if (warp == kRowsMmaWarp) {
+        // ------------------------------------------------------------ MMA issuer
+        // Two cursors over the same operations: Q.K^T runs ahead of P.V.  An
+        // operation on a slot's S follows the P.V that read P there: both are
+        // issued here, and MMAs execute in the order of issue.
+        const uint32_t qb = s_addr(sQ), kb = s_addr(sK), vb = s_addr(sV);
+        RowsItem qi, pi;
+        int kq = 0, kp = 0, jq = 0, jp = 0, tq = 0, tp = 0;
+        int ck = 0, cv = 0;                        // K / V tiles used up
+        int nq[2] = {0, 0}, nv[2] = {0, 0};        // operations issued on a slot
+        int qloads[2] = {0, 0}, outs[2] = {0, 0};  // items begun on a slot, by cursor
+        bool have_q = false, have_p = false, end_q = false, end_p = false, failed = false;
+        uint64_t t_idle = 0;
+        while (!end_p) {
+            bool progressed = false;
+            if (!end_q && !have_q) {
+                if (__all_sync(0xffffffffu, mbar_test(s_addr(&i_full[kq % kRowsItems]), (kq / kRowsItems) & 1))) {
+                    qi = items[kq % kRowsItems];
+                    if (qi.n_kt < 0) end_q = true;
+                    else if (qi.n_kt == 0) ++kq;
+                    else {
+                        have_q = true;
+                        jq = tq = 0;
+                    }
+                    progressed = true;
+                }
+            }
+            if (have_q) {
+                const bool pair = qi.ntok1 > 0;
+                const int s = pair ? tq : kq & 1;
+                const bool ready = nq[s] == nv[s] && mbar_test(s_addr(&k_full[ck % RING]), (ck / RING) & 1) &&
+                                   (jq > 0 || mbar_test(s_addr(&q_full[s]), qloads[s] & 1));
+                if (__all_sync(0xffffffffu, ready)) {
+                    tc_fence_after();
+                    const bool last_t = !pair || tq == 1, last_j = jq == qi.n_kt - 1;
+                    if (lane == 0) {
+                        const int np = min(8, ((qi.end + 15) >> 4) - (qi.slot0 >> 4) - 8 * jq);
+                        const uint32_t idesc = idesc_f16(128, 16 * np);
+                        const uint32_t q0 = qb + s * C::TILE, k0 = kb + (ck % RING) * C::TILE;
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk)
+                            tc_mma_f16_ss(tmem + s * 128, sw128_desc(q0 + (kk >> 2) * 16384 + (kk & 3) * 32),
+                                          sw128_desc(k0 + (kk >> 2) * 16384 + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+                        tc_commit(s_addr(&s_full[s]));
+                        if (last_t) tc_commit(s_addr(&k_empty[ck % RING]));
+                        if (last_j) tc_commit(s_addr(&q_empty[s]));
+                    }
+                    __syncwarp();
+                    ++nq[s];
+                    if (last_j) ++qloads[s];
+                    if (last_t) {
+                        tq = 0;
+                        ++ck;
+                        if (++jq == qi.n_kt) {
+                            have_q = false;
+                            ++kq;
+                        }
+                    } else {
+                        tq = 1;
+                    }
+                    progressed = true;
+                }
+            }
+            if (!have_p) {
+                if (__all_sync(0xffffffffu, mbar_test(s_addr(&i_full[kp % kRowsItems]), (kp / kRowsItems) & 1))) {
+                    pi = items[kp % kRowsItems];
+                    if (pi.n_kt < 0) end_p = true;
+                    else if (pi.n_kt == 0) {
+                        if (kq > kp) {
+                            done_item(kp);
+                            ++kp;
+                        }
+                    } else {
+                        have_p = true;
+                        jp = tp = 0;
+                    }
+                    progressed = true;
+                }
+            }
+            if (have_p) {
+                const bool pair = pi.ntok1 > 0;
+                const int s = pair ? tp : kp & 1;
+                const bool ready = nq[s] > nv[s] && mbar_test(s_addr(&p_full[s]), nv[s] & 1) &&
+                                   mbar_test(s_addr(&v_full[cv % RING]), (cv / RING) & 1) &&
+                                   (jp > 0 || outs[s] == 0 || mbar_test(s_addr(&o_free[s]), (outs[s] - 1) & 1));
+                if (__all_sync(0xffffffffu, ready)) {
+                    tc_fence_after();
+                    const bool last_t = !pair || tp == 1;
+                    if (lane == 0) {
+                        const int np = min(8, ((pi.end + 15) >> 4) - (pi.slot0 >> 4) - 8 * jp);
+                        const uint32_t v0 = vb + (cv % RING) * C::TILE;
+                        for (int i = 0; i < np; ++i)
+                            tc_mma_f16_ts(tmem + 256 + s * HD, tmem + s * 128 + i * 8,
+                                          sw128_mn_desc(v0 + i * NH * kBlockHalf, kBlockHalf, 1024),
+                                          idesc_f16_bmn(128, HD), (jp > 0 || i > 0) ? 1u : 0u);
+                        tc_commit(s_addr(&pv_done[s]));
+                        if (last_t) tc_commit(s_addr(&v_empty[cv % RING]));
+                    }
+                    __syncwarp();
+                    if (jp == 0) ++outs[s];
+                    ++nv[s];
+                    if (last_t) {
+                        tp = 0;
+                        ++cv;
+                        if (++jp == pi.n_kt) {
+                            have_p = false;
+                            done_item(kp);
+                            ++kp;
+                        }
+                    } else {
+                        tp = 1;
+                    }
+                    progressed = true;
+                }
+            }
+            if (progressed) {
+                t_idle = 0;
+            } else {
+                const uint64_t now = gtimer();
+                if (t_idle == 0) t_idle = now;
+                failed = __any_sync(0xffffffffu, now - t_idle > 2000000000ull);
+                if (failed || stopped()) break;
+            }
+        }
+        if (failed) give_up(24);
+        // every MMA has finished with shared and tensor memory before the CTA leaves
+        for (int s = 0; s < 2; ++s) {
+            if (nq[s]) (void)wait(&s_full[s], nq[s] - 1);
+            if (nv[s]) (void)wait(&pv_done[s], nv[s] - 1);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax, one thread per query row
+        const int ws = warp >> 2;                      // tile slot
+        const int quarter = warp & 3;                  // TMEM lanes of this warp
+        const int row = quarter * 32 + lane;
+        const int ti = row / a.G, g = row % a.G;       // token of the tile, head of the group
+        const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t t_s = t_lane + ws * 128, t_o = t_lane + 256 + ws * HD;
+        int c = 0;  // operations on this slot
+        bool ok = true;
+        RowsItem it;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+            const bool pair = it.ntok1 > 0;
+            if (!pair && (k & 1) != ws) {
+                done_item(k);
+                continue;
+            }
+            const int t = pair ? ws : 0;               // tile of the item
+            const int ntok = t ? it.ntok1 : it.ntok0;
+            const int i = it.i0 + t * a.tpt + ti;      // row of the segment
+            const bool real = ti < ntok;
+            const bool here = quarter * 32 < ntok * a.G;  // the warp holds a real row
+            const uint64_t bits = it.mode == kModeMask && real ? a.mask[i] : 0ull;
+            // slots below `every` are seen by all rows of the tile
+            const int every = it.mode == kModeCausal ? min(it.end, it.ctx + it.i0 + t * a.tpt + 1)
+                                                     : (it.mode == kModeMask ? min(it.end, it.ctx) : it.end);
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < it.n_kt; ++j, ++c) {
+                if (!(ok = wait(&s_full[ws], c)) || stopped()) break;
+                tc_fence_after();
+                if (here) {
+                    uint32_t sv[128];
+                    tc_ld_x32(t_s, sv);
+                    tc_ld_x32(t_s + 32, sv + 32);
+                    tc_ld_x32(t_s + 64, sv + 64);
+                    tc_ld_x32(t_s + 96, sv + 96);
+                    tc_wait_ld();
+                    const int key0 = it.slot0 + 128 * j;
+                    if (key0 + 128 > every) {
+                        uint32_t w[4];
+                        rows_seen(it, key0, i, bits, w);
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            if (!((w[e >> 5] >> (e & 31)) & 1u)) sv[e] = 0xFF800000u;  // -inf
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
+#pragma unroll
+                    for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[e]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+                    const bool grow = top > m + 8.0f;  // also where the row had seen nothing yet
+                    const float m_new = grow ? top : m;
+                    const float alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
+                    const float sub = m_new == -INFINITY ? 0.f : m_new;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t pw[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float x0 = rows_exp2(fmaf(__uint_as_float(sv[64 * half + 2 * e]), a.scale_log2, -sub));
+                            const float x1 =
+                                rows_exp2(fmaf(__uint_as_float(sv[64 * half + 2 * e + 1]), a.scale_log2, -sub));
+                            sum[(2 * e) & 3] += x0;
+                            sum[(2 * e + 1) & 3] += x1;
+                            const __half2 h = __floats2half2_rn(x0, x1);
+                            pw[e] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        tc_st_x32(t_s + 32 * half, pw);
+                    }
+                    // O holds the tiles before this one: rescale it once their P.V has landed
+                    if (j > 0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                        if (!(ok = wait(&pv_done[ws], c - 1))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < HD; c0 += 32) {
+                            uint32_t ov[32];
+                            tc_ld_x32(t_o + c0, ov);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                            tc_st_x32(t_o + c0, ov);
+                        }
+                    }
+                    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    m = m_new;
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_addr(&p_full[ws]));
+            }
+            if (!ok) give_up(25);
+            if (!ok || stopped()) break;
+            if (it.n_kt > 0) {
+                if (!(ok = wait(&pv_done[ws], c - 1))) {
+                    give_up(26);
+                    break;
+                }
+                tc_fence_after();
+            }
+            // ---- the item's rows: O / l, or O with (m, l) for the merge
+            if (here) {
+                const bool bad = it.n_kt > 0 && *reinterpret_cast<volatile int*>(&items[k % kRowsItems].bad) != 0;
+                const int head = it.kvh * a.G + g, tok = it.tok0 + t * a.tpt + ti;
+                const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+                const size_t prow = (size_t)(it.prow + t * a.tpt + ti) * a.Hq + head;
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    uint32_t ov[32];
+                    __syncwarp();  // rows that are not real skip the stores below
+                    if (it.n_kt > 0) {
+                        tc_ld_x32(t_o + c0, ov);
+                        tc_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] = 0u;
+                    }
+                    if (bad && real) {
+                        const int hi = min(it.end, it.slot0 + 128 * it.n_kt);
+                        for (int s = max(it.scan, it.slot0); s < hi; ++s) {
+                            const bool seen = it.mode == kModeCausal
+                                                  ? s <= it.ctx + i
+                                                  : (s - it.ctx < 64 && ((bits >> (s - it.ctx)) & 1ull));
+                            if (!seen) continue;
+                            const int x = a.tables[(size_t)it.trow * a.max_blocks + (s >> 4)];
+                            const int page = x < 0 || x >= a.num_blocks ? 0 : x;
+                            const __half* v = a.kv +
+                                              ((((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 + (s & 15)) * HD + c0;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float y = __half2float(v[e]);
+                                if (!isfinite(y)) ov[e] = __float_as_uint(__uint_as_float(ov[e]) + y);
+                            }
+                        }
+                    }
+                    if (real && it.prow < 0) {
+                        __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + c0;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 w;
+                            uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const __half2 h = __floats2half2_rn(__uint_as_float(ov[e + 2 * q]) * inv,
+                                                                    __uint_as_float(ov[e + 2 * q + 1]) * inv);
+                                wp[q] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            *reinterpret_cast<uint4*>(dst + e) = w;
+                        }
+                    } else if (real) {
+                        uint4* dst = reinterpret_cast<uint4*>(a.po + prow * HD + c0);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) dst[e / 4] = make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+                    }
+                }
+                if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
+            }
+            if (it.n_kt > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_addr(&o_free[ws]));
+            }
+            done_item(k);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kRowsMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kRowsTmemCols));
+    }
+}
+
+// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
+// their order.  One CTA per token row, a warp per head.
+template <int HD>
+__global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
+    constexpr int E = HD / 32;
+    pdl_wait();
+    const int tok = blockIdx.x, lane = threadIdx.x & 31;
+    int b, i;
+    if (a.row_off) {
+        int lo = 0, hi = a.B;  // first sequence whose end is past tok
         while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (a.row_off[mid + 1] > t) hi = mid;
+            const int mid = (lo + hi) >> 1;
+            if (a.row_off[mid + 1] > tok) hi = mid;
             else lo = mid + 1;
         }
         b = lo;
-        if (b >= a.B || t < a.row_off[b]) return;  // a row of no sequence
-        i = t - a.row_off[b];
-        n = a.row_off[b + 1] - a.row_off[b];
+        if (b >= a.B) return;
+        i = tok - max(0, a.row_off[b]);
+        if (i < 0) return;
     } else {
-        b = t / a.R;
-        i = t % a.R;
-        n = a.R;
+        b = tok / a.R;
+        i = tok % a.R;
     }
-    const int ctx = max(0, a.ctx_len[b]);
-    const long long cap = (long long)a.max_blocks * 16;
-    const int L = (int)min((long long)ctx + n, cap);
-    const uint64_t bits = a.mask ? a.mask[i] : 0;
-    float q[E], o[E];
-    const __half* qp = a.q + (size_t)t * a.ldq + (size_t)h * HD + lane * E;
+    const RowsMeta mt = a.meta[b];
+    const int n = mt.n_pre + mt.n_own;
+    if (n == 0) return;
+    for (int head = threadIdx.x >> 5; head < a.Hq; head += 8) {
+        auto at = [&](int p) -> size_t {
+            const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
+            return (size_t)(r + i) * a.Hq + head;
+        };
+        // up to 64 pieces: two a lane
+        float2 ml[2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = __half2float(qp[e]) * a.scale_log2;
-        o[e] = 0.f;
+        for (int u = 0; u < 2; ++u) ml[u] = lane + 32 * u < n ? a.pml[at(lane + 32 * u)] : make_float2(-INFINITY, 0.f);
+        const float M = warp_max(fmaxf(ml[0].x, ml[1].x));
+        const float sub = M == -INFINITY ? 0.f : M;
+        const float w0 = exp2f(ml[0].x - sub), w1 = exp2f(ml[1].x - sub);
+        const float l = warp_sum(w0 * ml[0].y + w1 * ml[1].y);
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+        for (int p = 0; p < n; ++p) {
+            const float w = __shfl_sync(0xffffffffu, p < 32 ? w0 : w1, p & 31);
+            const float* src = a.po + at(p) * HD + lane * E;
+            if (w == 0.f) continue;  // a piece without a seen slot, or far below
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += w * src[e];
+        }
+        __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[e] = __float2half_rn(o[e] * inv);
     }
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < L; ++j) {
-        const bool seen = j < ctx || (a.mask ? (j - ctx < 64 && ((bits >> (j - ctx)) & 1)) : j - ctx <= i);
-        if (!seen) continue;
-        int blk = a.tables[(size_t)b * a.max_blocks + j / 16];
-        if (blk < 0 || blk >= a.num_blocks) blk = 0;  // a malformed table reads block 0, never out of range
-        const __half* kp = a.kv + ((((size_t)blk * 2) * a.Hkv + kvh) * 16 + j % 16) * HD + lane * E;
-        const __half* vp = kp + (size_t)a.Hkv * 16 * HD;
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += q[e] * __half2float(kp[e]);
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s);
-        const float w = exp2f(m - mn), p = exp2f(s - mn);
-        l = l * w + p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * w + p * __half2float(vp[e]);
-        m = mn;
-    }
-    __half* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * E;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < E; ++e) op[e] = __float2half_rn(o[e] * inv);
 }
 
-static int launch_rows(const RowAttnArgs& a, int HD, cudaStream_t s) {
-    const long long warps = (long long)a.T * a.Hq;
-    const unsigned grid = (unsigned)((warps + 3) / 4);
-    if (HD == 128) row_attention_kernel<128><<<grid, 128, 0, s>>>(a);
-    else row_attention_kernel<64><<<grid, 128, 0, s>>>(a);
-    SD_LAUNCH_CHECK("row_attention_kernel");
+// ------------------------------------------------------------------ host side
+// The queries as [T][Hq][HD / 64][64]: one box is `tokens` tokens of one group
+// and column half, rows token * G + g of 128 bytes.
+static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq, int HD, int G, int tokens) {
+    auto enc = attn_encode();
+    SD_CHECK(enc, SPECDEC_ENOTSUP, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[4] = {64, (cuuint64_t)(HD / 64), (cuuint64_t)Hq, (cuuint64_t)T};
+    cuuint64_t strides[3] = {128, (cuuint64_t)HD * 2, (cuuint64_t)ldq * 2};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)G, (cuuint32_t)tokens};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(q), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    SD_CHECK(r == CUDA_SUCCESS, SPECDEC_EINVAL, "attention: cuTensorMapEncodeTiled failed for the queries");
+    return SPECDEC_OK;
+}
+
+constexpr int kRowsSplitTokens = 4096;   // prompts of more rows fill the GPU without splits
+constexpr int kRowsPartialRows = 8192;   // room for pieces beyond the first, in token rows
+
+// Rows of the partial buffers.
+static size_t prompt_partial_rows(int T) {
+    return T <= kRowsSplitTokens ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : 0;
+}
+static size_t shared_partial_rows(int T) {
+    return 2 * (size_t)T + std::min<size_t>(2 * (size_t)(kRowsMaxSplits - 1) * T, kRowsPartialRows);
+}
+static size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t rows_workspace(size_t prows, int B, int Hq, int HD) {
+    return 256 + align256(sizeof(RowsMeta) * (size_t)B) + align256(prows * Hq * sizeof(float2)) +
+           prows * Hq * HD * sizeof(float);
+}
+
+struct DeviceFacts {
+    std::atomic<int> sms{0};
+};
+static int rows_sms(int* out) {  // SMs of the current device; sets the kernels' shared memory on it once
+    static DeviceFacts facts[64];
+    int dev = 0;
+    SD_CUDA(cudaGetDevice(&dev));
+    SD_CHECK(dev >= 0 && dev < 64, SPECDEC_ENOTSUP, "attention: device index above 63");
+    int n = facts[dev].sms.load();
+    if (!n) {
+        SD_CUDA(cudaFuncSetAttribute(rows_attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)RowsCfg<128>::smem));
+        SD_CUDA(cudaFuncSetAttribute(rows_attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)RowsCfg<64>::smem));
+        SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        facts[dev].sms.store(n);
+    }
+    *out = n;
+    return SPECDEC_OK;
+}
+
+// Fills in what both calls share and launches.  tiles: an upper bound of the
+// items before splits.
+static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, int HD, size_t prows, long long tiles,
+                       void* ws, cudaStream_t s) {
+    int sms = 0;
+    int rc = rows_sms(&sms);
+    if (rc) return rc;
+    a.G = a.Hq / a.Hkv;
+    a.tpt = 128 / a.G;
+    a.tq_small = std::min(a.tq_small, a.tpt);
+    a.kv = kv;
+    a.slots_max = a.max_blocks * 16;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)HD));
+    a.status = device_status_ptr();
+    a.prows = (int)prows;
+    char* w = static_cast<char*>(ws);
+    // more items than CTAs: they are taken from a counter, the longest first
+    a.counter = tiles > sms ? reinterpret_cast<uint32_t*>(w) : nullptr;
+    a.meta = prows ? reinterpret_cast<RowsMeta*>(w + 256) : nullptr;
+    w += 256 + align256(sizeof(RowsMeta) * (size_t)a.B);
+    a.pml = reinterpret_cast<float2*>(w);
+    a.po = reinterpret_cast<float*>(w + align256(prows * a.Hq * sizeof(float2)));
+    CUtensorMap qmap, qsmall, kmap, vmap;
+    rc = make_q_tmap(&qmap, q, ldq, a.T, a.Hq, HD, a.G, a.tpt);
+    if (!rc) rc = make_q_tmap(&qsmall, q, ldq, a.T, a.Hq, HD, a.G, a.tq_small);
+    if (!rc) rc = make_kv_tmap(&kmap, kv, a.num_blocks, a.Hkv, HD, 1, 1);
+    if (!rc) rc = make_kv_tmap(&vmap, kv, a.num_blocks, a.Hkv, HD, HD / 64, 1);
+    if (rc) return rc;
+    if (a.counter) SD_CUDA(cudaMemsetAsync(a.counter, 0, sizeof(uint32_t), s));
+    const unsigned grid = (unsigned)(prows ? sms : std::min<long long>(sms, tiles));
+    if (HD == 128) rows_attention_kernel<128><<<grid, kRowsThreads, RowsCfg<128>::smem, s>>>(qmap, qsmall, kmap, vmap, a);
+    else rows_attention_kernel<64><<<grid, kRowsThreads, RowsCfg<64>::smem, s>>>(qmap, qsmall, kmap, vmap, a);
+    SD_LAUNCH_CHECK("rows_attention_kernel");
+    if (prows) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)a.T);
+        cfg.blockDim = dim3(256);
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (HD == 128) SD_CUDA(cudaLaunchKernelEx(&cfg, rows_merge_kernel<128>, a));
+        else SD_CUDA(cudaLaunchKernelEx(&cfg, rows_merge_kernel<64>, a));
+    }
     return SPECDEC_OK;
 }
 
@@ -104,10 +1099,15 @@ static int check_rows(const char* who, const void* q, const void* kv, const void
              w + ": bad head counts (at most 1024 query heads, 128 for each KV head)");
     SD_CHECK(num_blocks > 0 && max_blocks > 0 && max_blocks <= (1 << 26), SPECDEC_EINVAL,
              w + ": empty block pool or table");
-    SD_CHECK(B >= 0 && B <= kRowsMaxSeqs, SPECDEC_EINVAL, w + ": 0 to 4096 sequences");
+    SD_CHECK(B >= 0 && B <= kRowsMaxSeqs, SPECDEC_EINVAL, w + ": 0 to 1024 sequences");
     SD_CHECK(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv) | reinterpret_cast<uintptr_t>(out)) &
               15) == 0,
              SPECDEC_EINVAL, w + ": q, KV pool and out must be 16-byte aligned");
+    return SPECDEC_OK;
+}
+static int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
+    SD_CHECK(ws && have >= need && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, SPECDEC_EINVAL,
+             std::string(who) + ": workspace too small or not 16-byte aligned");
     return SPECDEC_OK;
 }
 
@@ -117,8 +1117,9 @@ using namespace specdec;
 
 extern "C" size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                            int max_blocks) {
-    (void)B, (void)T, (void)n_q_heads, (void)n_kv_heads, (void)head_dim, (void)max_blocks;
-    return 0;
+    (void)n_kv_heads, (void)max_blocks;
+    if (B <= 0 || T <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
+    return rows_workspace(prompt_partial_rows(T), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -132,33 +1133,36 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
     SD_CHECK(T >= 0 && T <= (1 << 24), SPECDEC_EINVAL, "attention_prompt: 0 to 2^24 rows");
     SD_CHECK(ldq >= n_q_heads * head_dim && ldq % 8 == 0 && ldo >= n_q_heads * head_dim && ldo % 8 == 0,
              SPECDEC_EINVAL, "attention_prompt: row strides hold all heads and are multiples of 8");
-    (void)workspace;
-    (void)workspace_bytes;
     if (B == 0 || T == 0) return SPECDEC_OK;
-    RowAttnArgs a = {};
-    a.q = reinterpret_cast<const __half*>(q);
-    a.ldq = ldq;
-    a.kv = reinterpret_cast<const __half*>(kv_layer);
+    const size_t prows = prompt_partial_rows(T);
+    if ((rc = check_workspace("attention_prompt", workspace, workspace_bytes,
+                              rows_workspace(prows, B, n_q_heads, head_dim))))
+        return rc;
+    RowsArgs a = {};
     a.num_blocks = num_blocks;
     a.Hkv = n_kv_heads;
     a.Hq = n_q_heads;
-    a.G = n_q_heads / n_kv_heads;
     a.tables = tables;
     a.max_blocks = max_blocks;
     a.ctx_len = ctx_len;
     a.row_off = row_off;
     a.B = B;
     a.T = T;
+    a.R = 1;
+    a.tq_small = 1;
     a.out = reinterpret_cast<__half*>(out);
     a.ldo = ldo;
-    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
-    return launch_rows(a, head_dim, as_stream(stream));
+    const int tpt2 = 2 * (128 / (n_q_heads / n_kv_heads));
+    return launch_rows(a, reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer), head_dim,
+                       prows, (long long)n_kv_heads * ((T + tpt2 - 1) / tpt2 + std::min(B, T)), workspace,
+                       as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads,
                                                                   int n_kv_heads, int head_dim, int max_blocks) {
-    (void)B, (void)R, (void)n_groups, (void)n_q_heads, (void)n_kv_heads, (void)head_dim, (void)max_blocks;
-    return 0;
+    (void)n_groups, (void)n_kv_heads, (void)max_blocks;
+    if (B <= 0 || R <= 0 || B > kRowsMaxSeqs || R > 64 || n_q_heads <= 0 || head_dim <= 0) return 0;
+    return rows_workspace(shared_partial_rows(B * R), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer, int num_blocks,
@@ -173,26 +1177,30 @@ extern "C" int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t
     if (rc) return rc;
     SD_CHECK(R >= 1 && R <= 64, SPECDEC_EINVAL, "attention_shared_prefix: 1 to 64 rows");
     SD_CHECK(n_groups >= 0 && n_groups <= B, SPECDEC_EINVAL, "attention_shared_prefix: 0 to B groups");
-    (void)workspace;
-    (void)workspace_bytes;
     if (B == 0) return SPECDEC_OK;
-    RowAttnArgs a = {};
-    a.q = reinterpret_cast<const __half*>(q);
-    a.ldq = n_q_heads * head_dim;
-    a.kv = reinterpret_cast<const __half*>(kv_layer);
+    const size_t prows = shared_partial_rows(B * R);
+    if ((rc = check_workspace("attention_shared_prefix", workspace, workspace_bytes,
+                              rows_workspace(prows, B, n_q_heads, head_dim))))
+        return rc;
+    RowsArgs a = {};
     a.num_blocks = num_blocks;
     a.Hkv = n_kv_heads;
     a.Hq = n_q_heads;
-    a.G = n_q_heads / n_kv_heads;
     a.tables = tables;
     a.max_blocks = max_blocks;
     a.ctx_len = ctx_len;
     a.mask = mask;
+    a.group_off = group_off;
+    a.shared_blocks = shared_blocks;
+    a.n_groups = n_groups;
     a.B = B;
-    a.R = R;
     a.T = B * R;
+    a.R = R;
+    a.tq_small = R;
     a.out = reinterpret_cast<__half*>(out);
-    a.ldo = a.ldq;
-    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
-    return launch_rows(a, head_dim, as_stream(stream));
+    a.ldo = n_q_heads * head_dim;
+    const int tpt2 = 2 * (128 / (n_q_heads / n_kv_heads));
+    const long long tiles = (long long)n_kv_heads * ((a.T + tpt2 - 1) / tpt2 + n_groups + (long long)B * ((R + tpt2 - 1) / tpt2));
+    return launch_rows(a, reinterpret_cast<const __half*>(q), a.ldo, reinterpret_cast<const __half*>(kv_layer),
+                       head_dim, prows, tiles, workspace, as_stream(stream));
 }

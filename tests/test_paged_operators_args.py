@@ -30,7 +30,7 @@ def shared(**kw):
 
 COMMON = [dict(q=None), dict(kv=None), dict(tables=None), dict(ctx=None), dict(out=None), dict(hd=96), dict(hd=256),
           dict(Hkv=3), dict(Hkv=0), dict(Hkv=-2), dict(Hq=0), dict(num_blocks=0), dict(max_blocks=0),
-          dict(max_blocks=(1 << 26) + 1), dict(B=-1), dict(B=4097), dict(q=PTR + 2), dict(kv=PTR + 8),
+          dict(max_blocks=(1 << 26) + 1), dict(B=-1), dict(B=1025), dict(q=PTR + 2), dict(kv=PTR + 8),
           dict(out=PTR + 4), dict(Hq=2048, Hkv=16)]
 
 
