@@ -368,6 +368,31 @@ int specdec_kv_append(specdec_kv* kv, const int32_t* reqs, const int32_t* n_toke
                       void* stream);
 int specdec_kv_free_request(specdec_kv* kv, int req, void* stream);
 int specdec_kv_share_prefix(specdec_kv* kv, int new_req, int src_req, int shared_len, void* stream);
+/* Forks (n samples of one prompt, beams that survive): request new_reqs[i]
+ * becomes a copy of src_reqs[i], i < n.  It shares the source's whole blocks
+ * (reference counts) and, where the source's last block is partly used, gets
+ * a block of its own (the lowest free ones, in the order of the call) into
+ * which the used rows are copied in each of `layers` layers of the fp16 pool
+ * (pool + l * layer_stride halves, [num_blocks, 2, Hkv, 16, hd]; layers = 0:
+ * tables only).  What new_reqs[i] held before is released first; a source may
+ * be forked many times.  Host arrays; synchronises the stream.  All or
+ * nothing: EINVAL (an id out of range, a source without a table, a target
+ * named twice or also a source) and ENOMEM change nothing.  Unlike
+ * specdec_kv_share_prefix, whose reference semantics overwrite the new
+ * request's table without releasing it and share the block in use. */
+int specdec_kv_fork(specdec_kv* kv, const int32_t* src_reqs, const int32_t* new_reqs, int n, uint16_t* pool,
+                    int layers, size_t layer_stride, int n_kv_heads, int head_dim, void* stream);
+/* The same on a caller's own tables, in device memory, without host
+ * synchronisation (may be captured): tables [max_reqs, max_blocks] (-1
+ * padded), n_blocks [max_reqs] (-1: no table), lens [max_reqs], refcounts
+ * [num_blocks] (0: free), src / dst [n].  *status (device) receives
+ * SPECDEC_OK, SPECDEC_EINVAL or SPECDEC_ENOMEM; only OK changes anything.
+ * Calls in flight at the same time need workspaces of their own. */
+size_t specdec_kv_fork_pages_workspace_bytes(int num_blocks, int max_reqs, int n);
+int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t* lens, int32_t* refcounts, int num_blocks,
+                          int max_reqs, int max_blocks, const int32_t* src, const int32_t* dst, int n, uint16_t* kv,
+                          int layers, size_t layer_stride, int n_kv_heads, int head_dim, int32_t* status,
+                          void* workspace, size_t workspace_bytes, void* stream);
 int specdec_kv_free_merged_blocks(specdec_kv* kv, int req, int n_blocks, void* stream);
 int specdec_kv_evict_tokens(specdec_kv* kv, int req, int n_tokens, int* evicted, void* stream);
 /* Token-granular rollback: new lengths (host array, -1 = unchanged); tail
@@ -456,6 +481,14 @@ int specdec_engine_admit(specdec_engine* e, int seq, int32_t request_id, const i
 /* Releases slot `seq`: its KV blocks (shared blocks survive while another
  * slot holds them) and, with an index, its prefix references. */
 int specdec_engine_retire(specdec_engine* e, int seq, specdec_radix* cache);
+/* Slots new_seqs[i], i < n, become copies of slot `seq` (specdec_kv_fork of
+ * its K/V in every layer, its pending token and draft state): n samples of
+ * one prompt from one prefill, or a branch of a running generation.  Their
+ * previous requests are retired (with an index, their prefix references);
+ * request_ids (may be NULL: none) are recorded for them.  EINVAL or ENOMEM
+ * leave every slot as it was.  Synchronises the engine stream. */
+int specdec_engine_fork(specdec_engine* e, int seq, const int32_t* new_seqs, const int32_t* request_ids, int n,
+                        specdec_radix* cache);
 /* The first half of specdec_engine_admit, for chunked admission: retires the
  * slot, shares the indexed prefix of the prompt's K/V tokens whose source
  * request holds a slot (whole blocks, at most prompt_len - 2 tokens) and

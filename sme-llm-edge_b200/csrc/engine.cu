@@ -1194,6 +1194,37 @@ extern "C" int specdec_engine_retire(specdec_engine* e, int seq, specdec_radix* 
     return specdec_kv_free_request(e->kvm, seq, e->stream);
 }
 
+extern "C" int specdec_engine_fork(specdec_engine* e, int seq, const int32_t* new_seqs, const int32_t* request_ids,
+                                   int n, specdec_radix* cache) {
+    SD_CHECK(e && seq >= 0 && seq < e->B && n >= 0 && n <= e->B && (n == 0 || new_seqs), SPECDEC_EINVAL,
+             "engine_fork: bad argument");
+    std::vector<char> named(e->B, 0);
+    for (int i = 0; i < n; ++i) {
+        const int d = new_seqs[i];
+        SD_CHECK(d >= 0 && d < e->B && d != seq && !named[d], SPECDEC_EINVAL,
+                 "engine_fork: a new slot out of range, named twice or the source");
+        named[d] = 1;
+    }
+    if (n == 0) return SPECDEC_OK;
+    cudaStream_t s = e->stream;
+    const int H = e->mc.hidden;
+    const std::vector<int32_t> src(n, seq);
+    // on an error nothing has changed: the new slots still hold their requests
+    int rc = specdec_kv_fork(e->kvm, src.data(), new_seqs, n, reinterpret_cast<uint16_t*>(e->kv), e->mc.layers,
+                             e->layer_stride, e->mc.n_kv_heads, e->mc.head_dim, s);
+    if (rc) return rc;
+    for (int i = 0; i < n; ++i) {
+        const int d = new_seqs[i];
+        if (cache && e->slot_request[d] >= 0 && (rc = specdec_radix_release(cache, e->slot_request[d]))) return rc;
+        e->slot_request[d] = request_ids ? request_ids[i] : -1;
+        SD_CUDA(cudaMemcpyAsync(e->pending + d, e->pending + seq, sizeof(int32_t), cudaMemcpyDeviceToDevice, s));
+        SD_CUDA(cudaMemcpyAsync(e->h0 + (size_t)d * H, e->h0 + (size_t)seq * H, sizeof(float) * H,
+                                cudaMemcpyDeviceToDevice, s));
+    }
+    SD_CUDA(cudaStreamSynchronize(s));
+    return SPECDEC_OK;
+}
+
 namespace {
 // Prompt tokens [c_begin, c_end) of slot seq (d_tok[0, T) on the device)
 // through the forward in chunks of at most 64 rows under the chain mask, each

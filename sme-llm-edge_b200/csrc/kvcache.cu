@@ -200,6 +200,7 @@ struct specdec_kv {
     KVState s;
     int32_t* h_tmp = nullptr;  // pinned staging
     int32_t* d_tmp = nullptr;  // device staging [3 * max_reqs + 8]
+    int32_t* d_fork = nullptr;  // workspace of a fork
 };
 
 namespace specdec {
@@ -236,6 +237,7 @@ extern "C" int specdec_kv_create(int num_blocks, int block_size, int max_reqs, i
     if (e == cudaSuccess) e = cudaMalloc(&s.scratch, sizeof(int32_t) * scratch);
     if (e == cudaSuccess) e = cudaMalloc(&s.status, sizeof(int32_t) * 4);
     if (e == cudaSuccess) e = cudaMalloc(&kv->d_tmp, sizeof(int32_t) * (3 * (size_t)max_reqs + 8));
+    if (e == cudaSuccess) e = cudaMalloc(&kv->d_fork, kv_fork_workspace(num_blocks, max_reqs, max_reqs));
     if (e == cudaSuccess) e = cudaMallocHost(&kv->h_tmp, sizeof(int32_t) * (3 * (size_t)max_reqs + 8));
     if (e == cudaSuccess) e = cudaMemset(s.tables, 0xff, sizeof(int32_t) * (size_t)max_reqs * max_blocks_per_req);
     if (e == cudaSuccess) e = cudaMemset(s.nblk, 0xff, sizeof(int32_t) * max_reqs);
@@ -262,6 +264,7 @@ extern "C" int specdec_kv_destroy(specdec_kv* kv) {
     cudaFree(s.scratch);
     cudaFree(s.status);
     cudaFree(kv->d_tmp);
+    cudaFree(kv->d_fork);
     cudaFreeHost(kv->h_tmp);
     delete kv;
     return SPECDEC_OK;
@@ -309,6 +312,34 @@ extern "C" int specdec_kv_share_prefix(specdec_kv* kv, int new_req, int src_req,
              SPECDEC_EINVAL, "kv_share_prefix: bad argument");
     kv_share_prefix_kernel<<<1, 1, 0, as_stream(stream)>>>(kv->s, new_req, src_req, shared_len);
     SD_LAUNCH_CHECK("kv_share_prefix_kernel");
+    return SPECDEC_OK;
+}
+
+extern "C" int specdec_kv_fork(specdec_kv* kv, const int32_t* src_reqs, const int32_t* new_reqs, int n, uint16_t* pool,
+                               int layers, size_t layer_stride, int n_kv_heads, int head_dim, void* stream) {
+    SD_CHECK(kv && n >= 0 && n <= kv->s.max_reqs && (n == 0 || (src_reqs && new_reqs)), SPECDEC_EINVAL,
+             "kv_fork: bad argument");
+    int rc = kv_fork_check_pool("kv_fork", pool, layers, layer_stride, kv->s.num_blocks, n_kv_heads, head_dim);
+    if (rc) return rc;
+    SD_CHECK(layers == 0 || kv->s.block_size == 16, SPECDEC_EINVAL, "kv_fork: a pool's blocks hold 16 tokens");
+    if (n == 0) return SPECDEC_OK;
+    cudaStream_t s = as_stream(stream);
+    int32_t* h = kv->h_tmp;
+    for (int i = 0; i < n; ++i) {
+        h[i] = src_reqs[i];
+        h[n + i] = new_reqs[i];
+    }
+    SD_CUDA(cudaMemcpyAsync(kv->d_tmp, h, sizeof(int32_t) * 2 * n, cudaMemcpyHostToDevice, s));
+    int32_t* d_status = kv->d_tmp + 2 * n;
+    rc = kv_fork_launch(kv->s, kv->d_tmp, kv->d_tmp + n, n, reinterpret_cast<__half*>(pool), layers, layer_stride,
+                        n_kv_heads, head_dim, d_status, kv->d_fork, s);
+    cudaError_t e = cudaMemcpyAsync(h, d_status, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (rc) return rc;
+    if (e != cudaSuccess) return cuda_status(e, "kv_fork");
+    SD_CHECK(h[0] != SPECDEC_EINVAL, SPECDEC_EINVAL,
+             "kv_fork: a request id out of range, a source without a table, or a target named twice or also a source");
+    SD_CHECK(h[0] != SPECDEC_ENOMEM, SPECDEC_ENOMEM, "kv_fork: KV block pool exhausted (nothing was changed)");
     return SPECDEC_OK;
 }
 

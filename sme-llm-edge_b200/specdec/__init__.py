@@ -120,6 +120,9 @@ _SIGS = {
     "specdec_kv_append": (I, [P, P, P, I, P, P]),
     "specdec_kv_free_request": (I, [P, I, P]),
     "specdec_kv_share_prefix": (I, [P, I, I, I, P]),
+    "specdec_kv_fork": (I, [P, P, P, I, P, I, SZ, I, I, P]),
+    "specdec_kv_fork_pages_workspace_bytes": (SZ, [I, I, I]),
+    "specdec_kv_fork_pages": (I, [P, P, P, P, I, I, I, P, P, I, P, I, SZ, I, I, P, P, SZ, P]),
     "specdec_kv_free_merged_blocks": (I, [P, I, I, P]),
     "specdec_kv_evict_tokens": (I, [P, I, I, C.POINTER(I), P]),
     "specdec_kv_truncate": (I, [P, P, I, P]),
@@ -133,6 +136,7 @@ _SIGS = {
     "specdec_engine_load_sme": (I, [P, P, U32]),
     "specdec_engine_admit": (I, [P, I, C.c_int32, P, I, P, C.POINTER(C.c_int32)]),
     "specdec_engine_retire": (I, [P, I, P]),
+    "specdec_engine_fork": (I, [P, I, P, P, I, P]),
     "specdec_engine_prefill_chunk": (I, [P, I, C.c_int32, P, I, I]),
     "specdec_engine_share_prefix": (I, [P, I, C.c_int32, P, I, P, C.POINTER(C.c_int32)]),
     "specdec_engine_draft": (I, [P]),
@@ -379,6 +383,16 @@ class PagedKVCache:
 
     def share_prefix(self, new_request_id: int, source_request_id: int, shared_length: int):
         check(_lib.specdec_kv_share_prefix(self._h, new_request_id, source_request_id, shared_length, None))
+
+    def fork(self, source_request_ids, new_request_ids):
+        """new_request_ids[i] becomes a copy of source_request_ids[i]: whole
+        blocks shared, a block of its own for a partly used last one (tables
+        only; the K/V payload lives in the engine's pool)."""
+        src = np.ascontiguousarray(source_request_ids, dtype=np.int32).reshape(-1)
+        new = np.ascontiguousarray(new_request_ids, dtype=np.int32).reshape(-1)
+        if src.size != new.size:
+            raise ValueError("fork: one source for each new request")
+        check(_lib.specdec_kv_fork(self._h, _p(src), _p(new), src.size, None, 0, 0, 0, 0, None))
 
     def free_merged_blocks(self, request_id: int, num_blocks_to_free: int):
         check(_lib.specdec_kv_free_merged_blocks(self._h, request_id, num_blocks_to_free, None))
@@ -653,6 +667,16 @@ class Engine:
 
     def retire(self, seq: int, cache: "RadixKVCache | None" = None):
         check(_lib.specdec_engine_retire(self._h, seq, cache.handle if cache is not None else None))
+
+    def fork(self, seq: int, new_seqs, request_ids=None, cache: "RadixKVCache | None" = None):
+        """Slots new_seqs become copies of slot `seq` (whole K/V blocks
+        shared, the one in use copied; pending token and draft state)."""
+        new = np.ascontiguousarray(new_seqs, dtype=np.int32).reshape(-1)
+        ids = None if request_ids is None else np.ascontiguousarray(request_ids, dtype=np.int32).reshape(-1)
+        if ids is not None and ids.size != new.size:
+            raise ValueError("fork: one request id for each new slot")
+        check(_lib.specdec_engine_fork(self._h, seq, _p(new), None if ids is None else _p(ids), new.size,
+                                       cache.handle if cache is not None else None))
 
     def share_prefix(self, seq: int, request_id: int, prompt, cache: "RadixKVCache | None" = None) -> int:
         """Starts slot `seq` on a new request for chunked admission: shares

@@ -58,3 +58,34 @@ def test_errors_of_the_binding():
     with pytest.raises(S.SpecdecError):
         S.check(prompt(hd=32))
     assert isinstance(C.c_size_t(L.specdec_attention_prompt_workspace_bytes(0, 0, 0, 0, 0, 0)).value, int)
+
+
+def fork(**kw):
+    a = dict(tables=PTR, nblk=PTR, lens=PTR, ref=PTR, num_blocks=8, max_reqs=4, max_blocks=3, src=PTR, dst=PTR, n=2,
+             kv=PTR, layers=2, stride=8 * 2 * 2 * 16 * 64, Hkv=2, hd=64, status=PTR, ws=PTR, ws_bytes=1 << 30)
+    a.update(kw)
+    return L.specdec_kv_fork_pages(a["tables"], a["nblk"], a["lens"], a["ref"], a["num_blocks"], a["max_reqs"],
+                                   a["max_blocks"], a["src"], a["dst"], a["n"], a["kv"], a["layers"], a["stride"],
+                                   a["Hkv"], a["hd"], a["status"], a["ws"], a["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(tables=None), dict(nblk=None), dict(lens=None), dict(ref=None), dict(src=None), dict(dst=None),
+    dict(status=None), dict(ws=None), dict(kv=None), dict(num_blocks=0), dict(max_reqs=0), dict(max_blocks=0),
+    dict(n=-1), dict(n=5), dict(layers=-1), dict(layers=65536), dict(stride=8 * 2 * 2 * 16 * 64 - 8),
+    dict(stride=8 * 2 * 2 * 16 * 64 + 4), dict(Hkv=0), dict(hd=0), dict(hd=60), dict(kv=PTR + 8), dict(ws=PTR + 2),
+    dict(ws_bytes=100)])
+def test_fork_refuses(bad):
+    assert fork(**bad) == S.EINVAL
+    assert "kv_fork_pages" in S.last_error()
+
+
+def test_null_handles_are_refused():
+    assert L.specdec_kv_fork(None, None, None, 0, None, 0, 0, 0, 0, None) == S.EINVAL
+    assert L.specdec_engine_fork(None, 0, None, None, 0, None) == S.EINVAL
+
+
+@pytest.mark.parametrize("ws", [dict(ws=None), dict(ws_bytes=64), dict(ws=PTR + 4)])
+def test_workspaces_are_checked(ws):
+    assert prompt(**ws) == S.EINVAL and "workspace" in S.last_error()
+    assert shared(**ws) == S.EINVAL and "workspace" in S.last_error()
