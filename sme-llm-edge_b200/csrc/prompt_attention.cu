@@ -8,8 +8,12 @@
 //   a group's rows against its shared pages      (specdec_attention_shared_prefix)
 //   a sequence's rows against its own pages,
 //   with the mask of its new rows                (specdec_attention_shared_prefix)
-// An item is two adjacent tiles (one, where no second is left) of a segment and
-// a KV head, and one of the S pieces into which the segment's key range is cut.
+// An item is a KV head, one of the S pieces into which the segment's key range
+// is cut, and
+//   a pair   two adjacent tiles of the segment against the same keys (the
+//            second may be empty),
+//   a dual   one tile, its even and odd 128-key tiles apart: two chains of
+//            Q.K^T, softmax and P.V at a time (short segments).
 //
 // Mathematics, with x = score * log2(e) / sqrt(hd): in blocks of 128 keys
 //   m' = max(m, rowmax x),  P = 2^(x - m'),  l = l 2^(m - m') + rowsum P,
@@ -18,19 +22,23 @@
 // 2^8), so O is rarely rescaled.  P is rounded to fp16 (at most 2^-11 of a
 // weight): the tensor core multiplies fp16 by fp16.  m, l, O are fp32.
 //
-// One persistent CTA per SM, 12 warps:
+// One persistent CTA per SM, 12 warps (registers moved to the softmax warps):
 //   warps 0-3, 4-7  softmax of tile slot 0 / 1, one thread per query row
-//   warp 8          MMA issuer: S = Q K^T and O += P V, whichever is ready
+//   warp 8          MMA issuer
 //   warp 9          TMA loads: the tiles' queries, 128-key tiles of K and V
 //   warp 10         makes V safe: zeroes the slots behind the range's end in its
 //                   last page, and replaces infinities and NaN in slots that
 //                   not every row sees (0 * NaN would reach rows that do not
 //                   see them); the rows that see them add them at the end
 //   warp 11         scheduler: takes items, decodes them, passes them on
-// Two tiles share each K / V tile, so while the softmax of one works on its
-// scores the tensor cores work for the other.  P overlays S in tensor memory
-// (columns: S0 0, S1 128, O0 256, O1 256 + hd).  Single tiles use slots 0 and 1
-// in turn.
+// An operation is S = Q K^T, softmax, O += P V for one tile and 128 keys.  The
+// operations of a CTA use tile slots 0 and 1 in turn, through all its items (a
+// pair's tile t is in the slot of its operation 2j + t), and one thread issues
+// their MMAs as P.V of an operation, then Q.K^T of the next on that slot: the
+// tensor cores work for one slot while the softmax of the other runs.  (With an
+// issuer for each slot the two interleave MMA by MMA, both softmaxes run at the
+// same time and then neither: 6,900 clocks a pair of operations.)
+// P overlays S in tensor memory (columns: S0 0, S1 128, O0 256, O1 256 + hd).
 //
 // Splits of the key range write unnormalised fp32 O with (m, l) into the
 // workspace; rows_merge_kernel joins them in their order.
@@ -39,6 +47,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -52,11 +61,14 @@ constexpr int kRowsMaxSplits = 32;   // pieces of one key range
 constexpr int kRowsSorted = 128;     // up to so many segments are taken longest first
 constexpr int kRowsThreads = 384;
 constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
+// 256 softmax threads with 200 registers and 128 others with 104: the 384 * 168 of the launch
+constexpr int kRowsSoftRegs = 200, kRowsOtherRegs = 104;
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
 constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte rows, 128B swizzle
 constexpr int kRowsTmemCols = 512;
 
 enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2 };
+enum { kPair = 0, kDual = 1 };
 
 // Where the partial results of a sequence's rows lie (rows of the partial buffers).
 struct RowsMeta {
@@ -103,9 +115,10 @@ struct RowsItem {
     int trow, kvh;
     int tok0, i0;      // first token row; its index within the segment
     int ntok0, ntok1;  // tokens of the two tiles
-    int ctx, mode;
+    int ctx, mode, kind;
     int scan;          // slots >= scan are not seen by every row
     int prow;          // row of the partial buffers for tok0, -1: the result is final
+    int pnext;         // a dual's odd tiles: so many rows behind (0: it has one tile only)
     int bad;           // warp 10 found an infinity or NaN past `scan`
 };
 
@@ -153,17 +166,25 @@ __device__ __forceinline__ int rows_item_end(const RowsArgs& a, const RowsSeg& s
 __device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s, int p) {
     return (rows_item_end(a, s, p) - s.base + 127) / 128;
 }
+// A segment of one tile and several key tiles is worked on as duals.
+__device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s) {
+    return a.prows > 0 && s.n <= a.tpt && s.kt >= 2;
+}
 // Pieces of the key range, for pieces of about `fine` tiles where there are few
 // rows (memory-bound: partial results are small) or `coarse`.
 __device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, int fine, int coarse) {
     const int S = s.n * a.G <= 64 ? (s.kt + fine - 1) / fine : (2 * s.kt + coarse) / (2 * coarse);
-    return rows_clamp(S, 1, max(1, min(kRowsMaxSplits, s.kt)));
+    const int most = rows_dual(a, s) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
+    return rows_clamp(S, 1, max(1, most));
 }
-__device__ __forceinline__ bool rows_partial(const RowsSeg& s, int S) { return s.mode == kModeAll || S > 1 || s.base > 0; }
+// Results of the segment's rows to join: 0 where the item's own is final.
+__device__ __forceinline__ int rows_parts(const RowsArgs& a, const RowsSeg& s, int S) {
+    return rows_dual(a, s) ? 2 * S : (s.mode == kModeAll || S > 1 || s.base > 0 ? S : 0);
+}
 
 // False only for group bounds that overlap: what would not fit is left out.
-__device__ __forceinline__ bool rows_fit(const RowsArgs& a, const RowsSeg& s, int S, int prow) {
-    return (long long)prow + (long long)s.n * S <= a.prows;
+__device__ __forceinline__ bool rows_fit(const RowsArgs& a, const RowsSeg& s, int parts, int prow) {
+    return (long long)prow + (long long)s.n * parts <= a.prows;
 }
 
 struct RowsPlan {
@@ -270,11 +291,11 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             const RowsSeg s = rows_seg(a, nseg <= kRowsSorted ? p.order[i] : i, p.group_pages, p.seq_pages);
             const int S = rows_splits(a, s, fine, coarse);
             items += s.tiles * S;
-            if (rows_partial(s, S)) prows += s.n * S;
+            prows += s.n * rows_parts(a, s, S);
         }
         rows_scan2(p, items, prows, &item0, &prow0, &tot_items, &tot_prows);
         if (tot_prows <= a.prows || round >= 8) break;
-        // fewer pieces until their results fit; at last one piece a segment, which always does
+        // fewer pieces until their results fit; at last one a segment, which always does
         fine = round == 7 ? 1 << 26 : 2 * fine;
         coarse = round == 7 ? 1 << 26 : 2 * coarse;
     }
@@ -282,26 +303,26 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         const int id = nseg <= kRowsSorted ? p.order[i] : i;
         const RowsSeg s = rows_seg(a, id, p.group_pages, p.seq_pages);
         const int S = rows_splits(a, s, fine, coarse);
-        const bool part = rows_partial(s, S);
+        const int parts = rows_parts(a, s, S);
         p.pre[i] = item0;
         p.prow[i] = prow0;
         if (blockIdx.x == 0 && a.meta) {
             if (s.mode == kModeAll) {
                 for (int b = s.lo / a.R; b < (s.lo + s.n) / a.R; ++b) {
-                    a.meta[b].n_pre = rows_fit(a, s, S, prow0) ? S : 0;
+                    a.meta[b].n_pre = rows_fit(a, s, parts, prow0) ? parts : 0;
                     a.meta[b].base_pre = prow0 + (b * a.R - s.lo);
                     a.meta[b].stride_pre = s.n;
                 }
             } else {
                 RowsMeta& m = a.meta[s.trow];
                 if (s.base == 0) m.n_pre = 0;
-                m.n_own = part && rows_fit(a, s, S, prow0) ? S : 0;
+                m.n_own = rows_fit(a, s, parts, prow0) ? parts : 0;
                 m.base_own = prow0;
                 m.stride_own = s.n;
             }
         }
         item0 += s.tiles * S;
-        if (part) prow0 += s.n * S;
+        prow0 += s.n * parts;
     }
     if (tid == 0) {
         p.pre[nseg] = tot_items;
@@ -313,7 +334,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     __syncthreads();
 }
 
-__device__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
+__device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
     RowsItem it;
     it.n_kt = -1;
     it.bad = 0;
@@ -330,9 +351,11 @@ __device__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
     const int S = rows_splits(a, s, p.fine, p.coarse);
     const int local = r - p.pre[lo];
     const int tile = s.tiles - 1 - local / S, piece = local % S;  // the longest first
-    const bool part = rows_partial(s, S);
-    if (local < 0 || tile < 0 || (part && !rows_fit(a, s, S, p.prow[lo]))) {  // bounds that overlap: an empty item
+    const int parts = rows_parts(a, s, S);
+    if (local < 0 || tile < 0 || (parts && !rows_fit(a, s, parts, p.prow[lo]))) {  // bounds that overlap: an empty item
         it.n_kt = it.ntok0 = it.ntok1 = 0;
+        it.kind = kDual;
+        it.pnext = 0;
         it.prow = -1;
         return it;
     }
@@ -349,7 +372,9 @@ __device__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
     it.ctx = s.ctx;
     it.mode = s.mode;
     it.scan = s.mode == kModeCausal ? s.ctx + it.i0 + 1 : (s.mode == kModeMask ? s.ctx : it.end);
-    it.prow = part ? p.prow[lo] + piece * s.n + it.i0 : -1;
+    it.kind = rows_dual(a, s) || (it.ntok1 == 0 && it.n_kt <= 1) ? kDual : kPair;
+    it.pnext = rows_dual(a, s) ? s.n : 0;
+    it.prow = parts ? p.prow[lo] + piece * (parts / S) * s.n + it.i0 : -1;
     return it;
 }
 
@@ -359,7 +384,7 @@ struct RowsCfg {
     static constexpr int NH = HD / 64;                  // 64-column halves
     static constexpr int TILE = NH * 16384;             // 128 rows x HD fp16
     static constexpr int RING = HD == 128 ? 2 : 4;      // K tiles and V tiles in flight
-    static constexpr int NBAR = 4 * 2 + 5 * RING + 2 + 2 + 2 * kRowsItems;
+    static constexpr int NBAR = 7 * 2 + 5 * RING + 2 * kRowsItems;
     static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
                                    NBAR * 8 + 16;
 };
@@ -389,10 +414,206 @@ __device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, u
     w[3] = (uint32_t)(hi >> 32);
 }
 
-__device__ __forceinline__ float rows_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+// Two fp32 values in a register pair: one instruction works on both.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t d, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float rows_max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x on the special-function unit (2 ulp); the result is rounded to fp16 next.
+__device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
+    float x0, x1, y0, y1;
+    unpack2(x, x0, x1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(x0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
+    return pack2(y0, y1);
+}
+// The same on the FMA units for x <= 127 and not NaN: x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 rounds to it), 2^f on [-1/2, 1/2] by a
+// polynomial of degree 4 with the least largest relative error (2.6e-6, found
+// by an exchange of its extrema), 2^n added to the exponent.  Below 2^-126 the
+// result is some value under 2^-125, which fp16 rounds to 0.
+// The special-function unit gives 16 results a clock and SM, and a tile pair
+// needs 32,768 while its MMAs take 2,048 clocks: one result in kRowsExpEvery
+// comes from here.
+constexpr int kRowsExpEvery = 4;
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+    float x0, x1;
+    unpack2(x, x0, x1);
+    x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t big = pack2(12582912.f, 12582912.f);
+    const uint64_t t = add2(x, big);
+    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
+    uint64_t p = pack2(0.009570102207362652f, 0.009570102207362652f);
+    p = fma2(p, f, pack2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float t0, t1, p0, p1;
+    unpack2(t, t0, t1);
+    unpack2(p, p0, p1);
+    return pack2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)),
+                 __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
+}
+
+// The CTA's barriers, in shared memory.
+template <int RING>
+struct RowsBars {
+    uint64_t *q_full, *q_empty;  // [2] queries of a slot landed; their last Q.K^T is done
+    uint64_t* s_full;            // [2] scores landed
+    uint64_t *p_half, *p_full;   // [2] P of the first 64 keys written and O rescaled; all of P (4 warps)
+    uint64_t* pv_done;           // [2]
+    uint64_t* o_free;            // [2] O of an item was read (4 warps)
+    uint64_t *k_full, *k_empty;  // [RING]
+    uint64_t *v_raw, *v_full, *v_empty;  // [RING] V landed; is safe to multiply
+    uint64_t *i_full, *i_empty;  // [kRowsItems] empty: 8 softmax warps, the MMA issuer, loads, fix
+    __device__ explicit RowsBars(uint64_t* b)
+        : q_full(b), q_empty(b + 2), s_full(b + 4), p_half(b + 6), p_full(b + 8), pv_done(b + 10), o_free(b + 12),
+          k_full(b + 14), k_empty(k_full + RING), v_raw(k_empty + RING), v_full(v_raw + RING), v_empty(v_full + RING),
+          i_full(v_empty + RING), i_empty(i_full + kRowsItems) {}
+};
+
+// The MMA issuer.  Q.K^T of operation i + 2 follows P.V of operation i, on the
+// same slot (MMAs execute in the order of issue, so it may overwrite the P that
+// P.V reads).  The whole warp walks the operations and one lane issues: with
+// all values warp-uniform the operands are worked out in uniform registers,
+// where a thread of its own took 110 to 260 cycles for each MMA of 64.  Keys
+// behind the range's end cost Q.K^T columns that the softmax masks; P.V takes
+// the pages that exist.
+template <int HD>
+__device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uint32_t tmem, uint32_t sq, uint32_t sk,
+                                         uint32_t sv, uint64_t* bars, volatile int* abort_flag) {
+    using C = RowsCfg<HD>;
+    constexpr int NH = C::NH, RING = C::RING;
+    const RowsBars<RING> bar(bars);
+    const uint64_t qd0 = sw128_desc(sq), kd0 = sw128_desc(sk), vd0 = sw128_mn_desc(sv, kBlockHalf, 1024);
+    const uint32_t on = (threadIdx.x & 31) == 0;
+    bool ok = true;
+    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    auto wait = [&](uint64_t* b, int parity) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(s_addr(b), (uint32_t)parity & 1u));
+        return ok;
+    };
+    // the next Q.K^T: operation x of the n of item k, on the CTA's key tile `tile`
+    int k = -1, x = 0, n = 0, tile = 0, pair = 0, np_last = 0;
+    // what P.V of a slot's operation needs to know
+    int r_tile[2] = {0, 0}, r_pages[2] = {0, 0}, r_first[2] = {0, 0}, r_last_use[2] = {0, 0};
+    int begun[2] = {0, 0}, asked[2] = {0, 0}, done[2] = {0, 0};  // on a slot: items, Q.K^T issued, P.V issued
+    auto issue_qk = [&](auto slot) -> bool {
+        constexpr int s = decltype(slot)::value;
+        while (x == n) {  // to the next item with operations
+            ++k;
+            const int d = k % kRowsItems;
+            if (!wait(&bar.i_full[d], k / kRowsItems)) return false;
+            const volatile RowsItem& it = items[d];
+            const int n_kt = same(it.n_kt);
+            if (n_kt < 0) return false;
+            pair = same(it.kind) == kPair;
+            np_last = same(((it.end + 15) >> 4) - (it.slot0 >> 4)) - 8 * (n_kt - 1);
+            x = 0;
+            n = pair ? 2 * n_kt : n_kt;
+            __syncwarp();
+            if (on) mbar_arrive(s_addr(&bar.i_empty[d]));
+        }
+        const int at = tile % RING;
+        if (!wait(&bar.k_full[at], tile / RING)) return false;
+        if (x < 2 && !wait(&bar.q_full[s], begun[s])) return false;
+        tc_fence_after();
+        const uint64_t kd = kd0 + (uint64_t)(at * (C::TILE >> 4));
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+            tc_mma_f16_ss_if(on, tmem + s * 128,
+                             qd0 + (uint64_t)((s * C::TILE + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                             kd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), idesc_f16(128, 128),
+                             kk > 0 ? 1u : 0u);
+        tc_commit_if(on, s_addr(&bar.s_full[s]));
+        ++asked[s];
+        r_tile[s] = tile;
+        r_first[s] = x < 2;
+        r_pages[s] = x + (pair ? 2 : 1) >= n ? np_last : 8;
+        r_last_use[s] = !pair || (x & 1);
+        if (x < 2) ++begun[s];
+        if (x + 2 >= n) tc_commit_if(on, s_addr(&bar.q_empty[s]));
+        if (r_last_use[s]) {
+            tc_commit_if(on, s_addr(&bar.k_empty[at]));
+            ++tile;
+        }
+        ++x;
+        return true;
+    };
+    auto issue_pv = [&](auto slot) -> bool {
+        constexpr int s = decltype(slot)::value;
+        if (done[s] == asked[s]) return false;  // the last operation was issued
+        const int at = r_tile[s] % RING, np = r_pages[s];
+        const uint64_t vd = vd0 + (uint64_t)(at * (C::TILE >> 4));
+        auto step = [&](int i, uint32_t add) {  // the 16 keys of page i
+            tc_mma_f16_ts_if(on, tmem + 256 + s * HD, tmem + s * 128 + i * 8,
+                             vd + (uint64_t)((i * NH * kBlockHalf) >> 4), idesc_f16_bmn(128, HD), add);
+        };
+        if (!wait(&bar.v_full[at], r_tile[s] / RING)) return false;
+        // O of the slot's item before was read
+        if (r_first[s] && begun[s] > 1 && !wait(&bar.o_free[s], begun[s] - 2)) return false;
+        if (!wait(&bar.p_half[s], done[s])) return false;
+        tc_fence_after();
+        step(0, r_first[s] ? 0u : 1u);
+        if (np >= 4) {
+#pragma unroll
+            for (int i = 1; i < 4; ++i) step(i, 1u);
+        } else {
+            for (int i = 1; i < np; ++i) step(i, 1u);
+        }
+        if (!wait(&bar.p_full[s], done[s])) return false;
+        tc_fence_after();
+        if (np == 8) {
+#pragma unroll
+            for (int i = 4; i < 8; ++i) step(i, 1u);
+        } else {
+            for (int i = 4; i < np; ++i) step(i, 1u);
+        }
+        tc_commit_if(on, s_addr(&bar.pv_done[s]));
+        ++done[s];
+        if (r_last_use[s]) tc_commit_if(on, s_addr(&bar.v_empty[at]));
+        return true;
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    bool more = issue_qk(S0()) && issue_qk(S1());
+    for (;;) {
+        if (!issue_pv(S0())) break;
+        more = more && issue_qk(S0());
+        if (!issue_pv(S1())) break;
+        more = more && issue_qk(S1());
+    }
+    if (!ok && on) {
+        *abort_flag = 1;
+        record_timeout(a.status, 24);
+    }
+    // every MMA has finished with shared and tensor memory before the CTA leaves
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (asked[s]) (void)mbar_wait(s_addr(&bar.s_full[s]), (uint32_t)(asked[s] - 1) & 1u);
+        if (done[s]) (void)mbar_wait(s_addr(&bar.pv_done[s]), (uint32_t)(done[s] - 1) & 1u);
+    }
+    __syncwarp();
 }
 
 template <int HD>
@@ -412,19 +633,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     RowsItem* items = reinterpret_cast<RowsItem*>(&plan + 1);
     uint64_t* bars = reinterpret_cast<uint64_t*>(
         (reinterpret_cast<uintptr_t>(items + kRowsItems) + 7) & ~uintptr_t(7));
-    uint64_t* q_full = bars;               // [2] queries of a slot landed
-    uint64_t* q_empty = q_full + 2;        // [2] their last Q.K^T is done
-    uint64_t* s_full = q_empty + 2;        // [2] scores landed
-    uint64_t* p_full = s_full + 2;         // [2] P written (4 warps)
-    uint64_t* pv_done = p_full + 2;        // [2]
-    uint64_t* o_free = pv_done + 2;        // [2] O of an item was read (4 warps)
-    uint64_t* k_full = o_free + 2;         // [RING]
-    uint64_t* k_empty = k_full + RING;     // [RING]
-    uint64_t* v_raw = k_empty + RING;      // [RING] V landed
-    uint64_t* v_full = v_raw + RING;       // [RING] V is safe to multiply
-    uint64_t* v_empty = v_full + RING;     // [RING]
-    uint64_t* i_full = v_empty + RING;     // [kRowsItems]
-    uint64_t* i_empty = i_full + kRowsItems;  // [kRowsItems] 8 softmax warps, MMA, loads, fix
+    const RowsBars<C::RING> bar(bars);
+    uint64_t *q_full = bar.q_full, *q_empty = bar.q_empty, *s_full = bar.s_full, *p_half = bar.p_half,
+             *p_full = bar.p_full, *pv_done = bar.pv_done, *o_free = bar.o_free, *k_full = bar.k_full,
+             *k_empty = bar.k_empty, *v_raw = bar.v_raw, *v_full = bar.v_full, *v_empty = bar.v_empty,
+             *i_full = bar.i_full, *i_empty = bar.i_empty;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + kRowsItems);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -435,6 +648,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             mbar_init(s_addr(&q_full[i]), 1);
             mbar_init(s_addr(&q_empty[i]), 1);
             mbar_init(s_addr(&s_full[i]), 1);
+            mbar_init(s_addr(&p_half[i]), 4);
             mbar_init(s_addr(&p_full[i]), 4);
             mbar_init(s_addr(&pv_done[i]), 1);
             mbar_init(s_addr(&o_free[i]), 4);
@@ -489,274 +703,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         if (lane == 0) mbar_arrive(s_addr(&i_empty[k % kRowsItems]));
     };
 
-    if (warp == kRowsSchedWarp) {
-        // ------------------------------------------------------------ scheduler
-        for (int k = 0;; ++k) {
-            const int d = k % kRowsItems;
-            if (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1)) {
-                give_up(21);
-                break;
-            }
-            if (stopped()) break;
-            int more = 0;
-            if (lane == 0) {
-                const int idx = a.counter ? (int)atomicAdd(a.counter, 1u) : (int)(blockIdx.x + k * gridDim.x);
-                const RowsItem it = rows_item(a, plan, idx);
-                items[d] = it;
-                more = it.n_kt >= 0;
-                mbar_arrive(s_addr(&i_full[d]));
-            }
-            if (!__shfl_sync(0xffffffffu, more, 0)) break;
-        }
-    } else if (warp == kRowsLoadWarp) {
-        // ------------------------------------------------------------ loads
-        int kc = 0, qn[2] = {0, 0};  // K / V tiles loaded; query loads of a slot
-        bool ok = true;
-        RowsItem it;
-        for (int k = 0; ok && next_item(k, it); ++k) {
-            const bool pair = it.ntok1 > 0;
-            const int page0 = it.slot0 >> 4, pages = ((it.end + 15) >> 4) - page0;
-            const int32_t* tab = a.tables + (size_t)it.trow * a.max_blocks + page0;
-            auto page_at = [&](int i) {
-                int x = i < pages ? tab[i] : 0;
-                return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
-            };
-            int pg = it.n_kt > 0 ? page_at(lane) : 0, pg_next = 0;  // pages of four tiles, one a lane
-            for (int j = 0; j < it.n_kt && ok; ++j) {
-                if ((j & 3) == 0) {
-                    if (j) pg = pg_next;
-                    pg_next = page_at(8 * j + 32 + lane);
-                }
-                const int np = min(8, pages - 8 * j), slot = kc % RING, turn = kc / RING;
-                const int mine_k = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + (lane / NH) % 8);
-                const int mine_v = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + lane % 8);
-                if (turn && !(ok = wait(&k_empty[slot], turn - 1))) break;
-                if (lane == 0) mbar_expect_tx(s_addr(&k_full[slot]), (uint32_t)(np * NH * kBlockHalf));
-                __syncwarp();
-                if (lane < np * NH)
-                    tma_load_5d(s_addr(sK + slot * C::TILE + (lane % NH) * 16384 + (lane / NH) * kBlockHalf), &kmap, 0,
-                                it.kvh * 16, lane % NH, 0, mine_k, s_addr(&k_full[slot]));
-                if (j == 0) {  // the queries, behind the first keys
-                    for (int t = 0; t < (pair ? 2 : 1) && ok; ++t) {
-                        const int qs = pair ? t : k & 1;
-                        if (qn[qs] && !(ok = wait(&q_empty[qs], qn[qs] - 1))) break;
-                        ++qn[qs];
-                        const int ntok = t ? it.ntok1 : it.ntok0;
-                        const bool small = ntok <= a.tq_small;
-                        const uint32_t bytes = (uint32_t)((small ? a.tq_small : a.tpt) * a.G * 128);
-                        if (lane == 0) {
-                            mbar_expect_tx(s_addr(&q_full[qs]), bytes * NH);
-                            for (int h = 0; h < NH; ++h)
-                                tma_load_4d(s_addr(sQ + qs * C::TILE + h * 16384), small ? &qmap_small : &qmap, 0, h,
-                                            it.kvh * a.G, it.tok0 + t * a.tpt, s_addr(&q_full[qs]));
-                        }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                }
-                if (turn && !(ok = wait(&v_empty[slot], turn - 1))) break;
-                if (lane == 0) mbar_expect_tx(s_addr(&v_raw[slot]), (uint32_t)(np * NH * kBlockHalf));
-                __syncwarp();
-                if (lane < np)
-                    tma_load_5d(s_addr(sV + slot * C::TILE + lane * NH * kBlockHalf), &vmap, 0, it.kvh * 16, 0, 1,
-                                mine_v, s_addr(&v_raw[slot]));
-                ++kc;
-                if (stopped()) break;
-            }
-            if (!ok) give_up(22);
-            if (!ok || stopped()) break;
-            done_item(k);
-        }
-        if (stopped()) {  // the copies in flight land before the CTA leaves
-            for (int s = 0; s < 2; ++s)
-                if (qn[s]) (void)wait(&q_full[s], qn[s] - 1);
-            for (int c = max(0, kc - RING); c < kc; ++c) {
-                (void)wait(&k_full[c % RING], c / RING);
-                (void)wait(&v_raw[c % RING], c / RING);
-            }
-            if (!ok || kc == 0) (void)wait(&k_full[kc % RING], kc / RING);
-        }
-    } else if (warp == kRowsFixWarp) {
-        // ------------------------------------------------------------ V made safe
-        int vc = 0;
-        bool ok = true;
-        RowsItem it;
-        for (int k = 0; ok && next_item(k, it); ++k) {
-            for (int j = 0; j < it.n_kt; ++j, ++vc) {
-                const int slot = vc % RING, key0 = it.slot0 + 128 * j;
-                if (!(ok = wait(&v_raw[slot], vc / RING)) || stopped()) break;
-                unsigned char* v = sV + slot * C::TILE;
-                const int n = min(128, it.end - key0);           // slots that exist
-                const int np = (n + 15) >> 4;
-                const int lo = rows_clamp(it.scan - key0, 0, n);  // from here not every row sees them
-                bool touched = false;
-                if (n < 16 * np) {
-                    for (int i = n * NH * 8 + lane; i < 16 * np * NH * 8; i += 32) {
-                        const int row = i / (NH * 8), h = i / 8 % NH;
-                        *reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
-                                                  (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    touched = true;
-                }
-                bool found = false;
-                for (int i = lo * NH * 8 + lane; i < n * NH * 8; i += 32) {
-                    const int row = i / (NH * 8), h = i / 8 % NH;
-                    uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
-                                                         (i & 7) * 16);
-                    uint4 x = *at;
-                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
-                    bool mine = false;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
-                        if (l16) xs[e] &= 0xFFFF0000u;
-                        if (h16) xs[e] &= 0x0000FFFFu;
-                        mine |= l16 || h16;
-                    }
-                    if (mine) *at = x;
-                    found |= mine;
-                }
-                found = __any_sync(0xffffffffu, found);
-                if (found && lane == 0) items[k % kRowsItems].bad = 1;
-                if (touched || found) fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_addr(&v_full[slot]));
-            }
-            if (!ok) give_up(23);
-            if (!ok || stopped()) break;
-            done_item(k);
-        }
-    } else if (warp == kRowsMmaWarp) {
-        // ------------------------------------------------------------ MMA issuer
-        // Two cursors over the same operations: Q.K^T runs ahead of P.V.  An
-        // operation on a slot's S follows the P.V that read P there: both are
-        // issued here, and MMAs execute in the order of issue.
-        const uint32_t qb = s_addr(sQ), kb = s_addr(sK), vb = s_addr(sV);
-        RowsItem qi, pi;
-        int kq = 0, kp = 0, jq = 0, jp = 0, tq = 0, tp = 0;
-        int ck = 0, cv = 0;                        // K / V tiles used up
-        int nq[2] = {0, 0}, nv[2] = {0, 0};        // operations issued on a slot
-        int qloads[2] = {0, 0}, outs[2] = {0, 0};  // items begun on a slot, by cursor
-        bool have_q = false, have_p = false, end_q = false, end_p = false, failed = false;
-        uint64_t t_idle = 0;
-        while (!end_p) {
-            bool progressed = false;
-            if (!end_q && !have_q) {
-                if (__all_sync(0xffffffffu, mbar_test(s_addr(&i_full[kq % kRowsItems]), (kq / kRowsItems) & 1))) {
-                    qi = items[kq % kRowsItems];
-                    if (qi.n_kt < 0) end_q = true;
-                    else if (qi.n_kt == 0) ++kq;
-                    else {
-                        have_q = true;
-                        jq = tq = 0;
-                    }
-                    progressed = true;
-                }
-            }
-            if (have_q) {
-                const bool pair = qi.ntok1 > 0;
-                const int s = pair ? tq : kq & 1;
-                const bool ready = nq[s] == nv[s] && mbar_test(s_addr(&k_full[ck % RING]), (ck / RING) & 1) &&
-                                   (jq > 0 || mbar_test(s_addr(&q_full[s]), qloads[s] & 1));
-                if (__all_sync(0xffffffffu, ready)) {
-                    tc_fence_after();
-                    const bool last_t = !pair || tq == 1, last_j = jq == qi.n_kt - 1;
-                    if (lane == 0) {
-                        const int np = min(8, ((qi.end + 15) >> 4) - (qi.slot0 >> 4) - 8 * jq);
-                        const uint32_t idesc = idesc_f16(128, 16 * np);
-                        const uint32_t q0 = qb + s * C::TILE, k0 = kb + (ck % RING) * C::TILE;
-#pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk)
-                            tc_mma_f16_ss(tmem + s * 128, sw128_desc(q0 + (kk >> 2) * 16384 + (kk & 3) * 32),
-                                          sw128_desc(k0 + (kk >> 2) * 16384 + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
-                        tc_commit(s_addr(&s_full[s]));
-                        if (last_t) tc_commit(s_addr(&k_empty[ck % RING]));
-                        if (last_j) tc_commit(s_addr(&q_empty[s]));
-                    }
-                    __syncwarp();
-                    ++nq[s];
-                    if (last_j) ++qloads[s];
-                    if (last_t) {
-                        tq = 0;
-                        ++ck;
-                        if (++jq == qi.n_kt) {
-                            have_q = false;
-                            ++kq;
-                        }
-                    } else {
-                        tq = 1;
-                    }
-                    progressed = true;
-                }
-            }
-            if (!have_p) {
-                if (__all_sync(0xffffffffu, mbar_test(s_addr(&i_full[kp % kRowsItems]), (kp / kRowsItems) & 1))) {
-                    pi = items[kp % kRowsItems];
-                    if (pi.n_kt < 0) end_p = true;
-                    else if (pi.n_kt == 0) {
-                        if (kq > kp) {
-                            done_item(kp);
-                            ++kp;
-                        }
-                    } else {
-                        have_p = true;
-                        jp = tp = 0;
-                    }
-                    progressed = true;
-                }
-            }
-            if (have_p) {
-                const bool pair = pi.ntok1 > 0;
-                const int s = pair ? tp : kp & 1;
-                const bool ready = nq[s] > nv[s] && mbar_test(s_addr(&p_full[s]), nv[s] & 1) &&
-                                   mbar_test(s_addr(&v_full[cv % RING]), (cv / RING) & 1) &&
-                                   (jp > 0 || outs[s] == 0 || mbar_test(s_addr(&o_free[s]), (outs[s] - 1) & 1));
-                if (__all_sync(0xffffffffu, ready)) {
-                    tc_fence_after();
-                    const bool last_t = !pair || tp == 1;
-                    if (lane == 0) {
-                        const int np = min(8, ((pi.end + 15) >> 4) - (pi.slot0 >> 4) - 8 * jp);
-                        const uint32_t v0 = vb + (cv % RING) * C::TILE;
-                        for (int i = 0; i < np; ++i)
-                            tc_mma_f16_ts(tmem + 256 + s * HD, tmem + s * 128 + i * 8,
-                                          sw128_mn_desc(v0 + i * NH * kBlockHalf, kBlockHalf, 1024),
-                                          idesc_f16_bmn(128, HD), (jp > 0 || i > 0) ? 1u : 0u);
-                        tc_commit(s_addr(&pv_done[s]));
-                        if (last_t) tc_commit(s_addr(&v_empty[cv % RING]));
-                    }
-                    __syncwarp();
-                    if (jp == 0) ++outs[s];
-                    ++nv[s];
-                    if (last_t) {
-                        tp = 0;
-                        ++cv;
-                        if (++jp == pi.n_kt) {
-                            have_p = false;
-                            done_item(kp);
-                            ++kp;
-                        }
-                    } else {
-                        tp = 1;
-                    }
-                    progressed = true;
-                }
-            }
-            if (progressed) {
-                t_idle = 0;
-            } else {
-                const uint64_t now = gtimer();
-                if (t_idle == 0) t_idle = now;
-                failed = __any_sync(0xffffffffu, now - t_idle > 2000000000ull);
-                if (failed || stopped()) break;
-            }
-        }
-        if (failed) give_up(24);
-        // every MMA has finished with shared and tensor memory before the CTA leaves
-        for (int s = 0; s < 2; ++s) {
-            if (nq[s]) (void)wait(&s_full[s], nq[s] - 1);
-            if (nv[s]) (void)wait(&pv_done[s], nv[s] - 1);
-        }
-    } else {
+    if (warp < kRowsMmaWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowsSoftRegs));
         // ------------------------------------------------------------ softmax, one thread per query row
         const int ws = warp >> 2;                      // tile slot
         const int quarter = warp & 3;                  // TMEM lanes of this warp
@@ -764,16 +712,20 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const int ti = row / a.G, g = row % a.G;       // token of the tile, head of the group
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_s = t_lane + ws * 128, t_o = t_lane + 256 + ws * HD;
-        int c = 0;  // operations on this slot
+        int c = 0, op = 0;  // operations on this slot; of the items before, on both
         bool ok = true;
         RowsItem it;
         for (int k = 0; ok && next_item(k, it); ++k) {
-            const bool pair = it.ntok1 > 0;
-            if (!pair && (k & 1) != ws) {
+            // this slot's part: a pair's tile, a dual's even (0) or odd (1) key tiles
+            const int role = (op ^ ws) & 1;
+            op += it.n_kt * (it.kind == kPair ? 2 : 1);
+            if (it.kind == kDual && role && !it.pnext) {
                 done_item(k);
                 continue;
             }
-            const int t = pair ? ws : 0;               // tile of the item
+            const int t = it.kind == kPair ? role : 0;
+            const int j0 = it.kind == kPair ? 0 : role, jstep = it.kind == kPair ? 1 : 2;
+            const bool ops = it.n_kt > j0;
             const int ntok = t ? it.ntok1 : it.ntok0;
             const int i = it.i0 + t * a.tpt + ti;      // row of the segment
             const bool real = ti < ntok;
@@ -783,8 +735,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             const int every = it.mode == kModeCausal ? min(it.end, it.ctx + it.i0 + t * a.tpt + 1)
                                                      : (it.mode == kModeMask ? min(it.end, it.ctx) : it.end);
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < it.n_kt; ++j, ++c) {
-                if (!(ok = wait(&s_full[ws], c)) || stopped()) break;
+            for (int j = j0; j < it.n_kt; j += jstep, ++c) {
+                if (!(ok = wait(&s_full[ws], c))) break;
                 tc_fence_after();
                 if (here) {
                     uint32_t sv[128];
@@ -805,53 +757,72 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
 #pragma unroll
-                    for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[e]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-                    const bool grow = top > m + 8.0f;  // also where the row had seen nothing yet
+                    for (int e = 4; e < 128; e += 8)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            mx[q] = e + 4 + q < 128 ? rows_max3(mx[q], __uint_as_float(sv[e + q]), __uint_as_float(sv[(e + 4 + q) & 127]))
+                                                    : rows_max3(mx[q], mx[q], __uint_as_float(sv[e + q]));
+                    const float top = rows_max3(rows_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.scale_log2;
+                    const bool grow = real && !(top <= m + 8.0f);  // also where the row had seen nothing yet, and for NaN
                     const float m_new = grow ? top : m;
+                    // O holds the tiles before this one: rescale it once their P.V has landed
                     const float alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
-                    const float sub = m_new == -INFINITY ? 0.f : m_new;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (j != j0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                        if (!(ok = wait(&pv_done[ws], c - 1))) break;
+                        tc_fence_after();
+                        const float f = grow && m != -INFINITY ? alpha : 1.f;
+#pragma unroll 1
+                        for (int c0 = 0; c0 < HD; c0 += 16) {
+                            uint32_t ov[16];
+                            tc_ld_x16(t_o + c0, ov);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+                            tc_st_x16(t_o + c0, ov);
+                        }
+                    }
+                    // a NaN or infinite maximum makes every weight, and so the row, NaN
+                    const float sub = m_new == -INFINITY ? 0.f : (m_new < INFINITY ? m_new : __int_as_float(0x7FC00000));
+                    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), sub2 = pack2(-sub, -sub);
+                    uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         uint32_t pw[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            const float x0 = rows_exp2(fmaf(__uint_as_float(sv[64 * half + 2 * e]), a.scale_log2, -sub));
-                            const float x1 =
-                                rows_exp2(fmaf(__uint_as_float(sv[64 * half + 2 * e + 1]), a.scale_log2, -sub));
-                            sum[(2 * e) & 3] += x0;
-                            sum[(2 * e + 1) & 3] += x1;
-                            const __half2 h = __floats2half2_rn(x0, x1);
+                            const uint64_t x = fma2(pack2(__uint_as_float(sv[64 * half + 2 * e]),
+                                                          __uint_as_float(sv[64 * half + 2 * e + 1])),
+                                                    scale2, sub2);
+                            const uint64_t y = e % kRowsExpEvery == kRowsExpEvery - 1 ? exp2_poly2(x) : exp2_unit2(x);
+                            sum2[e & 1] = add2(sum2[e & 1], y);
+                            float y0, y1;
+                            unpack2(y, y0, y1);
+                            const __half2 h = __floats2half2_rn(y0, y1);
                             pw[e] = *reinterpret_cast<const uint32_t*>(&h);
                         }
                         tc_st_x32(t_s + 32 * half, pw);
-                    }
-                    // O holds the tiles before this one: rescale it once their P.V has landed
-                    if (j > 0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
-                        if (!(ok = wait(&pv_done[ws], c - 1))) break;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c0 = 0; c0 < HD; c0 += 32) {
-                            uint32_t ov[32];
-                            tc_ld_x32(t_o + c0, ov);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-                            tc_st_x32(t_o + c0, ov);
+                        if (half == 0) {
+                            tc_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(s_addr(&p_half[ws]));
                         }
                     }
-                    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    float s0, s1;
+                    unpack2(add2(sum2[0], sum2[1]), s0, s1);
+                    l = l * alpha + (s0 + s1);
                     m = m_new;
                     tc_wait_st();
+                } else if (lane == 0) {
+                    mbar_arrive(s_addr(&p_half[ws]));
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_addr(&p_full[ws]));
             }
             if (!ok) give_up(25);
-            if (!ok || stopped()) break;
-            if (it.n_kt > 0) {
+            if (!ok) break;
+            if (ops) {
                 if (!(ok = wait(&pv_done[ws], c - 1))) {
                     give_up(26);
                     break;
@@ -860,15 +831,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             }
             // ---- the item's rows: O / l, or O with (m, l) for the merge
             if (here) {
-                const bool bad = it.n_kt > 0 && *reinterpret_cast<volatile int*>(&items[k % kRowsItems].bad) != 0;
+                const bool bad = ops && *reinterpret_cast<volatile int*>(&items[k % kRowsItems].bad) != 0;
                 const int head = it.kvh * a.G + g, tok = it.tok0 + t * a.tpt + ti;
                 const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-                const size_t prow = (size_t)(it.prow + t * a.tpt + ti) * a.Hq + head;
+                const size_t prow = (size_t)(it.prow + (it.kind == kDual ? role * it.pnext : 0) + t * a.tpt + ti) * a.Hq + head;
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     uint32_t ov[32];
                     __syncwarp();  // rows that are not real skip the stores below
-                    if (it.n_kt > 0) {
+                    if (ops) {
                         tc_ld_x32(t_o + c0, ov);
                         tc_wait_ld();
                     } else {
@@ -915,13 +886,156 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 }
                 if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
             }
-            if (it.n_kt > 0) {
+            if (ops) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_addr(&o_free[ws]));
             }
             done_item(k);
         }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsOtherRegs));
+    if (warp == kRowsSchedWarp) {
+        // ------------------------------------------------------------ scheduler
+        for (int k = 0;; ++k) {
+            const int d = k % kRowsItems;
+            if (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1)) {
+                give_up(21);
+                break;
+            }
+            if (stopped()) break;
+            int more = 0;
+            if (lane == 0) {
+                const int idx = a.counter ? (int)atomicAdd(a.counter, 1u) : (int)(blockIdx.x + k * gridDim.x);
+                const RowsItem it = rows_item(a, plan, idx);
+                items[d] = it;
+                more = it.n_kt >= 0;
+                mbar_arrive(s_addr(&i_full[d]));
+            }
+            if (!__shfl_sync(0xffffffffu, more, 0)) break;
+        }
+    } else if (warp == kRowsLoadWarp) {
+        // ------------------------------------------------------------ loads
+        int kc = 0, qn[2] = {0, 0};  // K / V tiles loaded; query loads of a slot
+        int op = 0;                  // operations of the items before
+        bool ok = true;
+        RowsItem it;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+            const int page0 = it.slot0 >> 4, pages = ((it.end + 15) >> 4) - page0;
+            const int32_t* tab = a.tables + (size_t)it.trow * a.max_blocks + page0;
+            auto page_at = [&](int i) {
+                int x = i < pages ? tab[i] : 0;
+                return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
+            };
+            int pg = it.n_kt > 0 ? page_at(lane) : 0, pg_next = 0;  // pages of four tiles, one a lane
+            for (int j = 0; j < it.n_kt && ok; ++j) {
+                if ((j & 3) == 0) {
+                    if (j) pg = pg_next;
+                    pg_next = page_at(8 * j + 32 + lane);
+                }
+                const int np = min(8, pages - 8 * j), slot = kc % RING, turn = kc / RING;
+                const int mine_k = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + (lane / NH) % 8);
+                const int mine_v = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + lane % 8);
+                if (turn && !(ok = wait(&k_empty[slot], turn - 1))) break;
+                if (lane == 0) mbar_expect_tx(s_addr(&k_full[slot]), (uint32_t)(np * NH * kBlockHalf));
+                __syncwarp();
+                if (lane < np * NH)
+                    tma_load_5d(s_addr(sK + slot * C::TILE + (lane % NH) * 16384 + (lane / NH) * kBlockHalf), &kmap, 0,
+                                it.kvh * 16, lane % NH, 0, mine_k, s_addr(&k_full[slot]));
+                if (j == 0) {  // the queries, behind the first keys
+                    const int loads = it.kind == kPair || it.n_kt > 1 ? 2 : 1;
+                    for (int u = 0; u < loads && ok; ++u) {
+                        const int qs = (op + u) & 1, t = it.kind == kPair && it.ntok1 > 0 ? u : 0;
+                        if (qn[qs] && !(ok = wait(&q_empty[qs], qn[qs] - 1))) break;
+                        ++qn[qs];
+                        const int ntok = t ? it.ntok1 : it.ntok0;
+                        const bool small = ntok <= a.tq_small;
+                        const uint32_t bytes = (uint32_t)((small ? a.tq_small : a.tpt) * a.G * 128);
+                        if (lane == 0) {
+                            mbar_expect_tx(s_addr(&q_full[qs]), bytes * NH);
+                            for (int h = 0; h < NH; ++h)
+                                tma_load_4d(s_addr(sQ + qs * C::TILE + h * 16384), small ? &qmap_small : &qmap, 0, h,
+                                            it.kvh * a.G, it.tok0 + t * a.tpt, s_addr(&q_full[qs]));
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                }
+                if (turn && !(ok = wait(&v_empty[slot], turn - 1))) break;
+                if (lane == 0) mbar_expect_tx(s_addr(&v_raw[slot]), (uint32_t)(np * NH * kBlockHalf));
+                __syncwarp();
+                if (lane < np)
+                    tma_load_5d(s_addr(sV + slot * C::TILE + lane * NH * kBlockHalf), &vmap, 0, it.kvh * 16, 0, 1,
+                                mine_v, s_addr(&v_raw[slot]));
+                ++kc;
+            }
+            op += it.n_kt * (it.kind == kPair ? 2 : 1);
+            if (!ok) give_up(22);
+            if (!ok) break;
+            done_item(k);
+        }
+        if (stopped()) {  // the copies in flight land before the CTA leaves
+            for (int s = 0; s < 2; ++s)
+                if (qn[s]) (void)wait(&q_full[s], qn[s] - 1);
+            for (int c = max(0, kc - RING); c < kc; ++c) {
+                (void)wait(&k_full[c % RING], c / RING);
+                (void)wait(&v_raw[c % RING], c / RING);
+            }
+            if (!ok || kc == 0) (void)wait(&k_full[kc % RING], kc / RING);
+        }
+    } else if (warp == kRowsFixWarp) {
+        // ------------------------------------------------------------ V made safe
+        int vc = 0;
+        bool ok = true;
+        RowsItem it;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+            for (int j = 0; j < it.n_kt; ++j, ++vc) {
+                const int slot = vc % RING, key0 = it.slot0 + 128 * j;
+                if (!(ok = wait(&v_raw[slot], vc / RING))) break;
+                unsigned char* v = sV + slot * C::TILE;
+                const int n = min(128, it.end - key0);           // slots that exist
+                const int np = (n + 15) >> 4;
+                const int lo = rows_clamp(it.scan - key0, 0, n);  // from here not every row sees them
+                bool touched = false;
+                if (n < 16 * np) {
+                    for (int i = n * NH * 8 + lane; i < 16 * np * NH * 8; i += 32) {
+                        const int row = i / (NH * 8), h = i / 8 % NH;
+                        *reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
+                                                  (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    touched = true;
+                }
+                bool found = false;
+                for (int i = lo * NH * 8 + lane; i < n * NH * 8; i += 32) {
+                    const int row = i / (NH * 8), h = i / 8 % NH;
+                    uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
+                                                         (i & 7) * 16);
+                    uint4 x = *at;
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+                    bool mine = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
+                        if (l16) xs[e] &= 0xFFFF0000u;
+                        if (h16) xs[e] &= 0x0000FFFFu;
+                        mine |= l16 || h16;
+                    }
+                    if (mine) *at = x;
+                    found |= mine;
+                }
+                found = __any_sync(0xffffffffu, found);
+                if (found && lane == 0) items[k % kRowsItems].bad = 1;
+                if (touched || found) fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_addr(&v_full[slot]));
+            }
+            if (!ok) give_up(23);
+            if (!ok) break;
+            done_item(k);
+        }
+    } else if (warp == kRowsMmaWarp) {
+        rows_mma<HD>(a, items, tmem, s_addr(sQ), s_addr(sK), s_addr(sV), bars, abort_flag);
+    }
     }
     tc_fence_before();
     __syncthreads();
@@ -1005,14 +1119,16 @@ static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq
 }
 
 constexpr int kRowsSplitTokens = 4096;   // prompts of more rows fill the GPU without splits
-constexpr int kRowsPartialRows = 8192;   // room for pieces beyond the first, in token rows
+constexpr int kRowsPartialRows = 8192;   // room for their pieces, in token rows (two for each row at least)
+constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece of every range
 
 // Rows of the partial buffers.
 static size_t prompt_partial_rows(int T) {
     return T <= kRowsSplitTokens ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : 0;
 }
 static size_t shared_partial_rows(int T) {
-    return 2 * (size_t)T + std::min<size_t>(2 * (size_t)(kRowsMaxSplits - 1) * T, kRowsPartialRows);
+    // prefix and own range of every row, each of which may be a dual
+    return 4 * (size_t)T + std::min<size_t>(2 * (size_t)(kRowsMaxSplits - 2) * T, kRowsMoreRows);
 }
 static size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 static size_t rows_workspace(size_t prows, int B, int Hq, int HD) {
