@@ -22,7 +22,7 @@
 // 2^8), so O is rarely rescaled.  P is rounded to fp16 (at most 2^-11 of a
 // weight): the tensor core multiplies fp16 by fp16.  m, l, O are fp32.
 //
-// One persistent CTA per SM, 12 warps (registers moved to the softmax warps):
+// One persistent CTA per SM, 12 warps:
 //   warps 0-3, 4-7  softmax of tile slot 0 / 1, one thread per query row
 //   warp 8          MMA issuer
 //   warp 9          TMA loads: the tiles' queries, 128-key tiles of K and V
@@ -61,8 +61,6 @@ constexpr int kRowsMaxSplits = 32;   // pieces of one key range
 constexpr int kRowsSorted = 128;     // up to so many segments are taken longest first
 constexpr int kRowsThreads = 384;
 constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
-// 256 softmax threads with 200 registers and 128 others with 104: the 384 * 168 of the launch
-constexpr int kRowsSoftRegs = 200, kRowsOtherRegs = 104;
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
 constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte rows, 128B swizzle
 constexpr int kRowsTmemCols = 512;
@@ -338,7 +336,7 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     RowsItem it;
     it.n_kt = -1;
     it.bad = 0;
-    if (idx >= p.items) return it;
+    if (idx < 0 || idx >= p.items) return it;
     it.kvh = idx % a.Hkv;
     const int r = idx / a.Hkv;
     int lo = 0, hi = p.nseg;  // last position with pre <= r
@@ -384,16 +382,57 @@ struct RowsCfg {
     static constexpr int NH = HD / 64;                  // 64-column halves
     static constexpr int TILE = NH * 16384;             // 128 rows x HD fp16
     static constexpr int RING = HD == 128 ? 2 : 4;      // K tiles and V tiles in flight
-    static constexpr int NBAR = 7 * 2 + 5 * RING + 2 * kRowsItems;
+    static constexpr int NBAR = 5 * 2 + 5 * RING + 2 * kRowsItems;
     static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
                                    NBAR * 8 + 16;
 };
 
-// Four words: bit c = slot key0 + c of a row is seen.
-__device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, uint64_t bits, uint32_t w[4]) {
+// The rows of an item without keys.
+template <int HD>
+__device__ void rows_zero(const RowsArgs& a, const RowsItem& it, int lane) {
+    const int rows = (it.ntok0 + it.ntok1) * a.G;
+    for (int r = lane; r < rows; r += 32) {
+        const int t = r / a.G, head = it.kvh * a.G + r % a.G;
+        if (it.prow < 0) {
+            uint4* dst = reinterpret_cast<uint4*>(a.out + (size_t)(it.tok0 + t) * a.ldo + (size_t)head * HD);
+            for (int e = 0; e < HD / 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
+        } else {  // a piece of no weight: the merge reads no O of it
+            a.pml[(size_t)(it.prow + t) * a.Hq + head] = make_float2(-INFINITY, 0.f);
+            if (it.pnext) a.pml[(size_t)(it.prow + it.pnext + t) * a.Hq + head] = make_float2(-INFINITY, 0.f);
+        }
+    }
+}
+
+// Adds the infinities and NaN of V that warp 10 took out to a row that sees
+// them; `at` is the row's token (final) or its place in the partial buffers.
+template <int HD>
+__device__ void rows_add_bad(const RowsArgs& a, const RowsItem& it, int i, uint64_t bits, int head, size_t at) {
+    const int hi = min(it.end, it.slot0 + 128 * it.n_kt);
+#pragma unroll 1
+    for (int s = max(it.scan, it.slot0); s < hi; ++s) {
+        const bool seen = it.mode == kModeCausal ? s <= it.ctx + i : (s - it.ctx < 64 && ((bits >> (s - it.ctx)) & 1ull));
+        if (!seen) continue;
+        const int x = a.tables[(size_t)it.trow * a.max_blocks + (s >> 4)];
+        const int page = x < 0 || x >= a.num_blocks ? 0 : x;
+        const __half* v = a.kv + ((((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 + (s & 15)) * HD;
+#pragma unroll 1
+        for (int e = 0; e < HD; ++e) {
+            const float y = __half2float(v[e]);
+            if (isfinite(y)) continue;
+            if (it.prow < 0) {
+                __half* o = a.out + at * a.ldo + (size_t)head * HD + e;
+                *o = __float2half_rn(__half2float(*o) + y);
+            } else {
+                a.po[at * HD + e] += y;
+            }
+        }
+    }
+}
+
+// Bit c = slot key0 + c of a row is seen.
+__device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, uint64_t bits, uint64_t& lo, uint64_t& hi) {
     auto below = [](int k) -> uint64_t { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); };
     const int n = it.end - key0;
-    uint64_t lo, hi;
     if (it.mode == kModeMask) {
         const int d = it.ctx - key0;  // column of the first new row
         lo = below(d);
@@ -408,10 +447,6 @@ __device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, u
         lo = below(k);
         hi = below(k - 64);
     }
-    w[0] = (uint32_t)lo;
-    w[1] = (uint32_t)(lo >> 32);
-    w[2] = (uint32_t)hi;
-    w[3] = (uint32_t)(hi >> 32);
 }
 
 // Two fp32 values in a register pair: one instruction works on both.
@@ -480,25 +515,24 @@ template <int RING>
 struct RowsBars {
     uint64_t *q_full, *q_empty;  // [2] queries of a slot landed; their last Q.K^T is done
     uint64_t* s_full;            // [2] scores landed
-    uint64_t *p_half, *p_full;   // [2] P of the first 64 keys written and O rescaled; all of P (4 warps)
-    uint64_t* pv_done;           // [2]
-    uint64_t* o_free;            // [2] O of an item was read (4 warps)
+    uint64_t* p_full;            // [2] P written, O rescaled, V safe, O of the item before read (4 warps)
+    uint64_t* o_full;            // [2] the item's last P.V is done
     uint64_t *k_full, *k_empty;  // [RING]
     uint64_t *v_raw, *v_full, *v_empty;  // [RING] V landed; is safe to multiply
     uint64_t *i_full, *i_empty;  // [kRowsItems] empty: 8 softmax warps, the MMA issuer, loads, fix
     __device__ explicit RowsBars(uint64_t* b)
-        : q_full(b), q_empty(b + 2), s_full(b + 4), p_half(b + 6), p_full(b + 8), pv_done(b + 10), o_free(b + 12),
-          k_full(b + 14), k_empty(k_full + RING), v_raw(k_empty + RING), v_full(v_raw + RING), v_empty(v_full + RING),
+        : q_full(b), q_empty(b + 2), s_full(b + 4), p_full(b + 6), o_full(b + 8), k_full(b + 10), k_empty(k_full + RING), v_raw(k_empty + RING), v_full(v_raw + RING), v_empty(v_full + RING),
           i_full(v_empty + RING), i_empty(i_full + kRowsItems) {}
 };
 
-// The MMA issuer.  Q.K^T of operation i + 2 follows P.V of operation i, on the
-// same slot (MMAs execute in the order of issue, so it may overwrite the P that
-// P.V reads).  The whole warp walks the operations and one lane issues: with
-// all values warp-uniform the operands are worked out in uniform registers,
-// where a thread of its own took 110 to 260 cycles for each MMA of 64.  Keys
-// behind the range's end cost Q.K^T columns that the softmax masks; P.V takes
-// the pages that exist.
+// The MMA issuer.  P.V of operation i and Q.K^T of operation i + 2 on the same
+// slot go out together (MMAs execute in the order of issue, so the second may
+// overwrite the P that the first reads), and one commit tells of all MMAs
+// before it: scores that have landed mean that the slot's P.V before them has,
+// too.  The whole warp walks the operations, so that the operands are
+// warp-uniform, and one lane issues.  The softmax warps answer for V and O; the
+// issuer waits for P alone.  Keys behind the range's end cost Q.K^T columns that
+// the softmax masks; P.V takes the pages that exist.
 template <int HD>
 __device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uint32_t tmem, uint32_t sq, uint32_t sk,
                                          uint32_t sv, uint64_t* bars, volatile int* abort_flag) {
@@ -506,113 +540,134 @@ __device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uin
     constexpr int NH = C::NH, RING = C::RING;
     const RowsBars<RING> bar(bars);
     const uint64_t qd0 = sw128_desc(sq), kd0 = sw128_desc(sk), vd0 = sw128_mn_desc(sv, kBlockHalf, 1024);
-    const uint32_t on = (threadIdx.x & 31) == 0;
-    bool ok = true;
+    const bool on = (threadIdx.x & 31) == 0;
+    bool ok = true, more = true;  // no wait ran out; items may be left
     auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    auto ready = [&](uint64_t* b, int parity) { return mbar_test_warp(s_addr(b), (uint32_t)parity & 1u); };
     auto wait = [&](uint64_t* b, int parity) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(s_addr(b), (uint32_t)parity & 1u));
+        ok = ok && mbar_spin_warp(s_addr(b), (uint32_t)parity & 1u);
         return ok;
     };
     // the next Q.K^T: operation x of the n of item k, on the CTA's key tile `tile`
     int k = -1, x = 0, n = 0, tile = 0, pair = 0, np_last = 0;
-    // what P.V of a slot's operation needs to know
-    int r_tile[2] = {0, 0}, r_pages[2] = {0, 0}, r_first[2] = {0, 0}, r_last_use[2] = {0, 0};
-    int begun[2] = {0, 0}, asked[2] = {0, 0}, done[2] = {0, 0};  // on a slot: items, Q.K^T issued, P.V issued
-    auto issue_qk = [&](auto slot) -> bool {
+    // what P.V of an operation needs to know: ring place | pages | first, last of the item on its slot | last use of V
+    int rec = -1, rec_next = -1;    // of the operation in turn and of the one after; -1: none
+    int begun[2] = {0, 0}, ended[2] = {0, 0};  // items whose Q.K^T began on a slot, whose P.V ended on it
+    // Is the operation of the next Q.K^T known, and has its data landed?
+    // block: waits for it.  False without block: not yet, or none is left.
+    auto next_ready = [&](auto slot, bool block) -> bool {
         constexpr int s = decltype(slot)::value;
-        while (x == n) {  // to the next item with operations
-            ++k;
-            const int d = k % kRowsItems;
-            if (!wait(&bar.i_full[d], k / kRowsItems)) return false;
+        while (x == n) {  // to the next item
+            const int d = (k + 1) % kRowsItems, turn = (k + 1) / kRowsItems;
+            if (block ? !wait(&bar.i_full[d], turn) : !ready(&bar.i_full[d], turn)) return false;
             const volatile RowsItem& it = items[d];
             const int n_kt = same(it.n_kt);
-            if (n_kt < 0) return false;
+            if (n_kt < 0) {
+                more = false;
+                return false;
+            }
             pair = same(it.kind) == kPair;
             np_last = same(((it.end + 15) >> 4) - (it.slot0 >> 4)) - 8 * (n_kt - 1);
+            ++k;
             x = 0;
             n = pair ? 2 * n_kt : n_kt;
             __syncwarp();
             if (on) mbar_arrive(s_addr(&bar.i_empty[d]));
         }
-        const int at = tile % RING;
-        if (!wait(&bar.k_full[at], tile / RING)) return false;
-        if (x < 2 && !wait(&bar.q_full[s], begun[s])) return false;
-        tc_fence_after();
-        const uint64_t kd = kd0 + (uint64_t)(at * (C::TILE >> 4));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_f16_ss_if(on, tmem + s * 128,
-                             qd0 + (uint64_t)((s * C::TILE + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
-                             kd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), idesc_f16(128, 128),
-                             kk > 0 ? 1u : 0u);
-        tc_commit_if(on, s_addr(&bar.s_full[s]));
-        ++asked[s];
-        r_tile[s] = tile;
-        r_first[s] = x < 2;
-        r_pages[s] = x + (pair ? 2 : 1) >= n ? np_last : 8;
-        r_last_use[s] = !pair || (x & 1);
-        if (x < 2) ++begun[s];
-        if (x + 2 >= n) tc_commit_if(on, s_addr(&bar.q_empty[s]));
-        if (r_last_use[s]) {
-            tc_commit_if(on, s_addr(&bar.k_empty[at]));
-            ++tile;
-        }
-        ++x;
-        return true;
+        if (block) return wait(&bar.k_full[tile % RING], tile / RING) && (x >= 2 || wait(&bar.q_full[s], begun[s]));
+        return ready(&bar.k_full[tile % RING], tile / RING) && (x >= 2 || ready(&bar.q_full[s], begun[s]));
     };
-    auto issue_pv = [&](auto slot) -> bool {
+    auto issue_qk = [&](auto slot) -> int {
         constexpr int s = decltype(slot)::value;
-        if (done[s] == asked[s]) return false;  // the last operation was issued
-        const int at = r_tile[s] % RING, np = r_pages[s];
-        const uint64_t vd = vd0 + (uint64_t)(at * (C::TILE >> 4));
-        auto step = [&](int i, uint32_t add) {  // the 16 keys of page i
-            tc_mma_f16_ts_if(on, tmem + 256 + s * HD, tmem + s * 128 + i * 8,
-                             vd + (uint64_t)((i * NH * kBlockHalf) >> 4), idesc_f16_bmn(128, HD), add);
-        };
-        if (!wait(&bar.v_full[at], r_tile[s] / RING)) return false;
-        // O of the slot's item before was read
-        if (r_first[s] && begun[s] > 1 && !wait(&bar.o_free[s], begun[s] - 2)) return false;
-        if (!wait(&bar.p_half[s], done[s])) return false;
-        tc_fence_after();
-        step(0, r_first[s] ? 0u : 1u);
-        if (np >= 4) {
+        const int at = tile % RING;
+        const uint64_t qd = qd0 + (uint64_t)(s * (C::TILE >> 4)), kd = kd0 + (uint64_t)(at * (C::TILE >> 4));
+        const bool first = x < 2, last = x + 2 >= n, last_use = !pair || (x & 1);
+        const int np = x + (pair ? 2 : 1) >= n ? np_last : 8;
+        const uint32_t d = tmem + s * 128, sb = s_addr(&bar.s_full[s]), qb = s_addr(&bar.q_empty[s]),
+                       kb = s_addr(&bar.k_empty[at]);
+        if (on) {
 #pragma unroll
-            for (int i = 1; i < 4; ++i) step(i, 1u);
-        } else {
-            for (int i = 1; i < np; ++i) step(i, 1u);
+            for (int kk = 0; kk < HD / 16; ++kk)
+                tc_mma_f16_ss(d, qd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                              kd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), idesc_f16(128, 128),
+                              kk > 0 ? 1u : 0u);
+            tc_commit(sb);
+            if (last) tc_commit(qb);
+            if (last_use) tc_commit(kb);
         }
-        if (!wait(&bar.p_full[s], done[s])) return false;
-        tc_fence_after();
-        if (np == 8) {
-#pragma unroll
-            for (int i = 4; i < 8; ++i) step(i, 1u);
-        } else {
-            for (int i = 4; i < np; ++i) step(i, 1u);
-        }
-        tc_commit_if(on, s_addr(&bar.pv_done[s]));
-        ++done[s];
-        if (r_last_use[s]) tc_commit_if(on, s_addr(&bar.v_empty[at]));
-        return true;
+        __syncwarp();
+        begun[s] += first;
+        tile += last_use;
+        ++x;
+        return at | np << 4 | (int)first << 8 | (int)last << 9 | (int)last_use << 10;
     };
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
-    bool more = issue_qk(S0()) && issue_qk(S1());
-    for (;;) {
-        if (!issue_pv(S0())) break;
-        more = more && issue_qk(S0());
-        if (!issue_pv(S1())) break;
-        more = more && issue_qk(S1());
+    if (next_ready(S0(), true)) {
+        tc_fence_after();
+        rec = issue_qk(S0());
+        if (next_ready(S1(), true)) {
+            tc_fence_after();
+            rec_next = issue_qk(S1());
+        }
+    }
+    int asked = (rec >= 0) + (rec_next >= 0);
+    // P.V of the operation in turn and Q.K^T of the slot's next
+    auto turn = [&](auto slot, int phase) {
+        constexpr int s = decltype(slot)::value;
+        const bool next = more && next_ready(slot, false);
+        if (!wait(&bar.p_full[s], phase)) return;
+        tc_fence_after();
+        const int at = rec & 15, np = (rec >> 4) & 15;
+        const bool first = (rec >> 8) & 1, last = (rec >> 9) & 1, last_use = (rec >> 10) & 1;
+        const uint64_t vd = vd0 + (uint64_t)(at * (C::TILE >> 4));
+        const uint32_t o = tmem + 256 + s * HD, pa = tmem + s * 128, ob = s_addr(&bar.o_full[s]),
+                       vb = s_addr(&bar.v_empty[at]);
+        auto step = [&](int i, uint32_t add) {  // the 16 keys of page i
+            tc_mma_f16_ts(o, pa + i * 8, vd + (uint64_t)((i * NH * kBlockHalf) >> 4), idesc_f16_bmn(128, HD), add);
+        };
+        if (on) {
+            if (first) step(0, 0u);
+            else step(0, 1u);
+            if (np == 8) {
+#pragma unroll
+                for (int i = 1; i < 8; ++i) step(i, 1u);
+            } else {
+#pragma unroll 1
+                for (int i = 1; i < np; ++i) step(i, 1u);
+            }
+            if (last) tc_commit(ob);
+        }
+        __syncwarp();
+        ended[s] += last;
+        int made = -1;
+        if (next) made = issue_qk(slot);
+        if (last_use && on) tc_commit(vb);
+        __syncwarp();
+        if (!next && more && next_ready(slot, true)) {
+            tc_fence_after();
+            made = issue_qk(slot);
+        }
+        asked += made >= 0;
+        rec = rec_next;
+        rec_next = made;
+    };
+#pragma unroll 1
+    for (int phase = 0; rec >= 0; ++phase) {
+        turn(S0(), phase);
+        if (!ok || rec < 0) break;
+        turn(S1(), phase);
+        if (!ok) break;
     }
     if (!ok && on) {
         *abort_flag = 1;
         record_timeout(a.status, 24);
     }
     // every MMA has finished with shared and tensor memory before the CTA leaves
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        if (asked[s]) (void)mbar_wait(s_addr(&bar.s_full[s]), (uint32_t)(asked[s] - 1) & 1u);
-        if (done[s]) (void)mbar_wait(s_addr(&bar.pv_done[s]), (uint32_t)(done[s] - 1) & 1u);
-    }
+    if (asked > 0) (void)mbar_spin_warp(s_addr(&bar.s_full[0]), (uint32_t)((asked + 1) / 2 - 1) & 1u);
+    if (asked > 1) (void)mbar_spin_warp(s_addr(&bar.s_full[1]), (uint32_t)(asked / 2 - 1) & 1u);
+    if (ended[0]) (void)mbar_spin_warp(s_addr(&bar.o_full[0]), (uint32_t)(ended[0] - 1) & 1u);
+    if (ended[1]) (void)mbar_spin_warp(s_addr(&bar.o_full[1]), (uint32_t)(ended[1] - 1) & 1u);
     __syncwarp();
 }
 
@@ -634,8 +689,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(
         (reinterpret_cast<uintptr_t>(items + kRowsItems) + 7) & ~uintptr_t(7));
     const RowsBars<C::RING> bar(bars);
-    uint64_t *q_full = bar.q_full, *q_empty = bar.q_empty, *s_full = bar.s_full, *p_half = bar.p_half,
-             *p_full = bar.p_full, *pv_done = bar.pv_done, *o_free = bar.o_free, *k_full = bar.k_full,
+    uint64_t *q_full = bar.q_full, *q_empty = bar.q_empty, *s_full = bar.s_full, *p_full = bar.p_full,
+             *o_full = bar.o_full, *k_full = bar.k_full,
              *k_empty = bar.k_empty, *v_raw = bar.v_raw, *v_full = bar.v_full, *v_empty = bar.v_empty,
              *i_full = bar.i_full, *i_empty = bar.i_empty;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + kRowsItems);
@@ -648,10 +703,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             mbar_init(s_addr(&q_full[i]), 1);
             mbar_init(s_addr(&q_empty[i]), 1);
             mbar_init(s_addr(&s_full[i]), 1);
-            mbar_init(s_addr(&p_half[i]), 4);
             mbar_init(s_addr(&p_full[i]), 4);
-            mbar_init(s_addr(&pv_done[i]), 1);
-            mbar_init(s_addr(&o_free[i]), 4);
+            mbar_init(s_addr(&o_full[i]), 1);
         }
         for (int i = 0; i < RING; ++i) {
             mbar_init(s_addr(&k_full[i]), 1);
@@ -685,7 +738,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     };
     auto stopped = [&]() { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };
     auto wait = [&](uint64_t* bar, int parity) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(s_addr(bar), (uint32_t)parity & 1u)) != 0;
+        return mbar_test_warp(s_addr(bar), (uint32_t)parity & 1u) ||
+               __all_sync(0xffffffffu, mbar_wait(s_addr(bar), (uint32_t)parity & 1u)) != 0;
     };
     // the k-th item of this CTA; false: none is left, or a wait ran out
     auto next_item = [&](int k, RowsItem& it) -> bool {
@@ -704,7 +758,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     };
 
     if (warp < kRowsMmaWarp) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowsSoftRegs));
         // ------------------------------------------------------------ softmax, one thread per query row
         const int ws = warp >> 2;                      // tile slot
         const int quarter = warp & 3;                  // TMEM lanes of this warp
@@ -712,13 +765,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const int ti = row / a.G, g = row % a.G;       // token of the tile, head of the group
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_s = t_lane + ws * 128, t_o = t_lane + 256 + ws * HD;
-        int c = 0, op = 0;  // operations on this slot; of the items before, on both
+        int c = 0, ended = 0;   // operations and items done on this slot
+        int op = 0, tile = 0;   // operations (on both slots) and key tiles of the items before
         bool ok = true;
         RowsItem it;
         for (int k = 0; ok && next_item(k, it); ++k) {
             // this slot's part: a pair's tile, a dual's even (0) or odd (1) key tiles
-            const int role = (op ^ ws) & 1;
+            const int role = (op ^ ws) & 1, tile0 = tile;
             op += it.n_kt * (it.kind == kPair ? 2 : 1);
+            tile += it.n_kt;
             if (it.kind == kDual && role && !it.pnext) {
                 done_item(k);
                 continue;
@@ -739,37 +794,48 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 if (!(ok = wait(&s_full[ws], c))) break;
                 tc_fence_after();
                 if (here) {
-                    uint32_t sv[128];
-                    tc_ld_x32(t_s, sv);
-                    tc_ld_x32(t_s + 32, sv + 32);
-                    tc_ld_x32(t_s + 64, sv + 64);
-                    tc_ld_x32(t_s + 96, sv + 96);
-                    tc_wait_ld();
+                    // two passes over the scores, 32 columns at a time with the next 32 on
+                    // their way: all 128 in registers at once made code that the
+                    // instruction cache does not hold
                     const int key0 = it.slot0 + 128 * j;
-                    if (key0 + 128 > every) {
-                        uint32_t w[4];
-                        rows_seen(it, key0, i, bits, w);
+                    const bool masked = key0 + 128 > every;
+                    uint64_t seen_lo = ~0ull, seen_hi = ~0ull;
+                    if (masked) rows_seen(it, key0, i, bits, seen_lo, seen_hi);
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    uint32_t va[32], vb[32];
+                    auto largest = [&](uint32_t(&v)[32], int q) {
+                        if (masked) {
+                            const uint32_t w = (uint32_t)((q & 2 ? seen_hi : seen_lo) >> (32 * (q & 1)));
 #pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            if (!((w[e >> 5] >> (e & 31)) & 1u)) sv[e] = 0xFF800000u;  // -inf
+                            for (int e = 0; e < 32; ++e)
+                                if (!((w >> e) & 1u)) v[e] = 0xFF800000u;  // -inf
+                            tc_st_x32(t_s + 32 * q, v);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            mx[0] = rows_max3(mx[0], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                            mx[1] = rows_max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                        }
+                    };
+                    tc_ld_x32(t_s, va);
+                    tc_wait_ld();
+#pragma unroll 1
+                    for (int q = 0; q < 4; q += 2) {
+                        tc_ld_x32(t_s + 32 * (q + 1), vb);
+                        largest(va, q);
+                        tc_wait_ld();
+                        if (q == 0) tc_ld_x32(t_s + 64, va);
+                        largest(vb, q + 1);
+                        tc_wait_ld();
                     }
-                    float mx[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
-#pragma unroll
-                    for (int e = 4; e < 128; e += 8)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            mx[q] = e + 4 + q < 128 ? rows_max3(mx[q], __uint_as_float(sv[e + q]), __uint_as_float(sv[(e + 4 + q) & 127]))
-                                                    : rows_max3(mx[q], mx[q], __uint_as_float(sv[e + q]));
-                    const float top = rows_max3(rows_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.scale_log2;
+                    if (masked) tc_wait_st();
+                    tc_ld_x32(t_s, va);
+                    const float top = rows_max3(mx[0], mx[1], mx[1]) * a.scale_log2;
                     const bool grow = real && !(top <= m + 8.0f);  // also where the row had seen nothing yet, and for NaN
                     const float m_new = grow ? top : m;
-                    // O holds the tiles before this one: rescale it once their P.V has landed
+                    // O holds the tiles before this one (their P.V came before these scores)
                     const float alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
                     if (j != j0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
-                        if (!(ok = wait(&pv_done[ws], c - 1))) break;
-                        tc_fence_after();
                         const float f = grow && m != -INFINITY ? alpha : 1.f;
 #pragma unroll 1
                         for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -785,14 +851,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     const float sub = m_new == -INFINITY ? 0.f : (m_new < INFINITY ? m_new : __int_as_float(0x7FC00000));
                     const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), sub2 = pack2(-sub, -sub);
                     uint64_t sum2[2] = {0ull, 0ull};
+                    auto weights = [&](uint32_t(&v)[32], int q) {
+                        uint32_t pw[16];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t pw[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const uint64_t x = fma2(pack2(__uint_as_float(sv[64 * half + 2 * e]),
-                                                          __uint_as_float(sv[64 * half + 2 * e + 1])),
-                                                    scale2, sub2);
+                        for (int e = 0; e < 16; ++e) {
+                            const uint64_t x =
+                                fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, sub2);
                             const uint64_t y = e % kRowsExpEvery == kRowsExpEvery - 1 ? exp2_poly2(x) : exp2_unit2(x);
                             sum2[e & 1] = add2(sum2[e & 1], y);
                             float y0, y1;
@@ -800,21 +864,27 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                             const __half2 h = __floats2half2_rn(y0, y1);
                             pw[e] = *reinterpret_cast<const uint32_t*>(&h);
                         }
-                        tc_st_x32(t_s + 32 * half, pw);
-                        if (half == 0) {
-                            tc_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(s_addr(&p_half[ws]));
-                        }
+                        tc_st_x16(t_s + 16 * q, pw);  // over scores that were read
+                    };
+                    tc_wait_ld();
+#pragma unroll 1
+                    for (int q = 0; q < 4; q += 2) {
+                        tc_ld_x32(t_s + 32 * (q + 1), vb);
+                        weights(va, q);
+                        tc_wait_ld();
+                        if (q == 0) tc_ld_x32(t_s + 64, va);
+                        weights(vb, q + 1);
+                        tc_wait_ld();
                     }
                     float s0, s1;
                     unpack2(add2(sum2[0], sum2[1]), s0, s1);
                     l = l * alpha + (s0 + s1);
                     m = m_new;
                     tc_wait_st();
-                } else if (lane == 0) {
-                    mbar_arrive(s_addr(&p_half[ws]));
+                }
+                if (quarter == 0) {  // V of these keys is there and safe
+                    const int at = tile0 + j;
+                    if (!(ok = wait(&v_full[at % RING], at / RING))) break;
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -823,7 +893,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (!ok) give_up(25);
             if (!ok) break;
             if (ops) {
-                if (!(ok = wait(&pv_done[ws], c - 1))) {
+                if (!(ok = wait(&o_full[ws], ended++))) {
                     give_up(26);
                     break;
                 }
@@ -846,24 +916,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 32; ++e) ov[e] = 0u;
                     }
-                    if (bad && real) {
-                        const int hi = min(it.end, it.slot0 + 128 * it.n_kt);
-                        for (int s = max(it.scan, it.slot0); s < hi; ++s) {
-                            const bool seen = it.mode == kModeCausal
-                                                  ? s <= it.ctx + i
-                                                  : (s - it.ctx < 64 && ((bits >> (s - it.ctx)) & 1ull));
-                            if (!seen) continue;
-                            const int x = a.tables[(size_t)it.trow * a.max_blocks + (s >> 4)];
-                            const int page = x < 0 || x >= a.num_blocks ? 0 : x;
-                            const __half* v = a.kv +
-                                              ((((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 + (s & 15)) * HD + c0;
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float y = __half2float(v[e]);
-                                if (!isfinite(y)) ov[e] = __float_as_uint(__uint_as_float(ov[e]) + y);
-                            }
-                        }
-                    }
                     if (real && it.prow < 0) {
                         __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + c0;
 #pragma unroll
@@ -885,18 +937,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     }
                 }
                 if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
+                if (bad && real) rows_add_bad<HD>(a, it, i, bits, head, it.prow < 0 ? (size_t)tok : prow);
             }
-            if (ops) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_addr(&o_free[ws]));
-            }
+            tc_fence_before();  // O was read before the slot's next P is announced
             done_item(k);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsOtherRegs));
     if (warp == kRowsSchedWarp) {
         // ------------------------------------------------------------ scheduler
+        // The items that it passes on have at least one operation: the MMA
+        // issuer may wait for an item while operations of the one before are
+        // open, which an empty one between would keep from ending.
+        int next = blockIdx.x;
         for (int k = 0;; ++k) {
             const int d = k % kRowsItems;
             if (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1)) {
@@ -905,14 +957,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             }
             if (stopped()) break;
             int more = 0;
-            if (lane == 0) {
-                const int idx = a.counter ? (int)atomicAdd(a.counter, 1u) : (int)(blockIdx.x + k * gridDim.x);
+            for (;;) {
+                int idx = next;
+                if (a.counter) idx = __shfl_sync(0xffffffffu, lane == 0 ? (int)atomicAdd(a.counter, 1u) : 0, 0);
+                else next += gridDim.x;
                 const RowsItem it = rows_item(a, plan, idx);
-                items[d] = it;
-                more = it.n_kt >= 0;
-                mbar_arrive(s_addr(&i_full[d]));
+                if (it.n_kt == 0) {  // no keys: the rows' results are zero
+                    rows_zero<HD>(a, it, lane);
+                    continue;
+                }
+                more = it.n_kt > 0;
+                if (lane == 0) {
+                    items[d] = it;
+                    mbar_arrive(s_addr(&i_full[d]));
+                }
+                break;
             }
-            if (!__shfl_sync(0xffffffffu, more, 0)) break;
+            __syncwarp();
+            if (!more) break;
         }
     } else if (warp == kRowsLoadWarp) {
         // ------------------------------------------------------------ loads

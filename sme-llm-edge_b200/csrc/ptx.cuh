@@ -73,6 +73,24 @@ __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity) {
         if (gtimer() - t0 > 2000000000ull) return false;
     }
 }
+// Probe and wait for a whole warp: the result is a vote, and so warp-uniform
+// (what depends on it may stay in uniform registers).  The wait probes without
+// sleeping.
+__device__ __forceinline__ bool mbar_test_warp(uint32_t a, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_test(a, parity));
+}
+__device__ __forceinline__ bool mbar_spin_warp(uint32_t a, uint32_t parity) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t n = 1;; ++n) {
+        if (mbar_test_warp(a, parity)) return true;
+        if ((n & 255u) == 0) {
+            const uint64_t now = gtimer();
+            if (t0 == 0) t0 = now;
+            if (__any_sync(0xffffffffu, now - t0 > 2000000000ull)) return false;
+        }
+    }
+}
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(mbar)
