@@ -280,7 +280,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     }
     __syncthreads();
     int fine = max(4, (int)min((long long)1 << 20, (work + 4 * gridDim.x - 1) / (4 * (long long)gridDim.x)));
-    int coarse = max(8, (int)min((long long)1 << 20, (work + gridDim.x - 1) / (long long)gridDim.x));
+    int coarse = max(8, (int)min((long long)1 << 20, (work + 4 * gridDim.x - 1) / (4 * (long long)gridDim.x)));
     if (a.prows == 0) fine = coarse = 1 << 26;
     int items, prows, item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
     for (int round = 0;; ++round) {
@@ -475,6 +475,9 @@ __device__ __forceinline__ float rows_max3(float a, float b, float c) {
     return d;
 }
 // 2^x on the special-function unit (2 ulp); the result is rounded to fp16 next.
+// A quarter of them by a polynomial on the FMA units instead cost 5% (8192-token
+// prompt 559 us against 532): a softmax warp is bound by the instructions that
+// it issues, not by that unit.
 __device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
     float x0, x1, y0, y1;
     unpack2(x, x0, x1);
@@ -482,34 +485,6 @@ __device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
     return pack2(y0, y1);
 }
-// The same on the FMA units for x <= 127 and not NaN: x = n + f with n the
-// nearest integer (adding 1.5 * 2^23 rounds to it), 2^f on [-1/2, 1/2] by a
-// polynomial of degree 4 with the least largest relative error (2.6e-6, found
-// by an exchange of its extrema), 2^n added to the exponent.  Below 2^-126 the
-// result is some value under 2^-125, which fp16 rounds to 0.
-// The special-function unit gives 16 results a clock and SM, and a tile pair
-// needs 32,768 while its MMAs take 2,048 clocks: one result in kRowsExpEvery
-// comes from here.
-constexpr int kRowsExpEvery = 4;
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-    float x0, x1;
-    unpack2(x, x0, x1);
-    x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-    const uint64_t big = pack2(12582912.f, 12582912.f);
-    const uint64_t t = add2(x, big);
-    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
-    uint64_t p = pack2(0.009570102207362652f, 0.009570102207362652f);
-    p = fma2(p, f, pack2(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-    float t0, t1, p0, p1;
-    unpack2(t, t0, t1);
-    unpack2(p, p0, p1);
-    return pack2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)),
-                 __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
-}
-
 // The CTA's barriers, in shared memory.
 template <int RING>
 struct RowsBars {
@@ -857,7 +832,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                         for (int e = 0; e < 16; ++e) {
                             const uint64_t x =
                                 fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, sub2);
-                            const uint64_t y = e % kRowsExpEvery == kRowsExpEvery - 1 ? exp2_poly2(x) : exp2_unit2(x);
+                            const uint64_t y = exp2_unit2(x);
                             sum2[e & 1] = add2(sum2[e & 1], y);
                             float y0, y1;
                             unpack2(y, y0, y1);
@@ -1108,12 +1083,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 }
 
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
-// their order.  One CTA per token row, a warp per head.
+// their order.  One warp per token row and head; a lane holds HD / 32
+// neighbouring columns, and the loads of eight pieces are in flight together
+// (one piece after the other took 18 to 34 us where this takes 4 to 6).
 template <int HD>
 __global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
     constexpr int E = HD / 32;
     pdl_wait();
     const int tok = blockIdx.x, lane = threadIdx.x & 31;
+    const int head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (head >= a.Hq) return;
     int b, i;
     if (a.row_off) {
         int lo = 0, hi = a.B;  // first sequence whose end is past tok
@@ -1133,34 +1112,52 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
     const RowsMeta mt = a.meta[b];
     const int n = mt.n_pre + mt.n_own;
     if (n == 0) return;
-    for (int head = threadIdx.x >> 5; head < a.Hq; head += 8) {
-        auto at = [&](int p) -> size_t {
-            const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
-            return (size_t)(r + i) * a.Hq + head;
-        };
-        // up to 64 pieces: two a lane
-        float2 ml[2];
+    auto at = [&](int p) -> size_t {
+        const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
+        return (size_t)(r + i) * a.Hq + head;
+    };
+    // up to 64 pieces: two a lane
+    float2 ml[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) ml[u] = lane + 32 * u < n ? a.pml[at(lane + 32 * u)] : make_float2(-INFINITY, 0.f);
-        const float M = warp_max(fmaxf(ml[0].x, ml[1].x));
-        const float sub = M == -INFINITY ? 0.f : M;
-        const float w0 = exp2f(ml[0].x - sub), w1 = exp2f(ml[1].x - sub);
-        const float l = warp_sum(w0 * ml[0].y + w1 * ml[1].y);
-        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-        float o[E];
+    for (int u = 0; u < 2; ++u) ml[u] = lane + 32 * u < n ? a.pml[at(lane + 32 * u)] : make_float2(-INFINITY, 0.f);
+    const float M = warp_max(fmaxf(ml[0].x, ml[1].x));
+    const float sub = M == -INFINITY ? 0.f : M;
+    const float w0 = exp2f(ml[0].x - sub), w1 = exp2f(ml[1].x - sub);
+    const float l = warp_sum(w0 * ml[0].y + w1 * ml[1].y);
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    float o[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int p = 0; p < n; ++p) {
-            const float w = __shfl_sync(0xffffffffu, p < 32 ? w0 : w1, p & 31);
-            const float* src = a.po + at(p) * HD + lane * E;
-            if (w == 0.f) continue;  // a piece without a seen slot, or far below
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int p0 = 0; p0 < n; p0 += 8) {
+        float v[8][E], w[8];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += w * src[e];
+        for (int u = 0; u < 8; ++u) {
+            const int p = p0 + u;
+            w[u] = __shfl_sync(0xffffffffu, p & 32 ? w1 : w0, p & 31);
+            if (p >= n) w[u] = 0.f;
+            if (w[u] != 0.f) {  // a piece of no weight may hold nothing
+                const float* src = a.po + at(p) * HD + lane * E;
+                if (E == 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(src);
+                    v[u][0] = x.x, v[u][1] = x.y, v[u][E - 2] = x.z, v[u][E - 1] = x.w;
+                } else {
+                    const float2 x = *reinterpret_cast<const float2*>(src);
+                    v[u][0] = x.x, v[u][1] = x.y;
+                }
+            }
         }
-        __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) dst[e] = __float2half_rn(o[e] * inv);
+        for (int u = 0; u < 8; ++u)
+            if (w[u] != 0.f)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += w[u] * v[u][e];
     }
+    __half h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = __float2half_rn(o[e] * inv);
+    __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
+    if (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
+    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1254,7 +1251,7 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     SD_LAUNCH_CHECK("rows_attention_kernel");
     if (prows) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)a.T);
+        cfg.gridDim = dim3((unsigned)a.T, (unsigned)((a.Hq + 7) / 8));
         cfg.blockDim = dim3(256);
         cfg.stream = s;
         cudaLaunchAttribute at[1];
