@@ -58,7 +58,7 @@ namespace specdec {
 
 constexpr int kRowsMaxSeqs = 1024;   // sequences of a call: the plan's tables live in shared memory
 constexpr int kRowsMaxSplits = 32;   // pieces of one key range
-constexpr int kRowsSorted = 128;     // up to so many segments are taken longest first
+constexpr int kRowsSorted = 128;     // up to so many segments are kept in shared memory and taken longest first
 constexpr int kRowsThreads = 384;
 constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
@@ -123,18 +123,20 @@ struct RowsItem {
 // ------------------------------------------------------------------ the plan
 __device__ __forceinline__ int rows_clamp(int v, int lo, int hi) { return max(lo, min(hi, v)); }
 
-__device__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* group_pages, const int* seq_pages) {
+// Segment i; off: the bounds of the sequences' rows (prompt) or of the groups.
+__device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* off, const int* ctx_len,
+                                            const int* group_pages, const int* seq_pages) {
     RowsSeg s;
     if (a.row_off) {
-        s.lo = rows_clamp(a.row_off[i], 0, a.T);
-        s.n = rows_clamp(a.row_off[i + 1], s.lo, a.T) - s.lo;
-        s.ctx = rows_clamp(a.ctx_len[i], 0, 1 << 30);
+        s.lo = rows_clamp(off[i], 0, a.T);
+        s.n = rows_clamp(off[i + 1], s.lo, a.T) - s.lo;
+        s.ctx = rows_clamp(ctx_len[i], 0, 1 << 30);
         s.base = 0;
         s.end = min(s.ctx + s.n, a.slots_max);
         s.trow = i;
         s.mode = kModeCausal;
     } else if (i < a.n_groups) {
-        const int b0 = rows_clamp(a.group_off[i], 0, a.B), b1 = rows_clamp(a.group_off[i + 1], b0, a.B);
+        const int b0 = rows_clamp(off[i], 0, a.B), b1 = rows_clamp(off[i + 1], b0, a.B);
         s.lo = b0 * a.R;
         s.n = (b1 - b0) * a.R;
         s.ctx = 0;
@@ -147,7 +149,7 @@ __device__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* group_pages, co
         const int b = i - a.n_groups;
         s.lo = b * a.R;
         s.n = a.R;
-        s.ctx = rows_clamp(a.ctx_len[b], 0, 1 << 30);
+        s.ctx = rows_clamp(ctx_len[b], 0, 1 << 30);
         s.base = seq_pages[b] * 16;
         s.end = max(s.base, min(s.ctx + a.R, a.slots_max));
         s.trow = b;
@@ -169,9 +171,12 @@ __device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s) {
     return a.prows > 0 && s.n <= a.tpt && s.kt >= 2;
 }
 // Pieces of the key range, for pieces of about `fine` tiles where there are few
-// rows (memory-bound: partial results are small) or `coarse`.
-__device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, int fine, int coarse) {
-    const int S = s.n * a.G <= 64 ? (s.kt + fine - 1) / fine : (2 * s.kt + coarse) / (2 * coarse);
+// rows (memory-bound: partial results are small) or `coarse`.  A segment of many
+// rows is cut only where one range is more than a CTA's share of the work
+// (`whole` tiles): the pieces' results cost as much as two key tiles each.
+__device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, int fine, int coarse, int whole) {
+    const int S = s.n * a.G <= 64 ? (s.kt + fine - 1) / fine
+                                  : (s.kt <= whole ? 1 : (2 * s.kt + coarse) / (2 * coarse));
     const int most = rows_dual(a, s) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
     return rows_clamp(S, 1, max(1, most));
 }
@@ -189,50 +194,61 @@ struct RowsPlan {
     int pre[2 * kRowsMaxSeqs + 1];  // items before position i (without the KV heads)
     int prow[2 * kRowsMaxSeqs];     // partial rows before position i
     int group_pages[kRowsMaxSeqs], seq_pages[kRowsMaxSeqs];
+    RowsSeg segs[kRowsSorted];
     int order[kRowsSorted];
-    int wsum[2][kRowsThreads / 32];
-    long long wwork[kRowsThreads / 32];
-    int nseg, items, fine, coarse;
+    int wsum[2][32];
+    float wwork[32];
+    int nseg, items, fine, coarse, whole;
 };
 
 // Sums over the CTA; every thread gets them.  before_*: the sums of the threads in front.
-__device__ void rows_scan2(RowsPlan& p, int va, int vb, int* before_a, int* before_b, int* tot_a, int* tot_b) {
+__device__ __forceinline__ void rows_scan2(RowsPlan& p, int va, int vb, int* before_a, int* before_b, int* tot_a,
+                                           int* tot_b) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int xa = va, xb = vb;
+    auto scan = [&](int& x, int& y) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int ya = __shfl_up_sync(0xffffffffu, xa, o), yb = __shfl_up_sync(0xffffffffu, xb, o);
-        if (lane >= o) {
-            xa += ya;
-            xb += yb;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) {
+                x += u;
+                y += v;
+            }
         }
-    }
+    };
+    int xa = va, xb = vb;
+    scan(xa, xb);
     __syncthreads();
     if (lane == 31) {
         p.wsum[0][w] = xa;
         p.wsum[1][w] = xb;
     }
     __syncthreads();
-    int ba = 0, bb = 0, ta = 0, tb = 0;
-    for (int i = 0; i < kRowsThreads / 32; ++i) {
-        if (i == w) {
-            ba = ta;
-            bb = tb;
-        }
-        ta += p.wsum[0][i];
-        tb += p.wsum[1][i];
-    }
-    *before_a = ba + xa - va;
-    *before_b = bb + xb - vb;
-    *tot_a = ta;
-    *tot_b = tb;
+    int ta = lane < kRowsThreads / 32 ? p.wsum[0][lane] : 0, tb = lane < kRowsThreads / 32 ? p.wsum[1][lane] : 0;
+    scan(ta, tb);
+    const int ba = __shfl_sync(0xffffffffu, ta, max(0, w - 1)), bb = __shfl_sync(0xffffffffu, tb, max(0, w - 1));
+    *tot_a = __shfl_sync(0xffffffffu, ta, 31);
+    *tot_b = __shfl_sync(0xffffffffu, tb, 31);
+    *before_a = (w ? ba : 0) + xa - va;
+    *before_b = (w ? bb : 0) + xb - vb;
 }
 
 // Every CTA makes the same plan from the lengths in device memory (so a
-// captured call serves other lengths); CTA 0 writes where the partials lie.
+// captured call serves other lengths); CTA 0 writes where the partials lie.  It
+// is on every call's path: lengths and bounds are loaded once, together, and up
+// to kRowsSorted segments stay in shared memory.
 __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const int tid = threadIdx.x;
     const int nseg = a.row_off ? a.B : a.n_groups + a.B;
+    const bool small = nseg <= kRowsSorted;
+    const int32_t* off = a.row_off ? a.row_off : a.group_off;
+    const int32_t* ctx = a.ctx_len;
+    if (small) {  // copies, where pre and prow will be
+        const int n_off = a.row_off ? a.B + 1 : (a.n_groups ? a.n_groups + 1 : 0);
+        if (tid < n_off) p.pre[tid] = off[tid];
+        if (tid < a.B) p.prow[tid] = ctx[tid];
+        off = p.pre;
+        ctx = p.prow;
+    }
     if (!a.row_off) {
         // shared pages of a group: announced, and within every member's context
         for (int g = tid; g < a.n_groups; g += kRowsThreads)
@@ -242,52 +258,55 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             int lo = 0, hi = a.n_groups;  // first group whose end is past b
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if (a.group_off[mid + 1] > b) hi = mid;
+                if (off[mid + 1] > b) hi = mid;
                 else lo = mid + 1;
             }
-            const int g = lo < a.n_groups && a.group_off[lo] <= b ? lo : -1;
+            const int g = lo < a.n_groups && off[lo] <= b ? lo : -1;
             p.seq_pages[b] = g;
             if (g >= 0) {
                 // a group of one shares nothing worth a second pass
-                const bool one = a.group_off[g + 1] - a.group_off[g] < 2;
-                atomicMin(&p.group_pages[g], one ? 0 : rows_clamp(a.ctx_len[b], 0, 1 << 30) / 16);
+                const bool one = off[g + 1] - off[g] < 2;
+                atomicMin(&p.group_pages[g], one ? 0 : rows_clamp(ctx[b], 0, 1 << 30) / 16);
             }
         }
         __syncthreads();
         for (int b = tid; b < a.B; b += kRowsThreads) p.seq_pages[b] = p.seq_pages[b] >= 0 ? p.group_pages[p.seq_pages[b]] : 0;
-        __syncthreads();
     }
-    const int per = (nseg + kRowsThreads - 1) / kRowsThreads;
+    __syncthreads();
+    const int per = small ? 1 : (nseg + kRowsThreads - 1) / kRowsThreads;
     const int s0 = min(nseg, tid * per), s1 = min(nseg, s0 + per);
-    // total work in key tiles, and the longest segments first
-    long long work = 0;
-    int len = 0;
+    auto seg_of = [&](int i) { return rows_seg(a, i, off, ctx, p.group_pages, p.seq_pages); };
+    // total work in key tiles (in fp32: an estimate, the same in every CTA)
+    float work = 0.f;
     for (int i = s0; i < s1; ++i) {
-        const RowsSeg s = rows_seg(a, i, p.group_pages, p.seq_pages);
-        if (s.tiles > 0) work += (long long)s.tiles * (rows_item_kt(a, s, 0) + s.kt) / 2 * a.Hkv;
-        len = s.tiles > 0 ? s.kt : 0;
-        p.pre[i] = len;
+        const RowsSeg s = seg_of(i);
+        if (s.tiles > 0) work += (float)s.tiles * 0.5f * (float)(rows_item_kt(a, s, 0) + s.kt) * (float)a.Hkv;
+        if (small) p.segs[i] = s;
     }
     work = warp_sum(work);
     if ((tid & 31) == 0) p.wwork[tid >> 5] = work;
     __syncthreads();
-    work = 0;
-    for (int i = 0; i < kRowsThreads / 32; ++i) work += p.wwork[i];
-    if (nseg <= kRowsSorted && tid < nseg) {  // here a thread has one segment
-        int rank = 0;
-        for (int j = 0; j < nseg; ++j) rank += p.pre[j] > len || (p.pre[j] == len && j < tid);
-        p.order[rank] = tid;
+    work = warp_sum((tid & 31) < kRowsThreads / 32 ? p.wwork[tid & 31] : 0.f);
+    if (small) {  // the longest first
+        if (tid < nseg) {
+            const int len = p.segs[tid].kt;
+            int rank = 0;
+            for (int j = 0; j < nseg; ++j) rank += p.segs[j].kt > len || (p.segs[j].kt == len && j < tid);
+            p.order[rank] = tid;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    int fine = max(4, (int)min((long long)1 << 20, (work + 4 * gridDim.x - 1) / (4 * (long long)gridDim.x)));
-    int coarse = max(8, (int)min((long long)1 << 20, (work + 4 * gridDim.x - 1) / (4 * (long long)gridDim.x)));
-    if (a.prows == 0) fine = coarse = 1 << 26;
-    int items, prows, item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
+    // pieces of about a quarter of a CTA's share
+    const float mean = work / (float)gridDim.x;
+    const int share = (int)fminf(ceilf(0.25f * mean), (float)(1 << 20));
+    const int whole = (int)fminf(1.1f * mean, (float)(1 << 26));
+    int fine = a.prows ? max(4, share) : 1 << 26, coarse = a.prows ? max(8, share) : 1 << 26;
+    int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
     for (int round = 0;; ++round) {
-        items = prows = 0;
+        int items = 0, prows = 0;
         for (int i = s0; i < s1; ++i) {
-            const RowsSeg s = rows_seg(a, nseg <= kRowsSorted ? p.order[i] : i, p.group_pages, p.seq_pages);
-            const int S = rows_splits(a, s, fine, coarse);
+            const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
+            const int S = rows_splits(a, s, fine, coarse, whole);
             items += s.tiles * S;
             prows += s.n * rows_parts(a, s, S);
         }
@@ -298,9 +317,8 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         coarse = round == 7 ? 1 << 26 : 2 * coarse;
     }
     for (int i = s0; i < s1; ++i) {
-        const int id = nseg <= kRowsSorted ? p.order[i] : i;
-        const RowsSeg s = rows_seg(a, id, p.group_pages, p.seq_pages);
-        const int S = rows_splits(a, s, fine, coarse);
+        const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
+        const int S = rows_splits(a, s, fine, coarse, whole);
         const int parts = rows_parts(a, s, S);
         p.pre[i] = item0;
         p.prow[i] = prow0;
@@ -328,6 +346,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         p.items = tot_items * a.Hkv;
         p.fine = fine;
         p.coarse = coarse;
+        p.whole = whole;
     }
     __syncthreads();
 }
@@ -345,8 +364,10 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
         if (p.pre[mid] <= r) lo = mid;
         else hi = mid;
     }
-    const RowsSeg s = rows_seg(a, p.nseg <= kRowsSorted ? p.order[lo] : lo, p.group_pages, p.seq_pages);
-    const int S = rows_splits(a, s, p.fine, p.coarse);
+    const RowsSeg s = p.nseg <= kRowsSorted
+                          ? p.segs[p.order[lo]]
+                          : rows_seg(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_pages);
+    const int S = rows_splits(a, s, p.fine, p.coarse, p.whole);
     const int local = r - p.pre[lo];
     const int tile = s.tiles - 1 - local / S, piece = local % S;  // the longest first
     const int parts = rows_parts(a, s, S);
@@ -1152,7 +1173,7 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] += w[u] * v[u][e];
     }
-    __half h[E];
+    alignas(8) __half h[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) h[e] = __float2half_rn(o[e] * inv);
     __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
@@ -1182,8 +1203,10 @@ constexpr int kRowsPartialRows = 8192;   // room for their pieces, in token rows
 constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece of every range
 
 // Rows of the partial buffers.
-static size_t prompt_partial_rows(int T) {
-    return T <= kRowsSplitTokens ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : 0;
+// Tables of up to 256 slots have two key tiles: no pieces, and no merge behind
+// them (a single row on 40 slots: 14.9 us a call with its launch, 12.2 without).
+static size_t prompt_partial_rows(int T, int max_blocks) {
+    return T <= kRowsSplitTokens && max_blocks > 16 ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : 0;
 }
 static size_t shared_partial_rows(int T) {
     // prefix and own range of every row, each of which may be a dual
@@ -1292,9 +1315,9 @@ using namespace specdec;
 
 extern "C" size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                            int max_blocks) {
-    (void)n_kv_heads, (void)max_blocks;
+    (void)n_kv_heads;
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
-    return rows_workspace(prompt_partial_rows(T), B, n_q_heads, head_dim);
+    return rows_workspace(prompt_partial_rows(T, max_blocks), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1309,7 +1332,7 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
     SD_CHECK(ldq >= n_q_heads * head_dim && ldq % 8 == 0 && ldo >= n_q_heads * head_dim && ldo % 8 == 0,
              SPECDEC_EINVAL, "attention_prompt: row strides hold all heads and are multiples of 8");
     if (B == 0 || T == 0) return SPECDEC_OK;
-    const size_t prows = prompt_partial_rows(T);
+    const size_t prows = prompt_partial_rows(T, max_blocks);
     if ((rc = check_workspace("attention_prompt", workspace, workspace_bytes,
                               rows_workspace(prows, B, n_q_heads, head_dim))))
         return rc;
