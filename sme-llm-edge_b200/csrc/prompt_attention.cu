@@ -74,6 +74,17 @@ struct RowsMeta {
     int n_own, base_own, stride_own;  // pieces of the own range; both 0: written by the main kernel
 };
 
+// x / d for 0 <= x < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d), 2^s >= d.
+struct RowsDiv {
+    uint32_t mul, shift;
+};
+static RowsDiv rows_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1u << s) < d) ++s;
+    return {(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ int rows_quot(int x, RowsDiv d) { return (int)(((uint64_t)(uint32_t)x * d.mul) >> d.shift); }
+
 struct RowsArgs {
     const __half* kv;
     int num_blocks, Hkv, Hq, G, tpt;  // tpt = tokens of a 128-row tile
@@ -86,6 +97,7 @@ struct RowsArgs {
     const int32_t* shared_blocks;
     int n_groups, B, T, R;
     int tq_small;  // tokens of the small query box
+    RowsDiv by_item, by_hkv;  // 2 * tpt tokens of an item; KV heads
     int slots_max;  // max_blocks * 16
     __half* out;
     int ldo;
@@ -155,7 +167,7 @@ __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int*
         s.trow = b;
         s.mode = kModeMask;
     }
-    s.tiles = (s.n + 2 * a.tpt - 1) / (2 * a.tpt);
+    s.tiles = rows_quot(s.n + 2 * a.tpt - 1, a.by_item);
     s.kt = (s.end - s.base + 127) / 128;
     return s;
 }
@@ -170,13 +182,18 @@ __device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s,
 __device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s) {
     return a.prows > 0 && s.n <= a.tpt && s.kt >= 2;
 }
-// Pieces of the key range, for pieces of about `fine` tiles where there are few
-// rows (memory-bound: partial results are small) or `coarse`.  A segment of many
-// rows is cut only where one range is more than a CTA's share of the work
-// (`whole` tiles): the pieces' results cost as much as two key tiles each.
-__device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, int fine, int coarse, int whole) {
-    const int S = s.n * a.G <= 64 ? (s.kt + fine - 1) / fine
-                                  : (s.kt <= whole ? 1 : (2 * s.kt + coarse) / (2 * coarse));
+// How long the pieces of a key range are, in key tiles: about `fine` where there
+// are few rows (memory-bound: partial results are small), about `coarse`
+// elsewhere.  A segment of many rows is cut only where one range is more than a
+// CTA's share of the work (`whole`): its pieces' results cost as much as two key
+// tiles each.
+struct RowsCut {
+    float per_fine, per_coarse;  // reciprocals
+    int whole;
+};
+__device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
+    const int S = s.n * a.G <= 64 ? (int)ceilf((float)s.kt * cut.per_fine)
+                                  : (s.kt <= cut.whole ? 1 : (int)rintf((float)s.kt * cut.per_coarse));
     const int most = rows_dual(a, s) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
     return rows_clamp(S, 1, max(1, most));
 }
@@ -195,10 +212,12 @@ struct RowsPlan {
     int prow[2 * kRowsMaxSeqs];     // partial rows before position i
     int group_pages[kRowsMaxSeqs], seq_pages[kRowsMaxSeqs];
     RowsSeg segs[kRowsSorted];
-    int order[kRowsSorted];
+    int order[kRowsSorted];   // segment at position i
+    int splits[kRowsSorted];  // its pieces
     int wsum[2][32];
     float wwork[32];
-    int nseg, items, fine, coarse, whole;
+    int nseg, items;
+    RowsCut cut;
 };
 
 // Sums over the CTA; every thread gets them.  before_*: the sums of the threads in front.
@@ -298,30 +317,31 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     }
     // pieces of about a quarter of a CTA's share
     const float mean = work / (float)gridDim.x;
-    const int share = (int)fminf(ceilf(0.25f * mean), (float)(1 << 20));
-    const int whole = (int)fminf(1.1f * mean, (float)(1 << 26));
-    int fine = a.prows ? max(4, share) : 1 << 26, coarse = a.prows ? max(8, share) : 1 << 26;
+    const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
+    RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.25f * mean) : none,
+                   (int)fminf(1.1f * mean, (float)(1 << 26))};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
     for (int round = 0;; ++round) {
         int items = 0, prows = 0;
         for (int i = s0; i < s1; ++i) {
             const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
-            const int S = rows_splits(a, s, fine, coarse, whole);
+            const int S = rows_splits(a, s, cut);
             items += s.tiles * S;
             prows += s.n * rows_parts(a, s, S);
         }
         rows_scan2(p, items, prows, &item0, &prow0, &tot_items, &tot_prows);
         if (tot_prows <= a.prows || round >= 8) break;
         // fewer pieces until their results fit; at last one a segment, which always does
-        fine = round == 7 ? 1 << 26 : 2 * fine;
-        coarse = round == 7 ? 1 << 26 : 2 * coarse;
+        cut.per_fine = round == 7 ? none : 0.5f * cut.per_fine;
+        cut.per_coarse = round == 7 ? none : 0.5f * cut.per_coarse;
     }
     for (int i = s0; i < s1; ++i) {
         const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
-        const int S = rows_splits(a, s, fine, coarse, whole);
+        const int S = rows_splits(a, s, cut);
         const int parts = rows_parts(a, s, S);
         p.pre[i] = item0;
         p.prow[i] = prow0;
+        if (small) p.splits[i] = S;
         if (blockIdx.x == 0 && a.meta) {
             if (s.mode == kModeAll) {
                 for (int b = s.lo / a.R; b < (s.lo + s.n) / a.R; ++b) {
@@ -344,9 +364,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         p.pre[nseg] = tot_items;
         p.nseg = nseg;
         p.items = tot_items * a.Hkv;
-        p.fine = fine;
-        p.coarse = coarse;
-        p.whole = whole;
+        p.cut = cut;
     }
     __syncthreads();
 }
@@ -356,8 +374,8 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     it.n_kt = -1;
     it.bad = 0;
     if (idx < 0 || idx >= p.items) return it;
-    it.kvh = idx % a.Hkv;
-    const int r = idx / a.Hkv;
+    const int r = rows_quot(idx, a.by_hkv);
+    it.kvh = idx - r * a.Hkv;
     int lo = 0, hi = p.nseg;  // last position with pre <= r
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -367,9 +385,10 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     const RowsSeg s = p.nseg <= kRowsSorted
                           ? p.segs[p.order[lo]]
                           : rows_seg(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_pages);
-    const int S = rows_splits(a, s, p.fine, p.coarse, p.whole);
+    const int S = p.nseg <= kRowsSorted ? p.splits[lo] : rows_splits(a, s, p.cut);
     const int local = r - p.pre[lo];
-    const int tile = s.tiles - 1 - local / S, piece = local % S;  // the longest first
+    const int along = S == 1 ? local : local / S;
+    const int tile = s.tiles - 1 - along, piece = local - along * S;  // the longest first
     const int parts = rows_parts(a, s, S);
     if (local < 0 || tile < 0 || (parts && !rows_fit(a, s, parts, p.prow[lo]))) {  // bounds that overlap: an empty item
         it.n_kt = it.ntok0 = it.ntok1 = 0;
@@ -379,7 +398,7 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
         return it;
     }
     const int kt = rows_item_kt(a, s, tile);
-    const int k0 = (int)((long long)piece * kt / S), k1 = (int)((long long)(piece + 1) * kt / S);
+    const int k0 = S == 1 ? 0 : piece * kt / S, k1 = S == 1 ? kt : (piece + 1) * kt / S;  // S <= 32, kt < 2^24
     it.n_kt = k1 - k0;
     it.slot0 = s.base + 128 * k0;
     it.end = min(rows_item_end(a, s, tile), s.base + 128 * k1);
@@ -393,7 +412,7 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     it.scan = s.mode == kModeCausal ? s.ctx + it.i0 + 1 : (s.mode == kModeMask ? s.ctx : it.end);
     it.kind = rows_dual(a, s) || (it.ntok1 == 0 && it.n_kt <= 1) ? kDual : kPair;
     it.pnext = rows_dual(a, s) ? s.n : 0;
-    it.prow = parts ? p.prow[lo] + piece * (parts / S) * s.n + it.i0 : -1;
+    it.prow = parts ? p.prow[lo] + piece * (parts > S ? 2 : 1) * s.n + it.i0 : -1;
     return it;
 }
 
@@ -1249,6 +1268,8 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     a.G = a.Hq / a.Hkv;
     a.tpt = 128 / a.G;
     a.tq_small = std::min(a.tq_small, a.tpt);
+    a.by_item = rows_div(2 * a.tpt);
+    a.by_hkv = rows_div(a.Hkv);
     a.kv = kv;
     a.slots_max = a.max_blocks * 16;
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)HD));
