@@ -422,7 +422,7 @@ struct RowsCfg {
     static constexpr int NH = HD / 64;                  // 64-column halves
     static constexpr int TILE = NH * 16384;             // 128 rows x HD fp16
     static constexpr int RING = HD == 128 ? 2 : 4;      // K tiles and V tiles in flight
-    static constexpr int NBAR = 5 * 2 + 5 * RING + 2 * kRowsItems;
+    static constexpr int NBAR = 5 * 2 + 5 * RING + 2 * kRowsItems + 1;
     static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
                                    NBAR * 8 + 16;
 };
@@ -535,9 +535,10 @@ struct RowsBars {
     uint64_t *k_full, *k_empty;  // [RING]
     uint64_t *v_raw, *v_full, *v_empty;  // [RING] V landed; is safe to multiply
     uint64_t *i_full, *i_empty;  // [kRowsItems] empty: 8 softmax warps, the MMA issuer, loads, fix
+    uint64_t* i_want;            // the loads of an item are nearly out: the next is wanted
     __device__ explicit RowsBars(uint64_t* b)
         : q_full(b), q_empty(b + 2), s_full(b + 4), p_full(b + 6), o_full(b + 8), k_full(b + 10), k_empty(k_full + RING), v_raw(k_empty + RING), v_full(v_raw + RING), v_empty(v_full + RING),
-          i_full(v_empty + RING), i_empty(i_full + kRowsItems) {}
+          i_full(v_empty + RING), i_empty(i_full + kRowsItems), i_want(i_empty + kRowsItems) {}
 };
 
 // The MMA issuer.  P.V of operation i and Q.K^T of operation i + 2 on the same
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
              *o_full = bar.o_full, *k_full = bar.k_full,
              *k_empty = bar.k_empty, *v_raw = bar.v_raw, *v_full = bar.v_full, *v_empty = bar.v_empty,
              *i_full = bar.i_full, *i_empty = bar.i_empty;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + kRowsItems);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar.i_want + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     pdl_trigger();
@@ -732,6 +733,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             mbar_init(s_addr(&i_full[i]), 1);
             mbar_init(s_addr(&i_empty[i]), 11);
         }
+        mbar_init(s_addr(bar.i_want), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -966,7 +968,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         int next = blockIdx.x;
         for (int k = 0;; ++k) {
             const int d = k % kRowsItems;
-            if (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1)) {
+            // An item is taken when the loads of the one before are nearly out: taken
+            // earlier it would wait here while other CTAs have none left.
+            if ((k && !wait(bar.i_want, k - 1)) || (k >= kRowsItems && !wait(&i_empty[d], k / kRowsItems - 1))) {
                 give_up(21);
                 break;
             }
@@ -1013,6 +1017,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 const int np = min(8, pages - 8 * j), slot = kc % RING, turn = kc / RING;
                 const int mine_k = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + (lane / NH) % 8);
                 const int mine_v = __shfl_sync(0xffffffffu, pg, 8 * (j & 3) + lane % 8);
+                if (j == max(0, it.n_kt - 2) && lane == 0) mbar_arrive(s_addr(bar.i_want));
                 if (turn && !(ok = wait(&k_empty[slot], turn - 1))) break;
                 if (lane == 0) mbar_expect_tx(s_addr(&k_full[slot]), (uint32_t)(np * NH * kBlockHalf));
                 __syncwarp();
