@@ -121,7 +121,7 @@ int kv_append_uniform(specdec_kv* kv, int n, int tokens, cudaStream_t s, int r0 
 int kv_truncate_dev(specdec_kv* kv, const int32_t* new_len_dev, int n, cudaStream_t s);
 
 // Forks (kv_fork.cu): dst[i] becomes a copy of src[i], i < n; kv null: tables only.
-size_t kv_fork_workspace(int num_blocks, int max_reqs, int n);
+size_t kv_fork_workspace(int num_blocks, int n);
 int kv_fork_launch(const KVState& st, const int32_t* src, const int32_t* dst, int n, __half* kv, int layers,
                    size_t layer_stride, int Hkv, int hd, int32_t* status, void* ws, cudaStream_t s);
 int kv_fork_check_pool(const char* who, const void* kv, int layers, size_t layer_stride, int num_blocks, int Hkv, int hd);

@@ -30,9 +30,8 @@ struct ForkArgs {
     int n;
     int32_t* status;
     // workspace
-    int32_t* head;   // [64]: 0 error, 1 pairs to copy, 16 + c free blocks counted by CTA c
+    int32_t* head;   // [64]: c error seen by CTA c, 8 pairs to copy, 16 + c free blocks counted by CTA c
     int32_t* refw;   // [num_blocks] reference counts in the making
-    int32_t* mark;   // [max_reqs] times a target
     int32_t* rank;   // [n] copies before this one that need a block
     int32_t* fresh;  // [n] blocks for them
     int32_t* pair;   // [n][3] block to read, block to write, rows
@@ -64,49 +63,54 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
     const int cta = blockIdx.x, tid = threadIdx.x;
     const int gt = cta * kForkThreads + tid, stride = kForkCtas * kForkThreads;
     const int bs = a.block_size;
-    auto fail = [&](int code) { atomicMax(&a.head[0], code); };
-    auto failed = [&]() { return __ldcg(&a.head[0]); };
-    auto leave = [&](int code) {
-        if (cta == 0 && tid == 0) *a.status = code;
-    };
-    if (gt < 64) a.head[gt] = 0;
-    for (int i = gt; i < a.num_blocks; i += stride) a.refw[i] = a.ref[i];
-    for (int i = gt; i < a.max_reqs; i += stride) a.mark[i] = 0;
-    cluster_sync_all();
-    // ids in range, targets distinct
-    for (int i = gt; i < a.n; i += stride) {
-        const int s = a.src[i], d = a.dst[i];
-        if (s < 0 || s >= a.max_reqs || d < 0 || d >= a.max_reqs) fail(SPECDEC_EINVAL);
-        else if (atomicAdd(&a.mark[d], 1)) fail(SPECDEC_EINVAL);
-    }
-    cluster_sync_all();
-    if (int e = failed()) return leave(e);
-    cluster_sync_all();  // nobody reports a later error before all have read this one
-    // sources have a table that holds their tokens and are no targets; the
-    // targets' old blocks are released.  A group of the cluster's 128 warps to
-    // each copy: one copy after the other in a CTA took most of 23 us for 48.
+    // Every check of the arguments reads what the call does not change yet, so one
+    // barrier stands between the checks and the first change; refw is a copy.
+    // Ids in range, targets distinct and no sources, sources with a table that
+    // holds their tokens.  A group of the cluster's 128 warps to each copy (one
+    // copy after the other in a CTA took most of 23 us for 48).
     const int warps = kForkCtas * kForkWarps, gw = gt >> 5, lane = tid & 31;
     const int group = max(1, warps / max(1, a.n)), groups = warps / group;
     const int mine = gw / group, part = gw % group * 32 + lane, step = group * 32;
-    for (int i = mine < groups ? mine : a.n; i < a.n; i += groups) {
+    const int first = mine < groups ? mine : a.n;
+    auto leave = [&](int code) {
+        if (cta == 0 && tid == 0) *a.status = code;
+    };
+    bool bad = false;
+    for (int i = first; i < a.n; i += groups) {
         const int s = a.src[i], d = a.dst[i];
-        const int ns = a.nblk[s], nd = a.nblk[d], L = a.len[s];
-        const int use = L < 0 ? 0 : (int)(((long long)L + bs - 1) / bs);
-        if (ns < 0 || ns > a.max_bpr || nd > a.max_bpr || L < 0 || use > ns || __ldcg(&a.mark[s])) {
-            if (part == 0) fail(SPECDEC_EINVAL);
+        if (s < 0 || s >= a.max_reqs || d < 0 || d >= a.max_reqs) {
+            bad = true;
             continue;
         }
-        for (int j = part; j < use; j += step) {
-            const int p = a.tables[(size_t)s * a.max_bpr + j];
-            if (p < 0 || p >= a.num_blocks) fail(SPECDEC_EINVAL);
+        for (int j = part; j < a.n; j += step) {
+            const int e = a.dst[j];
+            bad |= e == s || (e == d && j != i);
         }
+        const int ns = a.nblk[s], L = a.len[s];
+        const int use = L < 0 ? 0 : (int)(((long long)L + bs - 1) / bs);
+        bad |= ns < 0 || ns > a.max_bpr || a.nblk[d] > a.max_bpr || L < 0 || use > ns;
+        if (!bad)
+            for (int j = part; j < use; j += step) {
+                const int p = a.tables[(size_t)s * a.max_bpr + j];
+                bad |= p < 0 || p >= a.num_blocks;
+            }
+    }
+    bad = __syncthreads_or(bad);
+    if (tid == 0) a.head[cta] = bad;
+    if (gt == 0) a.head[kForkCtas] = 0;  // pairs to copy
+    for (int i = gt; i < a.num_blocks; i += stride) a.refw[i] = a.ref[i];
+    cluster_sync_all();
+    int any = 0;
+    for (int c = 0; c < kForkCtas; ++c) any |= __ldcg(&a.head[c]);
+    if (any) return leave(SPECDEC_EINVAL);
+    // the targets' old blocks are released
+    for (int i = first; i < a.n; i += groups) {
+        const int d = a.dst[i], nd = a.nblk[d];
         for (int j = part; j < nd; j += step) {
             const int p = a.tables[(size_t)d * a.max_bpr + j];
             if (p >= 0 && p < a.num_blocks) atomicSub(&a.refw[p], 1);
         }
     }
-    cluster_sync_all();
-    if (int e = failed()) return leave(e);
     // the copies that need a block, in order (every CTA counts; CTA 0 writes the ranks)
     int need = 0;
     for (int i0 = 0; i0 < a.n; i0 += kForkThreads) {
@@ -117,6 +121,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
         if (cta == 0 && i < a.n) a.rank[i] = t ? need + before : -1;
         need += tot;
     }
+    cluster_sync_all();
     // the lowest free blocks: each CTA takes a range, its threads neighbouring pieces of it
     const int per_cta = (a.num_blocks + kForkCtas - 1) / kForkCtas;
     const int b0 = min(a.num_blocks, cta * per_cta), b1 = min(a.num_blocks, b0 + per_cta);
@@ -140,7 +145,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
             if (__ldcg(&a.refw[b]) == 0) a.fresh[before++] = b;
     cluster_sync_all();
     // tables, lengths and counts of the copies
-    for (int i = mine < groups ? mine : a.n; i < a.n; i += groups) {
+    for (int i = first; i < a.n; i += groups) {
         const int s = a.src[i], d = a.dst[i], L = a.len[s], whole = L / bs, r = __ldcg(&a.rank[i]);
         const int page = r >= 0 ? __ldcg(&a.fresh[r]) : -1;
         int32_t* to = a.tables + (size_t)d * a.max_bpr;
@@ -169,7 +174,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
     cluster_sync_all();
     for (int i = gt; i < a.num_blocks; i += stride) a.ref[i] = __ldcg(&a.refw[i]);
     if (gt == 0) {
-        a.head[1] = need;
+        a.head[kForkCtas] = need;
         *a.status = SPECDEC_OK;
     }
 }
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const int32_t* head, 
                                                            size_t layer_stride, int Hkv, int hd) {
     pdl_wait();
     const int i = blockIdx.x;
-    if (i >= head[1]) return;
+    if (i >= head[kForkCtas]) return;
     const int rows = pair[3 * i + 2], run = rows * hd / 8, total = 2 * Hkv * run;  // 16-byte pieces
     const size_t block = (size_t)2 * Hkv * 16 * hd;
     const uint4* src = reinterpret_cast<const uint4*>(kv + layer_stride * blockIdx.y + block * pair[3 * i]);
@@ -201,9 +206,7 @@ __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const int32_t* head, 
     }
 }
 
-size_t kv_fork_workspace(int num_blocks, int max_reqs, int n) {
-    return sizeof(int32_t) * (64 + (size_t)num_blocks + max_reqs + 5 * (size_t)n);
-}
+size_t kv_fork_workspace(int num_blocks, int n) { return sizeof(int32_t) * (64 + (size_t)num_blocks + 5 * (size_t)n); }
 
 int kv_fork_launch(const KVState& st, const int32_t* src, const int32_t* dst, int n, __half* kv, int layers,
                    size_t layer_stride, int Hkv, int hd, int32_t* status, void* ws, cudaStream_t s) {
@@ -222,8 +225,7 @@ int kv_fork_launch(const KVState& st, const int32_t* src, const int32_t* dst, in
     a.status = status;
     a.head = static_cast<int32_t*>(ws);
     a.refw = a.head + 64;
-    a.mark = a.refw + st.num_blocks;
-    a.rank = a.mark + st.max_reqs;
+    a.rank = a.refw + st.num_blocks;
     a.fresh = a.rank + n;
     a.pair = a.fresh + n;
     kv_fork_kernel<<<kForkCtas, kForkThreads, 0, s>>>(a);
@@ -262,7 +264,7 @@ using namespace specdec;
 
 extern "C" size_t specdec_kv_fork_pages_workspace_bytes(int num_blocks, int max_reqs, int n) {
     if (num_blocks <= 0 || max_reqs <= 0 || n < 0) return 0;
-    return kv_fork_workspace(num_blocks, max_reqs, n);
+    return kv_fork_workspace(num_blocks, n);
 }
 
 extern "C" int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t* lens, int32_t* refcounts,
@@ -276,7 +278,7 @@ extern "C" int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t
              SPECDEC_EINVAL, "kv_fork_pages: bad sizes (at most max_reqs copies)");
     int rc = kv_fork_check_pool("kv_fork_pages", kv, layers, layer_stride, num_blocks, n_kv_heads, head_dim);
     if (rc) return rc;
-    SD_CHECK(workspace && workspace_bytes >= kv_fork_workspace(num_blocks, max_reqs, n) &&
+    SD_CHECK(workspace && workspace_bytes >= kv_fork_workspace(num_blocks, n) &&
                  (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
              SPECDEC_EINVAL, "kv_fork_pages: workspace too small or not 4-byte aligned");
     cudaStream_t s = as_stream(stream);

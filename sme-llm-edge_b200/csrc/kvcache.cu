@@ -237,7 +237,7 @@ extern "C" int specdec_kv_create(int num_blocks, int block_size, int max_reqs, i
     if (e == cudaSuccess) e = cudaMalloc(&s.scratch, sizeof(int32_t) * scratch);
     if (e == cudaSuccess) e = cudaMalloc(&s.status, sizeof(int32_t) * 4);
     if (e == cudaSuccess) e = cudaMalloc(&kv->d_tmp, sizeof(int32_t) * (3 * (size_t)max_reqs + 8));
-    if (e == cudaSuccess) e = cudaMalloc(&kv->d_fork, kv_fork_workspace(num_blocks, max_reqs, max_reqs));
+    if (e == cudaSuccess) e = cudaMalloc(&kv->d_fork, kv_fork_workspace(num_blocks, max_reqs));
     if (e == cudaSuccess) e = cudaMallocHost(&kv->h_tmp, sizeof(int32_t) * (3 * (size_t)max_reqs + 8));
     if (e == cudaSuccess) e = cudaMemset(s.tables, 0xff, sizeof(int32_t) * (size_t)max_reqs * max_blocks_per_req);
     if (e == cudaSuccess) e = cudaMemset(s.nblk, 0xff, sizeof(int32_t) * max_reqs);

@@ -104,6 +104,7 @@ struct RowsArgs {
     float scale_log2;
     // workspace
     uint32_t* counter;  // null: items go round the CTAs
+    int* any_parts;     // set by the plan: some rows have pieces to join
     RowsMeta* meta;
     float2* pml;
     float* po;
@@ -315,10 +316,11 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         }
         __syncthreads();
     }
-    // pieces of about a quarter of a CTA's share
+    // pieces of about a quarter of a CTA's share; of half of it where they have many rows (128 x 5 rows under 8192
+    // tokens: 171 us, with a quarter 181)
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
-    RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.25f * mean) : none,
+    RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
                    (int)fminf(1.1f * mean, (float)(1 << 26))};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
     for (int round = 0;; ++round) {
@@ -365,6 +367,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         p.nseg = nseg;
         p.items = tot_items * a.Hkv;
         p.cut = cut;
+        if (blockIdx.x == 0 && a.meta) *a.any_parts = tot_prows > 0;
     }
     __syncthreads();
 }
@@ -948,9 +951,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                             *reinterpret_cast<uint4*>(dst + e) = w;
                         }
                     } else if (real) {
-                        uint4* dst = reinterpret_cast<uint4*>(a.po + prow * HD + c0);
+                        // whole 32-byte sectors: a lane's row is far from the next lane's
+                        float* dst = a.po + prow * HD + c0;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) dst[e / 4] = make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+                        for (int e = 0; e < 32; e += 8)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + e),
+                                         "r"(ov[e]), "r"(ov[e + 1]), "r"(ov[e + 2]), "r"(ov[e + 3]), "r"(ov[e + 4]),
+                                         "r"(ov[e + 5]), "r"(ov[e + 6]), "r"(ov[e + 7])
+                                         : "memory");
                     }
                 }
                 if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
@@ -1130,14 +1138,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
 // their order.  One warp per token row and head; a lane holds HD / 32
 // neighbouring columns, and the loads of eight pieces are in flight together
-// (one piece after the other took 18 to 34 us where this takes 4 to 6).
+// (one piece after the other took 18 to 34 us where this takes 4 to 18).  The
+// CTAs go round the rows: one for each row cost 12 us where no row has pieces.
 template <int HD>
-__global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
+__device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int head) {
     constexpr int E = HD / 32;
-    pdl_wait();
-    const int tok = blockIdx.x, lane = threadIdx.x & 31;
-    const int head = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (head >= a.Hq) return;
+    const int lane = threadIdx.x & 31;
     int b, i;
     if (a.row_off) {
         int lo = 0, hi = a.B;  // first sequence whose end is past tok
@@ -1203,6 +1209,17 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
     __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
     if (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
     else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
+    pdl_wait();
+    if (*a.any_parts == 0) return;
+    const int groups = (a.Hq + 7) / 8;  // of 8 heads
+    for (int u = blockIdx.x; u < a.T * groups; u += gridDim.x) {
+        const int tok = u / groups, head = (u - tok * groups) * 8 + (threadIdx.x >> 5);
+        if (head < a.Hq) rows_merge_row<HD>(a, tok, head);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -1283,6 +1300,7 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     char* w = static_cast<char*>(ws);
     // more items than CTAs: they are taken from a counter, the longest first
     a.counter = tiles > sms ? reinterpret_cast<uint32_t*>(w) : nullptr;
+    a.any_parts = reinterpret_cast<int*>(w + 128);
     a.meta = prows ? reinterpret_cast<RowsMeta*>(w + 256) : nullptr;
     w += 256 + align256(sizeof(RowsMeta) * (size_t)a.B);
     a.pml = reinterpret_cast<float2*>(w);
@@ -1300,7 +1318,7 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     SD_LAUNCH_CHECK("rows_attention_kernel");
     if (prows) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)a.T, (unsigned)((a.Hq + 7) / 8));
+        cfg.gridDim = dim3((unsigned)std::min<long long>((long long)a.T * ((a.Hq + 7) / 8), 8LL * sms));
         cfg.blockDim = dim3(256);
         cfg.stream = s;
         cudaLaunchAttribute at[1];
@@ -1330,8 +1348,8 @@ static int check_rows(const char* who, const void* q, const void* kv, const void
     return SPECDEC_OK;
 }
 static int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
-    SD_CHECK(ws && have >= need && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, SPECDEC_EINVAL,
-             std::string(who) + ": workspace too small or not 16-byte aligned");
+    SD_CHECK(ws && have >= need && (reinterpret_cast<uintptr_t>(ws) & 31) == 0, SPECDEC_EINVAL,
+             std::string(who) + ": workspace too small or not 32-byte aligned");
     return SPECDEC_OK;
 }
 
