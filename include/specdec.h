@@ -323,7 +323,8 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
  * the pool reads block 0.  Up to 1024 sequences.  Long key ranges are split
  * across CTAs and merged through the workspace in a fixed order (the result
  * is deterministic); calls in flight at the same time, captured graphs
- * among them, need workspaces of their own.  The first call on a device
+ * among them, need workspaces (32-byte aligned) of their own.  All pointers
+ * are memory of the current device.  The first call on a device
  * comes before any stream capture.  The reference feeds prompts in chunks
  * (server/chunked_prefill.cpp:4-24) through one row of attention at a time
  * (server/paged_attention.cpp:16-111). */

@@ -95,6 +95,17 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
                 bad |= p < 0 || p >= a.num_blocks;
             }
     }
+    // the copies that need a block, in order (every CTA counts; CTA 0 writes the ranks)
+    int need = 0;
+    for (int i0 = 0; i0 < a.n; i0 += kForkThreads) {
+        const int i = i0 + tid;
+        const int s = i < a.n ? a.src[i] : -1;
+        const int t = s >= 0 && s < a.max_reqs && a.len[s] % bs != 0;
+        int tot;
+        const int before = fork_scan(t, sh, &tot);
+        if (cta == 0 && i < a.n) a.rank[i] = t ? need + before : -1;
+        need += tot;
+    }
     bad = __syncthreads_or(bad);
     if (tid == 0) a.head[cta] = bad;
     if (gt == 0) a.head[kForkCtas] = 0;  // pairs to copy
@@ -110,16 +121,6 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
             const int p = a.tables[(size_t)d * a.max_bpr + j];
             if (p >= 0 && p < a.num_blocks) atomicSub(&a.refw[p], 1);
         }
-    }
-    // the copies that need a block, in order (every CTA counts; CTA 0 writes the ranks)
-    int need = 0;
-    for (int i0 = 0; i0 < a.n; i0 += kForkThreads) {
-        const int i = i0 + tid;
-        const int t = i < a.n && a.len[a.src[i]] % bs != 0;
-        int tot;
-        const int before = fork_scan(t, sh, &tot);
-        if (cta == 0 && i < a.n) a.rank[i] = t ? need + before : -1;
-        need += tot;
     }
     cluster_sync_all();
     // the lowest free blocks: each CTA takes a range, its threads neighbouring pieces of it
@@ -282,6 +283,9 @@ extern "C" int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t
                  (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
              SPECDEC_EINVAL, "kv_fork_pages: workspace too small or not 4-byte aligned");
     cudaStream_t s = as_stream(stream);
+    if ((rc = check_on_device(tables, "kv_fork_pages: tables")) || (rc = check_on_device(status, "kv_fork_pages: status")) ||
+        (layers > 0 && (rc = check_on_device(kv, "kv_fork_pages: the pool"))))
+        return rc;
     if (n == 0) {
         SD_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), s));
         return SPECDEC_OK;

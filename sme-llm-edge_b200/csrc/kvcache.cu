@@ -323,6 +323,7 @@ extern "C" int specdec_kv_fork(specdec_kv* kv, const int32_t* src_reqs, const in
     if (rc) return rc;
     SD_CHECK(layers == 0 || kv->s.block_size == 16, SPECDEC_EINVAL, "kv_fork: a pool's blocks hold 16 tokens");
     if (n == 0) return SPECDEC_OK;
+    if (layers > 0 && (rc = check_on_device(pool, "kv_fork: the pool"))) return rc;
     cudaStream_t s = as_stream(stream);
     int32_t* h = kv->h_tmp;
     for (int i = 0; i < n; ++i) {

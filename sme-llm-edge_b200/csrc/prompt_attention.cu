@@ -193,7 +193,7 @@ struct RowsCut {
     int whole;
 };
 __device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
-    const int S = s.n * a.G <= 64 ? (int)ceilf((float)s.kt * cut.per_fine)
+    const int S = s.n <= 64 / a.G ? (int)ceilf((float)s.kt * cut.per_fine)
                                   : (s.kt <= cut.whole ? 1 : (int)rintf((float)s.kt * cut.per_coarse));
     const int most = rows_dual(a, s) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
     return rows_clamp(S, 1, max(1, most));
@@ -260,6 +260,8 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const int tid = threadIdx.x;
     const int nseg = a.row_off ? a.B : a.n_groups + a.B;
     const bool small = nseg <= kRowsSorted;
+    if (blockIdx.x == 0 && a.meta)  // before a barrier; a group's thread sets it behind
+        for (int b = tid; b < a.B; b += kRowsThreads) a.meta[b].n_pre = 0;
     const int32_t* off = a.row_off ? a.row_off : a.group_off;
     const int32_t* ctx = a.ctx_len;
     if (small) {  // copies, where pre and prow will be
@@ -353,7 +355,6 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
                 }
             } else {
                 RowsMeta& m = a.meta[s.trow];
-                if (s.base == 0) m.n_pre = 0;
                 m.n_own = rows_fit(a, s, parts, prow0) ? parts : 0;
                 m.base_own = prow0;
                 m.stride_own = s.n;
@@ -1165,7 +1166,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
     if (n == 0) return;
     auto at = [&](int p) -> size_t {
         const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
-        return (size_t)(r + i) * a.Hq + head;
+        return (size_t)min(r + i, a.prows - 1) * a.Hq + head;  // group bounds that overlap: never out of range
     };
     // up to 64 pieces: two a lane
     float2 ml[2];
@@ -1286,6 +1287,10 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
                        void* ws, cudaStream_t s) {
     int sms = 0;
     int rc = rows_sms(&sms);
+    if (!rc) rc = check_on_device(q, "attention: q");
+    if (!rc) rc = check_on_device(kv, "attention: the KV pool");
+    if (!rc) rc = check_on_device(a.out, "attention: out");
+    if (!rc) rc = check_on_device(ws, "attention: the workspace");
     if (rc) return rc;
     a.G = a.Hq / a.Hkv;
     a.tpt = 128 / a.G;

@@ -17,6 +17,17 @@ int cuda_status(cudaError_t e, const char* what) {
     return e == cudaErrorMemoryAllocation ? SPECDEC_ENOMEM : SPECDEC_ECUDA;
 }
 
+int check_on_device(const void* p, const char* what) {
+    cudaPointerAttributes at = {};
+    int dev = 0;
+    SD_CUDA(cudaGetDevice(&dev));
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    SD_CHECK(e == cudaSuccess && (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)),
+             SPECDEC_EINVAL, std::string(what) + " is not memory of the current device");
+    return SPECDEC_OK;
+}
+
 static std::mutex g_status_mu;
 static DeviceStatus* g_status[64] = {nullptr};
 

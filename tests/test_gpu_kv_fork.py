@@ -299,3 +299,16 @@ def test_engine_fork(cuda_device, T):
     assert eng.read("lens", np.int32, (B,))[1] > 0  # slot 1 kept its request
     eng.close()
     cache.close()
+
+
+def test_host_pointers_are_refused(cuda_device):
+    g = OnGpu(*make({0: 20}, 3, 8, 4))
+    g.fork([0], [1])
+    g.buf, keep = g.buf.cpu(), g.buf
+    with pytest.raises(S.SpecdecError) as e:
+        g.fork([0], [2])
+    assert e.value.code == S.EINVAL
+    g.buf = keep
+    g.fork([0], [2])
+    torch.cuda.synchronize()
+    assert int(g.status) == S.OK

@@ -268,3 +268,51 @@ def test_no_rows(cuda_device):
     verify(s)
     assert math.isclose(float(s["out"][0, 0, 0]), 7.0)
     del ws
+
+
+@pytest.mark.parametrize("n", [200, 1024])
+def test_many_sequences(cuda_device, n):
+    """More sequences than the plan keeps at hand: single tokens, empty ones, short prompts, a long cache."""
+    lens = [((7 * b) % 4, (37 * b) % 150) for b in range(n)]
+    lens[5], lens[n - 1] = (1, 3000), (90, 11)
+    s = make(lens, 8, 2, 64, seed=n)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_pools_past_32_bits(cuda_device):
+    """Pages whose offset passes 2^31 elements."""
+    s = make([(3, 700), (70, 100)], 8, 8, 128, seed=1)
+    blocks = 70000
+    big = torch.zeros((blocks, 2, 8, 16, 128), dtype=torch.float16, device=DEV)
+    big[blocks - s["nb"]:] = s["kv"]
+    s["tables"] = torch.where(s["tables"] >= 0, s["tables"] + (blocks - s["nb"]), -1).int()
+    s["kv"], s["nb"] = big, blocks
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_a_cut_range_of_which_a_tile_has_nothing(cuda_device):
+    """Pieces of the longest tile's range are empty for the first tiles."""
+    s = make([(2000, 0)], 8, 1, 128, seed=3)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_host_pointers_are_refused(cuda_device):
+    s = make([(3, 60)], 8, 2, 64)
+    ws = workspace(s)
+    host = torch.zeros(1 << 16, dtype=torch.float16)
+    for name in ("q", "kv", "out"):
+        t = dict(s)
+        t[name] = host.view(-1, s[name].shape[-1]) if name == "q" else host
+        if name == "out":
+            t["out"] = host[:3 * 8 * 64].view(3, 8, 64)
+        with pytest.raises(S.SpecdecError) as e:
+            call(t, ws)
+        assert e.value.code == S.EINVAL and "device" in str(e.value)
+    call(s, ws)
+    verify(s)

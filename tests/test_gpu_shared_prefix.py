@@ -213,3 +213,53 @@ def test_agrees_with_the_verify_attention(cuda_device):
                                       s["out"].data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream))
     verify(s, "specdec_attention")
     del ws
+
+
+def test_more_sequences_than_the_plan_keeps(cuda_device):
+    own = [(11 * b) % 90 for b in range(300)]
+    s = make([(120, 8), (3, 0), (150, 21), (1, 4)], own[:274], 3, 8, 2, 64, seed=4, alone=own[274:])
+    ws = call(s)
+    verify(s)
+    s = make([(1024, 3)], [b % 40 for b in range(1024)], 1, 4, 4, 64, seed=4)
+    ws2 = call(s)
+    verify(s)
+    del ws, ws2
+
+
+def test_new_rows_without_slots(cuda_device):
+    """A table that ends with the shared pages: the new rows' slots do not
+    exist, the rows see the prefix alone (and zeros where there is none)."""
+    s = make([(3, 6)], [0, 0, 0], 4, 8, 2, 64, seed=5, alone=(0,))
+    s["tables"] = s["tables"][:, :6].contiguous()
+    ws = call(s)
+    verify(s)
+    s["ctx_host"][3] = 6 * 16
+    s["ctx"][3] = 6 * 16
+    s["tables"][3] = s["tables"][0]
+    call(s, ws)
+    verify(s)
+
+
+def test_no_groups(cuda_device):
+    s = make([], [], 5, 8, 2, 64, seed=6, alone=(3, 40, 0, 700))
+    s["goff"] = s["pages"] = torch.empty(0, dtype=torch.int32, device=DEV)  # null pointers
+    assert s["goff"].data_ptr() == 0
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_groups_that_overlap_or_decrease_stay_in_bounds(cuda_device):
+    """Bounds that no caller should give: the call ends, and memory around the
+    workspace's and the output's is untouched."""
+    s = make([(2, 4), (2, 4)], [30, 5, 9, 100], 2, 8, 2, 64, seed=7)
+    need = S.lib().specdec_attention_shared_prefix_workspace_bytes(4, 2, 2, 8, 2, 64, s["tables"].shape[1])
+    ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=DEV)
+    for off in ([0, 4, 0], [3, 1, 4], [-5, 9, 2], [4, 4, 4], [0, 1 << 30, -1]):
+        s["goff"].copy_(torch.tensor(off))
+        call(s, ws[:need])
+        torch.cuda.synchronize()
+        assert bool((ws[need:] == 0x5A).all())
+    s["goff"].copy_(torch.tensor([0, 2, 4]))
+    call(s, ws[:need])
+    verify(s)
