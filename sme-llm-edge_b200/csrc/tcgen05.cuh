@@ -106,36 +106,4 @@ __host__ __device__ constexpr uint32_t idesc_f16_bmn(int M, int N) {
     return (1u << 4) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// The same for code that a whole warp runs: the lane with on != 0 issues.
-// Without a branch around them the operands stay in uniform registers and are
-// worked out there, so they may change from call to call.
-__device__ __forceinline__ void tc_mma_f16_ss_if(uint32_t on, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-        : "memory");
-}
-__device__ __forceinline__ void tc_mma_f16_ts_if(uint32_t on, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-        : "memory");
-}
-__device__ __forceinline__ void tc_commit_if(uint32_t on, uint32_t mbar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "setp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar),
-        "r"(on)
-        : "memory");
-}
-
 }  // namespace specdec
