@@ -1152,14 +1152,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 }
 
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
-// their order.  One warp per token row and head; a lane holds HD / 32
-// neighbouring columns, and the loads of eight pieces are in flight together
-// (one piece after the other took 18 to 34 us where this takes 4 to 18).  The
-// CTAs go round the rows: one for each row cost 12 us where no row has pieces.
+// their order, M being the largest so far.  Bound by L2 and by latency (where the
+// pieces lie, then their results: two loads that wait for one another).  Eight
+// lanes per token row and head; (m, l) and O of four pieces are in flight
+// together, O too before its weight is known.  Against a warp for each row, that
+// first shares out all weights: 128 x 5 rows under 8192 tokens 171 -> 162 us a
+// call, 16 x 21 under 2048 61 -> 57; two or eight pieces at a time, or 16 lanes a
+// row, gain in one case what they lose in another.  The CTAs go round the rows:
+// one for every few rows cost 12 us where no row has pieces.
 template <int HD>
 __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int head) {
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31;
+    constexpr int K = HD / 32, P = 4;  // 16-byte pieces of a lane's columns; pieces at a time
+    const int lane = threadIdx.x & 7;
     int b, i;
     if (a.row_off) {
         int lo = 0, hi = a.B;  // first sequence whose end is past tok
@@ -1174,67 +1178,76 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
         if (i < 0) return;
     } else {
         b = tok / a.R;
-        i = tok % a.R;
+        i = tok - b * a.R;
     }
     const RowsMeta mt = a.meta[b];
     const int n = mt.n_pre + mt.n_own;
     if (n == 0) return;
-    auto at = [&](int p) -> size_t {
-        const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
-        return (size_t)min(r + i, a.prows - 1) * a.Hq + head;  // group bounds that overlap: never out of range
-    };
-    // up to 64 pieces: two a lane
-    float2 ml[2];
+    float M = -INFINITY, l = 0.f;
+    float o[K][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) ml[u] = lane + 32 * u < n ? a.pml[at(lane + 32 * u)] : make_float2(-INFINITY, 0.f);
-    const float M = warp_max(fmaxf(ml[0].x, ml[1].x));
-    const float sub = M == -INFINITY ? 0.f : M;
-    const float w0 = exp2f(ml[0].x - sub), w1 = exp2f(ml[1].x - sub);
-    const float l = warp_sum(w0 * ml[0].y + w1 * ml[1].y);
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-    float o[E];
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int p0 = 0; p0 < n; p0 += 8) {
-        float v[8][E], w[8];
+        for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
+#pragma unroll 1
+    for (int p0 = 0; p0 < n; p0 += P) {
+        float2 ml[P];
+        float4 v[P][K];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int p = p0 + u;
-            w[u] = __shfl_sync(0xffffffffu, p & 32 ? w1 : w0, p & 31);
-            if (p >= n) w[u] = 0.f;
-            if (w[u] != 0.f) {  // a piece of no weight may hold nothing
-                const float* src = a.po + at(p) * HD + lane * E;
-                if (E == 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(src);
-                    v[u][0] = x.x, v[u][1] = x.y, v[u][E - 2] = x.z, v[u][E - 1] = x.w;
-                } else {
-                    const float2 x = *reinterpret_cast<const float2*>(src);
-                    v[u][0] = x.x, v[u][1] = x.y;
-                }
+        for (int u = 0; u < P; ++u) {
+            const int p = min(p0 + u, n - 1);
+            const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
+            const size_t at = (size_t)min(r + i, a.prows - 1) * a.Hq + head;  // bounds that overlap: never out of range
+            ml[u] = a.pml[at];
+            if (p0 + u >= n) ml[u] = make_float2(-INFINITY, 0.f);
+            const float4* src = reinterpret_cast<const float4*>(a.po + at * HD) + lane;
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[u][k] = src[8 * k];
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < P; ++u) top = fmaxf(top, ml[u].x);
+        const float sub = top == -INFINITY ? 0.f : top;
+        const float f = exp2f(M - sub);
+        M = top;
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][e] *= f;
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+            const float w = exp2f(ml[u].x - sub);
+            if (w == 0.f) continue;  // a piece of no weight may hold anything
+            l += w * ml[u].y;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                o[k][0] += w * v[u][k].x;
+                o[k][1] += w * v[u][k].y;
+                o[k][2] += w * v[u][k].z;
+                o[k][3] += w * v[u][k].w;
             }
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (w[u] != 0.f)
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] += w[u] * v[u][e];
     }
-    alignas(8) __half h[E];
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + 4 * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = __float2half_rn(o[e] * inv);
-    __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * E;
-    if (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
-    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
+    for (int k = 0; k < K; ++k) {
+        alignas(8) __half h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __float2half_rn(o[k][e] * inv);
+        *reinterpret_cast<uint2*>(dst + 32 * k) = *reinterpret_cast<const uint2*>(h);
+    }
 }
 
 template <int HD>
 __global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
     pdl_wait();
     if (*a.any_parts == 0) return;
-    const int groups = (a.Hq + 7) / 8;  // of 8 heads
-    for (int u = blockIdx.x; u < a.T * groups; u += gridDim.x) {
-        const int tok = u / groups, head = (u - tok * groups) * 8 + (threadIdx.x >> 5);
-        if (head < a.Hq) rows_merge_row<HD>(a, tok, head);
+    const int rows = a.T * a.Hq;
+    for (int r = blockIdx.x * 32 + (threadIdx.x >> 3); r < rows; r += gridDim.x * 32) {
+        const int tok = r / a.Hq;
+        rows_merge_row<HD>(a, tok, r - tok * a.Hq);
     }
 }
 
@@ -1338,7 +1351,7 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     SD_LAUNCH_CHECK("rows_attention_kernel");
     if (prows) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)std::min<long long>((long long)a.T * ((a.Hq + 7) / 8), 8LL * sms));
+        cfg.gridDim = dim3((unsigned)std::min<long long>(((long long)a.T * a.Hq + 31) / 32, 8LL * sms));
         cfg.blockDim = dim3(256);
         cfg.stream = s;
         cudaLaunchAttribute at[1];
