@@ -35,9 +35,10 @@ int cuda_status(cudaError_t e, const char* what);
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
-// SPECDEC_EINVAL unless p is memory of the current device (or managed): a host
-// pointer or another device's would fault in a kernel.
-int check_on_device(const void* p, const char* what);
+// SPECDEC_EINVAL unless p is memory of the current device (or managed) and
+// aligned to `align` bytes: a host pointer, another device's or a misaligned one
+// would fault in a kernel.
+int check_on_device(const void* p, const char* what, size_t align = 4);
 
 // Device-side error word (bounded waits that give up record here).
 struct DeviceStatus {

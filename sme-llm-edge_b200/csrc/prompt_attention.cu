@@ -1324,6 +1324,12 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     if (!rc) rc = check_on_device(kv, "attention: the KV pool");
     if (!rc) rc = check_on_device(a.out, "attention: out");
     if (!rc) rc = check_on_device(ws, "attention: the workspace");
+    if (!rc) rc = check_on_device(a.tables, "attention: tables");
+    if (!rc) rc = check_on_device(a.ctx_len, "attention: ctx_len");
+    if (!rc && a.row_off) rc = check_on_device(a.row_off, "attention: row_off");
+    if (!rc && a.mask) rc = check_on_device(a.mask, "attention: mask", sizeof(uint64_t));
+    if (!rc && a.n_groups) rc = check_on_device(a.group_off, "attention: group_off");
+    if (!rc && a.n_groups) rc = check_on_device(a.shared_blocks, "attention: shared_blocks");
     if (rc) return rc;
     a.G = a.Hq / a.Hkv;
     a.tpt = 128 / a.G;

@@ -17,7 +17,9 @@ int cuda_status(cudaError_t e, const char* what) {
     return e == cudaErrorMemoryAllocation ? SPECDEC_ENOMEM : SPECDEC_ECUDA;
 }
 
-int check_on_device(const void* p, const char* what) {
+int check_on_device(const void* p, const char* what, size_t align) {
+    SD_CHECK(reinterpret_cast<uintptr_t>(p) % align == 0, SPECDEC_EINVAL,
+             std::string(what) + " is not aligned to " + std::to_string(align) + " bytes");
     cudaPointerAttributes at = {};
     int dev = 0;
     SD_CUDA(cudaGetDevice(&dev));

@@ -312,3 +312,20 @@ def test_host_pointers_are_refused(cuda_device):
     g.fork([0], [2])
     torch.cuda.synchronize()
     assert int(g.status) == S.OK
+
+
+def test_host_tables_are_refused(cuda_device):
+    g = OnGpu(*make({0: 20}, 3, 8, 4))
+    for i in range(4):
+        g.t[i], keep = g.t[i].cpu(), g.t[i]
+        with pytest.raises(S.SpecdecError) as e:
+            g.fork([0], [1])
+        assert e.value.code == S.EINVAL and "device" in str(e.value)
+        g.t[i] = keep
+    need = S.lib().specdec_kv_fork_pages_workspace_bytes(8, 3, 1)
+    with pytest.raises(S.SpecdecError) as e:
+        g.fork([0], [1], ws=torch.zeros(need, dtype=torch.uint8))
+    assert e.value.code == S.EINVAL and "device" in str(e.value)
+    g.fork([0], [2])
+    torch.cuda.synchronize()
+    assert int(g.status) == S.OK and int(g.t[2][2]) == 20

@@ -316,3 +316,17 @@ def test_host_pointers_are_refused(cuda_device):
         assert e.value.code == S.EINVAL and "device" in str(e.value)
     call(s, ws)
     verify(s)
+
+
+@pytest.mark.parametrize("name", ["tables", "ctx", "off"])
+def test_host_tables_and_lengths_are_refused(cuda_device, name):
+    s = make([(3, 60), (1, 400)], 8, 2, 64)
+    with pytest.raises(S.SpecdecError) as e:
+        call(dict(s, **{name: s[name].cpu()}))
+    assert e.value.code == S.EINVAL and "device" in str(e.value)
+    with pytest.raises(S.SpecdecError) as e:
+        call(s, workspace(s).cpu())
+    assert e.value.code == S.EINVAL and "device" in str(e.value)
+    ws = call(s)
+    verify(s)
+    del ws

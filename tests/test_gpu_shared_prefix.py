@@ -263,3 +263,30 @@ def test_groups_that_overlap_or_decrease_stay_in_bounds(cuda_device):
     s["goff"].copy_(torch.tensor([0, 2, 4]))
     call(s, ws[:need])
     verify(s)
+
+
+@pytest.mark.parametrize("name", ["tables", "ctx", "mask", "goff", "pages"])
+def test_host_pointers_are_refused(cuda_device, name):
+    s = make([(3, 4)], [5, 20, 40], 2, 8, 2, 64)
+    with pytest.raises(S.SpecdecError) as e:
+        call(dict(s, **{name: s[name].cpu()}))
+    assert e.value.code == S.EINVAL and "device" in str(e.value)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_misaligned_pointers_are_refused(cuda_device):
+    s = make([(3, 4)], [5, 20, 40], 2, 8, 2, 64)
+    ws = workspace(s)
+    for at, step in ((5, 2), (7, 2), (8, 4), (9, 2), (10, 2)):  # tables, ctx_len, mask, group_off, shared_blocks
+        args = [s["q"].data_ptr(), s["kv"].data_ptr(), s["nb"], s["Hkv"], s["hd"], s["tables"].data_ptr(),
+                s["tables"].shape[1], s["ctx"].data_ptr(), s["mask"].data_ptr(), s["goff"].data_ptr(),
+                s["pages"].data_ptr(), s["ng"], s["B"], s["R"], s["Hq"], s["out"].data_ptr(), ws.data_ptr(),
+                ws.numel(), torch.cuda.current_stream().cuda_stream]
+        args[at] += step
+        with pytest.raises(S.SpecdecError) as e:
+            S.check(S.lib().specdec_attention_shared_prefix(*args))
+        assert e.value.code == S.EINVAL and "aligned" in str(e.value)
+    call(s, ws)
+    verify(s)
