@@ -6,9 +6,9 @@
 // copy's slot held before are released first.  Either all forks of a call
 // happen or none.
 //
-// Two launches: the tables by one cluster of 8 CTAs (its phases need a barrier,
-// not a grid: the tables of 48 copies of 1500 tokens are 4,500 entries), then
-// the copies by one CTA for each (copy, layer).  Bound by latency for few
+// Two launches: the tables by one CTA or one cluster of 8 (the phases need a
+// barrier, not a grid: the tables of 48 copies of 1500 tokens are 4,500 entries),
+// then the copies by one CTA for each (copy, layer).  Bound by latency for few
 // copies and by the copies' bytes for many: only the rows in use move, each as
 // runs of 16 * head_dim bytes or more.
 #include "common.cuh"
@@ -17,6 +17,7 @@
 
 namespace specdec {
 
+constexpr int kForkSmall = 2048;  // table entries and blocks of a call that one CTA works on
 constexpr int kForkCtas = 8, kForkThreads = 512, kForkWarps = kForkThreads / 32;
 
 struct ForkArgs {
@@ -58,73 +59,102 @@ __device__ int fork_scan(int v, int* sh, int* total) {
     return before + x - v;
 }
 
-__global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads) kv_fork_kernel(ForkArgs a) {
-    __shared__ int sh[kForkWarps];
+template <int CTAS>
+__device__ __forceinline__ void fork_sync() {
+    if constexpr (CTAS > 1) cluster_sync_all();
+    else __syncthreads();
+}
+
+template <int CTAS>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kForkThreads) kv_fork_kernel(ForkArgs a) {
+    __shared__ int sh[kForkWarps], ranks[kForkThreads];
     const int cta = blockIdx.x, tid = threadIdx.x;
-    const int gt = cta * kForkThreads + tid, stride = kForkCtas * kForkThreads;
+    const int gt = cta * kForkThreads + tid, stride = CTAS * kForkThreads;
     const int bs = a.block_size;
     // Every check of the arguments reads what the call does not change yet, so one
     // barrier stands between the checks and the first change; refw is a copy.
     // Ids in range, targets distinct and no sources, sources with a table that
-    // holds their tokens.  A group of the cluster's 128 warps to each copy (one
-    // copy after the other in a CTA took most of 23 us for 48).
-    const int warps = kForkCtas * kForkWarps, gw = gt >> 5, lane = tid & 31;
+    // holds their tokens.  A group of the cluster's warps to each copy (one copy
+    // after the other in a CTA took most of 23 us for 48).
+    const int warps = CTAS * kForkWarps, gw = gt >> 5, lane = tid & 31;
     const int group = max(1, warps / max(1, a.n)), groups = warps / group;
     const int mine = gw / group, part = gw % group * 32 + lane, step = group * 32;
     const int first = mine < groups ? mine : a.n;
     auto leave = [&](int code) {
         if (cta == 0 && tid == 0) *a.status = code;
     };
+    // A call waits for its loads, one round behind the other, far longer than it
+    // computes: what does not depend on one another is loaded together, and what a
+    // group knows of its first copy (most often its only one) it keeps.
+    struct Copy {
+        int s, d, have, L, old;  // source, target, source's blocks and tokens, target's blocks
+    };
+    auto ids_ok = [&](int s, int d) { return s >= 0 && s < a.max_reqs && d >= 0 && d < a.max_reqs; };
+    auto load = [&](int i) {
+        Copy c = {a.src[i], a.dst[i], -1, 0, -1};
+        if (ids_ok(c.s, c.d)) {
+            c.have = a.nblk[c.s];
+            c.L = a.len[c.s];
+            c.old = a.nblk[c.d];
+        }
+        return c;
+    };
+    const int scan_s = tid < a.n ? a.src[tid] : -1, ref0 = gt < a.num_blocks ? a.ref[gt] : 0;
+    Copy kept = {-1, -1, -1, 0, -1};
+    if (first < a.n) kept = load(first);
+    const int scan_L = scan_s >= 0 && scan_s < a.max_reqs ? a.len[scan_s] : 0;
+    auto copy = [&](int i) { return i == first ? kept : load(i); };
     bool bad = false;
     for (int i = first; i < a.n; i += groups) {
-        const int s = a.src[i], d = a.dst[i];
-        if (s < 0 || s >= a.max_reqs || d < 0 || d >= a.max_reqs) {
+        const Copy c = copy(i);
+        if (!ids_ok(c.s, c.d)) {
             bad = true;
             continue;
         }
+        const int use = c.L < 0 ? 0 : (int)(((long long)c.L + bs - 1) / bs);
+        const bool fits = c.have >= 0 && c.have <= a.max_bpr && c.old <= a.max_bpr && c.L >= 0 && use <= c.have;
+        bad |= !fits;
         for (int j = part; j < a.n; j += step) {
             const int e = a.dst[j];
-            bad |= e == s || (e == d && j != i);
+            bad |= e == c.s || (e == c.d && j != i);
         }
-        const int ns = a.nblk[s], L = a.len[s];
-        const int use = L < 0 ? 0 : (int)(((long long)L + bs - 1) / bs);
-        bad |= ns < 0 || ns > a.max_bpr || a.nblk[d] > a.max_bpr || L < 0 || use > ns;
-        if (!bad)
+        if (fits)
             for (int j = part; j < use; j += step) {
-                const int p = a.tables[(size_t)s * a.max_bpr + j];
+                const int p = a.tables[(size_t)c.s * a.max_bpr + j];
                 bad |= p < 0 || p >= a.num_blocks;
             }
     }
-    // the copies that need a block, in order (every CTA counts; CTA 0 writes the ranks)
+    // the copies that need a block, in order (every CTA counts; CTA 0 writes the ranks behind the first 512)
     int need = 0;
     for (int i0 = 0; i0 < a.n; i0 += kForkThreads) {
         const int i = i0 + tid;
-        const int s = i < a.n ? a.src[i] : -1;
-        const int t = s >= 0 && s < a.max_reqs && a.len[s] % bs != 0;
+        const int s = i0 == 0 ? scan_s : (i < a.n ? a.src[i] : -1);
+        const int t = s >= 0 && s < a.max_reqs && (i0 == 0 ? scan_L : a.len[s]) % bs != 0;
         int tot;
-        const int before = fork_scan(t, sh, &tot);
-        if (cta == 0 && i < a.n) a.rank[i] = t ? need + before : -1;
+        const int before = fork_scan(t, sh, &tot), r = t ? need + before : -1;
+        if (i0 == 0) ranks[tid] = r;
+        else if (cta == 0 && i < a.n) a.rank[i] = r;
         need += tot;
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) a.head[cta] = bad;
     if (gt == 0) a.head[kForkCtas] = 0;  // pairs to copy
-    for (int i = gt; i < a.num_blocks; i += stride) a.refw[i] = a.ref[i];
-    cluster_sync_all();
+    for (int i = gt; i < a.num_blocks; i += stride) a.refw[i] = i == gt ? ref0 : a.ref[i];
+    fork_sync<CTAS>();
     int any = 0;
-    for (int c = 0; c < kForkCtas; ++c) any |= __ldcg(&a.head[c]);
+    for (int c = 0; c < CTAS; ++c) any |= __ldcg(&a.head[c]);
     if (any) return leave(SPECDEC_EINVAL);
     // the targets' old blocks are released
     for (int i = first; i < a.n; i += groups) {
-        const int d = a.dst[i], nd = a.nblk[d];
-        for (int j = part; j < nd; j += step) {
-            const int p = a.tables[(size_t)d * a.max_bpr + j];
+        const Copy c = copy(i);
+        for (int j = part; j < c.old; j += step) {
+            const int p = a.tables[(size_t)c.d * a.max_bpr + j];
             if (p >= 0 && p < a.num_blocks) atomicSub(&a.refw[p], 1);
         }
     }
-    cluster_sync_all();
+    fork_sync<CTAS>();
     // the lowest free blocks: each CTA takes a range, its threads neighbouring pieces of it
-    const int per_cta = (a.num_blocks + kForkCtas - 1) / kForkCtas;
+    const int per_cta = (a.num_blocks + CTAS - 1) / CTAS;
     const int b0 = min(a.num_blocks, cta * per_cta), b1 = min(a.num_blocks, b0 + per_cta);
     const int per = (b1 - b0 + kForkThreads - 1) / kForkThreads;
     const int lo = min(b1, b0 + tid * per), hi = min(b1, lo + per);
@@ -133,9 +163,9 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
     int here;
     int before = fork_scan(cnt, sh, &here);
     if (tid == 0) a.head[16 + cta] = here;
-    cluster_sync_all();
+    fork_sync<CTAS>();
     int total = 0;
-    for (int c = 0; c < kForkCtas; ++c) {
+    for (int c = 0; c < CTAS; ++c) {
         const int x = __ldcg(&a.head[16 + c]);
         if (c < cta) before += x;
         total += x;
@@ -144,10 +174,11 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
     if (before < need)
         for (int b = lo; b < hi && before < need; ++b)
             if (__ldcg(&a.refw[b]) == 0) a.fresh[before++] = b;
-    cluster_sync_all();
+    fork_sync<CTAS>();
     // tables, lengths and counts of the copies
     for (int i = first; i < a.n; i += groups) {
-        const int s = a.src[i], d = a.dst[i], L = a.len[s], whole = L / bs, r = __ldcg(&a.rank[i]);
+        const Copy c = copy(i);
+        const int s = c.s, d = c.d, L = c.L, whole = L / bs, r = i < kForkThreads ? ranks[i] : __ldcg(&a.rank[i]);
         const int page = r >= 0 ? __ldcg(&a.fresh[r]) : -1;
         int32_t* to = a.tables + (size_t)d * a.max_bpr;
         const int32_t* from = a.tables + (size_t)s * a.max_bpr;
@@ -172,7 +203,7 @@ __global__ void __cluster_dims__(kForkCtas, 1, 1) __launch_bounds__(kForkThreads
             }
         }
     }
-    cluster_sync_all();
+    fork_sync<CTAS>();
     for (int i = gt; i < a.num_blocks; i += stride) a.ref[i] = __ldcg(&a.refw[i]);
     if (gt == 0) {
         a.head[kForkCtas] = need;
@@ -229,7 +260,10 @@ int kv_fork_launch(const KVState& st, const int32_t* src, const int32_t* dst, in
     a.rank = a.refw + st.num_blocks;
     a.fresh = a.rank + n;
     a.pair = a.fresh + n;
-    kv_fork_kernel<<<kForkCtas, kForkThreads, 0, s>>>(a);
+    // Few entries: one CTA, whose barriers cost little (4 copies of 205 tokens in a pool of 256 blocks: 8.0 us a call,
+    // a cluster 10.6; 8 of 1500 in 2048: 11.7 and 11.9; 16 of 1500 in 4096: 15.4 and 12.2).
+    if ((long long)n * st.max_bpr + st.num_blocks <= kForkSmall) kv_fork_kernel<1><<<1, kForkThreads, 0, s>>>(a);
+    else kv_fork_kernel<kForkCtas><<<kForkCtas, kForkThreads, 0, s>>>(a);
     SD_LAUNCH_CHECK("kv_fork_kernel");
     if (kv && layers > 0) {
         cudaLaunchConfig_t cfg = {};

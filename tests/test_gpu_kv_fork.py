@@ -329,3 +329,13 @@ def test_host_tables_are_refused(cuda_device):
     g.fork([0], [2])
     torch.cuda.synchronize()
     assert int(g.status) == S.OK and int(g.t[2][2]) == 20
+
+
+@pytest.mark.parametrize("state,src,dst", CASES)
+def test_wide_tables(cuda_device, state, src, dst):
+    """The same calls on tables that one CTA does not work on alone."""
+    st = make(**dict(state, max_blocks=2500))
+    g = OnGpu(*st)
+    status = plain_fork(*st[:4], src, dst, st[4])
+    g.fork(src, dst)
+    g.same(*st, status)
