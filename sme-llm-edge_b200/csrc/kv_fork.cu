@@ -317,13 +317,20 @@ extern "C" int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t
                  (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
              SPECDEC_EINVAL, "kv_fork_pages: workspace too small or not 4-byte aligned");
     cudaStream_t s = as_stream(stream);
-    if ((rc = check_on_device(tables, "kv_fork_pages: tables")) ||
-        (rc = check_on_device(n_blocks, "kv_fork_pages: n_blocks")) || (rc = check_on_device(lens, "kv_fork_pages: lens")) ||
-        (rc = check_on_device(refcounts, "kv_fork_pages: refcounts")) || (n && (rc = check_on_device(src, "kv_fork_pages: src"))) ||
-        (n && (rc = check_on_device(dst, "kv_fork_pages: dst"))) || (rc = check_on_device(status, "kv_fork_pages: status")) ||
-        (rc = check_on_device(workspace, "kv_fork_pages: the workspace")) ||
-        (layers > 0 && (rc = check_on_device(kv, "kv_fork_pages: the pool"))))
-        return rc;
+    const struct {
+        const void* p;
+        const char* what;
+    } given[] = {{tables, "kv_fork_pages: tables"},
+                 {n_blocks, "kv_fork_pages: n_blocks"},
+                 {lens, "kv_fork_pages: lens"},
+                 {refcounts, "kv_fork_pages: refcounts"},
+                 {status, "kv_fork_pages: status"},
+                 {workspace, "kv_fork_pages: the workspace"},
+                 {n ? src : tables, "kv_fork_pages: src"},
+                 {n ? dst : tables, "kv_fork_pages: dst"},
+                 {layers ? (const void*)kv : tables, "kv_fork_pages: the pool"}};
+    for (const auto& g : given)
+        if ((rc = check_on_device(g.p, g.what))) return rc;
     if (n == 0) {
         SD_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), s));
         return SPECDEC_OK;

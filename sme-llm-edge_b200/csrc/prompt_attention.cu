@@ -319,7 +319,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         __syncthreads();
     }
     // pieces of about a quarter of a CTA's share; of half of it where they have many rows (128 x 5 rows under 8192
-    // tokens: 171 us, with a quarter 181)
+    // tokens: 158 us, with a third 168, with three quarters 179)
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
@@ -520,8 +520,7 @@ __device__ __forceinline__ float rows_max3(float a, float b, float c) {
 }
 // 2^x on the special-function unit (2 ulp); the result is rounded to fp16 next.
 // A quarter of them by a polynomial on the FMA units instead cost 5% (8192-token
-// prompt 559 us against 532): a softmax warp is bound by the instructions that
-// it issues, not by that unit.
+// prompt 559 us against 532): that unit is 44% busy there, and the code grows.
 __device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
     float x0, x1, y0, y1;
     unpack2(x, x0, x1);
@@ -529,6 +528,7 @@ __device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
     return pack2(y0, y1);
 }
+
 // A row's O times f.
 template <int HD>
 __device__ __forceinline__ void rows_rescale(uint32_t t_o, float f) {
@@ -542,6 +542,7 @@ __device__ __forceinline__ void rows_rescale(uint32_t t_o, float f) {
         tc_st_x16(t_o + c0, ov);
     }
 }
+
 // The CTA's barriers, in shared memory.
 template <int RING>
 struct RowsBars {
@@ -554,8 +555,19 @@ struct RowsBars {
     uint64_t *i_full, *i_empty;  // [kRowsItems] empty: 8 softmax warps, the MMA issuer, loads, fix
     uint64_t* i_want;            // the loads of an item are nearly out: the next is wanted
     __device__ explicit RowsBars(uint64_t* b)
-        : q_full(b), q_empty(b + 2), s_full(b + 4), p_full(b + 6), o_full(b + 8), k_full(b + 10), k_empty(k_full + RING), v_raw(k_empty + RING), v_full(v_raw + RING), v_empty(v_full + RING),
-          i_full(v_empty + RING), i_empty(i_full + kRowsItems), i_want(i_empty + kRowsItems) {}
+        : q_full(b),
+          q_empty(b + 2),
+          s_full(b + 4),
+          p_full(b + 6),
+          o_full(b + 8),
+          k_full(b + 10),
+          k_empty(k_full + RING),
+          v_raw(k_empty + RING),
+          v_full(v_raw + RING),
+          v_empty(v_full + RING),
+          i_full(v_empty + RING),
+          i_empty(i_full + kRowsItems),
+          i_want(i_empty + kRowsItems) {}
 };
 
 // The MMA issuer.  P.V of operation i and Q.K^T of operation i + 2 on the same
@@ -983,8 +995,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             tc_fence_before();  // O was read before the slot's next P is announced
             done_item(k);
         }
-    } else {
-    if (warp == kRowsSchedWarp) {
+    } else if (warp == kRowsSchedWarp) {
         // ------------------------------------------------------------ scheduler
         // The items that it passes on have at least one operation: the MMA
         // issuer may wait for an item while operations of the one before are
@@ -1146,7 +1157,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
     } else if (warp == kRowsMmaWarp) {
         rows_mma<HD>(a, items, tmem, s_addr(sQ), s_addr(sK), s_addr(sV), bars, abort_flag);
-    }
     }
     tc_fence_before();
     __syncthreads();
