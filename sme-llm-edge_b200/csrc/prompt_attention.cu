@@ -179,10 +179,6 @@ __device__ __forceinline__ int rows_item_end(const RowsArgs& a, const RowsSeg& s
 __device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s, int p) {
     return (rows_item_end(a, s, p) - s.base + 127) / 128;
 }
-// A segment of one tile and several key tiles is worked on as duals.
-__device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s) {
-    return a.prows > 0 && s.n <= a.tpt && s.kt >= 2;
-}
 // How long the pieces of a key range are, in key tiles: about `fine` where there
 // are few rows (memory-bound: partial results are small), about `coarse`
 // elsewhere.  A segment of many rows is cut only where one range is more than a
@@ -191,16 +187,21 @@ __device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s) {
 struct RowsCut {
     float per_fine, per_coarse;  // reciprocals
     int whole;
+    bool duals;
 };
+// A segment of one tile and several key tiles is worked on as duals.
+__device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
+    return cut.duals && s.n <= a.tpt && s.kt >= 2;
+}
 __device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
     const int S = s.n <= 64 / a.G ? (int)ceilf((float)s.kt * cut.per_fine)
                                   : (s.kt <= cut.whole ? 1 : (int)rintf((float)s.kt * cut.per_coarse));
-    const int most = rows_dual(a, s) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
+    const int most = rows_dual(a, s, cut) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
     return rows_clamp(S, 1, max(1, most));
 }
 // Results of the segment's rows to join: 0 where the item's own is final.
-__device__ __forceinline__ int rows_parts(const RowsArgs& a, const RowsSeg& s, int S) {
-    return rows_dual(a, s) ? 2 * S : (s.mode == kModeAll || S > 1 || s.base > 0 ? S : 0);
+__device__ __forceinline__ int rows_parts(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut, int S) {
+    return rows_dual(a, s, cut) ? 2 * S : (s.mode == kModeAll || S > 1 || s.base > 0 ? S : 0);
 }
 
 // False only for group bounds that overlap: what would not fit is left out.
@@ -323,7 +324,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
-                   (int)fminf(1.1f * mean, (float)(1 << 26))};
+                   (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows > 0};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
     for (int round = 0;; ++round) {
         int items = 0, prows = 0;
@@ -331,18 +332,19 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
             const int S = rows_splits(a, s, cut);
             items += s.tiles * S;
-            prows += s.n * rows_parts(a, s, S);
+            prows += s.n * rows_parts(a, s, cut, S);
         }
         rows_scan2(p, items, prows, &item0, &prow0, &tot_items, &tot_prows);
         if (tot_prows <= a.prows || round >= 8) break;
-        // fewer pieces until their results fit; at last one a segment, which always does
+        // fewer pieces until their results fit; at last one a segment and no duals, which always does
         cut.per_fine = round == 7 ? none : 0.5f * cut.per_fine;
         cut.per_coarse = round == 7 ? none : 0.5f * cut.per_coarse;
+        cut.duals = round < 7;
     }
     for (int i = s0; i < s1; ++i) {
         const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
         const int S = rows_splits(a, s, cut);
-        const int parts = rows_parts(a, s, S);
+        const int parts = rows_parts(a, s, cut, S);
         p.pre[i] = item0;
         p.prow[i] = prow0;
         if (small) p.splits[i] = S;
@@ -393,7 +395,7 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     const int local = r - p.pre[lo];
     const int along = S == 1 ? local : local / S;
     const int tile = s.tiles - 1 - along, piece = local - along * S;  // the longest first
-    const int parts = rows_parts(a, s, S);
+    const int parts = rows_parts(a, s, p.cut, S);
     if (local < 0 || tile < 0 || (parts && !rows_fit(a, s, parts, p.prow[lo]))) {  // bounds that overlap: an empty item
         it.n_kt = it.ntok0 = it.ntok1 = 0;
         it.kind = kDual;
@@ -414,8 +416,8 @@ __device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p,
     it.ctx = s.ctx;
     it.mode = s.mode;
     it.scan = s.mode == kModeCausal ? s.ctx + it.i0 + 1 : (s.mode == kModeMask ? s.ctx : it.end);
-    it.kind = rows_dual(a, s) || (it.ntok1 == 0 && it.n_kt <= 1) ? kDual : kPair;
-    it.pnext = rows_dual(a, s) ? s.n : 0;
+    it.kind = rows_dual(a, s, p.cut) || (it.ntok1 == 0 && it.n_kt <= 1) ? kDual : kPair;
+    it.pnext = rows_dual(a, s, p.cut) ? s.n : 0;
     it.prow = parts ? p.prow[lo] + piece * (parts > S ? 2 : 1) * s.n + it.i0 : -1;
     return it;
 }
@@ -1283,15 +1285,19 @@ static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq
     return SPECDEC_OK;
 }
 
-constexpr int kRowsSplitTokens = 4096;   // prompts of more rows fill the GPU without splits
-constexpr int kRowsPartialRows = 8192;   // room for their pieces, in token rows (two for each row at least)
+constexpr int kRowsSplitTokens = 4096;   // calls of more rows fill the GPU, but for long ranges of few rows among them
+constexpr int kRowsPartialRows = 8192;   // room for pieces, in token rows (two for each row at least)
+constexpr int kRowsPartialMany = 2048;   // the same in calls of more rows
 constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece of every range
 
 // Rows of the partial buffers.
 // Tables of up to 256 slots have two key tiles: no pieces, and no merge behind
 // them (a single row on 40 slots: 14.9 us a call with its launch, 12.2 without).
-static size_t prompt_partial_rows(int T, int max_blocks) {
-    return T <= kRowsSplitTokens && max_blocks > 16 ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : 0;
+// In calls of many rows there is room for those of short segments: a single token
+// on 100,000 slots beside 6000 rows of prompts: 1,529 us without pieces, 373 with.
+static size_t prompt_partial_rows(int T, int Hq, int max_blocks) {
+    if (max_blocks <= 16 || (long long)T * Hq >= 1 << 30) return 0;
+    return T <= kRowsSplitTokens ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : kRowsPartialMany;
 }
 static size_t shared_partial_rows(int T) {
     // prefix and own range of every row, each of which may be a dual
@@ -1415,7 +1421,7 @@ extern "C" size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q
                                                            int max_blocks) {
     (void)n_kv_heads;
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
-    return rows_workspace(prompt_partial_rows(T, max_blocks), B, n_q_heads, head_dim);
+    return rows_workspace(prompt_partial_rows(T, n_q_heads, max_blocks), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1430,7 +1436,7 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
     SD_CHECK(ldq >= n_q_heads * head_dim && ldq % 8 == 0 && ldo >= n_q_heads * head_dim && ldo % 8 == 0,
              SPECDEC_EINVAL, "attention_prompt: row strides hold all heads and are multiples of 8");
     if (B == 0 || T == 0) return SPECDEC_OK;
-    const size_t prows = prompt_partial_rows(T, max_blocks);
+    const size_t prows = prompt_partial_rows(T, n_q_heads, max_blocks);
     if ((rc = check_workspace("attention_prompt", workspace, workspace_bytes,
                               rows_workspace(prows, B, n_q_heads, head_dim))))
         return rc;

@@ -330,3 +330,16 @@ def test_host_tables_and_lengths_are_refused(cuda_device, name):
     ws = call(s)
     verify(s)
     del ws
+
+
+@pytest.mark.parametrize("lens", [
+    [(4700, 0), (1, 30000), (3, 2000), (0, 50), (1, 5)],
+    [(7, 300)] * 700,  # as many results as there is no room for
+    [(1, 3000)] * 60 + [(4200, 100)] + [(1, 700)] * 70,
+])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)])
+def test_long_ranges_of_few_rows_beside_many(cuda_device, lens, heads):
+    s = make(lens, *heads, seed=5)
+    ws = call(s)
+    verify(s)
+    del ws
