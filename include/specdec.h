@@ -317,15 +317,15 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
  * 0 .. ctx_len[b] + i.  q [T, Hq, hd] and out [T, Hq, hd] fp16 with row
  * strides ldq / ldo in elements (multiples of 8, so q may lie in the fused
  * QKV rows); T = rows of the buffers.  A sequence may have no rows; rows
- * behind row_off[B] are neither read nor written.  Slots a row does not see
- * may hold anything (NaN and infinities too), pages past the last slot are
- * not read; slots past max_blocks * 16 do not exist; a table entry outside
- * the pool reads block 0.  Up to 1024 sequences.  Long key ranges are split
- * across CTAs and merged through the workspace in a fixed order (the result
- * is deterministic); calls in flight at the same time, captured graphs
+ * behind row_off[B] may hold anything and stay as they are.  Slots a row does
+ * not see may hold anything (NaN and infinities too), pages past the last
+ * slot are not read; slots past max_blocks * 16 do not exist; a table entry
+ * outside the pool reads block 0.  Up to 1024 sequences.  Long key ranges are
+ * split across CTAs and merged through the workspace in a fixed order (the
+ * result is deterministic); calls in flight at the same time, captured graphs
  * among them, need workspaces (32-byte aligned) of their own.  All pointers
- * are memory of the current device.  The first call on a device
- * comes before any stream capture.  The reference feeds prompts in chunks
+ * are memory of the current device.  The first call on a device comes before
+ * any stream capture.  The reference feeds prompts in chunks
  * (server/chunked_prefill.cpp:4-24) through one row of attention at a time
  * (server/paged_attention.cpp:16-111). */
 size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
