@@ -256,12 +256,14 @@ __device__ __forceinline__ void rows_scan2(RowsPlan& p, int va, int vb, int* bef
 // Every CTA makes the same plan from the lengths in device memory (so a
 // captured call serves other lengths); CTA 0 writes where the partials lie.  It
 // is on every call's path: lengths and bounds are loaded once, together, and up
-// to kRowsSorted segments stay in shared memory.
+// to kRowsSorted segments stay in shared memory.  What it takes is the fetching of
+// code that runs once: its loops are not unrolled.
 __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const int tid = threadIdx.x;
     const int nseg = a.row_off ? a.B : a.n_groups + a.B;
     const bool small = nseg <= kRowsSorted;
     if (blockIdx.x == 0 && a.meta)  // before a barrier; a group's thread sets it behind
+#pragma unroll 1
         for (int b = tid; b < a.B; b += kRowsThreads) a.meta[b].n_pre = 0;
     const int32_t* off = a.row_off ? a.row_off : a.group_off;
     const int32_t* ctx = a.ctx_len;
@@ -274,9 +276,11 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     }
     if (!a.row_off) {
         // shared pages of a group: announced, and within every member's context
+#pragma unroll 1
         for (int g = tid; g < a.n_groups; g += kRowsThreads)
             p.group_pages[g] = rows_clamp(a.shared_blocks[g], 0, a.max_blocks);
         __syncthreads();
+#pragma unroll 1
         for (int b = tid; b < a.B; b += kRowsThreads) {
             int lo = 0, hi = a.n_groups;  // first group whose end is past b
             while (lo < hi) {
@@ -293,6 +297,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             }
         }
         __syncthreads();
+#pragma unroll 1
         for (int b = tid; b < a.B; b += kRowsThreads) p.seq_pages[b] = p.seq_pages[b] >= 0 ? p.group_pages[p.seq_pages[b]] : 0;
     }
     __syncthreads();
@@ -301,6 +306,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     auto seg_of = [&](int i) { return rows_seg(a, i, off, ctx, p.group_pages, p.seq_pages); };
     // total work in key tiles (in fp32: an estimate, the same in every CTA)
     float work = 0.f;
+#pragma unroll 1
     for (int i = s0; i < s1; ++i) {
         const RowsSeg s = seg_of(i);
         if (s.tiles > 0) work += (float)s.tiles * 0.5f * (float)(rows_item_kt(a, s, 0) + s.kt) * (float)a.Hkv;
@@ -314,6 +320,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         if (tid < nseg) {
             const int len = p.segs[tid].kt;
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < nseg; ++j) rank += p.segs[j].kt > len || (p.segs[j].kt == len && j < tid);
             p.order[rank] = tid;
         }
@@ -326,8 +333,10 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
                    (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows > 0};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
+#pragma unroll 1
     for (int round = 0;; ++round) {
         int items = 0, prows = 0;
+#pragma unroll 1
         for (int i = s0; i < s1; ++i) {
             const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
             const int S = rows_splits(a, s, cut);
@@ -341,6 +350,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         cut.per_coarse = round == 7 ? none : 0.5f * cut.per_coarse;
         cut.duals = round < 7;
     }
+#pragma unroll 1
     for (int i = s0; i < s1; ++i) {
         const RowsSeg s = small ? p.segs[p.order[i]] : seg_of(i);
         const int S = rows_splits(a, s, cut);
@@ -350,6 +360,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         if (small) p.splits[i] = S;
         if (blockIdx.x == 0 && a.meta) {
             if (s.mode == kModeAll) {
+#pragma unroll 1
                 for (int b = s.lo / a.R; b < (s.lo + s.n) / a.R; ++b) {
                     a.meta[b].n_pre = rows_fit(a, s, parts, prow0) ? parts : 0;
                     a.meta[b].base_pre = prow0 + (b * a.R - s.lo);
@@ -375,7 +386,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     __syncthreads();
 }
 
-__device__ __noinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
+__device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
     RowsItem it;
     it.n_kt = -1;
     it.bad = 0;
