@@ -58,7 +58,9 @@ namespace specdec {
 
 constexpr int kRowsMaxSeqs = 1024;   // sequences of a call: the plan's tables live in shared memory
 constexpr int kRowsMaxSplits = 32;   // pieces of one key range
-constexpr int kRowsSorted = 128;     // up to so many segments are kept in shared memory and taken longest first
+// Up to so many segments are kept in shared memory and taken longest first (128 x 5 rows under 8192 tokens, 129
+// segments: 150 us, unsorted 155; 200 single rows on 4096 tokens: 184 and 180).
+constexpr int kRowsSorted = 256;
 constexpr int kRowsThreads = 384;
 constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
@@ -138,7 +140,7 @@ __device__ __forceinline__ int rows_clamp(int v, int lo, int hi) { return max(lo
 
 // Segment i; off: the bounds of the sequences' rows (prompt) or of the groups.
 __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* off, const int* ctx_len,
-                                            const int* group_pages, const int* seq_pages) {
+                                            const int* group_pages, const int16_t* seq_group) {
     RowsSeg s;
     if (a.row_off) {
         s.lo = rows_clamp(off[i], 0, a.T);
@@ -163,7 +165,7 @@ __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int*
         s.lo = b * a.R;
         s.n = a.R;
         s.ctx = rows_clamp(ctx_len[b], 0, 1 << 30);
-        s.base = seq_pages[b] * 16;
+        s.base = seq_group[b] >= 0 ? group_pages[seq_group[b]] * 16 : 0;
         s.end = max(s.base, min(s.ctx + a.R, a.slots_max));
         s.trow = b;
         s.mode = kModeMask;
@@ -212,10 +214,11 @@ __device__ __forceinline__ bool rows_fit(const RowsArgs& a, const RowsSeg& s, in
 struct RowsPlan {
     int pre[2 * kRowsMaxSeqs + 1];  // items before position i (without the KV heads)
     int prow[2 * kRowsMaxSeqs];     // partial rows before position i
-    int group_pages[kRowsMaxSeqs], seq_pages[kRowsMaxSeqs];
+    int group_pages[kRowsMaxSeqs];
+    int16_t seq_group[kRowsMaxSeqs];  // -1: of no group
     RowsSeg segs[kRowsSorted];
-    int order[kRowsSorted];   // segment at position i
-    int splits[kRowsSorted];  // its pieces
+    uint8_t order[kRowsSorted];   // segment at position i
+    uint8_t splits[kRowsSorted];  // its pieces
     int wsum[2][32];
     float wwork[32];
     int nseg, items;
@@ -289,21 +292,18 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
                 else lo = mid + 1;
             }
             const int g = lo < a.n_groups && off[lo] <= b ? lo : -1;
-            p.seq_pages[b] = g;
+            p.seq_group[b] = (int16_t)g;
             if (g >= 0) {
                 // a group of one shares nothing worth a second pass
                 const bool one = off[g + 1] - off[g] < 2;
                 atomicMin(&p.group_pages[g], one ? 0 : rows_clamp(ctx[b], 0, 1 << 30) / 16);
             }
         }
-        __syncthreads();
-#pragma unroll 1
-        for (int b = tid; b < a.B; b += kRowsThreads) p.seq_pages[b] = p.seq_pages[b] >= 0 ? p.group_pages[p.seq_pages[b]] : 0;
     }
     __syncthreads();
     const int per = small ? 1 : (nseg + kRowsThreads - 1) / kRowsThreads;
     const int s0 = min(nseg, tid * per), s1 = min(nseg, s0 + per);
-    auto seg_of = [&](int i) { return rows_seg(a, i, off, ctx, p.group_pages, p.seq_pages); };
+    auto seg_of = [&](int i) { return rows_seg(a, i, off, ctx, p.group_pages, p.seq_group); };
     // total work in key tiles (in fp32: an estimate, the same in every CTA)
     float work = 0.f;
 #pragma unroll 1
@@ -322,7 +322,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             int rank = 0;
 #pragma unroll 4
             for (int j = 0; j < nseg; ++j) rank += p.segs[j].kt > len || (p.segs[j].kt == len && j < tid);
-            p.order[rank] = tid;
+            p.order[rank] = (uint8_t)tid;
         }
         __syncthreads();
     }
@@ -357,7 +357,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         const int parts = rows_parts(a, s, cut, S);
         p.pre[i] = item0;
         p.prow[i] = prow0;
-        if (small) p.splits[i] = S;
+        if (small) p.splits[i] = (uint8_t)S;
         if (blockIdx.x == 0 && a.meta) {
             if (s.mode == kModeAll) {
 #pragma unroll 1
@@ -401,7 +401,7 @@ __device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan&
     }
     const RowsSeg s = p.nseg <= kRowsSorted
                           ? p.segs[p.order[lo]]
-                          : rows_seg(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_pages);
+                          : rows_seg(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_group);
     const int S = p.nseg <= kRowsSorted ? p.splits[lo] : rows_splits(a, s, p.cut);
     const int local = r - p.pre[lo];
     const int along = S == 1 ? local : local / S;
@@ -442,6 +442,7 @@ struct RowsCfg {
     static constexpr int NBAR = 5 * 2 + 5 * RING + 2 * kRowsItems + 1;
     static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
                                    NBAR * 8 + 16;
+    static_assert(smem <= 232448, "shared memory of a CTA");
 };
 
 // The rows of an item without keys.
