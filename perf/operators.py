@@ -24,27 +24,27 @@ def listed():
         # one pending token of one short request: latency alone
         dict(name="prompt one token", op="prompt", heads=8, kv_heads=2, head_dim=64, batch=1, rows=1, cached=40, spread=0),
         # short questions of the small model, packed for one forward
-        dict(name="prompt short 4 packed", op="prompt", heads=8, kv_heads=2, head_dim=64, batch=4, rows=333, cached=0, spread=3),
+        dict(name="prompt short, 4 packed", op="prompt", heads=8, kv_heads=2, head_dim=64, batch=4, rows=333, cached=0, spread=3),
         # one token a request, long ragged caches: the decode form
-        dict(name="prompt 1 row x 64 on 8k", op="prompt", heads=32, kv_heads=8, head_dim=128, batch=64, rows=1, cached=8192, spread=5),
+        dict(name="prompt 1 row x 64, cached 8k", op="prompt", heads=32, kv_heads=8, head_dim=128, batch=64, rows=1, cached=8192, spread=5),
         # the next chunk of prompts whose beginning is in the cache (40 query heads: 5 for each kv head)
         dict(name="prompt chunks 512 on 4k", op="prompt", heads=40, kv_heads=8, head_dim=128, batch=4, rows=512, cached=4096, spread=0),
         # packed prompts of very different lengths
-        dict(name="prompt ragged 8 packed", op="prompt", heads=32, kv_heads=8, head_dim=128, batch=8, rows=4001, cached=0, spread=11),
+        dict(name="prompt ragged, 8 packed", op="prompt", heads=32, kv_heads=8, head_dim=128, batch=8, rows=4001, cached=0, spread=11),
         # one long prompt from its first token: bound by the tensor cores
         dict(name="prompt 8192", op="prompt", heads=32, kv_heads=8, head_dim=128, batch=1, rows=8192, cached=0, spread=0),
         # single tokens of a few requests under one short system prompt
-        dict(name="shared 4 x 1 on 512", op="shared", heads=8, kv_heads=2, head_dim=64, batch=4, rows=1, groups=1, prefix=512, suffix=75, spread=2, tree=False),
+        dict(name="shared 4 x 1, 512", op="shared", heads=8, kv_heads=2, head_dim=64, batch=4, rows=1, groups=1, prefix=512, suffix=75, spread=2, tree=False),
         # chain verify rows of a batch under one system prompt
-        dict(name="shared 32 x 5 on 4k", op="shared", heads=32, kv_heads=8, head_dim=128, batch=32, rows=5, groups=1, prefix=4096, suffix=600, spread=4, tree=False),
+        dict(name="shared 32 x 5, 4k", op="shared", heads=32, kv_heads=8, head_dim=128, batch=32, rows=5, groups=1, prefix=4096, suffix=600, spread=4, tree=False),
         # draft trees, two system prompts
-        dict(name="shared 16 x 21 trees on 2 x 2k", op="shared", heads=40, kv_heads=8, head_dim=128, batch=16, rows=21, groups=2, prefix=2048, suffix=999, spread=6, tree=True),
+        dict(name="shared 16 x 21 tree, 2 of 2k", op="shared", heads=40, kv_heads=8, head_dim=128, batch=16, rows=21, groups=2, prefix=2048, suffix=999, spread=6, tree=True),
         # a large batch of chain verify rows under a long document
-        dict(name="shared 128 x 5 on 8k", op="shared", heads=32, kv_heads=8, head_dim=128, batch=128, rows=5, groups=1, prefix=8192, suffix=1024, spread=8, tree=False),
+        dict(name="shared 128 x 5, 8k", op="shared", heads=32, kv_heads=8, head_dim=128, batch=128, rows=5, groups=1, prefix=8192, suffix=1024, spread=8, tree=False),
         # one prompt sampled four times, small model
         dict(name="fork 1 to 4", op="fork", layers=4, kv_heads=2, head_dim=64, slots=8, sources=1, copies=4, tokens=205, pages=256, spread=0),
         # a beam step: 16 survivors continue as 48 requests in all 32 layers
-        dict(name="fork 16 to 48 in 32 layers", op="fork", layers=32, kv_heads=8, head_dim=128, slots=64, sources=16, copies=3, tokens=1500, pages=1800, spread=9),
+        dict(name="fork 16 to 48, 32 layers", op="fork", layers=32, kv_heads=8, head_dim=128, slots=64, sources=16, copies=3, tokens=1500, pages=1800, spread=9),
     ]
 
 
