@@ -16,11 +16,15 @@
 //            Q.K^T, softmax and P.V at a time (short segments).
 //
 // Mathematics, with x = score * log2(e) / sqrt(hd): in blocks of 128 keys
-//   m' = max(m, rowmax x),  P = 2^(x - m'),  l = l 2^(m - m') + rowsum P,
+//   m' = max(m, rowmax x),  P = 2^(x - m' + 7),  l = l 2^(m - m') + rowsum P,
 //   O = O 2^(m - m') + P V;  out = O / l.
-// m only moves when a row's maximum has grown by more than 8 (P stays below
-// 2^8), so O is rarely rescaled.  P is rounded to fp16 (at most 2^-11 of a
-// weight): the tensor core multiplies fp16 by fp16.  m, l, O are fp32.
+// m only moves when a row's maximum has grown by more than 8, so O is rarely
+// rescaled.  P is rounded to fp16, as the tensor core multiplies fp16 by fp16:
+// at most 2^-11 of a weight, or 2^-32 of the row's largest where that is more.
+// The 7 is what takes P, up to 2^15 with the 8, near the end of fp16's range:
+// without it weights below 2^-14 of the largest lost bits and those below 2^-25
+// were gone, which a long context of small weights shows (131,072 of 2^-25.2
+// beside one of 1: 3.4e-3 of V).  m, l, O are fp32.
 //
 // One persistent CTA per SM, 12 warps:
 //   warps 0-3, 4-7  softmax of tile slot 0 / 1, one thread per query row
@@ -66,6 +70,8 @@ constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSched
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
 constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte rows, 128B swizzle
 constexpr int kRowsTmemCols = 512;
+constexpr float kRowsLag = 8.0f;     // what a row's maximum may grow by before m follows
+constexpr float kRowsLift = 7.0f;    // P is 2^7 times the weight: at most 2^(8 + 7) < 65504
 
 enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2 };
 enum { kPair = 0, kDual = 1 };
@@ -900,7 +906,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     }
                     tc_ld_x32(t_s, va);
                     const float top = rows_max3(mx[0], mx[1], mx[1]) * a.scale_log2;
-                    const bool grow = real && !(top <= m + 8.0f);  // also where the row had seen nothing yet, and for NaN
+                    const bool grow = real && !(top <= m + kRowsLag);  // also where the row had seen nothing yet, and for NaN
                     float alpha = 1.f;
                     if (__any_sync(0xffffffffu, grow)) {
                         // O holds the tiles before this one (their P.V came before these scores)
@@ -912,14 +918,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     }
                     // a NaN or infinite maximum makes every weight, and so the row, NaN
                     const float sub = m == -INFINITY ? 0.f : (m < INFINITY ? m : __int_as_float(0x7FC00000));
-                    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), sub2 = pack2(-sub, -sub);
+                    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2),
+                                   lift2 = pack2(kRowsLift - sub, kRowsLift - sub);
                     uint64_t sum2[2] = {0ull, 0ull};
                     auto weights = [&](uint32_t(&v)[32], int q) {
                         uint32_t pw[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const uint64_t x =
-                                fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, sub2);
+                                fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, lift2);
                             const uint64_t y = exp2_unit2(x);
                             sum2[e & 1] = add2(sum2[e & 1], y);
                             float y0, y1;

@@ -1,0 +1,96 @@
+"""specdec_attention_prompt and specdec_attention_shared_prefix where values are
+at their limits: weights far below a row's largest, infinities and NaN in slots
+that every row sees, values and scores near the ends of their types."""
+import math
+
+import pytest
+import torch
+
+import test_gpu_prompt_attention as P
+import test_gpu_shared_prefix as X
+from attn_plain import close, rows_plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def slots_of(s, b, plane, n):
+    """K or V [Hkv, n, hd] of sequence b's first n slots (a copy)."""
+    pages = s["tables"][b, :(n + 15) // 16].long()
+    return s["kv"][pages, plane].permute(1, 0, 2, 3).reshape(s["Hkv"], -1, s["hd"])[:, :n].clone()
+
+
+def put_slots(s, b, plane, x):
+    n = x.shape[1]
+    pages = s["tables"][b, :(n + 15) // 16].long()
+    full = s["kv"][pages, plane].permute(1, 0, 2, 3).reshape(s["Hkv"], -1, s["hd"])
+    full[:, :n] = x.half()
+    s["kv"][pages, plane] = full.reshape(s["Hkv"], -1, 16, s["hd"]).permute(1, 0, 2, 3)
+
+
+def put_scores(s, b, x):
+    """Makes the scores of every row of sequence b against its slots x[j], up to
+    the keys' rounding: channel 0 alone counts."""
+    k = slots_of(s, b, 0, x.numel())
+    k[:] = 0
+    k[:, :, 0] = (x * math.sqrt(s["hd"]) / 8.0)[None]
+    put_slots(s, b, 0, k)
+    s["q"].view(-1, s["q"].shape[-1] // s["hd"], s["hd"])[:, :, 0] = 8.0
+
+
+def put_value(s, b, slot, value, head, column):
+    s["kv"][int(s["tables"][b, slot // 16]), 1, head, slot % 16, column] = value
+
+
+# ------------------------------------------------------------- small weights
+def small_weights_bound(s, q, b, seen):
+    """As attn_plain's bound, but for weights that are subnormal in fp16: P holds
+    2^7 times a weight (the row's largest weight is at least 1), so that what a
+    weight loses is at most half a subnormal step, 2^-25, over 2^7."""
+    o, tol = rows_plain(q, s["kv"], s["tables"][b], seen)
+    n = seen.shape[1]
+    v = slots_of(s, b, 1, n).double().abs()
+    G = s["Hq"] // s["Hkv"]
+    S = torch.stack([seen.double() @ v[h // G] for h in range(s["Hq"])], 1)
+    return o, tol - (2.0 ** -25 - 2.0 ** -32) * S
+
+
+@pytest.mark.parametrize("lens", [[(1, 131072)], [(300, 20000)]])
+@pytest.mark.parametrize("below", [22.3, 25.2])
+def test_many_small_weights(cuda_device, lens, below):
+    """One key of weight 1 and many thousands of 2^-22 to 2^-25: their sum is
+    what the output holds, as the large key's value is zero."""
+    s = P.make(lens, 8, 2, 64, seed=11)
+    (n, c), = lens
+    x = torch.full((n + c,), -below * math.log(2.0), device=DEV)
+    x[7] = 0.0
+    put_scores(s, 0, x)
+    v = slots_of(s, 0, 1, n + c).abs() + 0.5
+    v[:, 7] = 0.0
+    put_slots(s, 0, 1, v)
+    ws = P.call(s)
+    torch.cuda.synchronize()
+    q = s["q"][:n].reshape(n, 8, 64)
+    seen = torch.arange(n + c, device=DEV)[None] <= c + torch.arange(n, device=DEV)[:, None]
+    close(s["out"][:n], *small_weights_bound(s, q, 0, seen))
+    del ws
+
+
+def test_many_small_weights_under_a_shared_prefix(cuda_device):
+    s = X.make([(3, 2500)], [5, 30, 0], 4, 8, 2, 64, seed=12)
+    for b in range(3):
+        n = s["ctx_host"][b] + 4
+        x = torch.full((n,), -24.4 * math.log(2.0), device=DEV)
+        x[7] = 0.0
+        put_scores(s, b, x)
+        v = slots_of(s, b, 1, n)
+        v[:, :] = v.abs() + 0.5
+        v[:, 7] = 0.0
+        put_slots(s, b, 1, v.clamp(max=3))
+    ws = X.call(s)
+    torch.cuda.synchronize()
+    for b in range(3):
+        n = s["ctx_host"][b] + 4
+        seen = torch.arange(n, device=DEV)[None] <= s["ctx_host"][b] + torch.arange(4, device=DEV)[:, None]
+        close(s["out"][b], *small_weights_bound(s, s["q"][b], b, seen), f"sequence {b}")
+    del ws
