@@ -72,6 +72,11 @@ constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte ro
 constexpr int kRowsTmemCols = 512;
 constexpr float kRowsLag = 8.0f;     // what a row's maximum may grow by before m follows
 constexpr float kRowsLift = 7.0f;    // P is 2^7 times the weight: at most 2^(8 + 7) < 65504
+// From this maximum on (in units of x) score * scale - m is not one fused
+// operation: that leaves the rounding of m = score * scale in x, 32 at 2^29, and
+// P would be 2^(x + 7).  Product and difference apart, the largest gives 0.  Below
+// it x is off by 2^-13 at most (where 7 - m takes a bit more than m).
+constexpr float kRowsHuge = 4096.0f;
 
 enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2 };
 enum { kPair = 0, kDual = 1 };
@@ -563,6 +568,22 @@ __device__ __forceinline__ void rows_rescale(uint32_t t_o, float f) {
     }
 }
 
+// A row's scores v become (v scale - m) / scale, product and difference rounded apart.
+__device__ __noinline__ void rows_subtract(uint32_t t_s, float scale, float m) {
+    const float back = 1.0f / scale;
+#pragma unroll 1
+    for (int q = 0; q < 8; ++q) {
+        uint32_t v[16];
+        tc_ld_x16(t_s + 16 * q, v);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            v[e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[e]), scale), m) * back);
+        tc_st_x16(t_s + 16 * q, v);
+    }
+    tc_wait_st();
+}
+
 // The CTA's barriers, in shared memory.
 template <int RING>
 struct RowsBars {
@@ -855,7 +876,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             // slots below `every` are seen by all rows of the tile
             const int every = it.mode == kModeCausal ? min(it.end, it.ctx + it.i0 + t * a.tpt + 1)
                                                      : (it.mode == kModeMask ? min(it.end, it.ctx) : it.end);
-            float m = -INFINITY, l = 0.f;
+            float m = real ? -INFINITY : 0.f, l = 0.f;
             for (int j = j0; j < it.n_kt; j += jstep, ++c) {
                 if (!(ok = wait(&s_full[ws], c))) break;
                 tc_fence_after();
@@ -908,16 +929,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     const float top = rows_max3(mx[0], mx[1], mx[1]) * a.scale_log2;
                     const bool grow = real && !(top <= m + kRowsLag);  // also where the row had seen nothing yet, and for NaN
                     float alpha = 1.f;
-                    if (__any_sync(0xffffffffu, grow)) {
+                    bool huge = false;
+                    if (__any_sync(0xffffffffu, grow || fabsf(m) >= kRowsHuge)) {
                         // O holds the tiles before this one (their P.V came before these scores)
                         if (grow) {
                             alpha = m == -INFINITY ? 0.f : exp2f(m - top);
                             m = top;
                         }
-                        if (j != j0) rows_rescale<HD>(t_o, alpha);
+                        if (j != j0 && __any_sync(0xffffffffu, grow)) rows_rescale<HD>(t_o, alpha);
+                        huge = __any_sync(0xffffffffu, fabsf(m) >= kRowsHuge && fabsf(m) < INFINITY);
                     }
                     // a NaN or infinite maximum makes every weight, and so the row, NaN
-                    const float sub = m == -INFINITY ? 0.f : (m < INFINITY ? m : __int_as_float(0x7FC00000));
+                    float sub = m == -INFINITY ? 0.f : (m < INFINITY ? m : __int_as_float(0x7FC00000));
+                    if (huge) {
+                        tc_wait_ld();
+                        rows_subtract(t_s, a.scale_log2, sub);
+                        tc_ld_x32(t_s, va);
+                        sub = 0.f;
+                    }
                     const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2),
                                    lift2 = pack2(kRowsLift - sub, kRowsLift - sub);
                     uint64_t sum2[2] = {0ull, 0ull};

@@ -94,3 +94,25 @@ def test_many_small_weights_under_a_shared_prefix(cuda_device):
         seen = torch.arange(n, device=DEV)[None] <= s["ctx_host"][b] + torch.arange(4, device=DEV)[:, None]
         close(s["out"][b], *small_weights_bound(s, s["q"][b], b, seen), f"sequence {b}")
     del ws
+
+
+# --------------------------------------------------- the ends of the types
+@pytest.mark.parametrize("size", [900.0, 7000.0, 40000.0])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("lens", [[(60, 700)], [(1, 5000), (1, 40), (2, 300)], [(500, 0)]])
+def test_very_large_scores(cuda_device, size, heads, lens):
+    """Scores up to 2^37, a quarter of the largest apart: the softmax is the mean
+    of the largest score's values.  (Each of q and k is one number in all
+    channels, so equal keys have equal scores, however a product rounds.)"""
+    s = P.make(lens, *heads, seed=19)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    s["q"].fill_(size)
+    s["q"].view(-1, heads[0], heads[2])[:, 1::2] = -size
+    for b, (n, c) in enumerate(lens):
+        k = slots_of(s, b, 0, n + c)
+        k[:] = (torch.randint(-4, 5, (n + c,), generator=g, device=DEV) * size / 4)[None, :, None]
+        put_slots(s, b, 0, k)
+    ws = P.call(s)
+    P.verify(s)
+    del ws
