@@ -33,7 +33,7 @@
 //   warp 10         makes V safe: zeroes the slots behind the range's end in its
 //                   last page, and replaces infinities and NaN in slots that
 //                   not every row sees (0 * NaN would reach rows that do not
-//                   see them); the rows that see them add them at the end
+//                   see them)
 //   warp 11         scheduler: takes items, decodes them, passes them on
 // An operation is S = Q K^T, softmax, O += P V for one tile and 128 keys.  The
 // operations of a CTA use tile slots 0 and 1 in turn, through all its items (a
@@ -46,6 +46,12 @@
 //
 // Splits of the key range write unnormalised fp32 O with (m, l) into the
 // workspace; rows_merge_kernel joins them in their order.
+//
+// An infinity or a NaN of V reaches every row that sees its slot, whatever the
+// weight: no weight is 0 by the definition, though in fp16 (or beside a larger
+// piece) it may be, and 0 times infinity would be NaN.  Rows that hold one at the
+// end, or whose item warp 10 found one in, look their slots through again
+// (rows_nonfinite); a piece with one carries its l negative.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -472,30 +478,70 @@ __device__ void rows_zero(const RowsArgs& a, const RowsItem& it, int lane) {
     }
 }
 
-// Adds the infinities and NaN of V that warp 10 took out to a row that sees
-// them; `at` is the row's token (final) or its place in the partial buffers.
+// Sets the columns of a row in which it sees an infinity or a NaN of V; `at` is
+// the row's token (final) or its place in the partial buffers.  The whole warp
+// goes through the slots (all: from the item's first, else those warp 10 looked
+// at), a lane's columns being lane * (HD / 32) + j; only rows that are `mine` are
+// written.  True where a column was.
 template <int HD>
-__device__ void rows_add_bad(const RowsArgs& a, const RowsItem& it, int i, uint64_t bits, int head, size_t at) {
-    const int hi = min(it.end, it.slot0 + 128 * it.n_kt);
+__device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& it, bool mine, bool all, int i,
+                                            uint64_t bits, int head, size_t at) {
+    constexpr int W = HD / 32;  // columns of a lane
+    const int lane = threadIdx.x & 31;
+    const int mode = it.mode, ctx = it.ctx, end = min(it.end, it.slot0 + 128 * it.n_kt);
+    const int32_t* tab = a.tables + (size_t)it.trow * a.max_blocks;
+    uint32_t up[W], down[W];  // bit l of [j]: an infinity (NaN: both) in column l * W + j
+#pragma unroll
+    for (int j = 0; j < W; ++j) up[j] = down[j] = 0;
+    const int start = all ? it.slot0 : max(it.scan, it.slot0);
 #pragma unroll 1
-    for (int s = max(it.scan, it.slot0); s < hi; ++s) {
-        const bool seen = it.mode == kModeCausal ? s <= it.ctx + i : (s - it.ctx < 64 && ((bits >> (s - it.ctx)) & 1ull));
-        if (!seen) continue;
-        const int x = a.tables[(size_t)it.trow * a.max_blocks + (s >> 4)];
-        const int page = x < 0 || x >= a.num_blocks ? 0 : x;
-        const __half* v = a.kv + ((((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 + (s & 15)) * HD;
-#pragma unroll 1
-        for (int e = 0; e < HD; ++e) {
-            const float y = __half2float(v[e]);
-            if (isfinite(y)) continue;
-            if (it.prow < 0) {
-                __half* o = a.out + at * a.ldo + (size_t)head * HD + e;
-                *o = __float2half_rn(__half2float(*o) + y);
-            } else {
-                a.po[at * HD + e] += y;
+    for (int s0 = start & ~15; s0 < end; s0 += 16) {  // a page
+        const int x = tab[s0 >> 4], page = x < 0 || x >= a.num_blocks ? 0 : x;
+        const __half* src = a.kv + (((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 * HD + lane * W;
+        alignas(8) uint16_t v[16][W];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const __half* at_u = src + rows_clamp(u, max(0, start - s0), min(15, end - 1 - s0)) * HD;
+            if constexpr (W == 4) *reinterpret_cast<uint2*>(v[u]) = *reinterpret_cast<const uint2*>(at_u);
+            else *reinterpret_cast<uint32_t*>(v[u]) = *reinterpret_cast<const uint32_t*>(at_u);
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < W; ++j) any |= (v[u][j] & 0x7C00) == 0x7C00;
+            if (!__any_sync(0xffffffffu, any)) continue;
+            const int d = s0 + rows_clamp(u, max(0, start - s0), min(15, end - 1 - s0)) - ctx;
+            const bool seen = mode == kModeAll ||
+                              (mode == kModeCausal ? d <= i : d < 0 || (d < 64 && ((bits >> d) & 1ull)));
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const uint32_t y = v[u][j];  // 0x7C00 infinity, 0xFC00 its opposite, above either NaN
+                const uint32_t plus = __ballot_sync(0xffffffffu, (y & 0x7FFF) > 0x7C00 || y == 0x7C00);
+                const uint32_t minus = __ballot_sync(0xffffffffu, (y & 0x7FFF) > 0x7C00 || y == 0xFC00);
+                if (seen) {
+                    up[j] |= plus;
+                    down[j] |= minus;
+                }
             }
         }
     }
+    bool found = false;
+    if (mine) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            for (uint32_t left = up[j] | down[j]; left; left &= left - 1) {
+                const int l = __ffs(left) - 1, e = l * W + j;
+                const bool p = (up[j] >> l) & 1u, n = (down[j] >> l) & 1u;
+                const float y = p && n ? __int_as_float(0x7FC00000) : (p ? INFINITY : -INFINITY);
+                if (it.prow < 0) a.out[at * a.ldo + (size_t)head * HD + e] = __float2half_rn(y);
+                else a.po[at * HD + e] = y;
+                found = true;
+            }
+        }
+    }
+    __syncwarp();
+    return found;
 }
 
 // Bit c = slot key0 + c of a row is seen.
@@ -1003,6 +1049,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 const int head = it.kvh * a.G + g, tok = it.tok0 + t * a.tpt + ti;
                 const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
                 const size_t prow = (size_t)(it.prow + (it.kind == kDual ? role * it.pnext : 0) + t * a.tpt + ti) * a.Hq + head;
+                float far = 0.f;  // the row's largest |O|; NaN if one is
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     uint32_t ov[32];
@@ -1014,6 +1061,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 32; ++e) ov[e] = 0u;
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        far = rows_max3(far, fabsf(__uint_as_float(ov[e])), fabsf(__uint_as_float(ov[e + 1])));
                     if (real && it.prow < 0) {
                         __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + c0;
 #pragma unroll
@@ -1039,8 +1089,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                                          : "memory");
                     }
                 }
+                // (a row whose l is NaN is NaN in every column already)
+                const bool spoilt = !(far < INFINITY), mine = real && l == l && (bad || spoilt);
+                if (__any_sync(0xffffffffu, mine)) {
+                    const bool all = __any_sync(0xffffffffu, mine && spoilt);
+                    if (rows_nonfinite<HD>(a, items[k % kRowsItems], mine, all, i, bits, head,
+                                           it.prow < 0 ? (size_t)tok : prow))
+                        l = -l;
+                }
                 if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
-                if (bad && real) rows_add_bad<HD>(a, it, i, bits, head, it.prow < 0 ? (size_t)tok : prow);
             }
             tc_fence_before();  // O was read before the slot's next P is announced
             done_item(k);
@@ -1225,6 +1282,36 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 // call, 16 x 21 under 2048 61 -> 57; two or eight pieces at a time, or 16 lanes a
 // row, gain in one case what they lose in another.  The CTAs go round the rows:
 // one for every few rows cost 12 us where no row has pieces.
+// The same where a piece holds an infinity or a NaN (its l is negative or NaN):
+// they stay, whatever the piece's weight.
+template <int HD>
+__device__ __noinline__ void rows_merge_nonfinite(const RowsArgs& a, const RowsMeta mt, int i, int tok, int head) {
+    const int n = mt.n_pre + mt.n_own;
+    auto place = [&](int p) {
+        const int r = p < mt.n_pre ? mt.base_pre + p * mt.stride_pre : mt.base_own + (p - mt.n_pre) * mt.stride_own;
+        return (size_t)min(r + i, a.prows - 1) * a.Hq + head;
+    };
+    float top = -INFINITY, l = 0.f;
+    for (int p = 0; p < n; ++p) top = fmaxf(top, a.pml[place(p)].x);
+    const float sub = top == -INFINITY ? 0.f : top;
+    for (int p = 0; p < n; ++p) {
+        const float2 ml = a.pml[place(p)];
+        l += exp2f(ml.x - sub) * fabsf(ml.y);
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    for (int e = threadIdx.x & 7; e < HD; e += 8) {
+        float sum = 0.f, bad = 0.f;
+        for (int p = 0; p < n; ++p) {
+            const float2 ml = a.pml[place(p)];
+            if (ml.x == -INFINITY) continue;  // no key of the piece is seen
+            const float y = a.po[place(p) * HD + e];
+            if (isfinite(y)) sum += exp2f(ml.x - sub) * y;
+            else bad += y;
+        }
+        a.out[(size_t)tok * a.ldo + (size_t)head * HD + e] = __float2half_rn(l == l && bad != 0.f ? bad : sum * inv);
+    }
+}
+
 template <int HD>
 __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int head) {
     constexpr int K = HD / 32, P = 4;  // 16-byte pieces of a lane's columns; pieces at a time
@@ -1249,6 +1336,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
     const int n = mt.n_pre + mt.n_own;
     if (n == 0) return;
     float M = -INFINITY, l = 0.f;
+    bool bad = false;
     float o[K][4];
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -1265,6 +1353,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
             const size_t at = (size_t)min(r + i, a.prows - 1) * a.Hq + head;  // bounds that overlap: never out of range
             ml[u] = a.pml[at];
             if (p0 + u >= n) ml[u] = make_float2(-INFINITY, 0.f);
+            bad |= !(ml[u].y >= 0.f);
             const float4* src = reinterpret_cast<const float4*>(a.po + at * HD) + lane;
 #pragma unroll
             for (int k = 0; k < K; ++k) v[u][k] = src[8 * k];
@@ -1283,7 +1372,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
 #pragma unroll
         for (int u = 0; u < P; ++u) {
             const float w = exp2f(ml[u].x - sub);
-            if (w == 0.f) continue;  // a piece of no weight may hold anything
+            if (w == 0.f) continue;  // a piece without keys may hold anything
             l += w * ml[u].y;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -1294,7 +1383,11 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
             }
         }
     }
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    if (bad) {
+        rows_merge_nonfinite<HD>(a, mt, i, tok, head);
+        return;
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
     __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + 4 * lane;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -1306,7 +1399,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
 }
 
 template <int HD>
-__global__ void __launch_bounds__(256) rows_merge_kernel(RowsArgs a) {
+__global__ void __launch_bounds__(256) rows_merge_kernel(const __grid_constant__ RowsArgs a) {
     pdl_wait();
     if (*a.any_parts == 0) return;
     const int rows = a.T * a.Hq;

@@ -96,6 +96,87 @@ def test_many_small_weights_under_a_shared_prefix(cuda_device):
     del ws
 
 
+# ------------------------------------------- infinities and NaN that rows see
+def some_bad_values(s, b, slots):
+    """An infinity, its opposite (both in one column as well) and a NaN of head
+    0 and the last in the given slots."""
+    last, hd = s["Hkv"] - 1, s["hd"]
+    for head in {0, last}:
+        put_value(s, b, slots[0], math.inf, head, 0)
+        put_value(s, b, slots[1], -math.inf, head, hd - 1)
+        put_value(s, b, slots[2], math.nan, head, 5)
+        put_value(s, b, slots[0], math.inf, head, 33)
+        put_value(s, b, slots[1], -math.inf, head, 33)
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (5, 1, 128)])
+@pytest.mark.parametrize("lens", [[(40, 900)], [(200, 5)], [(1, 6000)], [(1, 300), (3, 4000)], [(600, 1500)]])
+@pytest.mark.parametrize("weight", ["ordinary", "small", "none"])
+def test_infinities_and_nan_of_slots_that_all_rows_see(cuda_device, heads, lens, weight):
+    """They reach every row, whatever their weight: 2^-30 (nothing in fp16) and
+    2^-300 (nothing in 32 bits) are weights."""
+    s = P.make(lens, *heads, seed=13)
+    for b, (n, c) in enumerate(lens):
+        slots = [c // 3, c // 2, min(c, 3)]
+        if weight != "ordinary":
+            x = torch.randn(n + c, device=DEV)
+            x[slots] = -30 * math.log(2.0) if weight == "small" else -300 * math.log(2.0)
+            put_scores(s, b, x)
+        some_bad_values(s, b, slots)
+    ws = P.call(s)
+    P.verify(s)
+    del ws
+
+
+def test_a_cache_of_nan(cuda_device):
+    """Every value of a long context NaN: rows that see it are NaN, in time."""
+    s = P.make([(300, 5000), (1, 8000), (70, 0)], 8, 2, 128, seed=14)
+    for b, c in ((0, 5000), (1, 8000)):
+        v = slots_of(s, b, 1, c)
+        v[:] = math.nan
+        put_slots(s, b, 1, v)
+    ws = P.call(s)
+    P.verify(s)
+    del ws
+
+
+@pytest.mark.parametrize("R", [1, 5])
+@pytest.mark.parametrize("weight", ["ordinary", "small", "none"])
+def test_infinities_and_nan_of_a_shared_prefix(cuda_device, R, weight):
+    s = X.make([(4, 70), (2, 9)], [9, 0, 200, 33, 500, 3], R, 8, 2, 128, seed=15, alone=(700,))
+    for b in range(7):
+        n = s["ctx_host"][b] + R
+        slots = [100, 130, 3]
+        if weight != "ordinary":
+            x = torch.randn(n, device=DEV) if b in (0, 4, 6) else torch.zeros(n, device=DEV)
+            if b in (0, 4, 6):
+                x[slots] = -30 * math.log(2.0) if weight == "small" else -300 * math.log(2.0)
+                put_scores(s, b, x)
+        if b in (0, 4, 6):
+            some_bad_values(s, b, slots)
+    ws = X.call(s)
+    X.verify(s)
+    del ws
+
+
+@pytest.mark.parametrize("lens", [[(1, 6000)], [(40, 900)], [(3, 4000), (1, 50)]])
+@pytest.mark.parametrize("large_first", [False, True])
+def test_a_nan_key_of_little_weight_beside_large_scores(cuda_device, lens, large_first):
+    """A NaN score makes its rows NaN, also where the keys around it weigh
+    nothing against the row's others."""
+    s = P.make(lens, 8, 2, 64, seed=16)
+    n, c = lens[0]
+    x = torch.zeros(n + c, device=DEV)
+    (x[:c // 2] if large_first else x[c // 2:]).fill_(250.0)
+    put_scores(s, 0, x)
+    slot = c - c // 4 if large_first else 19
+    s["kv"][int(s["tables"][0, slot // 16]), 0, 1, slot % 16, 9] = math.nan
+    ws = P.call(s)
+    P.verify(s)
+    assert bool(torch.isnan(s["out"][:n, 4:]).all()) and not bool(torch.isnan(s["out"][:n, :4]).any())
+    del ws
+
+
 # --------------------------------------------------- the ends of the types
 @pytest.mark.parametrize("size", [900.0, 7000.0, 40000.0])
 @pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)])
