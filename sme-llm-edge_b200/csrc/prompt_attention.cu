@@ -76,6 +76,7 @@ constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSched
 constexpr int kRowsItems = 3;        // items known ahead in a CTA
 constexpr int kBlockHalf = 2048;     // 16 tokens x 64 columns fp16, 128-byte rows, 128B swizzle
 constexpr int kRowsTmemCols = 512;
+constexpr float kHalfMax = 65504.0f, kHalfOver = 65520.0f;  // fp16's largest; from here on it rounds to infinity
 constexpr float kRowsLag = 8.0f;     // what a row's maximum may grow by before m follows
 constexpr float kRowsLift = 7.0f;    // P is 2^7 times the weight: at most 2^(8 + 7) < 65504
 // From this maximum on (in units of x) score * scale - m is not one fused
@@ -482,7 +483,8 @@ __device__ void rows_zero(const RowsArgs& a, const RowsItem& it, int lane) {
 // the row's token (final) or its place in the partial buffers.  The whole warp
 // goes through the slots (all: from the item's first, else those warp 10 looked
 // at), a lane's columns being lane * (HD / 32) + j; only rows that are `mine` are
-// written.  True where a column was.
+// written.  True where a column was.  Before it, a final row's infinities become
+// kHalfMax: its finite means that the weights' rounding (2^-11) took past 65520.
 template <int HD>
 __device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& it, bool mine, bool all, int i,
                                             uint64_t bits, int head, size_t at) {
@@ -527,6 +529,14 @@ __device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& i
         }
     }
     bool found = false;
+    if (mine && it.prow < 0) {
+#pragma unroll 1
+        for (int e = 0; e < HD; ++e) {
+            __half* o = a.out + at * a.ldo + (size_t)head * HD + e;
+            const float y = __half2float(*o);
+            if (fabsf(y) == INFINITY) *o = __float2half_rn(copysignf(kHalfMax, y));
+        }
+    }
     if (mine) {
 #pragma unroll
         for (int j = 0; j < W; ++j) {
@@ -1090,7 +1100,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     }
                 }
                 // (a row whose l is NaN is NaN in every column already)
-                const bool spoilt = !(far < INFINITY), mine = real && l == l && (bad || spoilt);
+                const bool spoilt = !(far < INFINITY);
+                const bool over = it.prow < 0 ? !(far * inv < kHalfOver) : spoilt;
+                const bool mine = real && l == l && (bad || over);
                 if (__any_sync(0xffffffffu, mine)) {
                     const bool all = __any_sync(0xffffffffu, mine && spoilt);
                     if (rows_nonfinite<HD>(a, items[k % kRowsItems], mine, all, i, bits, head,
@@ -1308,7 +1320,9 @@ __device__ __noinline__ void rows_merge_nonfinite(const RowsArgs& a, const RowsM
             if (isfinite(y)) sum += exp2f(ml.x - sub) * y;
             else bad += y;
         }
-        a.out[(size_t)tok * a.ldo + (size_t)head * HD + e] = __float2half_rn(l == l && bad != 0.f ? bad : sum * inv);
+        float y = sum * inv;
+        if (fabsf(y) > kHalfMax) y = copysignf(kHalfMax, y);
+        a.out[(size_t)tok * a.ldo + (size_t)head * HD + e] = __float2half_rn(l == l && bad != 0.f ? bad : y);
     }
 }
 
@@ -1393,7 +1407,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
     for (int k = 0; k < K; ++k) {
         alignas(8) __half h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = __float2half_rn(o[k][e] * inv);
+        for (int e = 0; e < 4; ++e) h[e] = __float2half_rn(fminf(fmaxf(o[k][e] * inv, -kHalfMax), kHalfMax));
         *reinterpret_cast<uint2*>(dst + 32 * k) = *reinterpret_cast<const uint2*>(h);
     }
 }

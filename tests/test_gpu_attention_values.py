@@ -178,6 +178,57 @@ def test_a_nan_key_of_little_weight_beside_large_scores(cuda_device, lens, large
 
 
 # --------------------------------------------------- the ends of the types
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("lens", [[(60, 700)], [(1, 5000), (1, 40), (2, 300)], [(500, 0)]])
+def test_the_largest_values(cuda_device, heads, lens):
+    """All values 65504: a mean of them is 65504 and no infinity."""
+    s = P.make(lens, *heads, seed=17)
+    for b, (n, c) in enumerate(lens):
+        v = slots_of(s, b, 1, n + c)
+        v[:] = 65504.0
+        v[:, :, 1::2] = -65504.0
+        put_slots(s, b, 1, v)
+    ws = P.call(s)
+    P.verify(s)
+    del ws
+
+
+@pytest.mark.parametrize("lens", [[(200, 300)], [(2, 3000)] * 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_the_largest_values_with_one_key_of_most_weight(cuda_device, lens, hd):
+    """One weight, of every fraction between 1 and 2, carries the rows: half its
+    rounding to fp16 would take 65504 over the next step, to infinity."""
+    s = P.make(lens, 8, 2, hd, seed=20)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    for b, (n, c) in enumerate(lens):
+        x = torch.full((n + c,), -30.0, device=DEV)
+        x[3], x[200] = 0.0, 3.55
+        put_scores(s, b, x)
+        k = slots_of(s, b, 0, n + c)
+        k[:, 200, 1] = 1.0
+        put_slots(s, b, 0, k)
+        v = slots_of(s, b, 1, n + c)
+        v[:] = 65504.0
+        put_slots(s, b, 1, v)
+    q = s["q"].view(-1, 8, hd)
+    q[:, :, 1] = (torch.rand(q.shape[:2], generator=g, device=DEV) * math.sqrt(hd) * 0.2).half()
+    ws = P.call(s)
+    P.verify(s)
+    del ws
+
+
+def test_the_largest_values_under_a_shared_prefix(cuda_device):
+    s = X.make([(4, 40)], [9, 0, 200, 33], 5, 8, 2, 128, seed=18, alone=(60,))
+    for b in range(5):
+        v = slots_of(s, b, 1, s["ctx_host"][b] + 5)
+        v[:] = -65504.0
+        put_slots(s, b, 1, v)
+    ws = X.call(s)
+    X.verify(s)
+    del ws
+
+
 @pytest.mark.parametrize("size", [900.0, 7000.0, 40000.0])
 @pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)])
 @pytest.mark.parametrize("lens", [[(60, 700)], [(1, 5000), (1, 40), (2, 300)], [(500, 0)]])
