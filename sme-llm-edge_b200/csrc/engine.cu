@@ -1205,6 +1205,14 @@ extern "C" int specdec_engine_fork(specdec_engine* e, int seq, const int32_t* ne
                  "engine_fork: a new slot out of range, named twice or the source");
         named[d] = 1;
     }
+    // An id stands for one request: a prefix index that releases a copy would release a running one's prefix with it.
+    for (int i = 0; request_ids && i < n; ++i) {
+        const int32_t id = request_ids[i];
+        bool taken = false;
+        for (int j = 0; j < i; ++j) taken |= request_ids[j] == id;
+        for (int b = 0; b < e->B; ++b) taken |= !named[b] && e->slot_request[b] == id;
+        SD_CHECK(id < 0 || !taken, SPECDEC_EINVAL, "engine_fork: a request id named twice or held by another slot");
+    }
     if (n == 0) return SPECDEC_OK;
     cudaStream_t s = e->stream;
     const int H = e->mc.hidden;
