@@ -487,8 +487,10 @@ int specdec_engine_retire(specdec_engine* e, int seq, specdec_radix* cache);
  * one prompt from one prefill, or a branch of a running generation.  Their
  * previous requests are retired (with an index, their prefix references);
  * request_ids (may be NULL: none) are recorded for them; an id >= 0 that
- * another slot holds or that is named twice is EINVAL.  EINVAL or ENOMEM leave
- * every slot as it was.  Synchronises the engine stream. */
+ * another slot holds or that is named twice is EINVAL.  A slot whose prompt is
+ * not complete (specdec_engine_prefill_chunk) may be forked: like it, its
+ * copies take their own rest of a prompt before they step.  EINVAL or ENOMEM
+ * leave every slot as it was.  Synchronises the engine stream. */
 int specdec_engine_fork(specdec_engine* e, int seq, const int32_t* new_seqs, const int32_t* request_ids, int n,
                         specdec_radix* cache);
 /* The first half of specdec_engine_admit, for chunked admission: retires the
