@@ -207,11 +207,10 @@ __device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s,
 struct RowsCut {
     float per_fine, per_coarse;  // reciprocals
     int whole;
-    bool duals;
+    int dual;  // key tiles from which a segment of one tile is worked on as duals
 };
-// A segment of one tile and several key tiles is worked on as duals.
 __device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
-    return cut.duals && s.n <= a.tpt && s.kt >= 2;
+    return s.n <= a.tpt && s.kt >= cut.dual;
 }
 __device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
     const int S = s.n <= 64 / a.G ? (int)ceilf((float)s.kt * cut.per_fine)
@@ -349,7 +348,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
-                   (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows > 0};
+                   (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows ? 2 : 1 << 30};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
 #pragma unroll 1
     for (int round = 0;; ++round) {
@@ -362,11 +361,17 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
             prows += s.n * rows_parts(a, s, cut, S);
         }
         rows_scan2(p, items, prows, &item0, &prow0, &tot_items, &tot_prows);
-        if (tot_prows <= a.prows || round >= 8) break;
-        // fewer pieces until their results fit; at last one a segment and no duals, which always does
-        cut.per_fine = round == 7 ? none : 0.5f * cut.per_fine;
-        cut.per_coarse = round == 7 ? none : 0.5f * cut.per_coarse;
-        cut.duals = round < 7;
+        if (tot_prows <= a.prows || round >= 11) break;
+        // Less until the results fit.  First the duals of short ranges, whose two halves take room and need no
+        // piece (all duals after three rounds), then pieces; at last one a segment, which always does.  (With duals
+        // of any length kept, 250 sequences of 5 rows beside one token on 100,000 slots used the room up, and
+        // that token's range was not cut at all.)
+        if (round < 3) {
+            cut.dual = round < 2 ? 4 * cut.dual : 1 << 30;
+        } else {
+            cut.per_fine = round == 10 ? none : 0.5f * cut.per_fine;
+            cut.per_coarse = round == 10 ? none : 0.5f * cut.per_coarse;
+        }
     }
 #pragma unroll 1
     for (int i = s0; i < s1; ++i) {
