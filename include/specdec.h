@@ -323,8 +323,10 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
  * outside the pool reads block 0.  Up to 1024 sequences.  Long key ranges are
  * split across CTAs and merged through the workspace in a fixed order (the
  * result is deterministic); calls in flight at the same time, captured graphs
- * among them, need workspaces (32-byte aligned) of their own.  All pointers
- * are memory of the current device.  The first call on a device comes before
+ * among them, need workspaces (32-byte aligned) of their own.  The size does
+ * not fall where B, T or max_blocks grows: the largest call's does for all (at
+ * most 8192 rows of n_q_heads * (head_dim + 2) floats and 24 bytes a sequence).
+ * All pointers are memory of the current device.  The first call on a device comes before
  * any stream capture.  The reference feeds prompts in chunks
  * (server/chunked_prefill.cpp:4-24) through one row of attention at a time
  * (server/paged_attention.cpp:16-111). */

@@ -1445,19 +1445,18 @@ static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq
     return SPECDEC_OK;
 }
 
-constexpr int kRowsSplitTokens = 4096;   // calls of more rows fill the GPU, but for long ranges of few rows among them
-constexpr int kRowsPartialRows = 8192;   // room for pieces, in token rows (two for each row at least)
-constexpr int kRowsPartialMany = 2048;   // the same in calls of more rows
+constexpr int kRowsPartialRows = 8192;   // room for pieces, in token rows
 constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece of every range
 
 // Rows of the partial buffers.
 // Tables of up to 256 slots have two key tiles: no pieces, and no merge behind
 // them (a single row on 40 slots: 14.9 us a call with its launch, 12.2 without).
-// In calls of many rows there is room for those of short segments: a single token
-// on 100,000 slots beside 6000 rows of prompts: 1,529 us without pieces, 373 with.
-static size_t prompt_partial_rows(int T, int Hq, int max_blocks) {
-    if (max_blocks <= 16 || (long long)T * Hq >= 1 << 30) return 0;
-    return T <= kRowsSplitTokens ? std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows) : kRowsPartialMany;
+// More rows never have less room: a workspace for a server's largest call does
+// for the smaller ones (and 2800 rows of prompts beside 250 sequences of 5 rows
+// and a token on 100,000 slots take 304 us, 2900 rows 314; with a quarter of the
+// room from 4096 rows in all on, 343).
+static size_t prompt_partial_rows(int T, int max_blocks) {
+    return max_blocks <= 16 ? 0 : std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows);
 }
 static size_t shared_partial_rows(int T) {
     // prefix and own range of every row, each of which may be a dual
@@ -1581,7 +1580,7 @@ extern "C" size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q
                                                            int max_blocks) {
     (void)n_kv_heads;
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
-    return rows_workspace(prompt_partial_rows(T, n_q_heads, max_blocks), B, n_q_heads, head_dim);
+    return rows_workspace(prompt_partial_rows(T, max_blocks), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1596,10 +1595,11 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
     SD_CHECK(ldq >= n_q_heads * head_dim && ldq % 8 == 0 && ldo >= n_q_heads * head_dim && ldo % 8 == 0,
              SPECDEC_EINVAL, "attention_prompt: row strides hold all heads and are multiples of 8");
     if (B == 0 || T == 0) return SPECDEC_OK;
-    const size_t prows = prompt_partial_rows(T, n_q_heads, max_blocks);
+    size_t prows = prompt_partial_rows(T, max_blocks);
     if ((rc = check_workspace("attention_prompt", workspace, workspace_bytes,
                               rows_workspace(prows, B, n_q_heads, head_dim))))
         return rc;
+    if ((long long)T * n_q_heads >= 1 << 30) prows = 0;  // the merge counts rows and heads in 32 bits
     RowsArgs a = {};
     a.num_blocks = num_blocks;
     a.Hkv = n_kv_heads;

@@ -1,0 +1,27 @@
+"""Workspace sizes of the prompt and shared-prefix attention (no GPU here): a
+server asks for its largest call's and makes every smaller call with it."""
+import itertools
+
+import pytest
+
+import specdec as S
+
+L = S.lib()
+HEADS = [(8, 2, 64), (32, 8, 128), (128, 8, 128)]
+
+
+def never_less(size, ranges):
+    """`size` does not fall where one of its arguments grows."""
+    for args in itertools.product(*ranges):
+        for i, values in enumerate(ranges):
+            more = [v for v in values if v > args[i]]
+            if more:
+                larger = args[:i] + (more[0],) + args[i + 1:]
+                assert size(*larger) >= size(*args), (args, larger)
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", HEADS)
+def test_prompt_sizes_grow_with_the_call(Hq, Hkv, hd):
+    never_less(lambda B, T, mb: L.specdec_attention_prompt_workspace_bytes(B, T, Hq, Hkv, hd, mb),
+               [(1, 5, 64, 1024), (1, 2, 200, 4095, 4096, 4097, 8192, 1 << 17, 1 << 23, 1 << 24),
+                (1, 16, 17, 512, 1 << 20)])
