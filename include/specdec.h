@@ -347,7 +347,9 @@ int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_laye
  * of no group share nothing.  The other arguments and the result are
  * specdec_attention's (the result up to the order of the sums); slots no row
  * sees may hold anything.  Up to 1024 sequences; workspace, capture and
- * determinism as for specdec_attention_prompt. */
+ * determinism as for specdec_attention_prompt (the size does not fall where B,
+ * R, n_groups or max_blocks grows; with groups, at most 2 B R + 8192 rows of
+ * n_q_heads * (head_dim + 2) floats, without 2 B R less). */
 size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads, int n_kv_heads,
                                                        int head_dim, int max_blocks);
 int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,

@@ -1446,7 +1446,7 @@ static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq
 }
 
 constexpr int kRowsPartialRows = 8192;   // room for pieces, in token rows
-constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece of every range
+constexpr int kRowsMoreRows = 4096;      // shared prefix: room for duals, and for pieces
 
 // Rows of the partial buffers.
 // Tables of up to 256 slots have two key tiles: no pieces, and no merge behind
@@ -1458,9 +1458,15 @@ constexpr int kRowsMoreRows = 4096;      // shared prefix: room beyond one piece
 static size_t prompt_partial_rows(int T, int max_blocks) {
     return max_blocks <= 16 ? 0 : std::min<size_t>((size_t)kRowsMaxSplits * T, kRowsPartialRows);
 }
-static size_t shared_partial_rows(int T) {
-    // prefix and own range of every row, each of which may be a dual
-    return 4 * (size_t)T + std::min<size_t>(2 * (size_t)(kRowsMaxSplits - 2) * T, kRowsMoreRows);
+// Under a shared prefix every row has two results to join, its own range's and
+// the prefix's; what lies beyond is for duals and pieces, and limited, as it only
+// makes the call faster (128 sequences of 64 rows, 32 heads of 128: 24,576 rows,
+// 409 MB).  Without groups, short tables have none.
+static size_t shared_partial_rows(int T, int n_groups, int max_blocks) {
+    if (n_groups == 0 && max_blocks <= 16) return 0;
+    const size_t t = (size_t)T, duals = std::min<size_t>(2 * t, kRowsMoreRows);
+    const size_t pieces = max_blocks <= 16 ? 0 : std::min<size_t>(2 * (kRowsMaxSplits - 2) * t, kRowsMoreRows);
+    return (n_groups ? 2 * t : 0) + duals + pieces;
 }
 static size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 static size_t rows_workspace(size_t prows, int B, int Hq, int HD) {
@@ -1622,9 +1628,9 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
 
 extern "C" size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads,
                                                                   int n_kv_heads, int head_dim, int max_blocks) {
-    (void)n_groups, (void)n_kv_heads, (void)max_blocks;
+    (void)n_kv_heads;
     if (B <= 0 || R <= 0 || B > kRowsMaxSeqs || R > 64 || n_q_heads <= 0 || head_dim <= 0) return 0;
-    return rows_workspace(shared_partial_rows(B * R), B, n_q_heads, head_dim);
+    return rows_workspace(shared_partial_rows(B * R, n_groups, max_blocks), B, n_q_heads, head_dim);
 }
 
 extern "C" int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer, int num_blocks,
@@ -1640,7 +1646,7 @@ extern "C" int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t
     SD_CHECK(R >= 1 && R <= 64, SPECDEC_EINVAL, "attention_shared_prefix: 1 to 64 rows");
     SD_CHECK(n_groups >= 0 && n_groups <= B, SPECDEC_EINVAL, "attention_shared_prefix: 0 to B groups");
     if (B == 0) return SPECDEC_OK;
-    const size_t prows = shared_partial_rows(B * R);
+    const size_t prows = shared_partial_rows(B * R, n_groups, max_blocks);
     if ((rc = check_workspace("attention_shared_prefix", workspace, workspace_bytes,
                               rows_workspace(prows, B, n_q_heads, head_dim))))
         return rc;

@@ -25,3 +25,20 @@ def test_prompt_sizes_grow_with_the_call(Hq, Hkv, hd):
     never_less(lambda B, T, mb: L.specdec_attention_prompt_workspace_bytes(B, T, Hq, Hkv, hd, mb),
                [(1, 5, 64, 1024), (1, 2, 200, 4095, 4096, 4097, 8192, 1 << 17, 1 << 23, 1 << 24),
                 (1, 16, 17, 512, 1 << 20)])
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", HEADS)
+def test_shared_prefix_sizes_grow_with_the_call(Hq, Hkv, hd):
+    size = L.specdec_attention_shared_prefix_workspace_bytes
+    never_less(lambda B, R, ng, mb: size(B, R, min(ng, B), Hq, Hkv, hd, mb),
+               [(1, 5, 64, 128, 1024), (1, 2, 5, 21, 64), (0, 1, 3, 64), (1, 16, 17, 512, 1 << 20)])
+
+
+def test_shared_prefix_sizes_stay_near_what_the_rows_need():
+    """Two results a row where there are groups; without groups and with one key
+    tile or two a table, none."""
+    size, row = L.specdec_attention_shared_prefix_workspace_bytes, 32 * (128 + 2) * 4
+    for B, R in ((128, 64), (1024, 64), (1024, 5)):
+        assert 2 * B * R * row <= size(B, R, 1, 32, 8, 128, 512) <= (2 * B * R + 8192) * row + 24 * B + 1024
+        assert size(B, R, 0, 32, 8, 128, 512) <= 8192 * row + 24 * B + 1024
+        assert size(B, R, 0, 32, 8, 128, 16) <= 24 * B + 1024

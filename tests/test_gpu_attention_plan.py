@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import test_gpu_prompt_attention as P
+import test_gpu_shared_prefix as X
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +27,16 @@ def test_a_long_range_is_cut_beside_many_short_ones(cuda_device, prompt):
     off = s["off"].tolist()
     for b in (0, 1, 249, 250, 251):
         P.close(s["out"][off[b]:off[b + 1]], *P.want(s, b), f"sequence {b}")
+    del ws
+
+
+@pytest.mark.parametrize("groups,R,own,alone", [
+    ([(200, 30)], 21, 90, ()), ([(40, 12), (0, 3), (60, 5)], 64, 33, (70, 5)),  # more rows than there is room for duals
+    ([(3, 4)], 5, 40, (90,)), ([], 5, 0, (3, 40, 0, 200)), ([], 64, 0, (150,) * 60), ([], 3, 0, (900, 5000) * 30)])
+def test_shared_prefixes_in_the_room_there_is(cuda_device, groups, R, own, alone):
+    """Calls of many rows, of short tables (16 pages at most) and of no groups."""
+    n = sum(g for g, _ in groups)
+    s = X.make(groups, [(own * b) % (own + 1) for b in range(n)], R, 8, 2, 64, seed=R + n, alone=alone)
+    ws = X.call(s)
+    X.verify(s)
     del ws
