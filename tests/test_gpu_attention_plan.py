@@ -40,3 +40,69 @@ def test_shared_prefixes_in_the_room_there_is(cuda_device, groups, R, own, alone
     ws = X.call(s)
     X.verify(s)
     del ws
+
+
+class Guarded:
+    """A tensor with a pattern in front of it and behind."""
+    N = 1 << 16
+
+    def __init__(self, like):
+        size = like.numel() * like.element_size()
+        self.buf = torch.full((size + 2 * self.N,), 0x5A, dtype=torch.uint8, device=like.device)
+        self.at = self.buf[self.N:self.N + size].view(like.dtype).view(like.shape)
+
+    def check(self):
+        end = self.buf.numel() - self.N
+        assert bool((self.buf[:self.N] == 0x5A).all()) and bool((self.buf[end:] == 0x5A).all())
+
+
+def timed(f):
+    """Far below the two seconds after which a kernel's wait gives up."""
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    e[0].record()
+    f()
+    e[1].record()
+    torch.cuda.synchronize()
+    assert e[0].elapsed_time(e[1]) < 200.0
+
+
+def test_group_bounds_that_no_caller_should_give(cuda_device):
+    """The call ends in time and writes in its output and its workspace alone."""
+    s = X.make([(2, 20), (3, 14)], [30, 5, 9, 700, 41], 2, 8, 2, 64, seed=7, alone=(333,))
+    out, ws = Guarded(s["out"]), Guarded(X.workspace(s))
+    s["out"] = out.at
+    X.call(s, ws.at)
+    for off in ([0, 6, 0], [3, 1, 4], [-5, 9, 2], [6, 6, 6], [0, 1 << 30, -1], [-(1 << 31), (1 << 31) - 1, 0], [5, 0, 6]):
+        for pages in ([20, 14], [1 << 30, -1], [-(1 << 31), (1 << 31) - 1]):
+            s["goff"].copy_(torch.tensor(off))
+            s["pages"].copy_(torch.tensor(pages))
+            timed(lambda: X.call(s, ws.at))
+            out.check()
+            ws.check()
+    s["goff"].copy_(torch.tensor([0, 2, 5]))
+    s["pages"].copy_(torch.tensor([20, 14]))
+    X.call(s, ws.at)
+    X.verify(s)
+
+
+@pytest.mark.parametrize("spare", [0, 40])
+def test_row_bounds_and_lengths_that_no_caller_should_give(cuda_device, spare):
+    s = P.make([(3, 2000), (130, 7), (0, 0), (1, 300)], 8, 2, 64, seed=8, tail_rows=spare)
+    good = s["off"].clone(), s["ctx"].clone()
+    out, ws = Guarded(s["out"]), Guarded(P.workspace(s))
+    s["out"] = out.at
+    P.call(s, ws.at)
+    big = (1 << 31) - 1
+    for off in ([0, 134, 0, 134, 0], [134, 3, 2, 1, 0], [-5, 1 << 30, -1, 7, big], [-big - 1] * 5, [big] * 5,
+                [0, big, -big, big, 134]):
+        for ctx in ([2000, 7, 0, 300], [big, -1, -big - 1, 1 << 30], [1 << 30] * 4):
+            s["off"].copy_(torch.tensor(off))
+            s["ctx"].copy_(torch.tensor(ctx))
+            timed(lambda: P.call(s, ws.at))
+            out.check()
+            ws.check()
+    s["off"].copy_(good[0])
+    s["ctx"].copy_(good[1])
+    s["out"].fill_(7.0)
+    P.call(s, ws.at)
+    P.verify(s)
