@@ -1106,8 +1106,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 }
                 // (a row whose l is NaN is NaN in every column already)
                 const bool spoilt = !(far < INFINITY);
-                const bool over = it.prow < 0 ? !(far * inv < kHalfOver) : spoilt;
-                const bool mine = real && l == l && (bad || over);
+                const bool mine = real && l == l && (bad || !(far * inv < kHalfOver));
                 if (__any_sync(0xffffffffu, mine)) {
                     const bool all = __any_sync(0xffffffffu, mine && spoilt);
                     if (rows_nonfinite<HD>(a, items[k % kRowsItems], mine, all, i, bits, head,
