@@ -1592,7 +1592,9 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
                                         int n_kv_heads, int head_dim, const int32_t* tables, int max_blocks,
                                         const int32_t* ctx_len, const int32_t* row_off, int B, int T, int n_q_heads,
                                         uint16_t* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    SD_CHECK(q && kv_layer && tables && ctx_len && row_off && out, SPECDEC_EINVAL, "attention_prompt: null argument");
+    // (an empty call's tensors may have no memory)
+    SD_CHECK(B == 0 || T == 0 || (q && kv_layer && tables && ctx_len && row_off && out), SPECDEC_EINVAL,
+             "attention_prompt: null argument");
     int rc = check_rows("attention_prompt", q, kv_layer, out, num_blocks, n_kv_heads, head_dim, max_blocks, B,
                         n_q_heads);
     if (rc) return rc;
@@ -1637,7 +1639,8 @@ extern "C" int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t
                                                const int32_t* ctx_len, const uint64_t* mask, const int32_t* group_off,
                                                const int32_t* shared_blocks, int n_groups, int B, int R, int n_q_heads,
                                                uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
-    SD_CHECK(q && kv_layer && tables && ctx_len && mask && out && (n_groups == 0 || (group_off && shared_blocks)),
+    SD_CHECK(B == 0 || (q && kv_layer && tables && ctx_len && mask && out &&
+                        (n_groups == 0 || (group_off && shared_blocks))),
              SPECDEC_EINVAL, "attention_shared_prefix: null argument");
     int rc = check_rows("attention_shared_prefix", q, kv_layer, out, num_blocks, n_kv_heads, head_dim, max_blocks, B,
                         n_q_heads);
