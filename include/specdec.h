@@ -318,16 +318,20 @@ int specdec_attention(const uint16_t* q, const uint16_t* kv_layer, int num_block
  * strides ldq / ldo in elements (multiples of 8, so q may lie in the fused
  * QKV rows); T = rows of the buffers.  A sequence may have no rows; rows
  * behind row_off[B] may hold anything and stay as they are.  Slots a row does
- * not see may hold anything (NaN and infinities too), pages past the last
- * slot are not read; slots past max_blocks * 16 do not exist; a table entry
- * outside the pool reads block 0.  Up to 1024 sequences.  Long key ranges are
- * split across CTAs and merged through the workspace in a fixed order (the
- * result is deterministic); calls in flight at the same time, captured graphs
- * among them, need workspaces (32-byte aligned) of their own.  The size does
- * not fall where B, T or max_blocks grows: the largest call's does for all (at
+ * not see may hold anything (NaN and infinities too; those of V that it sees
+ * reach it whatever their weight), pages past the last slot are not read;
+ * slots past max_blocks * 16 do not exist; a table entry outside the pool
+ * reads block 0.  Up to 1024 sequences.  Long key ranges are split across CTAs
+ * and merged through the workspace in a fixed order (the result is
+ * deterministic); calls in flight at the same time, captured graphs among
+ * them, need workspaces (32-byte aligned) of their own.  The size does not
+ * fall where B, T or max_blocks grows: the largest call's does for all (at
  * most 8192 rows of n_q_heads * (head_dim + 2) floats and 24 bytes a sequence).
- * All pointers are memory of the current device.  The first call on a device comes before
- * any stream capture.  The reference feeds prompts in chunks
+ * All pointers are memory of the current device.  The first call on a device
+ * comes before any stream capture.  Single tokens alone are faster by
+ * specdec_attention (64 on 2048 slots, 32/8 heads of 128: 95 us against 115),
+ * unless few sequences have very long contexts (one token on 65,536: 131
+ * against 65).  The reference feeds prompts in chunks
  * (server/chunked_prefill.cpp:4-24) through one row of attention at a time
  * (server/paged_attention.cpp:16-111). */
 size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
@@ -346,10 +350,13 @@ int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_laye
  * blocks past any member's ctx_len / 16 are taken as not shared).  Sequences
  * of no group share nothing.  The other arguments and the result are
  * specdec_attention's (the result up to the order of the sums); slots no row
- * sees may hold anything.  Up to 1024 sequences; workspace, capture and
- * determinism as for specdec_attention_prompt (the size does not fall where B,
- * R, n_groups or max_blocks grows; with groups, at most 2 B R + 8192 rows of
- * n_q_heads * (head_dim + 2) floats, without 2 B R less). */
+ * sees may hold anything.  It pays from about 30,000 shared tokens on, counted
+ * once for each sequence (16 x 21 rows under 2048: 48 us against 50; 32 x 5
+ * under 1024: 37 against 31, under 4096: 47 against 79; 128 x 5 under 8192:
+ * 167 against 637); below, specdec_attention is faster.  Up to 1024 sequences;
+ * workspace, capture and determinism as for specdec_attention_prompt (the size
+ * does not fall where B, R, n_groups or max_blocks grows; with groups, at most
+ * 2 B R + 8192 rows of n_q_heads * (head_dim + 2) floats, without 2 B R less). */
 size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads, int n_kv_heads,
                                                        int head_dim, int max_blocks);
 int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,

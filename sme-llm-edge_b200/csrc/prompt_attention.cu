@@ -68,8 +68,10 @@ namespace specdec {
 
 constexpr int kRowsMaxSeqs = 1024;   // sequences of a call: the plan's tables live in shared memory
 constexpr int kRowsMaxSplits = 32;   // pieces of one key range
-// Up to so many segments are kept in shared memory and taken longest first (128 x 5 rows under 8192 tokens, 129
-// segments: 150 us, unsorted 155; 200 single rows on 4096 tokens: 184 and 180).
+// Up to so many segments are kept in shared memory (it holds no more beside the tiles, and their places are bytes) and
+// taken longest first.  Sorted and as they come, in us: 128 x 5 rows under 8192 tokens (129 segments) 143.6 and 148.5;
+// 256 single rows on 64 to 16,384 tokens 152 and 158, on 4096 tokens each 199 and 196.5.  Of 257, as they come and read
+// from global memory for every item, the same calls take 158 and 200.
 constexpr int kRowsSorted = 256;
 constexpr int kRowsThreads = 384;
 constexpr int kRowsMmaWarp = 8, kRowsLoadWarp = 9, kRowsFixWarp = 10, kRowsSchedWarp = 11;
@@ -344,7 +346,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
         __syncthreads();
     }
     // pieces of about a quarter of a CTA's share; of half of it where they have many rows (128 x 5 rows under 8192
-    // tokens: 158 us, with a third 168, with three quarters 179)
+    // tokens: 144 us, with a third 158, with three quarters 171)
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
@@ -605,8 +607,8 @@ __device__ __forceinline__ float rows_max3(float a, float b, float c) {
     return d;
 }
 // 2^x on the special-function unit (2 ulp); the result is rounded to fp16 next.
-// A quarter of them by a polynomial on the FMA units instead cost 5% (8192-token
-// prompt 559 us against 532): that unit is 44% busy there, and the code grows.
+// A quarter of them by a polynomial on the FMA units instead made an 8192-token
+// prompt 5% slower: that unit is 44% busy there, and the code grows.
 __device__ __forceinline__ uint64_t exp2_unit2(uint64_t x) {
     float x0, x1, y0, y1;
     unpack2(x, x0, x1);
@@ -945,8 +947,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     // Two passes over the scores, 32 columns at a time with the next 32 on
                     // their way.  What counts is code that the instruction cache holds: all
                     // 128 columns unrolled, in one pass with the maximum of the tiles before,
-                    // took 680 us for an 8192-token prompt where this takes 541, and masking
-                    // within the first pass 555.
+                    // took a quarter longer for an 8192-token prompt, and masking within the
+                    // first pass 3%.
                     const int key0 = it.slot0 + 128 * j;
                     const bool masked = key0 + 128 > every;
                     uint64_t seen_lo = ~0ull, seen_hi = ~0ull;
