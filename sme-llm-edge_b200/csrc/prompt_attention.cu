@@ -1291,17 +1291,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     }
 }
 
-// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
-// their order, M being the largest so far.  Bound by L2 and by latency (where the
-// pieces lie, then their results: two loads that wait for one another).  Eight
-// lanes per token row and head; (m, l) and O of four pieces are in flight
-// together, O too before its weight is known.  Against a warp for each row, that
-// first shares out all weights: 128 x 5 rows under 8192 tokens 171 -> 162 us a
-// call, 16 x 21 under 2048 61 -> 57; two or eight pieces at a time, or 16 lanes a
-// row, gain in one case what they lose in another.  The CTAs go round the rows:
-// one for every few rows cost 12 us where no row has pieces.
-// The same where a piece holds an infinity or a NaN (its l is negative or NaN):
-// they stay, whatever the piece's weight.
+// A row's merge (below) where a piece holds an infinity or a NaN (its l is
+// negative or NaN): they stay, whatever the piece's weight.
 template <int HD>
 __device__ __noinline__ void rows_merge_nonfinite(const RowsArgs& a, const RowsMeta mt, int i, int tok, int head) {
     const int n = mt.n_pre + mt.n_own;
@@ -1332,6 +1323,15 @@ __device__ __noinline__ void rows_merge_nonfinite(const RowsArgs& a, const RowsM
     }
 }
 
+// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in
+// their order, M being the largest so far.  Bound by L2 and by latency (where the
+// pieces lie, then their results: two loads that wait for one another).  Eight
+// lanes per token row and head; (m, l) and O of four pieces are in flight
+// together, O too before its weight is known.  Against a warp for each row, that
+// first shares out all weights: 128 x 5 rows under 8192 tokens 171 -> 162 us a
+// call, 16 x 21 under 2048 61 -> 57; two or eight pieces at a time, or 16 lanes a
+// row, gain in one case what they lose in another.  The CTAs go round the rows:
+// one for every few rows cost 12 us where no row has pieces.
 template <int HD>
 __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int head) {
     constexpr int K = HD / 32, P = 4;  // 16-byte pieces of a lane's columns; pieces at a time
