@@ -1224,12 +1224,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (!ok) break;
             done_item(k);
         }
-        if (stopped()) {  // the copies in flight land before the CTA leaves
-            for (int s = 0; s < 2; ++s)
-                if (qn[s]) (void)wait(&q_full[s], qn[s] - 1);
-            for (int c = max(0, kc - RING); c < kc; ++c) (void)wait(&k_full[c % RING], c / RING);
-            for (int c = max(0, vc - RING); c < vc; ++c) (void)wait(&v_raw[c % RING], c / RING);
-        }
+        // the copies in flight land before the CTA leaves, also where another role's wait runs out after this
+        for (int s = 0; s < 2; ++s)
+            if (qn[s]) (void)wait(&q_full[s], qn[s] - 1);
+        for (int c = max(0, kc - RING); c < kc; ++c) (void)wait(&k_full[c % RING], c / RING);
+        for (int c = max(0, vc - RING); c < vc; ++c) (void)wait(&v_raw[c % RING], c / RING);
     } else if (warp == kRowsFixWarp) {
         // ------------------------------------------------------------ V made safe
         int vc = 0;
