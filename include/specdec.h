@@ -365,6 +365,62 @@ int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer,
                                     int n_groups, int B, int R, int n_q_heads, uint16_t* out, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* Causal attention of packed rows, as specdec_attention_prompt, whose rows see
+ * a window and the first tokens: the row in slot p sees slot j iff j <= p and
+ * (j < sinks or j > p - window).  window >= 1, sinks >= 0 (a window that
+ * reaches the first slot is plain causal attention).  The other arguments,
+ * what rows without a sequence hold and the treatment of slots that a row does
+ * not see are specdec_attention_prompt's; pages of which no row of a sequence
+ * sees a slot are not read, so their table entries may be anything (-1 where
+ * they were given back).  Rows keep their slots: a slot is a position here.
+ * Single tokens and prompts are both served by this call. */
+size_t specdec_attention_window_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
+                                                int max_blocks);
+int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
+                             int head_dim, const int32_t* tables, int max_blocks, const int32_t* ctx_len,
+                             const int32_t* row_off, int B, int T, int n_q_heads, int window, int sinks,
+                             uint16_t* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/* specdec_attention_prompt that also adds up what weight each slot received:
+ * weights[b][h][j] += the sum, over sequence b's rows that see slot j and the
+ * query heads of KV head h, of the row's softmax weight of j.  weights fp32
+ * [B, n_kv_heads, ldw] (ldw >= max_blocks * 16, a multiple of 4, 16-byte
+ * aligned); entries of slots that no row sees stay as they are.  A step's
+ * single tokens keep a running sum; the last rows of a prompt (ctx_len the
+ * tokens before them) weigh the whole prompt.  Layers may add into the same
+ * weights one after another.  The sums run in a fixed order: the result is
+ * deterministic.  Up to 32 query heads for each KV head, and 16 rows a
+ * sequence are what it is made for; T <= 65536.  The rest as for
+ * specdec_attention_prompt. */
+size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
+                                                    int max_blocks);
+int specdec_attention_accumulate(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
+                                 int head_dim, const int32_t* tables, int max_blocks, const int32_t* ctx_len,
+                                 const int32_t* row_off, int B, int T, int n_q_heads, float* weights, int ldw,
+                                 uint16_t* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What stands between the projection and the attention: the queries and keys
+ * of packed rows are normed per head and rotated, and keys and values go into
+ * their slots.  Row r of qkv is [q | k | v] (n_q_heads, n_kv_heads, n_kv_heads
+ * heads of head_dim; fp32, or fp16 with qkv_f16 = 1; row stride ldqkv in
+ * elements).  y = x / sqrt(mean(x^2) + eps) * norm for each head of q and k
+ * (q_norm / k_norm fp32 [head_dim], NULL: not normed); then the pairs (d, d +
+ * rot_dim / 2), d < rot_dim / 2, become (a cos - b sin, b cos + a sin) with
+ * row pos[r] of the tables cos_t / sin_t [max_pos, rot_dim / 2] (fp32; pos
+ * NULL: the row's slot; a position outside the tables takes the nearest row;
+ * rot_dim 0: no rotation, else a multiple of 16); all in 32 bits, rounded to
+ * fp16 once.  Rows, sequences and slots are specdec_attention_prompt's:
+ * sequence b owns rows row_off[b] .. row_off[b+1]-1, and its row i goes into
+ * slot ctx_len[b] + i of the pages of tables[b].  q_out [T, n_q_heads,
+ * head_dim] fp16 with row stride ldq.  Rows of no sequence are left alone; a
+ * row whose slot has no page in the pool writes its queries only.  Positions
+ * and slots part when tokens were evicted (specdec_kv_evict_pages). */
+int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, const float* q_norm, const float* k_norm,
+                            float eps, const float* cos_t, const float* sin_t, int max_pos, int rot_dim,
+                            const int32_t* pos, uint16_t* kv_layer, int num_blocks, int n_kv_heads, int head_dim,
+                            const int32_t* tables, int max_blocks, const int32_t* ctx_len, const int32_t* row_off,
+                            int B, int T, int n_q_heads, uint16_t* q_out, int ldq, void* stream);
+
 /* ===================================================================== */
 /* 3. Paged KV block manager (device resident).  Mirrors PagedKVCache      */
 /*    (server/paged_kv_cache.h:28-63): lowest-free-index allocation with   */
@@ -405,6 +461,42 @@ int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t* lens, int
                           int max_reqs, int max_blocks, const int32_t* src, const int32_t* dst, int n, uint16_t* kv,
                           int layers, size_t layer_stride, int n_kv_heads, int head_dim, int32_t* status,
                           void* workspace, size_t workspace_bytes, void* stream);
+/* Eviction by weight: each request reqs[i], i < n, that holds more than `keep`
+ * tokens keeps its first `first`, its last `last` and, of the others, the
+ * heaviest, `keep` in all (first + last <= keep).  A token's weight is the sum
+ * over the weight_heads rows of weights[request] (fp32 [max_reqs,
+ * weight_heads, ldw], as specdec_attention_accumulate leaves them), taken in
+ * 64 bits and rounded to 32; of equal weights the lower slot stays; NaN is
+ * above all numbers.  The tokens that stay keep their order and move up to
+ * slots 0 .. keep-1, in all `layers` layers of the pool (as for
+ * specdec_kv_fork; 0: tables and weights only) and in the weights, whose
+ * entries from slot `keep` on become 0.  Pages behind are released; a page
+ * that a token moves into and that others hold too is replaced by a free one
+ * (the lowest, in the order of the call; pages that this call releases are not
+ * free yet).  Keys stay rotated by the positions they were written with.
+ * kept [n, keep] int32 (may be NULL) receives the former slot of each token
+ * that stays, -1 behind (requests of up to `keep` tokens: 0, 1, ..): the way to
+ * carry what the caller holds for each slot.  tables, n_blocks, lens and
+ * refcounts are specdec_kv_fork_pages's.  All or nothing: *status (device)
+ * receives SPECDEC_OK, SPECDEC_EINVAL (an id out of range or named twice, a
+ * request without a table or with entries outside the pool, or tokens that its
+ * pages or ldw do not hold) or SPECDEC_ENOMEM; only OK changes anything (kept
+ * aside).  No host synchronisation; may be captured.  Calls in flight at the
+ * same time need workspaces (16-byte aligned) of their own.  The reference
+ * names this evict_least_important_blocks (server/paged_kv_cache.cpp:207-228)
+ * and drops a request's last blocks. */
+size_t specdec_kv_evict_pages_workspace_bytes(int num_blocks, int max_reqs, int max_blocks, int n, int keep);
+int specdec_kv_evict_pages(int32_t* tables, int32_t* n_blocks, int32_t* lens, int32_t* refcounts, int num_blocks,
+                           int max_reqs, int max_blocks, const int32_t* reqs, int n, int keep, int first, int last,
+                           float* weights, int weight_heads, int ldw, uint16_t* kv, int layers, size_t layer_stride,
+                           int n_kv_heads, int head_dim, int32_t* kept, int32_t* status, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* The same on the manager's tables: reqs a host array, weights [max_reqs,
+ * weight_heads, ldw] and kept (may be NULL) in device memory.  Synchronises
+ * the stream; EINVAL and ENOMEM change nothing. */
+int specdec_kv_evict(specdec_kv* kv, const int32_t* reqs, int n, int keep, int first, int last, float* weights,
+                     int weight_heads, int ldw, uint16_t* pool, int layers, size_t layer_stride, int n_kv_heads,
+                     int head_dim, int32_t* kept, void* stream);
 int specdec_kv_free_merged_blocks(specdec_kv* kv, int req, int n_blocks, void* stream);
 int specdec_kv_evict_tokens(specdec_kv* kv, int req, int n_tokens, int* evicted, void* stream);
 /* Token-granular rollback: new lengths (host array, -1 = unchanged); tail

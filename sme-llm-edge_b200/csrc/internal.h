@@ -126,6 +126,14 @@ int kv_fork_launch(const KVState& st, const int32_t* src, const int32_t* dst, in
                    size_t layer_stride, int Hkv, int hd, int32_t* status, void* ws, cudaStream_t s);
 int kv_fork_check_pool(const char* who, const void* kv, int layers, size_t layer_stride, int num_blocks, int Hkv, int hd);
 
+// Eviction by weight (kv_evict.cu); layers 0: tables and weights only.
+size_t kv_evict_workspace(int max_bpr, int block_size, int n, int keep);
+int kv_evict_check(const char* who, int max_reqs, int n, int keep, int first, int last, const float* weights, int wheads,
+                   int ldw);
+int kv_evict_launch(const KVState& st, const int32_t* reqs, int n, int keep, int first, int last, float* weights,
+                    int wheads, int ldw, __half* kv, int layers, size_t layer_stride, int Hkv, int hd, int32_t* kept,
+                    int32_t* status, void* ws, cudaStream_t s);
+
 // ------------------------------------------------------------ .sme weights
 // Rows of a source weight on the device: int8 with the writer's per-row
 // factor (value = q / rs) or fp32; fold = optional per-column multiplier

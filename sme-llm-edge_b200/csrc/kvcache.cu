@@ -201,6 +201,8 @@ struct specdec_kv {
     int32_t* h_tmp = nullptr;  // pinned staging
     int32_t* d_tmp = nullptr;  // device staging [3 * max_reqs + 8]
     int32_t* d_fork = nullptr;  // workspace of a fork
+    void* d_evict = nullptr;    // workspace of an eviction, made by the first and grown
+    size_t evict_bytes = 0;
 };
 
 namespace specdec {
@@ -265,6 +267,7 @@ extern "C" int specdec_kv_destroy(specdec_kv* kv) {
     cudaFree(s.status);
     cudaFree(kv->d_tmp);
     cudaFree(kv->d_fork);
+    cudaFree(kv->d_evict);
     cudaFreeHost(kv->h_tmp);
     delete kv;
     return SPECDEC_OK;
@@ -341,6 +344,46 @@ extern "C" int specdec_kv_fork(specdec_kv* kv, const int32_t* src_reqs, const in
     SD_CHECK(h[0] != SPECDEC_EINVAL, SPECDEC_EINVAL,
              "kv_fork: a request id out of range, a source without a table, or a target named twice or also a source");
     SD_CHECK(h[0] != SPECDEC_ENOMEM, SPECDEC_ENOMEM, "kv_fork: KV block pool exhausted (nothing was changed)");
+    return SPECDEC_OK;
+}
+
+extern "C" int specdec_kv_evict(specdec_kv* kv, const int32_t* reqs, int n, int keep, int first, int last, float* weights,
+                                int weight_heads, int ldw, uint16_t* pool, int layers, size_t layer_stride,
+                                int n_kv_heads, int head_dim, int32_t* kept, void* stream) {
+    SD_CHECK(kv && (n <= 0 || reqs), SPECDEC_EINVAL, "kv_evict: bad argument");
+    int rc = kv_evict_check("kv_evict", kv->s.max_reqs, n, keep, first, last, weights, weight_heads, ldw);
+    if (!rc) rc = kv_fork_check_pool("kv_evict", pool, layers, layer_stride, kv->s.num_blocks, n_kv_heads, head_dim);
+    if (rc) return rc;
+    SD_CHECK(layers == 0 || kv->s.block_size == 16, SPECDEC_EINVAL, "kv_evict: a pool's blocks hold 16 tokens");
+    if (n == 0) return SPECDEC_OK;
+    if ((rc = check_on_device(weights, "kv_evict: weights"))) return rc;
+    if (layers > 0 && (rc = check_on_device(pool, "kv_evict: the pool"))) return rc;
+    if (kept && (rc = check_on_device(kept, "kv_evict: kept"))) return rc;
+    cudaStream_t s = as_stream(stream);
+    const size_t need = kv_evict_workspace(kv->s.max_bpr, kv->s.block_size, n, keep);
+    if (need > kv->evict_bytes) {
+        cudaFree(kv->d_evict);  // waits for what still uses it
+        kv->d_evict = nullptr;
+        kv->evict_bytes = 0;
+        const cudaError_t e = cudaMalloc(&kv->d_evict, need);
+        if (e != cudaSuccess) return cuda_status(e, "kv_evict");
+        kv->evict_bytes = need;
+    }
+    int32_t* h = kv->h_tmp;
+    for (int i = 0; i < n; ++i) h[i] = reqs[i];
+    SD_CUDA(cudaMemcpyAsync(kv->d_tmp, h, sizeof(int32_t) * n, cudaMemcpyHostToDevice, s));
+    int32_t* d_status = kv->d_tmp + n;
+    rc = kv_evict_launch(kv->s, kv->d_tmp, n, keep, first, last, weights, weight_heads, ldw,
+                         reinterpret_cast<__half*>(pool), layers, layer_stride, n_kv_heads, head_dim, kept, d_status,
+                         kv->d_evict, s);
+    cudaError_t e = cudaMemcpyAsync(h, d_status, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (rc) return rc;
+    if (e != cudaSuccess) return cuda_status(e, "kv_evict");
+    SD_CHECK(h[0] != SPECDEC_EINVAL, SPECDEC_EINVAL,
+             "kv_evict: a request id out of range or named twice, or a request without a table or with more tokens than "
+             "its blocks or ldw hold");
+    SD_CHECK(h[0] != SPECDEC_ENOMEM, SPECDEC_ENOMEM, "kv_evict: KV block pool exhausted (nothing was changed)");
     return SPECDEC_OK;
 }
 

@@ -1,0 +1,232 @@
+// qk_norm_rope.cu -- queries and keys of packed rows normed per head and
+// rotated, keys and values into their pages: what stands between the fused QKV
+// projection and the attention calls (specdec_qk_norm_rope_kv).
+//
+// For each head x of q and k, in 32 bits and rounded to fp16 once:
+//   y = x / sqrt(mean(x^2) + eps) * w
+//   (y_d, y_{d + r/2}) -> (y_d c_d - y_{d + r/2} s_d, y_{d + r/2} c_d + y_d s_d), d < r/2
+// A row's values are read once and written once; HBM bounds many rows, the chain
+// bounds -> sequence -> page number -> store a few.
+//
+// head_dim / 8 lanes hold a head, 8 values each, so that an fp16 head is loaded
+// and stored in 16-byte pieces, and 2 (head_dim 128) or 4 heads are in a warp.
+// The sum of squares and the pair's other half come by shuffles (r / 16 lanes
+// away).
+#include "common.cuh"
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace specdec {
+
+constexpr int kNormMaxSeqs = 1024;
+constexpr int kNormWarps = 8;
+
+struct NormArgs {
+    const void* qkv;
+    int ld;
+    const float* qw;
+    const float* kw;
+    float eps;
+    const float* cos_t;
+    const float* sin_t;
+    int max_pos, half;  // half: pairs of a head that rotate
+    const int32_t* pos;
+    __half* kv;
+    int num_blocks, Hkv, Hq;
+    const int32_t* tables;
+    int max_blocks;
+    const int32_t* ctx_len;
+    const int32_t* row_off;
+    int B, T;
+    __half* q_out;
+    int ldq;
+    int parts;  // warps of a row
+};
+
+// The sequence of packed row r, -1 where it has none: bounds in two rounds of 32.
+__device__ __forceinline__ int norm_sequence(const NormArgs& a, int r) {
+    const int lane = threadIdx.x & 31, step = (a.B + 31) / 32;
+    auto below = [&](int b) { return b < a.B && a.row_off[b + 1] <= r; };  // sequence b ends before the row
+    const int c = __popc(__ballot_sync(0xffffffffu, (lane + 1) * step <= a.B && below((lane + 1) * step - 1)));
+    const int b = c * step + __popc(__ballot_sync(0xffffffffu, lane < step && below(c * step + lane)));
+    return b < a.B && a.row_off[b] <= r ? b : -1;
+}
+
+template <typename In>
+__device__ __forceinline__ void norm_load(const In* src, float (&x)[8]) {
+    if constexpr (sizeof(In) == 4) {
+        const float4 u = __ldcs(reinterpret_cast<const float4*>(src)), v = __ldcs(reinterpret_cast<const float4*>(src) + 1);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+        x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(src));
+        const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(h[e]);
+            x[2 * e] = f.x, x[2 * e + 1] = f.y;
+        }
+    }
+}
+__device__ __forceinline__ void norm_load8(const float* src, float (&x)[8]) {
+    const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 4);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+}
+
+template <int HD, typename In>
+__global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int LPH = HD / 8, HS = 32 / LPH;  // lanes of a head, heads of a warp at a time
+    const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH, d0 = 8 * l;
+    const long long w = (long long)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
+    const int r = (int)(w / a.parts), part = (int)(w % a.parts);
+    if (r >= a.T) return;
+    const int heads = a.Hq + 2 * a.Hkv;
+    const In* row = static_cast<const In*>(a.qkv) + (size_t)r * a.ld;
+    const int b = norm_sequence(a, r);
+    if (b < 0) return;
+    const int slot = max(0, min(a.ctx_len[b], 1 << 30)) + (r - max(0, a.row_off[b]));
+    const int page = slot < a.max_blocks * 16 ? a.tables[(size_t)b * a.max_blocks + (slot >> 4)] : -1;
+    const bool paged = page >= 0 && page < a.num_blocks;
+    // what this lane's values turn by: its pairs are pair0 .. pair0 + 7 of the head
+    const bool turns = d0 < 2 * a.half;
+    const bool upper = d0 >= a.half;
+    const int away = a.half / 8;  // lanes to the pair's other half
+    float c[8], s[8];
+    if (turns) {
+        const int p = max(0, min(a.pos ? a.pos[r] : slot, a.max_pos - 1));
+        const size_t at = (size_t)p * a.half + (upper ? d0 - a.half : d0);
+        norm_load8(a.cos_t + at, c);
+        norm_load8(a.sin_t + at, s);
+    }
+    float qw[8], kw[8];
+    if (a.qw) norm_load8(a.qw + d0, qw);
+    if (a.kw) norm_load8(a.kw + d0, kw);
+    for (int h0 = part * HS; h0 < heads; h0 += a.parts * HS) {
+        const int h = h0 + sub;
+        const bool real = h < heads, is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
+        float x[8] = {};
+        if (real) norm_load(row + (size_t)h * HD + d0, x);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+        for (int o = LPH / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((is_q && a.qw) || (is_k && a.kw)) {
+            const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (is_q ? qw[e] : kw[e]);
+        }
+        const int other = sub * LPH + (upper ? l - away : l + away);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], turns ? other : lane);
+        if (turns && (is_q || is_k)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = upper ? x[e] * c[e] + y[e] * s[e] : x[e] * c[e] - y[e] * s[e];
+        }
+        uint4 out;
+        __half2* o2 = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o2[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        if (!real) continue;
+        if (is_q) {
+            *reinterpret_cast<uint4*>(a.q_out + (size_t)r * a.ldq + (size_t)h * HD + d0) = out;
+        } else if (paged) {
+            const int kvh = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
+            __half* dst = a.kv + ((((size_t)page * 2 + (is_k ? 0 : 1)) * a.Hkv + kvh) * 16 + (slot & 15)) * HD + d0;
+            *reinterpret_cast<uint4*>(dst) = out;
+        }
+    }
+}
+
+}  // namespace specdec
+
+using namespace specdec;
+
+extern "C" int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, const float* q_norm,
+                                       const float* k_norm, float eps, const float* cos_t, const float* sin_t,
+                                       int max_pos, int rot_dim, const int32_t* pos, uint16_t* kv_layer, int num_blocks,
+                                       int n_kv_heads, int head_dim, const int32_t* tables, int max_blocks,
+                                       const int32_t* ctx_len, const int32_t* row_off, int B, int T, int n_q_heads,
+                                       uint16_t* q_out, int ldq, void* stream) {
+    const char* who = "qk_norm_rope_kv";
+    const std::string w(who);
+    const bool empty = B == 0 || T == 0;  // an empty call's tensors may have no memory
+    SD_CHECK(empty || (qkv && kv_layer && tables && ctx_len && row_off && q_out && (rot_dim == 0 || (cos_t && sin_t))),
+             SPECDEC_EINVAL, w + ": null argument");
+    SD_CHECK(qkv_f16 == 0 || qkv_f16 == 1, SPECDEC_EINVAL, w + ": qkv_f16 is 0 (fp32) or 1 (fp16)");
+    SD_CHECK(head_dim == 64 || head_dim == 128, SPECDEC_EINVAL, w + ": head_dim must be 64 or 128");
+    SD_CHECK(n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0 && n_q_heads <= 1024, SPECDEC_EINVAL,
+             w + ": bad head counts (at most 1024 query heads)");
+    SD_CHECK(num_blocks > 0 && max_blocks > 0 && max_blocks <= (1 << 26), SPECDEC_EINVAL, w + ": empty block pool or table");
+    SD_CHECK(B >= 0 && B <= kNormMaxSeqs && T >= 0 && T <= (1 << 24), SPECDEC_EINVAL,
+             w + ": 0 to 1024 sequences and 0 to 2^24 rows");
+    SD_CHECK(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 16 == 0 && (rot_dim == 0 || max_pos > 0), SPECDEC_EINVAL,
+             w + ": rot_dim is a multiple of 16 up to head_dim, with a table of at least one position");
+    SD_CHECK(eps >= 0.f && eps < INFINITY, SPECDEC_EINVAL, w + ": eps must be finite and not negative");
+    const int per16 = qkv_f16 ? 8 : 4;
+    SD_CHECK(ldqkv >= (n_q_heads + 2 * n_kv_heads) * head_dim && ldqkv % per16 == 0 && ldq >= n_q_heads * head_dim &&
+                 ldq % 8 == 0,
+             SPECDEC_EINVAL, w + ": row strides hold all heads and are multiples of 16 bytes");
+    SD_CHECK(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(kv_layer) |
+               reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_norm) |
+               reinterpret_cast<uintptr_t>(k_norm) | reinterpret_cast<uintptr_t>(cos_t) |
+               reinterpret_cast<uintptr_t>(sin_t)) &
+              15) == 0,
+             SPECDEC_EINVAL, w + ": qkv, norms, cos / sin tables, KV pool and q_out must be 16-byte aligned");
+    if (empty) return SPECDEC_OK;
+    const struct {
+        const void* p;
+        const char* what;
+    } given[] = {{qkv, "qk_norm_rope_kv: qkv"},
+                 {kv_layer, "qk_norm_rope_kv: the KV pool"},
+                 {q_out, "qk_norm_rope_kv: q_out"},
+                 {tables, "qk_norm_rope_kv: tables"},
+                 {ctx_len, "qk_norm_rope_kv: ctx_len"},
+                 {row_off, "qk_norm_rope_kv: row_off"},
+                 {q_norm ? q_norm : qkv, "qk_norm_rope_kv: q_norm"},
+                 {k_norm ? k_norm : qkv, "qk_norm_rope_kv: k_norm"},
+                 {rot_dim ? (const void*)cos_t : qkv, "qk_norm_rope_kv: cos_t"},
+                 {rot_dim ? (const void*)sin_t : qkv, "qk_norm_rope_kv: sin_t"},
+                 {pos && rot_dim ? (const void*)pos : qkv, "qk_norm_rope_kv: pos"}};
+    int rc;
+    for (const auto& g : given)
+        if ((rc = check_on_device(g.p, g.what))) return rc;
+    NormArgs a = {};
+    a.qkv = qkv;
+    a.ld = ldqkv;
+    a.qw = q_norm;
+    a.kw = k_norm;
+    a.eps = eps;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.max_pos = max_pos;
+    a.half = rot_dim / 2;
+    a.pos = pos;
+    a.kv = reinterpret_cast<__half*>(kv_layer);
+    a.num_blocks = num_blocks;
+    a.Hkv = n_kv_heads;
+    a.Hq = n_q_heads;
+    a.tables = tables;
+    a.max_blocks = max_blocks;
+    a.ctx_len = ctx_len;
+    a.row_off = row_off;
+    a.B = B;
+    a.T = T;
+    a.q_out = reinterpret_cast<__half*>(q_out);
+    a.ldq = ldq;
+    a.parts = 1;
+    const long long warps = (long long)T * a.parts;
+    const unsigned grid = (unsigned)((warps + kNormWarps - 1) / kNormWarps);
+    cudaStream_t s = as_stream(stream);
+    if (head_dim == 128) {
+        if (qkv_f16) qk_norm_rope_kernel<128, __half><<<grid, 32 * kNormWarps, 0, s>>>(a);
+        else qk_norm_rope_kernel<128, float><<<grid, 32 * kNormWarps, 0, s>>>(a);
+    } else {
+        if (qkv_f16) qk_norm_rope_kernel<64, __half><<<grid, 32 * kNormWarps, 0, s>>>(a);
+        else qk_norm_rope_kernel<64, float><<<grid, 32 * kNormWarps, 0, s>>>(a);
+    }
+    SD_LAUNCH_CHECK("qk_norm_rope_kernel");
+    return SPECDEC_OK;
+}

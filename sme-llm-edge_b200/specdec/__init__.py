@@ -115,6 +115,11 @@ _SIGS = {
     "specdec_attention_prompt": (I, [P, I, P, I, I, I, P, I, P, P, I, I, I, P, I, P, SZ, P]),
     "specdec_attention_shared_prefix_workspace_bytes": (SZ, [I, I, I, I, I, I, I]),
     "specdec_attention_shared_prefix": (I, [P, P, I, I, I, P, I, P, P, P, P, I, I, I, I, P, P, SZ, P]),
+    "specdec_attention_window_workspace_bytes": (SZ, [I, I, I, I, I, I]),
+    "specdec_attention_window": (I, [P, I, P, I, I, I, P, I, P, P, I, I, I, I, I, P, I, P, SZ, P]),
+    "specdec_attention_accumulate_workspace_bytes": (SZ, [I, I, I, I, I, I]),
+    "specdec_attention_accumulate": (I, [P, I, P, I, I, I, P, I, P, P, I, I, I, P, I, P, I, P, SZ, P]),
+    "specdec_qk_norm_rope_kv": (I, [P, I, I, P, P, F, P, P, I, I, P, P, I, I, I, P, I, P, P, I, I, I, P, I, P]),
     "specdec_kv_create": (I, [I, I, I, I, C.POINTER(P)]),
     "specdec_kv_destroy": (I, [P]),
     "specdec_kv_append": (I, [P, P, P, I, P, P]),
@@ -123,6 +128,9 @@ _SIGS = {
     "specdec_kv_fork": (I, [P, P, P, I, P, I, SZ, I, I, P]),
     "specdec_kv_fork_pages_workspace_bytes": (SZ, [I, I, I]),
     "specdec_kv_fork_pages": (I, [P, P, P, P, I, I, I, P, P, I, P, I, SZ, I, I, P, P, SZ, P]),
+    "specdec_kv_evict_pages_workspace_bytes": (SZ, [I, I, I, I, I]),
+    "specdec_kv_evict_pages": (I, [P, P, P, P, I, I, I, P, I, I, I, I, P, I, I, P, I, SZ, I, I, P, P, P, SZ, P]),
+    "specdec_kv_evict": (I, [P, P, I, I, I, I, P, I, I, P, I, SZ, I, I, P, P]),
     "specdec_kv_free_merged_blocks": (I, [P, I, I, P]),
     "specdec_kv_evict_tokens": (I, [P, I, I, C.POINTER(I), P]),
     "specdec_kv_truncate": (I, [P, P, I, P]),
@@ -393,6 +401,16 @@ class PagedKVCache:
         if src.size != new.size:
             raise ValueError("fork: one source for each new request")
         check(_lib.specdec_kv_fork(self._h, _p(src), _p(new), src.size, None, 0, 0, 0, 0, None))
+
+    def evict_by_weight(self, request_ids, keep: int, first: int, last: int, weights, weight_heads: int, ldw: int,
+                        kept=None):
+        """Each request keeps its first `first`, its last `last` and its
+        heaviest other tokens, `keep` in all (tables and weights only; the K/V
+        payload lives in the engine's pool).  weights: device pointer of fp32
+        [max_requests, weight_heads, ldw]; kept: of int32 [n, keep], or None."""
+        reqs = np.ascontiguousarray(request_ids, dtype=np.int32).reshape(-1)
+        check(_lib.specdec_kv_evict(self._h, _p(reqs), reqs.size, keep, first, last, weights, weight_heads, ldw, None,
+                                    0, 0, 0, 0, kept, None))
 
     def free_merged_blocks(self, request_id: int, num_blocks_to_free: int):
         check(_lib.specdec_kv_free_merged_blocks(self._h, request_id, num_blocks_to_free, None))
