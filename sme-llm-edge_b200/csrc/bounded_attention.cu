@@ -4,10 +4,15 @@
 //
 // With x = q.k / sqrt(hd) over the slots that a row sees, m = max x:
 //   l = sum e^(x - m),  out = sum e^(x - m) v / l,  weights[slot] += e^(x - m) / l.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "internal.h"
+#include "ptx.cuh"
 
 namespace specdec {
 
@@ -23,11 +28,8 @@ struct BoundArgs {
     const int32_t* ctx_len;
     const int32_t* row_off;
     int B, T, window, sinks;
-    float* weights;
-    int ldw;
     __half* out;
     int ldo;
-    float2* ml;  // [T][Hq] a row's largest x and sum (accumulate)
     float scale;
 };
 
@@ -99,34 +101,863 @@ __global__ void __launch_bounds__(256) bound_rows_kernel(const __grid_constant__
         if (fabsf(y) > 65504.f) y = copysignf(65504.f, y);
         a.out[(size_t)r * a.ldo + (size_t)head * HD + lane * W + e] = __float2half_rn(y == y && bad[e] != 0.f ? bad[e] : y);
     }
-    if (a.ml && lane == 0) a.ml[(size_t)r * a.Hq + head] = make_float2(m, l);
 }
 
-// A warp for each slot of a sequence's KV head.
+// ------------------------------------------------------------------ few rows
+//
+// A warp works for itself: it streams pages (16 tokens of one KV head, K and V
+// together, one TMA request) through a ring of its own, so no barrier of the CTA
+// stands between its loads and its arithmetic.  The call's pages, in the order
+// (sequence, tile of rows, KV head, page), are cut into equal ranges, one for
+// each warp of the grid: ragged lengths balance by themselves.  A tile is as many
+// whole tokens as fit into 8 * NT rows (row = token * G + g).  For a page
+//   S^T [16 keys][rows] = K Q^T,  P = 2^(S' - m + 15),  O^T [hd][rows] += V^T P
+// in mma.sync of 16 x 8 x 16: 16 keys of 8 rows are 4 FLOP for each byte of the
+// cache, far from what the tensor cores of either kind can do, and the fragments
+// stay in registers (128 rows of tensor memory for 4 to 32 real ones would not).
+// A row's largest score m is exact after each page, and 15 takes the largest
+// weight to fp16's upper end: weights keep their 11 bits down to 2^-29 of it.
+// m, sums and O are fp32.
+//
+// Ranges that a warp shares with others leave unnormalised O with (m, l); they
+// are joined in their order.
+constexpr int kFewWarps = 8;
+constexpr int kFewMaxCtas = 148;   // ranges: at most so many CTAs of warps
+constexpr int kFewMaxRows = 32;    // rows of a tile
+constexpr int kFewMinPages = 4;    // of a range
+constexpr float kFewLift = 15.0f;
+constexpr float kFewMax = 65504.0f;
+
+struct FewArgs {
+    const __half* q;
+    int ldq;
+    const __half* kv;
+    int num_blocks, Hkv, Hq, G, tpt;  // tpt: tokens of a tile
+    const int32_t* tables;
+    int max_blocks, slots_max;
+    const int32_t* ctx_len;
+    const int32_t* row_off;
+    int B, T, window, sinks;
+    float* weights;
+    int ldw;
+    __half* out;
+    int ldo;
+    float scale_log2;
+    int ranges;
+    // workspace
+    long long* pre;     // [B + 1] pages before sequence b, then the pages of a range
+    int32_t* np;        // [B] pages of each (tile, head) of sequence b
+    int32_t* chunks;    // [B + 1] chunks of slots before sequence b (weights)
+    float2* pml;        // [2 * ranges][rows] m, l of a piece (l < 0: it met an infinity or NaN of V)
+    float* po;          // [2 * ranges][rows][hd]
+    float2* ml;         // [T][Hq] m, 1 / l (weights)
+    float* scores;      // [T][Hkv][slots_max][G] (weights)
+    DeviceStatus* status;
+};
+
+struct FewSeq {
+    int lo, n, ctx;
+};
+__device__ __forceinline__ FewSeq few_seq(const FewArgs& a, int b) {
+    FewSeq s;
+    s.lo = max(0, min(a.row_off[b], a.T));
+    s.n = max(s.lo, min(a.row_off[b + 1], a.T)) - s.lo;
+    s.ctx = max(0, min(a.ctx_len[b], 1 << 30));
+    return s;
+}
+// Pages of a sequence's tile at most.
+__device__ __forceinline__ int few_pages(const FewArgs& a, const FewSeq& s) {
+    const int last = (min(s.ctx + s.n, a.slots_max) + 15) >> 4;
+    const long long most = ((long long)min(a.sinks, a.slots_max) + 15) / 16 + ((long long)a.window + a.tpt - 2) / 16 + 2;
+    return max(1, (int)min((long long)last, most));
+}
+
+// What tile `tile` of a sequence reads: pages 0 .. sinkp - 1 of its table, and
+// from there on page v + gap.
+struct FewTile {
+    int tokens, row, p0;  // its tokens, first packed row, first row's slot
+    int np, sinkp, gap;
+};
+__device__ __forceinline__ FewTile few_tile(const FewArgs& a, const FewSeq& s, int tile) {
+    FewTile t;
+    const int i0 = tile * a.tpt;
+    t.tokens = min(a.tpt, s.n - i0);
+    t.row = s.lo + i0;
+    t.p0 = s.ctx + i0;
+    const int end = min(t.p0 + t.tokens, a.slots_max);
+    const int wp = max(0, t.p0 - a.window + 1) >> 4, last = (end + 15) >> 4;
+    t.sinkp = (min(a.sinks, end) + 15) >> 4;
+    t.gap = max(0, wp - t.sinkp);
+    t.np = t.gap ? t.sinkp + max(0, last - wp) : last;
+    return t;
+}
+
+// A warp's way through the pages of its range.
+struct FewWalk {
+    long long u, hi;    // next page of the call, end of the range
+    int b, tile, kvh;
+    int v, ve;          // pages of the tile still to come
+    long long begun;    // the segment's first page of the call
+    bool whole;         // the segment is all of the tile's pages
+    FewTile t;
+};
+// To the next segment; false: the range is done.
+__device__ __forceinline__ bool few_next(const FewArgs& a, const long long* pre, const int* np, FewWalk& w) {
+    if (w.u >= w.hi) return false;
+    int lo = 0, hi = a.B;  // last sequence with pre <= u
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= w.u) lo = mid;
+        else hi = mid;
+    }
+    w.b = lo;
+    const long long local = w.u - pre[lo];
+    const int n = np[lo], pair = (int)(local / n);
+    w.v = (int)(local - (long long)pair * n);
+    w.tile = pair / a.Hkv;
+    w.kvh = pair - w.tile * a.Hkv;
+    w.t = few_tile(a, few_seq(a, lo), w.tile);
+    w.begun = w.u;
+    const int take = (int)min((long long)(n - w.v), w.hi - w.u);
+    w.u += take;
+    w.ve = min(w.v + take, w.t.np);
+    w.whole = w.v == 0 && w.ve == w.t.np;
+    return true;
+}
+
+__device__ __forceinline__ void few_mma(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void few_ldm(uint32_t (&x)[4], uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t few_turn(uint32_t x) {  // an 8 x 8 tile of halves, transposed
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float few_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float few_max(float x, float y) {  // NaN if one is
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+
+// Sets the columns of a row in which it sees an infinity or a NaN of V: no weight
+// is 0 by the definition, so they reach the row whatever the weight.  A warp for
+// each row and head.
 template <int HD>
-__global__ void __launch_bounds__(256) bound_weights_kernel(const __grid_constant__ BoundArgs a) {
+__device__ __noinline__ void few_nonfinite(const FewArgs& a, int b, int p, int kvh, __half* dst) {
     constexpr int W = HD / 32;
-    const int lane = threadIdx.x & 31, b = blockIdx.z, kvh = blockIdx.y;
-    const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int r0 = max(0, min(a.row_off[b], a.T)), r1 = max(r0, min(a.row_off[b + 1], a.T));
-    const int ctx = max(0, min(a.ctx_len[b], 1 << 30));
-    if (j >= a.max_blocks * 16 || j >= ctx + (r1 - r0)) return;
-    const __half* k = bound_slot(a, b, j, 0, kvh, HD) + lane * W;
-    float kf[W], sum = 0.f;
+    const int lane = threadIdx.x & 31, last = min(p, a.slots_max - 1);
+    const int from = max(0, p - a.window + 1), first = min(a.sinks, from);
+    float bad[W] = {};
+    bool any = false;
+    for (int j = first > 0 ? 0 : from; j <= last; j = j + 1 == first ? from : j + 1) {
+        const int x = a.tables[(size_t)b * a.max_blocks + (j >> 4)], page = x < 0 || x >= a.num_blocks ? 0 : x;
+        const __half* v = a.kv + ((((size_t)page * 2 + 1) * a.Hkv + kvh) * 16 + (j & 15)) * HD + lane * W;
 #pragma unroll
-    for (int e = 0; e < W; ++e) kf[e] = __half2float(k[e]);
-    for (int r = max(r0, r0 + j - ctx); r < r1; ++r)
-        for (int g = 0; g < a.G; ++g) {
-            const int head = kvh * a.G + g;
-            float x = 0.f;
-#pragma unroll
-            for (int e = 0; e < W; ++e)
-                x = fmaf(__half2float(a.q[(size_t)r * a.ldq + (size_t)head * HD + lane * W + e]) * a.scale, kf[e], x);
-            x = warp_sum(x);
-            const float2 ml = a.ml[(size_t)r * a.Hq + head];
-            sum += ml.y > 0.f || ml.y != ml.y ? expf(x - ml.x) / ml.y : 0.f;
+        for (int e = 0; e < W; ++e) {
+            const float y = __half2float(v[e]);
+            if (!isfinite(y)) {
+                bad[e] += y;
+                any = true;
+            }
         }
-    if (lane == 0) a.weights[((size_t)b * a.Hkv + kvh) * a.ldw + j] += sum;
+    }
+    if (any)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (bad[e] != 0.f) dst[lane * W + e] = __float2half_rn(bad[e]);
+}
+
+template <int HD>
+struct FewCfg {
+    static constexpr int PAGE = 64 * HD;                 // bytes of a page's K and V of a head
+    static constexpr int RING = HD == 128 ? 3 : 6;       // pages in flight of a warp
+    static constexpr size_t smem(int B) {
+        return 1024 + (size_t)kFewWarps * RING * PAGE + kFewWarps * RING * 8 + (size_t)(B + 1) * 8 + (size_t)B * 4 + 16;
+    }
+};
+static_assert(FewCfg<128>::smem(kBoundMaxSeqs) <= 232448 && FewCfg<64>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a CTA");
+
+// Pages before each sequence, by every CTA for itself from the lengths in device
+// memory (so a captured call serves other lengths); CTA 0 leaves them for the
+// kernels that follow.
+__device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, int* np, bool acc) {
+    __shared__ long long wsum[kFewWarps];
+    __shared__ int csum[kFewWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.B + 32 * kFewWarps - 1) / (32 * kFewWarps);
+    const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    long long x = 0;
+    int c = 0;
+    for (int b = b0; b < b1; ++b) {
+        const FewSeq s = few_seq(a, b);
+        const int n = few_pages(a, s);
+        np[b] = n;
+        const long long all = (long long)((s.n + a.tpt - 1) / a.tpt) * a.Hkv * n;
+        pre[b] = all;
+        x += all;
+        if (acc && s.n > 0) c += a.Hkv * ((n + 7) / 8);
+    }
+    const long long mine = x;
+    const int cmine = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        const int d = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) {
+            x += y;
+            c += d;
+        }
+    }
+    if (lane == 31) {
+        wsum[warp] = x;
+        csum[warp] = c;
+    }
+    __syncthreads();
+    long long before = 0, total = 0;
+    int cbefore = 0, ctotal = 0;
+    for (int w = 0; w < kFewWarps; ++w) {
+        if (w == warp) {
+            before = total;
+            cbefore = ctotal;
+        }
+        total += wsum[w];
+        ctotal += csum[w];
+    }
+    before += x - mine;
+    cbefore += c - cmine;
+    for (int b = b0; b < b1; ++b) {
+        const long long all = pre[b];
+        pre[b] = before;
+        if (blockIdx.x == 0) {
+            a.pre[b] = before;
+            a.np[b] = np[b];
+            if (acc) {
+                a.chunks[b] = cbefore;
+                if (all > 0) cbefore += a.Hkv * ((np[b] + 7) / 8);
+            }
+        }
+        before += all;
+    }
+    if (tid == 0) {
+        pre[a.B] = total;
+        if (blockIdx.x == 0) {
+            a.pre[a.B] = total;
+            if (acc) a.chunks[a.B] = ctotal;
+        }
+    }
+    __syncthreads();
+    return total;
+}
+// Pages of a range.
+__device__ __forceinline__ long long few_per(const FewArgs& a, long long total) {
+    return max((long long)kFewMinPages, (total + a.ranges - 1) / a.ranges);
+}
+
+template <int HD, int NT, bool ACC>
+__global__ void __launch_bounds__(32 * kFewWarps, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
+    using C = FewCfg<HD>;
+    constexpr int KS = HD / 16, NH = HD / 64, RING = C::RING;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + kFewWarps * RING * C::PAGE);
+    long long* pre = reinterpret_cast<long long*>(bars + kFewWarps * RING);
+    int* np = reinterpret_cast<int*>(pre + a.B + 1);
+    pdl_trigger();
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring = s_addr(base + warp * RING * C::PAGE), bar = s_addr(bars + warp * RING);
+    if (lane == 0) {
+        for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const long long total = few_plan(a, pre, np, ACC);  // ends with a CTA-wide barrier
+    const long long per = few_per(a, total);
+    // neighbouring ranges on different SMs: a call of few ranges has them to itself
+    const int range = warp * gridDim.x + blockIdx.x;
+    const long long u0 = min(total, range * per), u1 = min(total, u0 + per);
+    if (u0 >= u1) return;
+
+    // ---- loads: as many pages ahead as the ring holds
+    FewWalk ld = {};
+    ld.u = u0;
+    ld.hi = u1;
+    int asked = 0, tb = 0, ent = 0, ent_next = 0;  // pages asked for; table entries tb + lane, tb + 32 + lane
+    bool more = true;
+    auto entry = [&](int v) -> int {
+        if (v >= ld.ve) return 0;
+        const int x = a.tables[(size_t)ld.b * a.max_blocks + (v < ld.t.sinkp ? v : v + ld.t.gap)];
+        return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
+    };
+    auto load = [&]() {
+        while (more && ld.v >= ld.ve) {
+            more = few_next(a, pre, np, ld);
+            if (more) {
+                tb = ld.v;
+                ent = entry(tb + lane);
+                ent_next = entry(tb + 32 + lane);
+            }
+        }
+        if (!more) return;
+        if (ld.v - tb >= 32) {
+            tb += 32;
+            ent = ent_next;
+            ent_next = entry(tb + 32 + lane);
+        }
+        const int page = __shfl_sync(0xffffffffu, ent, ld.v - tb);
+        if (lane == 0) {
+            const uint32_t b = bar + 8 * (asked % RING);
+            mbar_expect_tx(b, C::PAGE);
+            tma_load_5d(ring + (asked % RING) * C::PAGE, &kvmap, 0, ld.kvh * 16, 0, 0, page, b);
+        }
+        ++asked;
+        ++ld.v;
+    };
+    for (int i = 0; i < RING; ++i) load();
+
+    // ---- arithmetic
+    const uint32_t k_row = (uint32_t)(lane & 15), k_chunk = (uint32_t)(lane >> 4);
+    const uint32_t v_row = (uint32_t)((lane & 7) + ((lane >> 4) & 1) * 8), v_chunk = (uint32_t)((lane >> 3) & 1);
+    FewWalk w = {};
+    w.u = u0;
+    w.hi = u1;
+    int done = 0;
+    bool ok = true;
+    while (ok && few_next(a, pre, np, w)) {
+        const FewTile& t = w.t;
+        const int rows = t.tokens * a.G, p1 = t.p0 + t.tokens - 1;
+        uint32_t qf[NT][KS][2];
+        int slot_of[NT][2];  // slots of this lane's rows 2 t4, 2 t4 + 1 (of those behind the tile: the last one's)
+        float m[NT][2], l[NT][2], o[KS][NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = 8 * n + g;
+            const bool real = row < rows;
+            const int tok = real ? row / a.G : 0;
+            const __half* src = a.q + (size_t)(t.row + tok) * a.ldq + (size_t)(w.kvh * a.G + (real ? row - tok * a.G : 0)) * HD + 2 * t4;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                qf[n][k][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+                qf[n][k][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                slot_of[n][e] = t.p0 + min(t.tokens - 1, (8 * n + 2 * t4 + e) / a.G);
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
+        bool bad = false;
+        for (int v = w.v; v < w.ve; ++v) {
+            const int at = done % RING;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
+            const uint32_t sk = ring + at * C::PAGE, sv = sk + NH * 2048;
+            const int s0 = 16 * (v < t.sinkp ? v : v + t.gap);
+            // every row sees every slot of the page
+            const bool clear = s0 + 15 <= t.p0 && (s0 + 15 < a.sinks || s0 > p1 - a.window);
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t x[4];
+                few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) few_mma(s[n], x, qf[n][k][0], qf[n][k][1]);
+            }
+            uint32_t pb[NT][2];
+            float top[NT][2];
+            bool grow = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] *= a.scale_log2;
+                    if (!clear) {
+                        const int slot = s0 + g + 8 * (e >> 1), p = slot_of[n][e & 1];
+                        if (!(slot <= p && (slot < a.sinks || slot > p - a.window))) s[n][e] = -INFINITY;
+                    }
+                }
+                if constexpr (ACC) {  // the rows' scores, for their weights once the rows' sums are known
+                    const int row = 8 * n + 2 * t4, tok = row / a.G, gg = row - tok * a.G;
+                    float* dst = a.scores + (((size_t)(t.row + tok) * a.Hkv + w.kvh) * a.slots_max + s0 + g) * a.G + gg;
+                    if ((a.G & 1) == 0) {
+                        if (row < rows) {
+                            *reinterpret_cast<float2*>(dst) = make_float2(s[n][0], s[n][1]);
+                            *reinterpret_cast<float2*>(dst + 8 * a.G) = make_float2(s[n][2], s[n][3]);
+                        }
+                    } else {
+                        if (row < rows) {
+                            dst[0] = s[n][0];
+                            dst[8 * a.G] = s[n][2];
+                        }
+                        if (row + 1 < rows) {
+                            const int tok1 = (row + 1) / a.G, g1 = row + 1 - tok1 * a.G;
+                            float* d1 = a.scores + (((size_t)(t.row + tok1) * a.Hkv + w.kvh) * a.slots_max + s0 + g) * a.G + g1;
+                            d1[0] = s[n][1];
+                            d1[8 * a.G] = s[n][3];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = few_max(s[n][e], s[n][2 + e]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = few_max(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    top[n][e] = x;
+                    grow |= !(x <= m[n][e]);  // also for NaN
+                }
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float now = few_max(m[n][e], top[n][e]);
+                        f[e] = m[n][e] == now || m[n][e] == -INFINITY ? 1.f : exp2f(m[n][e] - now);
+                        m[n][e] = now;
+                        l[n][e] *= f[e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[k][n][e] *= f[e & 1];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // a NaN or infinite maximum makes every weight, and so the row, NaN
+                    const float mm = m[n][e & 1];
+                    const float sub = mm == -INFINITY ? 0.f : (mm < INFINITY ? mm : __int_as_float(0x7FC00000));
+                    y[e] = few_exp2((s[n][e] - sub) + kFewLift);
+                }
+                l[n][0] += y[0] + y[2];
+                l[n][1] += y[1] + y[3];
+                const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
+                pb[n][0] = few_turn(*reinterpret_cast<const uint32_t*>(&h0));
+                pb[n][1] = few_turn(*reinterpret_cast<const uint32_t*>(&h1));
+            }
+            // V: slots that no row sees may hold anything and become 0; infinities and NaN of slots that some rows see
+            // too (0 * NaN would reach the others), and the rows look them up at the end
+            uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, some[2] = {0u, 0u};
+            if (!clear) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int slot = s0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
+                    const bool any = slot <= p1 && (slot < a.sinks || slot > t.p0 - a.window);
+                    const bool all = slot <= t.p0 && (slot < a.sinks || slot > p1 - a.window);
+                    const uint32_t half = e & 1 ? 0xFFFF0000u : 0xFFFFu;
+                    if (!any) keep[e >> 1] &= ~half;
+                    else if (!all) some[e >> 1] |= half;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t x[4];
+                few_ldm<true>(x, sv + (k >> 2) * 2048 + v_row * 128 + (((2 * (k & 3) + v_chunk) ^ (v_row & 7)) << 4));
+                if (!clear) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] &= keep[e >> 1];
+                        uint32_t wild = 0;
+                        if ((x[e] & 0x7C00u) == 0x7C00u) wild |= 0xFFFFu;
+                        if ((x[e] & 0x7C000000u) == 0x7C000000u) wild |= 0xFFFF0000u;
+                        wild &= some[e >> 1];
+                        bad |= wild != 0;
+                        x[e] &= ~wild;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) few_mma(o[k][n], x, pb[n][0], pb[n][1]);
+            }
+            ++done;
+            __syncwarp();  // the page has been read
+            load();
+        }
+        if (!ok) break;
+        // ---- the segment's rows
+        bad = __any_sync(0xffffffffu, bad);
+        const int piece = 2 * range + (w.begun == u0 ? 0 : 1);
+        if (w.v >= w.ve && !w.whole) continue;  // behind the tile's pages
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[n][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int row = 8 * n + 2 * t4 + e;
+                const bool real = row < rows;
+                const int tok = row / a.G, head = w.kvh * a.G + (row - tok * a.G), r = t.row + tok;
+                bool wild = bad;
+                if (w.whole) {
+                    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+                    __half* dst = a.out + (size_t)r * a.ldo + (size_t)head * HD;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float y = o[k][n][e + 2 * h] * inv;
+                            wild |= !(fabsf(y) < INFINITY);
+                            // (a finite mean that rounding took past fp16's largest)
+                            if (real) dst[16 * k + 8 * h + g] = __float2half_rn(y == y ? fminf(fmaxf(y, -kFewMax), kFewMax) : y);
+                        }
+                    if (ACC && real && g == 0) a.ml[(size_t)r * a.Hq + head] = make_float2(m[n][e], inv);
+                    const uint32_t look = __ballot_sync(0xffffffffu, real && wild && sum == sum);
+                    for (int q = 0; q < 4; ++q) {  // rows that met an infinity or a NaN
+                        if (!(look & (0x11111111u << q))) continue;
+                        const int row_q = 8 * n + 2 * q + e, tok_q = row_q / a.G, head_q = w.kvh * a.G + (row_q - tok_q * a.G);
+                        __syncwarp();
+                        few_nonfinite<HD>(a, w.b, t.p0 + tok_q, w.kvh,
+                                          a.out + (size_t)(t.row + tok_q) * a.ldo + (size_t)head_q * HD);
+                    }
+                } else {
+                    float* dst = a.po + ((size_t)piece * (8 * NT) + row) * HD;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float y = o[k][n][e + 2 * h];
+                            wild |= !(fabsf(y) < INFINITY);
+                            if (real) dst[16 * k + 8 * h + g] = y;
+                        }
+                    wild = (__ballot_sync(0xffffffffu, wild) & (0x11111111u << t4)) != 0;
+                    if (real && g == 0) a.pml[(size_t)piece * (8 * NT) + row] = make_float2(m[n][e], wild ? -sum : sum);
+                }
+            }
+        }
+    }
+    if (!ok) {
+        if (lane == 0) record_timeout(a.status, 40);
+        // the copies in flight land before the CTA leaves
+        for (int c = done; c < asked; ++c) (void)mbar_wait(bar + 8 * (c % RING), (uint32_t)(c / RING) & 1u);
+    }
+}
+
+// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in their
+// order: a warp for each row and head of up to 8 pieces, else the CTA's four warps
+// take every fourth piece and are joined in their order.
+template <int HD>
+__global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
+    constexpr int W = HD / 32;
+    __shared__ float sm[4], sl[4], so[4][HD];
+    __shared__ int sbad[4];
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long total = a.pre[a.B], per = few_per(a, total);
+    const long long rows = (long long)a.T * a.Hq, first = 4LL * blockIdx.x;
+    struct Row {
+        int n, b, p, kvh, row;
+        long long r0, u0;
+        __half* dst;
+        size_t at;
+    };
+    auto find = [&](long long idx) {
+        Row x;
+        x.n = 0;
+        if (idx >= rows) return x;
+        const int r = (int)(idx / a.Hq), head = (int)(idx - (long long)r * a.Hq);
+        int lo = 0, hi = a.B;  // first sequence whose end is past the row
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.row_off[mid + 1] > r) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo >= a.B) return x;
+        const FewSeq s = few_seq(a, lo);
+        const int i = r - s.lo;
+        if (i < 0 || i >= s.n) return x;
+        const int tile = i / a.tpt;
+        const FewTile t = few_tile(a, s, tile);
+        x.b = lo;
+        x.p = s.ctx + i;
+        x.kvh = head / a.G;
+        x.row = (i - tile * a.tpt) * a.G + head - x.kvh * a.G;
+        x.u0 = a.pre[lo] + ((long long)tile * a.Hkv + x.kvh) * a.np[lo];
+        x.r0 = x.u0 / per;
+        x.n = t.np > 0 ? (int)((x.u0 + t.np - 1) / per - x.r0) + 1 : 0;
+        x.dst = a.out + (size_t)r * a.ldo + (size_t)head * HD;
+        x.at = (size_t)r * a.Hq + head;
+        return x;
+    };
+    float m, l, o[W];
+    bool bad;
+    auto join = [&](const Row& x, int k0, int step) {  // pieces k0, k0 + step, ..
+        m = -INFINITY;
+        l = 0.f;
+        bad = false;
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[e] = 0.f;
+        constexpr int P = 4;
+        for (int k = k0; k < x.n; k += P * step) {
+            float2 ml[P];
+            float v[P][W];
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const long long range = x.r0 + min(x.n - 1, k + u * step);
+                const size_t at = (size_t)(2 * range + (x.u0 > range * per ? 1 : 0)) * tile_rows + x.row;
+                ml[u] = a.pml[at];
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[u][e] = a.po[at * HD + lane * W + e];
+                if (k + u * step >= x.n) ml[u] = make_float2(-INFINITY, 0.f);
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                top = few_max(top, ml[u].x);
+                bad |= !(ml[u].y >= 0.f);
+            }
+            const float sub = top == -INFINITY ? 0.f : top;
+            const float f = exp2f(m - sub);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < W; ++e) o[e] *= f;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const float w = exp2f(ml[u].x - sub);
+                if (w == 0.f) continue;  // a piece without weight may hold anything
+                l += w * fabsf(ml[u].y);
+#pragma unroll
+                for (int e = 0; e < W; ++e) o[e] += w * v[u][e];
+            }
+        }
+    };
+    auto finish = [&](const Row& x) {
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+            const float y = o[e] * inv;
+            bad |= !(fabsf(y) < INFINITY);
+            x.dst[lane * W + e] = __float2half_rn(y == y ? fminf(fmaxf(y, -kFewMax), kFewMax) : y);
+        }
+        if (a.ml && lane == 0) a.ml[x.at] = make_float2(m, inv);
+        if (__any_sync(0xffffffffu, bad) && l == l) few_nonfinite<HD>(a, x.b, x.p, x.kvh, x.dst);
+    };
+    const Row mine = find(first + warp);
+    if (mine.n > 1 && mine.n <= 8) {
+        join(mine, 0, 1);
+        finish(mine);
+    }
+    if (!__syncthreads_or(mine.n > 8)) return;
+    for (int k = 0; k < 4; ++k) {
+        const Row x = find(first + k);
+        if (x.n <= 8) continue;  // (the same for all)
+        join(x, warp, 4);
+        if (lane == 0) {
+            sm[warp] = m;
+            sl[warp] = l;
+            sbad[warp] = bad;
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) so[warp][lane * W + e] = o[e];
+        __syncthreads();
+        if (warp == 0) {
+            float top = sm[0];
+            for (int q = 1; q < 4; ++q) top = few_max(top, sm[q]);
+            const float sub = top == -INFINITY ? 0.f : top;
+            m = top;
+            l = 0.f;
+            bad = false;
+#pragma unroll
+            for (int e = 0; e < W; ++e) o[e] = 0.f;
+            for (int q = 0; q < 4; ++q) {
+                const float w = exp2f(sm[q] - sub);
+                bad |= sbad[q] != 0;
+                if (w == 0.f) continue;
+                l += w * sl[q];
+#pragma unroll
+                for (int e = 0; e < W; ++e) o[e] += w * so[q][lane * W + e];
+            }
+            finish(x);
+        }
+        __syncthreads();
+    }
+}
+
+// weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
+// of 2^(x - m) / l, from the scores that few_rows_kernel left.  A warp for 128
+// slots of a head, four a lane.
+__global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant__ FewArgs a) {
+    extern __shared__ int chunks[];
+    pdl_wait();
+    for (int b = threadIdx.x; b <= a.B; b += 256) chunks[b] = a.chunks[b];
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, total = chunks[a.B];
+    for (int c = blockIdx.x * 8 + warp; c < total; c += gridDim.x * 8) {
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (chunks[mid] <= c) lo = mid;
+            else hi = mid;
+        }
+        const FewSeq s = few_seq(a, lo);
+        const int per_head = (chunks[lo + 1] - chunks[lo]) / a.Hkv, local = c - chunks[lo];
+        const int kvh = local / per_head, j0 = 128 * (local - kvh * per_head);
+        const int end = min(min(s.ctx + s.n, a.slots_max), j0 + 128);
+        float sum[4] = {};
+        for (int i = max(0, j0 - s.ctx); i < s.n; ++i) {
+            const int r = s.lo + i, p = s.ctx + i;
+            const float* src = a.scores + ((size_t)r * a.Hkv + kvh) * a.slots_max * a.G;
+            const float2* ml = a.ml + (size_t)r * a.Hq + kvh * a.G;
+            for (int g = 0; g < a.G; ++g) {
+                const float2 y = ml[g];
+                const float sub = y.x == -INFINITY ? 0.f : y.x;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int j = j0 + 32 * u + lane;
+                    if (j < end && j <= p) sum[u] += few_exp2((src[(size_t)j * a.G + g] - sub) + kFewLift) * y.y;
+                }
+            }
+        }
+        float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = j0 + 32 * u + lane;
+            if (j < end) dst[j] += sum[u];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Sizes that do not fall where B, T or max_blocks grows.
+struct FewSpace {
+    int ctas, rows;
+    size_t pre, np, chunks, pml, po, ml, scores, bytes;  // offsets, and all
+};
+static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks, bool acc) {
+    FewSpace s = {};
+    const long long rows = (long long)T * (Hq / Hkv);
+    s.rows = (int)std::min<long long>(kFewMaxRows, (rows + 7) / 8 * 8);
+    s.ctas = (int)std::min<long long>(kFewMaxCtas, ((long long)T * Hkv * max_blocks + kFewMinPages - 1) / kFewMinPages);
+    const size_t pieces = (size_t)2 * kFewWarps * s.ctas * s.rows;
+    size_t at = 0;
+    auto room = [&](size_t n) {
+        const size_t here = at;
+        at += up256(n);
+        return here;
+    };
+    s.pre = room((size_t)(B + 1) * 8);
+    s.np = room((size_t)B * 4);
+    s.chunks = room((size_t)(B + 1) * 4);
+    s.pml = room(pieces * sizeof(float2));
+    s.po = room(pieces * HD * sizeof(float));
+    if (acc) {
+        s.ml = room((size_t)T * Hq * sizeof(float2));
+        s.scores = room((size_t)T * Hq * max_blocks * 16 * sizeof(float));
+    }
+    s.bytes = at;
+    return s;
+}
+
+static const void* few_fn(int HD, int NT, bool acc) {
+#define FEW_NT(hd, ac) \
+    (NT == 1 ? (const void*)few_rows_kernel<hd, 1, ac> \
+             : NT == 2 ? (const void*)few_rows_kernel<hd, 2, ac> \
+                       : NT == 3 ? (const void*)few_rows_kernel<hd, 3, ac> : (const void*)few_rows_kernel<hd, 4, ac>)
+    if (HD == 128) return acc ? FEW_NT(128, true) : FEW_NT(128, false);
+    return acc ? FEW_NT(64, true) : FEW_NT(64, false);
+#undef FEW_NT
+}
+static int few_sms(int* out) {  // SMs of the current device; sets the kernels' shared memory on it once
+    static std::atomic<int> facts[64];
+    int dev = 0;
+    SD_CUDA(cudaGetDevice(&dev));
+    SD_CHECK(dev >= 0 && dev < 64, SPECDEC_ENOTSUP, "attention: device index above 63");
+    int n = facts[dev].load();
+    if (!n) {
+        for (int nt = 1; nt <= 4; ++nt)
+            for (int acc = 0; acc < 2; ++acc) {
+                SD_CUDA(cudaFuncSetAttribute(few_fn(128, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)FewCfg<128>::smem(kBoundMaxSeqs)));
+                SD_CUDA(cudaFuncSetAttribute(few_fn(64, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)FewCfg<64>::smem(kBoundMaxSeqs)));
+            }
+        SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        facts[dev].store(n);
+    }
+    *out = n;
+    return SPECDEC_OK;
+}
+
+static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
+    int sms = 0;
+    int rc = few_sms(&sms);
+    if (rc) return rc;
+    const FewSpace sp = few_space(a.B, a.T, a.Hq, a.Hkv, HD, a.max_blocks, acc);
+    char* w = static_cast<char*>(ws);
+    a.pre = reinterpret_cast<long long*>(w + sp.pre);
+    a.np = reinterpret_cast<int32_t*>(w + sp.np);
+    a.chunks = reinterpret_cast<int32_t*>(w + sp.chunks);
+    a.pml = reinterpret_cast<float2*>(w + sp.pml);
+    a.po = reinterpret_cast<float*>(w + sp.po);
+    a.ml = acc ? reinterpret_cast<float2*>(w + sp.ml) : nullptr;
+    a.scores = acc ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
+    a.status = device_status_ptr();
+    a.slots_max = a.max_blocks * 16;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)HD));
+    // rows of a tile: what a sequence has on average
+    const long long want = std::min<long long>(kFewMaxRows, (((long long)a.T + a.B - 1) / a.B) * a.G);
+    const int NT = (int)((want + 7) / 8);
+    a.tpt = 8 * NT / a.G;
+    const int ctas = std::min(sp.ctas, sms);
+    a.ranges = ctas * kFewWarps;
+    CUtensorMap map;
+    if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 2))) return rc;
+    const size_t smem = HD == 128 ? FewCfg<128>::smem(a.B) : FewCfg<64>::smem(a.B);
+    void* args[] = {&map, &a};
+    SD_CUDA(cudaLaunchKernel(few_fn(HD, NT, acc), dim3((unsigned)ctas), dim3(32 * kFewWarps), args, smem, s));
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(((long long)a.T * a.Hq + 3) / 4));
+    cfg.blockDim = dim3(128);
+    if (HD == 128) SD_CUDA(cudaLaunchKernelEx(&cfg, few_merge_kernel<128>, a, 8 * NT));
+    else SD_CUDA(cudaLaunchKernelEx(&cfg, few_merge_kernel<64>, a, 8 * NT));
+    if (acc) {
+        const long long chunks = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
+        cfg.gridDim = dim3((unsigned)std::min<long long>((chunks + 7) / 8, 8LL * sms));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = (size_t)(a.B + 1) * 4;
+        SD_CUDA(cudaLaunchKernelEx(&cfg, few_weights_kernel, a));
+    }
+    return SPECDEC_OK;
 }
 
 static int check_bound(const char* who, const void* q, int ldq, const void* kv, const void* out, int ldo, int num_blocks,
@@ -168,19 +999,36 @@ static int launch_bound(const BoundArgs& a, int HD, cudaStream_t s) {
     if (HD == 128) bound_rows_kernel<128><<<grid, 256, 0, s>>>(a);
     else bound_rows_kernel<64><<<grid, 256, 0, s>>>(a);
     SD_LAUNCH_CHECK("bound_rows_kernel");
-    if (a.weights) {
-        const dim3 g2((unsigned)(2 * (size_t)a.max_blocks), (unsigned)a.Hkv, (unsigned)a.B);
-        if (HD == 128) bound_weights_kernel<128><<<g2, 256, 0, s>>>(a);
-        else bound_weights_kernel<64><<<g2, 256, 0, s>>>(a);
-        SD_LAUNCH_CHECK("bound_weights_kernel");
-    }
     return SPECDEC_OK;
+}
+static bool few_rows(int B, int T, int G) { return G <= kFewMaxRows && T <= (long long)B * (kFewMaxRows / G); }
+static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
+                        const int32_t* tables, int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B,
+                        int T, int n_q_heads, uint16_t* out, int ldo) {
+    FewArgs a = {};
+    a.q = reinterpret_cast<const __half*>(q);
+    a.ldq = ldq;
+    a.kv = reinterpret_cast<const __half*>(kv_layer);
+    a.num_blocks = num_blocks;
+    a.Hkv = n_kv_heads;
+    a.Hq = n_q_heads;
+    a.G = n_q_heads / n_kv_heads;
+    a.tables = tables;
+    a.max_blocks = max_blocks;
+    a.ctx_len = ctx_len;
+    a.row_off = row_off;
+    a.B = B;
+    a.T = T;
+    a.window = 1 << 30;
+    a.out = reinterpret_cast<__half*>(out);
+    a.ldo = ldo;
+    return a;
 }
 
 extern "C" size_t specdec_attention_window_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                            int max_blocks) {
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_blocks <= 0) return 0;
-    return 256;
+    return few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes;
 }
 
 extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -199,6 +1047,13 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
                  workspace_bytes >= specdec_attention_window_workspace_bytes(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks),
              SPECDEC_EINVAL, "attention_window: workspace too small or not 32-byte aligned");
     if ((rc = check_bound_memory(who, q, kv_layer, out, tables, ctx_len, row_off, workspace))) return rc;
+    if (few_rows(B, T, n_q_heads / n_kv_heads)) {
+        FewArgs f = few_args(q, ldq, kv_layer, num_blocks, n_kv_heads, tables, max_blocks, ctx_len, row_off, B, T,
+                             n_q_heads, out, ldo);
+        f.window = window;
+        f.sinks = sinks;
+        return launch_few(f, head_dim, false, workspace, as_stream(stream));
+    }
     BoundArgs a = {};
     a.q = reinterpret_cast<const __half*>(q);
     a.ldq = ldq;
@@ -224,7 +1079,7 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
 extern "C" size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads,
                                                                int head_dim, int max_blocks) {
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_blocks <= 0) return 0;
-    return (size_t)T * n_q_heads * sizeof(float2);
+    return few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, true).bytes;
 }
 
 extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -249,26 +1104,9 @@ extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const ui
              SPECDEC_EINVAL, "attention_accumulate: workspace too small or not 32-byte aligned");
     if ((rc = check_bound_memory(who, q, kv_layer, out, tables, ctx_len, row_off, workspace))) return rc;
     if ((rc = check_on_device(weights, "attention_accumulate: weights"))) return rc;
-    BoundArgs a = {};
-    a.q = reinterpret_cast<const __half*>(q);
-    a.ldq = ldq;
-    a.kv = reinterpret_cast<const __half*>(kv_layer);
-    a.num_blocks = num_blocks;
-    a.Hkv = n_kv_heads;
-    a.Hq = n_q_heads;
-    a.G = n_q_heads / n_kv_heads;
-    a.tables = tables;
-    a.max_blocks = max_blocks;
-    a.ctx_len = ctx_len;
-    a.row_off = row_off;
-    a.B = B;
-    a.T = T;
-    a.window = 1 << 30;
-    a.weights = weights;
-    a.ldw = ldw;
-    a.out = reinterpret_cast<__half*>(out);
-    a.ldo = ldo;
-    a.ml = static_cast<float2*>(workspace);
-    a.scale = (float)(1.0 / sqrt((double)head_dim));
-    return launch_bound(a, head_dim, as_stream(stream));
+    FewArgs f = few_args(q, ldq, kv_layer, num_blocks, n_kv_heads, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads,
+                         out, ldo);
+    f.weights = weights;
+    f.ldw = ldw;
+    return launch_few(f, head_dim, true, workspace, as_stream(stream));
 }
