@@ -17,91 +17,7 @@
 namespace specdec {
 
 constexpr int kBoundMaxSeqs = 1024;
-
-struct BoundArgs {
-    const __half* q;
-    int ldq;
-    const __half* kv;
-    int num_blocks, Hkv, Hq, G;
-    const int32_t* tables;
-    int max_blocks;
-    const int32_t* ctx_len;
-    const int32_t* row_off;
-    int B, T, window, sinks;
-    __half* out;
-    int ldo;
-    float scale;
-};
-
-struct BoundRow {
-    int b, slot, last;  // sequence (-1: none), the row's slot, last slot that exists for it
-};
-__device__ __forceinline__ BoundRow bound_row(const BoundArgs& a, int r) {
-    int lo = 0, hi = a.B;  // first sequence whose end is past the row
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.row_off[mid + 1] > r) hi = mid;
-        else lo = mid + 1;
-    }
-    if (lo >= a.B || a.row_off[lo] > r) return {-1, 0, 0};
-    const int slot = max(0, min(a.ctx_len[lo], 1 << 30)) + r - max(0, a.row_off[lo]);
-    return {lo, slot, min(slot, a.max_blocks * 16 - 1)};
-}
-__device__ __forceinline__ const __half* bound_slot(const BoundArgs& a, int b, int slot, int plane, int kvh, int hd) {
-    const int p = a.tables[(size_t)b * a.max_blocks + (slot >> 4)];
-    const int page = p < 0 || p >= a.num_blocks ? 0 : p;
-    return a.kv + ((((size_t)page * 2 + plane) * a.Hkv + kvh) * 16 + (slot & 15)) * hd;
-}
-
-// A warp for each row and query head.
-template <int HD>
-__global__ void __launch_bounds__(256) bound_rows_kernel(const __grid_constant__ BoundArgs a) {
-    constexpr int W = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int r = (int)(w / a.Hq), head = (int)(w % a.Hq);
-    if (r >= a.T) return;
-    const BoundRow row = bound_row(a, r);
-    if (row.b < 0) return;
-    const int kvh = head / a.G;
-    float q[W], o[W], bad[W];
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-        q[e] = __half2float(a.q[(size_t)r * a.ldq + (size_t)head * HD + lane * W + e]) * a.scale;
-        o[e] = bad[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    const int from = max(0, row.slot - a.window + 1), first = min(a.sinks, from);
-    for (int j = first > 0 ? 0 : from; j <= row.last; j = j + 1 == first ? from : j + 1) {
-        const __half* k = bound_slot(a, row.b, j, 0, kvh, HD) + lane * W;
-        const __half* v = bound_slot(a, row.b, j, 1, kvh, HD) + lane * W;
-        float x = 0.f;
-#pragma unroll
-        for (int e = 0; e < W; ++e) x = fmaf(q[e], __half2float(k[e]), x);
-        x = warp_sum(x);
-        const float top = x > m || x != x ? x : m;
-        const float sub = top == -INFINITY ? 0.f : top;
-        const float f = expf(m - sub), p = expf(x - sub);
-        m = top;
-        l = l * f + p;
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-            const float y = __half2float(v[e]);
-            if (isfinite(y)) o[e] = o[e] * f + p * y;
-            else {
-                o[e] *= f;
-                bad[e] += y;  // reaches the row whatever its weight
-            }
-        }
-    }
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-        float y = o[e] * inv;
-        if (fabsf(y) > 65504.f) y = copysignf(65504.f, y);
-        a.out[(size_t)r * a.ldo + (size_t)head * HD + lane * W + e] = __float2half_rn(y == y && bad[e] != 0.f ? bad[e] : y);
-    }
-}
+constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a call at most
 
 // ------------------------------------------------------------------ few rows
 //
@@ -994,13 +910,6 @@ static int check_bound_memory(const char* who, const void* q, const void* kv, co
 
 using namespace specdec;
 
-static int launch_bound(const BoundArgs& a, int HD, cudaStream_t s) {
-    const unsigned grid = (unsigned)(((long long)a.T * a.Hq + 7) / 8);
-    if (HD == 128) bound_rows_kernel<128><<<grid, 256, 0, s>>>(a);
-    else bound_rows_kernel<64><<<grid, 256, 0, s>>>(a);
-    SD_LAUNCH_CHECK("bound_rows_kernel");
-    return SPECDEC_OK;
-}
 static bool few_rows(int B, int T, int G) { return G <= kFewMaxRows && T <= (long long)B * (kFewMaxRows / G); }
 static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
                         const int32_t* tables, int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B,
@@ -1019,7 +928,7 @@ static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, in
     a.row_off = row_off;
     a.B = B;
     a.T = T;
-    a.window = 1 << 30;
+    a.window = kBoundSlots;
     a.out = reinterpret_cast<__half*>(out);
     a.ldo = ldo;
     return a;
@@ -1028,7 +937,8 @@ static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, in
 extern "C" size_t specdec_attention_window_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                            int max_blocks) {
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_blocks <= 0) return 0;
-    return few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes;
+    return std::max(few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes,
+                    rows_packed_workspace(B, T, n_q_heads, head_dim, max_blocks));
 }
 
 extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1047,6 +957,9 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
                  workspace_bytes >= specdec_attention_window_workspace_bytes(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks),
              SPECDEC_EINVAL, "attention_window: workspace too small or not 32-byte aligned");
     if ((rc = check_bound_memory(who, q, kv_layer, out, tables, ctx_len, row_off, workspace))) return rc;
+    // past the last slot that a row could have both change nothing (and sums with them stay in 32 bits)
+    window = std::min(window, kBoundSlots);
+    sinks = std::min(sinks, 16 * max_blocks);
     if (few_rows(B, T, n_q_heads / n_kv_heads)) {
         FewArgs f = few_args(q, ldq, kv_layer, num_blocks, n_kv_heads, tables, max_blocks, ctx_len, row_off, B, T,
                              n_q_heads, out, ldo);
@@ -1054,26 +967,9 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
         f.sinks = sinks;
         return launch_few(f, head_dim, false, workspace, as_stream(stream));
     }
-    BoundArgs a = {};
-    a.q = reinterpret_cast<const __half*>(q);
-    a.ldq = ldq;
-    a.kv = reinterpret_cast<const __half*>(kv_layer);
-    a.num_blocks = num_blocks;
-    a.Hkv = n_kv_heads;
-    a.Hq = n_q_heads;
-    a.G = n_q_heads / n_kv_heads;
-    a.tables = tables;
-    a.max_blocks = max_blocks;
-    a.ctx_len = ctx_len;
-    a.row_off = row_off;
-    a.B = B;
-    a.T = T;
-    a.window = window;
-    a.sinks = sinks;
-    a.out = reinterpret_cast<__half*>(out);
-    a.ldo = ldo;
-    a.scale = (float)(1.0 / sqrt((double)head_dim));
-    return launch_bound(a, head_dim, as_stream(stream));
+    return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
+                              num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads,
+                              window, sinks, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads,

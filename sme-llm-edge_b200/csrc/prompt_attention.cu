@@ -5,6 +5,8 @@
 // query heads together, row = token * G + g, as many whole tokens as fit into
 // 128 rows) against a range of one block table's slots.  A segment is
 //   a sequence's packed rows, causal             (specdec_attention_prompt)
+//   the same within a window and behind the first
+//   tokens                                       (specdec_attention_window)
 //   a group's rows against its shared pages      (specdec_attention_shared_prefix)
 //   a sequence's rows against its own pages,
 //   with the mask of its new rows                (specdec_attention_shared_prefix)
@@ -43,6 +45,11 @@
 // issuer for each slot the two interleave MMA by MMA, both softmaxes run at the
 // same time and then neither: 6,900 clocks a pair of operations.)
 // P overlays S in tensor memory (columns: S0 0, S1 128, O0 256, O1 256 + hd).
+//
+// With a window (WIN) an item's slots are numbered without the pages between the
+// first tokens and the item's first row's window: what lies there is not read, and
+// the rest of the kernel sees one range.  A row sees slot j of it iff
+// j <= its own and (j < sinks or j > its own - window).
 //
 // Splits of the key range write unnormalised fp32 O with (m, l) into the
 // workspace; rows_merge_kernel joins them in their order.
@@ -87,7 +94,7 @@ constexpr float kRowsLift = 7.0f;    // P is 2^7 times the weight: at most 2^(8 
 // it x is off by 2^-13 at most (where 7 - m takes a bit more than m).
 constexpr float kRowsHuge = 4096.0f;
 
-enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2 };
+enum { kModeCausal = 0, kModeAll = 1, kModeMask = 2, kModeWindow = 3 };
 enum { kPair = 0, kDual = 1 };
 
 // Where the partial results of a sequence's rows lie (rows of the partial buffers).
@@ -119,6 +126,7 @@ struct RowsArgs {
     const int32_t* shared_blocks;
     int n_groups, B, T, R;
     int tq_small;  // tokens of the small query box
+    int window, sinks;  // kModeWindow
     RowsDiv by_item, by_hkv;  // 2 * tpt tokens of an item; KV heads
     int slots_max;  // max_blocks * 16
     __half* out;
@@ -154,11 +162,18 @@ struct RowsItem {
     int pnext;         // a dual's odd tiles: so many rows behind (0: it has one tile only)
     int bad;           // warp 10 found an infinity or NaN past `scan`
 };
+struct RowsGap {
+    int sinkp, gap;  // pages of the first tokens; of the table between them and the window
+};
+struct RowsWinItem : RowsItem, RowsGap {};
+template <bool WIN>
+using RowsItemOf = std::conditional_t<WIN, RowsWinItem, RowsItem>;
 
 // ------------------------------------------------------------------ the plan
 __device__ __forceinline__ int rows_clamp(int v, int lo, int hi) { return max(lo, min(hi, v)); }
 
 // Segment i; off: the bounds of the sequences' rows (prompt) or of the groups.
+template <bool WIN>
 __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int* off, const int* ctx_len,
                                             const int* group_pages, const int16_t* seq_group) {
     RowsSeg s;
@@ -169,7 +184,7 @@ __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int*
         s.base = 0;
         s.end = min(s.ctx + s.n, a.slots_max);
         s.trow = i;
-        s.mode = kModeCausal;
+        s.mode = WIN ? kModeWindow : kModeCausal;
     } else if (i < a.n_groups) {
         const int b0 = rows_clamp(off[i], 0, a.B), b1 = rows_clamp(off[i + 1], b0, a.B);
         s.lo = b0 * a.R;
@@ -192,14 +207,31 @@ __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int*
     }
     s.tiles = rows_quot(s.n + 2 * a.tpt - 1, a.by_item);
     s.kt = (s.end - s.base + 127) / 128;
+    // of any item: the first tokens' pages, its tokens' windows and the rest of a page at each end
+    if constexpr (WIN) s.kt = min(s.kt, (int)(((uint32_t)((a.sinks + 15) & ~15) + a.window + 2 * a.tpt + 30 + 127) / 128));
     return s;
 }
+// What of a sequence's table the item p along the rows leaves out.
+__device__ __forceinline__ RowsGap rows_gap(const RowsArgs& a, const RowsSeg& s, int p) {
+    const int first = s.ctx + p * 2 * a.tpt, end = min(s.end, s.ctx + min(s.n, (p + 1) * 2 * a.tpt));
+    RowsGap g;
+    g.sinkp = (min(a.sinks, end) + 15) >> 4;
+    g.gap = max(0, (max(0, first - a.window + 1) >> 4) - g.sinkp);
+    return g;
+}
 // 128-key tiles of the segment's item p along the rows
+template <bool WIN>
 __device__ __forceinline__ int rows_item_end(const RowsArgs& a, const RowsSeg& s, int p) {
+    if constexpr (WIN) {
+        const int end = min(s.end, s.ctx + min(s.n, (p + 1) * 2 * a.tpt));
+        const RowsGap g = rows_gap(a, s, p);
+        return g.gap ? max(min(end, 16 * g.sinkp), end - 16 * g.gap) : end;
+    }
     return s.mode == kModeCausal ? min(s.end, s.ctx + min(s.n, (p + 1) * 2 * a.tpt)) : s.end;
 }
+template <bool WIN>
 __device__ __forceinline__ int rows_item_kt(const RowsArgs& a, const RowsSeg& s, int p) {
-    return (rows_item_end(a, s, p) - s.base + 127) / 128;
+    return (rows_item_end<WIN>(a, s, p) - s.base + 127) / 128;
 }
 // How long the pieces of a key range are, in key tiles: about `fine` where there
 // are few rows (memory-bound: partial results are small), about `coarse`
@@ -280,6 +312,7 @@ __device__ __forceinline__ void rows_scan2(RowsPlan& p, int va, int vb, int* bef
 // is on every call's path: lengths and bounds are loaded once, together, and up
 // to kRowsSorted segments stay in shared memory.  What it takes is the fetching of
 // code that runs once: its loops are not unrolled.
+template <bool WIN>
 __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const int tid = threadIdx.x;
     const int nseg = a.row_off ? a.B : a.n_groups + a.B;
@@ -322,13 +355,13 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     __syncthreads();
     const int per = small ? 1 : (nseg + kRowsThreads - 1) / kRowsThreads;
     const int s0 = min(nseg, tid * per), s1 = min(nseg, s0 + per);
-    auto seg_of = [&](int i) { return rows_seg(a, i, off, ctx, p.group_pages, p.seq_group); };
+    auto seg_of = [&](int i) { return rows_seg<WIN>(a, i, off, ctx, p.group_pages, p.seq_group); };
     // total work in key tiles (in fp32: an estimate, the same in every CTA)
     float work = 0.f;
 #pragma unroll 1
     for (int i = s0; i < s1; ++i) {
         const RowsSeg s = seg_of(i);
-        if (s.tiles > 0) work += (float)s.tiles * 0.5f * (float)(rows_item_kt(a, s, 0) + s.kt) * (float)a.Hkv;
+        if (s.tiles > 0) work += (float)s.tiles * 0.5f * (float)(rows_item_kt<WIN>(a, s, 0) + s.kt) * (float)a.Hkv;
         if (small) p.segs[i] = s;
     }
     work = warp_sum(work);
@@ -411,8 +444,9 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     __syncthreads();
 }
 
-__device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
-    RowsItem it;
+template <bool WIN>
+__device__ __forceinline__ RowsItemOf<WIN> rows_item(const RowsArgs& a, const RowsPlan& p, int idx) {
+    RowsItemOf<WIN> it;
     it.n_kt = -1;
     it.bad = 0;
     if (idx < 0 || idx >= p.items) return it;
@@ -426,7 +460,7 @@ __device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan&
     }
     const RowsSeg s = p.nseg <= kRowsSorted
                           ? p.segs[p.order[lo]]
-                          : rows_seg(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_group);
+                          : rows_seg<WIN>(a, lo, a.row_off ? a.row_off : a.group_off, a.ctx_len, p.group_pages, p.seq_group);
     const int S = p.nseg <= kRowsSorted ? p.splits[lo] : rows_splits(a, s, p.cut);
     const int local = r - p.pre[lo];
     const int along = S == 1 ? local : local / S;
@@ -439,11 +473,11 @@ __device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan&
         it.prow = -1;
         return it;
     }
-    const int kt = rows_item_kt(a, s, tile);
+    const int kt = rows_item_kt<WIN>(a, s, tile);
     const int k0 = S == 1 ? 0 : piece * kt / S, k1 = S == 1 ? kt : (piece + 1) * kt / S;  // S <= 32, kt < 2^24
     it.n_kt = k1 - k0;
     it.slot0 = s.base + 128 * k0;
-    it.end = min(rows_item_end(a, s, tile), s.base + 128 * k1);
+    it.end = min(rows_item_end<WIN>(a, s, tile), s.base + 128 * k1);
     it.trow = s.trow;
     it.i0 = tile * 2 * a.tpt;
     it.tok0 = s.lo + it.i0;
@@ -452,6 +486,13 @@ __device__ __forceinline__ RowsItem rows_item(const RowsArgs& a, const RowsPlan&
     it.ctx = s.ctx;
     it.mode = s.mode;
     it.scan = s.mode == kModeCausal ? s.ctx + it.i0 + 1 : (s.mode == kModeMask ? s.ctx : it.end);
+    if constexpr (WIN) {
+        const RowsGap g = rows_gap(a, s, tile);
+        it.sinkp = g.sinkp;
+        it.gap = g.gap;
+        it.ctx -= 16 * g.gap;
+        it.scan = it.ctx + it.i0 + 1;
+    }
     it.kind = rows_dual(a, s, p.cut) || (it.ntok1 == 0 && it.n_kt <= 1) ? kDual : kPair;
     it.pnext = rows_dual(a, s, p.cut) ? s.n : 0;
     it.prow = parts ? p.prow[lo] + piece * (parts > S ? 2 : 1) * s.n + it.i0 : -1;
@@ -465,8 +506,8 @@ struct RowsCfg {
     static constexpr int TILE = NH * 16384;             // 128 rows x HD fp16
     static constexpr int RING = HD == 128 ? 2 : 4;      // K tiles and V tiles in flight
     static constexpr int NBAR = 5 * 2 + 5 * RING + 2 * kRowsItems + 1;
-    static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) + kRowsItems * sizeof(RowsItem) +
-                                   NBAR * 8 + 16;
+    static constexpr size_t smem = 1024 + (size_t)TILE * (2 + 2 * RING) + sizeof(RowsPlan) +
+                                   kRowsItems * sizeof(RowsWinItem) + NBAR * 8 + 16;
     static_assert(smem <= 232448, "shared memory of a CTA");
 };
 
@@ -492,8 +533,8 @@ __device__ void rows_zero(const RowsArgs& a, const RowsItem& it, int lane) {
 // at), a lane's columns being lane * (HD / 32) + j; only rows that are `mine` are
 // written.  True where a column was.  Before it, a final row's infinities become
 // kHalfMax: its finite means that the weights' rounding (2^-11) took past 65520.
-template <int HD>
-__device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& it, bool mine, bool all, int i,
+template <int HD, bool WIN>
+__device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItemOf<WIN>& it, bool mine, bool all, int i,
                                             uint64_t bits, int head, size_t at) {
     constexpr int W = HD / 32;  // columns of a lane
     const int lane = threadIdx.x & 31;
@@ -502,10 +543,13 @@ __device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& i
     uint32_t up[W], down[W];  // bit l of [j]: an infinity (NaN: both) in column l * W + j
 #pragma unroll
     for (int j = 0; j < W; ++j) up[j] = down[j] = 0;
-    const int start = all ? it.slot0 : max(it.scan, it.slot0);
+    const int start = all || WIN ? it.slot0 : max(it.scan, it.slot0);
 #pragma unroll 1
     for (int s0 = start & ~15; s0 < end; s0 += 16) {  // a page
-        const int x = tab[s0 >> 4], page = x < 0 || x >= a.num_blocks ? 0 : x;
+        int x;
+        if constexpr (WIN) x = tab[(s0 >> 4) + (s0 >> 4 < it.sinkp ? 0 : it.gap)];
+        else x = tab[s0 >> 4];
+        const int page = x < 0 || x >= a.num_blocks ? 0 : x;
         const __half* src = a.kv + (((size_t)page * 2 + 1) * a.Hkv + it.kvh) * 16 * HD + lane * W;
         alignas(8) uint16_t v[16][W];
 #pragma unroll
@@ -521,8 +565,9 @@ __device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& i
             for (int j = 0; j < W; ++j) any |= (v[u][j] & 0x7C00) == 0x7C00;
             if (!__any_sync(0xffffffffu, any)) continue;
             const int d = s0 + rows_clamp(u, max(0, start - s0), min(15, end - 1 - s0)) - ctx;
-            const bool seen = mode == kModeAll ||
-                              (mode == kModeCausal ? d <= i : d < 0 || (d < 64 && ((bits >> d) & 1ull)));
+            const bool seen = WIN ? d <= i && (d + ctx < a.sinks || d > i - a.window)
+                                  : mode == kModeAll ||
+                                        (mode == kModeCausal ? d <= i : d < 0 || (d < 64 && ((bits >> d) & 1ull)));
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const uint32_t y = v[u][j];  // 0x7C00 infinity, 0xFC00 its opposite, above either NaN
@@ -562,10 +607,16 @@ __device__ __noinline__ bool rows_nonfinite(const RowsArgs& a, const RowsItem& i
 }
 
 // Bit c = slot key0 + c of a row is seen.
-__device__ __forceinline__ void rows_seen(const RowsItem& it, int key0, int i, uint64_t bits, uint64_t& lo, uint64_t& hi) {
+template <bool WIN>
+__device__ __forceinline__ void rows_seen(const RowsArgs& a, const RowsItem& it, int key0, int i, uint64_t bits,
+                                          uint64_t& lo, uint64_t& hi) {
     auto below = [](int k) -> uint64_t { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); };
     const int n = it.end - key0;
-    if (it.mode == kModeMask) {
+    if constexpr (WIN) {
+        const int p = it.ctx + i + 1 - key0, k = min(n, p), w = p - a.window, f = a.sinks - key0;
+        lo = below(k) & (~below(w) | below(f));
+        hi = below(k - 64) & (~below(w - 64) | below(f - 64));
+    } else if (it.mode == kModeMask) {
         const int d = it.ctx - key0;  // column of the first new row
         lo = below(d);
         hi = below(d - 64);
@@ -682,8 +733,8 @@ struct RowsBars {
 // warp-uniform, and one lane issues.  The softmax warps answer for V and O; the
 // issuer waits for P alone.  Keys behind the range's end cost Q.K^T columns that
 // the softmax masks; P.V takes the pages that exist.
-template <int HD>
-__device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uint32_t tmem, uint32_t sq, uint32_t sk,
+template <int HD, bool WIN>
+__device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItemOf<WIN>* items, uint32_t tmem, uint32_t sq, uint32_t sk,
                                          uint32_t sv, uint64_t* bars, volatile int* abort_flag) {
     using C = RowsCfg<HD>;
     constexpr int NH = C::NH, RING = C::RING;
@@ -709,7 +760,7 @@ __device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uin
         while (x == n) {  // to the next item
             const int d = (k + 1) % kRowsItems, turn = (k + 1) / kRowsItems;
             if (block ? !wait(&bar.i_full[d], turn) : !ready(&bar.i_full[d], turn)) return false;
-            const volatile RowsItem& it = items[d];
+            const volatile RowsItem& it = static_cast<const RowsItem&>(items[d]);
             const int n_kt = same(it.n_kt);
             if (n_kt < 0) {
                 more = false;
@@ -820,7 +871,7 @@ __device__ __forceinline__ void rows_mma(const RowsArgs& a, RowsItem* items, uin
     __syncwarp();
 }
 
-template <int HD>
+template <int HD, bool WIN>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     rows_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_small,
                           const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -834,7 +885,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     unsigned char* sK = sQ + 2 * C::TILE;           // [RING][NH][128 keys][128 B]
     unsigned char* sV = sK + RING * C::TILE;        // [RING][8 pages][NH][16][128 B]
     RowsPlan& plan = *reinterpret_cast<RowsPlan*>(sV + RING * C::TILE);
-    RowsItem* items = reinterpret_cast<RowsItem*>(&plan + 1);
+    using Item = RowsItemOf<WIN>;
+    Item* items = reinterpret_cast<Item*>(&plan + 1);
     uint64_t* bars = reinterpret_cast<uint64_t*>(
         (reinterpret_cast<uintptr_t>(items + kRowsItems) + 7) & ~uintptr_t(7));
     const RowsBars<C::RING> bar(bars);
@@ -876,7 +928,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tc_fence_before();
     }
-    rows_plan(a, plan);  // ends with a CTA-wide barrier
+    rows_plan<WIN>(a, plan);  // ends with a CTA-wide barrier
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -892,7 +944,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                __all_sync(0xffffffffu, mbar_wait(s_addr(bar), (uint32_t)parity & 1u)) != 0;
     };
     // the k-th item of this CTA; false: none is left, or a wait ran out
-    auto next_item = [&](int k, RowsItem& it) -> bool {
+    auto next_item = [&](int k, Item& it) -> bool {
         const int d = k % kRowsItems;
         if (!wait(&i_full[d], k / kRowsItems)) {
             give_up(20);
@@ -918,7 +970,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         int c = 0, ended = 0;   // operations and items done on this slot
         int op = 0, tile = 0;   // operations (on both slots) and key tiles of the items before
         bool ok = true;
-        RowsItem it;
+        Item it;
         for (int k = 0; ok && next_item(k, it); ++k) {
             // this slot's part: a pair's tile, a dual's even (0) or odd (1) key tiles
             const int role = (op ^ ws) & 1, tile0 = tile;
@@ -937,8 +989,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             const bool here = quarter * 32 < ntok * a.G;  // the warp holds a real row
             const uint64_t bits = it.mode == kModeMask && real ? a.mask[i] : 0ull;
             // slots below `every` are seen by all rows of the tile
-            const int every = it.mode == kModeCausal ? min(it.end, it.ctx + it.i0 + t * a.tpt + 1)
-                                                     : (it.mode == kModeMask ? min(it.end, it.ctx) : it.end);
+            const int every = WIN || it.mode == kModeCausal ? min(it.end, it.ctx + it.i0 + t * a.tpt + 1)
+                                                            : (it.mode == kModeMask ? min(it.end, it.ctx) : it.end);
+            // the last slot behind the first tokens that not every row of the tile sees
+            const int far = WIN ? it.ctx + it.i0 + t * a.tpt + max(ntok, 1) - 1 - a.window : 0;
             float m = real ? -INFINITY : 0.f, l = 0.f;
             for (int j = j0; j < it.n_kt; j += jstep, ++c) {
                 if (!(ok = wait(&s_full[ws], c))) break;
@@ -950,9 +1004,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     // took a quarter longer for an 8192-token prompt, and masking within the
                     // first pass 3%.
                     const int key0 = it.slot0 + 128 * j;
-                    const bool masked = key0 + 128 > every;
+                    const bool masked = key0 + 128 > every || (WIN && key0 <= far && key0 + 128 > a.sinks);
                     uint64_t seen_lo = ~0ull, seen_hi = ~0ull;
-                    if (masked) rows_seen(it, key0, i, bits, seen_lo, seen_hi);
+                    if (masked) rows_seen<WIN>(a, it, key0, i, bits, seen_lo, seen_hi);
                     float mx[2] = {-INFINITY, -INFINITY};
                     uint32_t va[32], vb[32];
                     auto largest = [&](uint32_t(&v)[32], int q) {
@@ -1111,7 +1165,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 const bool mine = real && l == l && (bad || !(far * inv < kHalfOver));
                 if (__any_sync(0xffffffffu, mine)) {
                     const bool all = __any_sync(0xffffffffu, mine && spoilt);
-                    if (rows_nonfinite<HD>(a, items[k % kRowsItems], mine, all, i, bits, head,
+                    if (rows_nonfinite<HD, WIN>(a, items[k % kRowsItems], mine, all, i, bits, head,
                                            it.prow < 0 ? (size_t)tok : prow))
                         l = -l;
                 }
@@ -1140,7 +1194,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 int idx = next;
                 if (a.counter) idx = __shfl_sync(0xffffffffu, lane == 0 ? (int)atomicAdd(a.counter, 1u) : 0, 0);
                 else next += gridDim.x;
-                const RowsItem it = rows_item(a, plan, idx);
+                const Item it = rows_item<WIN>(a, plan, idx);
                 if (it.n_kt == 0) {  // no keys: the rows' results are zero
                     rows_zero<HD>(a, it, lane);
                     continue;
@@ -1160,12 +1214,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         int kc = 0, vc = 0, qn[2] = {0, 0};  // K and V tiles loaded; query loads of a slot
         int op = 0;                          // operations of the items before
         bool ok = true;
-        RowsItem it;
+        Item it;
         for (int k = 0; ok && next_item(k, it); ++k) {
             const int page0 = it.slot0 >> 4, pages = ((it.end + 15) >> 4) - page0;
             const int32_t* tab = a.tables + (size_t)it.trow * a.max_blocks + page0;
             auto page_at = [&](int i) {
-                int x = i < pages ? tab[i] : 0;
+                int x = 0;
+                if (i < pages) {
+                    if constexpr (WIN) x = tab[page0 + i < it.sinkp ? i : i + it.gap];
+                    else x = tab[i];
+                }
                 return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
             };
             int pg = page_at(lane), pg_next = 0;  // pages of four tiles, one a lane
@@ -1233,7 +1291,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         // ------------------------------------------------------------ V made safe
         int vc = 0;
         bool ok = true;
-        RowsItem it;
+        Item it;
         for (int k = 0; ok && next_item(k, it); ++k) {
             for (int j = 0; j < it.n_kt; ++j, ++vc) {
                 const int slot = vc % RING, key0 = it.slot0 + 128 * j;
@@ -1252,23 +1310,30 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     touched = true;
                 }
                 bool found = false;
-                for (int i = lo * NH * 8 + lane; i < n * NH * 8; i += 32) {
-                    const int row = i / (NH * 8), h = i / 8 % NH;
-                    uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
-                                                         (i & 7) * 16);
-                    uint4 x = *at;
-                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
-                    bool mine = false;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
-                        if (l16) xs[e] &= 0xFFFF0000u;
-                        if (h16) xs[e] &= 0x0000FFFFu;
-                        mine |= l16 || h16;
+                auto look = [&](int from, int to) {
+                    for (int i = from * NH * 8 + lane; i < to * NH * 8; i += 32) {
+                        const int row = i / (NH * 8), h = i / 8 % NH;
+                        uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
+                                                             (i & 7) * 16);
+                        uint4 x = *at;
+                        uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+                        bool mine = false;
+    #pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
+                            if (l16) xs[e] &= 0xFFFF0000u;
+                            if (h16) xs[e] &= 0x0000FFFFu;
+                            mine |= l16 || h16;
+                        }
+                        if (mine) *at = x;
+                        found |= mine;
                     }
-                    if (mine) *at = x;
-                    found |= mine;
-                }
+                };
+                look(lo, n);
+                // and between the first tokens and the last row's window
+                if constexpr (WIN)
+                    look(rows_clamp(a.sinks - key0, 0, lo),
+                         rows_clamp(it.ctx + it.i0 + it.ntok0 + it.ntok1 - key0 - a.window, 0, lo));
                 found = __any_sync(0xffffffffu, found);
                 if (found && lane == 0) items[k % kRowsItems].bad = 1;
                 if (touched || found) fence_async_smem();
@@ -1280,7 +1345,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             done_item(k);
         }
     } else if (warp == kRowsMmaWarp) {
-        rows_mma<HD>(a, items, tmem, s_addr(sQ), s_addr(sK), s_addr(sV), bars, abort_flag);
+        rows_mma<HD, WIN>(a, items, tmem, s_addr(sQ), s_addr(sK), s_addr(sV), bars, abort_flag);
     }
     tc_fence_before();
     __syncthreads();
@@ -1484,10 +1549,13 @@ static int rows_sms(int* out) {  // SMs of the current device; sets the kernels'
     SD_CHECK(dev >= 0 && dev < 64, SPECDEC_ENOTSUP, "attention: device index above 63");
     int n = facts[dev].sms.load();
     if (!n) {
-        SD_CUDA(cudaFuncSetAttribute(rows_attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)RowsCfg<128>::smem));
-        SD_CUDA(cudaFuncSetAttribute(rows_attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)RowsCfg<64>::smem));
+        const auto room = [](const void* fn, size_t bytes) {
+            return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        };
+        SD_CUDA(room((const void*)rows_attention_kernel<128, false>, RowsCfg<128>::smem));
+        SD_CUDA(room((const void*)rows_attention_kernel<64, false>, RowsCfg<64>::smem));
+        SD_CUDA(room((const void*)rows_attention_kernel<128, true>, RowsCfg<128>::smem));
+        SD_CUDA(room((const void*)rows_attention_kernel<64, true>, RowsCfg<64>::smem));
         SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         facts[dev].sms.store(n);
     }
@@ -1538,8 +1606,9 @@ static int launch_rows(RowsArgs a, const __half* q, int ldq, const __half* kv, i
     if (rc) return rc;
     if (a.counter) SD_CUDA(cudaMemsetAsync(a.counter, 0, sizeof(uint32_t), s));
     const unsigned grid = (unsigned)(prows ? sms : std::min<long long>(sms, tiles));
-    if (HD == 128) rows_attention_kernel<128><<<grid, kRowsThreads, RowsCfg<128>::smem, s>>>(qmap, qsmall, kmap, vmap, a);
-    else rows_attention_kernel<64><<<grid, kRowsThreads, RowsCfg<64>::smem, s>>>(qmap, qsmall, kmap, vmap, a);
+    const auto fn = HD == 128 ? (a.window ? rows_attention_kernel<128, true> : rows_attention_kernel<128, false>)
+                              : (a.window ? rows_attention_kernel<64, true> : rows_attention_kernel<64, false>);
+    fn<<<grid, kRowsThreads, HD == 128 ? RowsCfg<128>::smem : RowsCfg<64>::smem, s>>>(qmap, qsmall, kmap, vmap, a);
     SD_LAUNCH_CHECK("rows_attention_kernel");
     if (prows) {
         cudaLaunchConfig_t cfg = {};
@@ -1578,6 +1647,35 @@ static int check_workspace(const char* who, const void* ws, size_t have, size_t 
     return SPECDEC_OK;
 }
 
+// Packed rows within a window (window > 0) and behind the first tokens, or causal (0).
+size_t rows_packed_workspace(int B, int T, int Hq, int HD, int max_blocks) {
+    return rows_workspace(prompt_partial_rows(T, max_blocks), B, Hq, HD);
+}
+int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_blocks, int Hkv, int HD, const int32_t* tables,
+                       int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B, int T, int Hq, int window,
+                       int sinks, __half* out, int ldo, void* ws, cudaStream_t s) {
+    size_t prows = prompt_partial_rows(T, max_blocks);
+    if ((long long)T * Hq >= 1 << 30) prows = 0;  // the merge counts rows and heads in 32 bits
+    RowsArgs a = {};
+    a.num_blocks = num_blocks;
+    a.Hkv = Hkv;
+    a.Hq = Hq;
+    a.tables = tables;
+    a.max_blocks = max_blocks;
+    a.ctx_len = ctx_len;
+    a.row_off = row_off;
+    a.B = B;
+    a.T = T;
+    a.R = 1;
+    a.tq_small = 1;
+    a.window = window;
+    a.sinks = sinks;
+    a.out = out;
+    a.ldo = ldo;
+    const int tpt2 = 2 * (128 / (Hq / Hkv));
+    return launch_rows(a, q, ldq, kv, HD, prows, (long long)Hkv * ((T + tpt2 - 1) / tpt2 + std::min(B, T)), ws, s);
+}
+
 }  // namespace specdec
 
 using namespace specdec;
@@ -1586,7 +1684,7 @@ extern "C" size_t specdec_attention_prompt_workspace_bytes(int B, int T, int n_q
                                                            int max_blocks) {
     (void)n_kv_heads;
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
-    return rows_workspace(prompt_partial_rows(T, max_blocks), B, n_q_heads, head_dim);
+    return rows_packed_workspace(B, T, n_q_heads, head_dim, max_blocks);
 }
 
 extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1603,29 +1701,12 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
     SD_CHECK(ldq >= n_q_heads * head_dim && ldq % 8 == 0 && ldo >= n_q_heads * head_dim && ldo % 8 == 0,
              SPECDEC_EINVAL, "attention_prompt: row strides hold all heads and are multiples of 8");
     if (B == 0 || T == 0) return SPECDEC_OK;
-    size_t prows = prompt_partial_rows(T, max_blocks);
     if ((rc = check_workspace("attention_prompt", workspace, workspace_bytes,
-                              rows_workspace(prows, B, n_q_heads, head_dim))))
+                              rows_packed_workspace(B, T, n_q_heads, head_dim, max_blocks))))
         return rc;
-    if ((long long)T * n_q_heads >= 1 << 30) prows = 0;  // the merge counts rows and heads in 32 bits
-    RowsArgs a = {};
-    a.num_blocks = num_blocks;
-    a.Hkv = n_kv_heads;
-    a.Hq = n_q_heads;
-    a.tables = tables;
-    a.max_blocks = max_blocks;
-    a.ctx_len = ctx_len;
-    a.row_off = row_off;
-    a.B = B;
-    a.T = T;
-    a.R = 1;
-    a.tq_small = 1;
-    a.out = reinterpret_cast<__half*>(out);
-    a.ldo = ldo;
-    const int tpt2 = 2 * (128 / (n_q_heads / n_kv_heads));
-    return launch_rows(a, reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer), head_dim,
-                       prows, (long long)n_kv_heads * ((T + tpt2 - 1) / tpt2 + std::min(B, T)), workspace,
-                       as_stream(stream));
+    return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
+                              num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads, 0,
+                              0, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads,
