@@ -27,13 +27,15 @@ constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a ca
 // (sequence, tile of rows, KV head, page), are cut into equal ranges, one for
 // each warp of the grid: ragged lengths balance by themselves.  A tile is as many
 // whole tokens as fit into 8 * NT rows (row = token * G + g).  For a page
-//   S^T [16 keys][rows] = K Q^T,  P = 2^(S' - m + 15),  O^T [hd][rows] += V^T P
+//   S^T [16 keys][rows] = K Q^T,  P = 2^(S' - m),  O^T [hd][rows] += V^T P
 // in mma.sync of 16 x 8 x 16: 16 keys of 8 rows are 4 FLOP for each byte of the
 // cache, far from what the tensor cores of either kind can do, and the fragments
 // stay in registers (128 rows of tensor memory for 4 to 32 real ones would not).
-// A row's largest score m is exact after each page, and 15 takes the largest
-// weight to fp16's upper end: weights keep their 11 bits down to 2^-29 of it.
-// m, sums and O are fp32.
+// The reference m of a row is 11 below its largest score at the time it was set and
+// follows only when a score is more than 15 above it, so most pages move nothing
+// and need no maximum across lanes.  P, rounded to fp16 for the product, is 2^15 at
+// most, and weights keep their 11 bits down to 2^-25 of the largest (2^-29 where m
+// is as high as it can be).  m, sums and O are fp32.
 //
 // Ranges that a warp shares with others leave unnormalised O with (m, l); they
 // are joined in their order.
@@ -41,7 +43,8 @@ constexpr int kFewWarps = 8;
 constexpr int kFewMaxCtas = 148;   // ranges: at most so many CTAs of warps
 constexpr int kFewMaxRows = 32;    // rows of a tile
 constexpr int kFewMinPages = 4;    // of a range
-constexpr float kFewLift = 15.0f;
+constexpr float kFewLift = 11.0f, kFewTop = 15.0f;
+constexpr float kFewNone = -3e38f;  // m of a row that has seen no slot: below all scores
 constexpr float kFewMax = 65504.0f;
 
 struct FewArgs {
@@ -73,9 +76,11 @@ struct FewArgs {
 
 struct FewSeq {
     int lo, n, ctx;
+    int np;  // pages of each of its (tile, head)
 };
 __device__ __forceinline__ FewSeq few_seq(const FewArgs& a, int b) {
     FewSeq s;
+    s.np = 0;
     s.lo = max(0, min(a.row_off[b], a.T));
     s.n = max(s.lo, min(a.row_off[b + 1], a.T)) - s.lo;
     s.ctx = max(0, min(a.ctx_len[b], 1 << 30));
@@ -118,7 +123,7 @@ struct FewWalk {
     FewTile t;
 };
 // To the next segment; false: the range is done.
-__device__ __forceinline__ bool few_next(const FewArgs& a, const long long* pre, const int* np, FewWalk& w) {
+__device__ __forceinline__ bool few_next(const FewArgs& a, const long long* pre, const FewSeq* seqs, FewWalk& w) {
     if (w.u >= w.hi) return false;
     int lo = 0, hi = a.B;  // last sequence with pre <= u
     while (hi - lo > 1) {
@@ -128,11 +133,12 @@ __device__ __forceinline__ bool few_next(const FewArgs& a, const long long* pre,
     }
     w.b = lo;
     const long long local = w.u - pre[lo];
-    const int n = np[lo], pair = (int)(local / n);
+    const FewSeq s = seqs[lo];
+    const int n = s.np, pair = n < 1 ? 0 : local >> 31 ? (int)(local / n) : (int)local / n;
     w.v = (int)(local - (long long)pair * n);
     w.tile = pair / a.Hkv;
     w.kvh = pair - w.tile * a.Hkv;
-    w.t = few_tile(a, few_seq(a, lo), w.tile);
+    w.t = few_tile(a, s, w.tile);
     w.begun = w.u;
     const int take = (int)min((long long)(n - w.v), w.hi - w.u);
     w.u += take;
@@ -204,7 +210,7 @@ struct FewCfg {
     static constexpr int PAGE = 64 * HD;                 // bytes of a page's K and V of a head
     static constexpr int RING = HD == 128 ? 3 : 6;       // pages in flight of a warp
     static constexpr size_t smem(int B) {
-        return 1024 + (size_t)kFewWarps * RING * PAGE + kFewWarps * RING * 8 + (size_t)(B + 1) * 8 + (size_t)B * 4 + 16;
+        return 1024 + (size_t)kFewWarps * RING * PAGE + kFewWarps * RING * 8 + (size_t)(B + 1) * 8 + (size_t)B * sizeof(FewSeq) + 16;
     }
 };
 static_assert(FewCfg<128>::smem(kBoundMaxSeqs) <= 232448 && FewCfg<64>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a CTA");
@@ -212,7 +218,7 @@ static_assert(FewCfg<128>::smem(kBoundMaxSeqs) <= 232448 && FewCfg<64>::smem(kBo
 // Pages before each sequence, by every CTA for itself from the lengths in device
 // memory (so a captured call serves other lengths); CTA 0 leaves them for the
 // kernels that follow.
-__device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, int* np, bool acc) {
+__device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, FewSeq* seqs, bool acc) {
     __shared__ long long wsum[kFewWarps];
     __shared__ int csum[kFewWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -221,9 +227,9 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     long long x = 0;
     int c = 0;
     for (int b = b0; b < b1; ++b) {
-        const FewSeq s = few_seq(a, b);
-        const int n = few_pages(a, s);
-        np[b] = n;
+        FewSeq s = few_seq(a, b);
+        const int n = s.np = few_pages(a, s);
+        seqs[b] = s;
         const long long all = (long long)((s.n + a.tpt - 1) / a.tpt) * a.Hkv * n;
         pre[b] = all;
         x += all;
@@ -262,10 +268,10 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
         pre[b] = before;
         if (blockIdx.x == 0) {
             a.pre[b] = before;
-            a.np[b] = np[b];
+            a.np[b] = seqs[b].np;
             if (acc) {
                 a.chunks[b] = cbefore;
-                if (all > 0) cbefore += a.Hkv * ((np[b] + 7) / 8);
+                if (all > 0) cbefore += a.Hkv * ((seqs[b].np + 7) / 8);
             }
         }
         before += all;
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + kFewWarps * RING * C::PAGE);
     long long* pre = reinterpret_cast<long long*>(bars + kFewWarps * RING);
-    int* np = reinterpret_cast<int*>(pre + a.B + 1);
+    FewSeq* seqs = reinterpret_cast<FewSeq*>(pre + a.B + 1);
     pdl_trigger();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int g = lane >> 2, t4 = lane & 3;
@@ -304,7 +310,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
         for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const long long total = few_plan(a, pre, np, ACC);  // ends with a CTA-wide barrier
+    const long long total = few_plan(a, pre, seqs, ACC);  // ends with a CTA-wide barrier
     const long long per = few_per(a, total);
     // neighbouring ranges on different SMs: a call of few ranges has them to itself
     const int range = warp * gridDim.x + blockIdx.x;
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
     };
     auto load = [&]() {
         while (more && ld.v >= ld.ve) {
-            more = few_next(a, pre, np, ld);
+            more = few_next(a, pre, seqs, ld);
             if (more) {
                 tb = ld.v;
                 ent = entry(tb + lane);
@@ -356,12 +362,17 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
     w.hi = u1;
     int done = 0;
     bool ok = true;
-    while (ok && few_next(a, pre, np, w)) {
+    while (ok && few_next(a, pre, seqs, w)) {
         const FewTile& t = w.t;
         const int rows = t.tokens * a.G, p1 = t.p0 + t.tokens - 1;
         uint32_t qf[NT][KS][2];
         int slot_of[NT][2];  // slots of this lane's rows 2 t4, 2 t4 + 1 (of those behind the tile: the last one's)
         float m[NT][2], l[NT][2], o[KS][NT][4];
+        float* score[NT];  // of this lane's rows at its slot of a page
+        auto score_at = [&](int row0, int row) {
+            const int tok = row / a.G;
+            return a.scores + ((size_t)(row0 + tok) * a.Hkv + w.kvh) * a.slots_max * a.G + (row - tok * a.G);
+        };
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int row = 8 * n + g;
@@ -376,9 +387,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 slot_of[n][e] = t.p0 + min(t.tokens - 1, (8 * n + 2 * t4 + e) / a.G);
-                m[n][e] = -INFINITY;
+                m[n][e] = kFewNone;
                 l[n][e] = 0.f;
             }
+            if constexpr (ACC) score[n] = score_at(t.row, 8 * n + 2 * t4) + (size_t)g * a.G;
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -394,7 +406,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
             const int s0 = 16 * (v < t.sinkp ? v : v + t.gap);
             // every row sees every slot of the page
             const bool clear = s0 + 15 <= t.p0 && (s0 + 15 < a.sinks || s0 > p1 - a.window);
-            float s[NT][4];
+            float s[NT][4], s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile of rows: two chains
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -404,10 +416,11 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
                 uint32_t x[4];
                 few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
 #pragma unroll
-                for (int n = 0; n < NT; ++n) few_mma(s[n], x, qf[n][k][0], qf[n][k][1]);
+                for (int n = 0; n < NT; ++n) few_mma(NT == 1 && (k & 1) ? s2 : s[n], x, qf[n][k][0], qf[n][k][1]);
             }
-            uint32_t pb[NT][2];
-            float top[NT][2];
+            if constexpr (NT == 1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[0][e] += s2[e];
             bool grow = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -420,8 +433,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
                     }
                 }
                 if constexpr (ACC) {  // the rows' scores, for their weights once the rows' sums are known
-                    const int row = 8 * n + 2 * t4, tok = row / a.G, gg = row - tok * a.G;
-                    float* dst = a.scores + (((size_t)(t.row + tok) * a.Hkv + w.kvh) * a.slots_max + s0 + g) * a.G + gg;
+                    const int row = 8 * n + 2 * t4;
+                    float* dst = score[n] + (size_t)s0 * a.G;
                     if ((a.G & 1) == 0) {
                         if (row < rows) {
                             *reinterpret_cast<float2*>(dst) = make_float2(s[n][0], s[n][1]);
@@ -433,21 +446,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
                             dst[8 * a.G] = s[n][2];
                         }
                         if (row + 1 < rows) {
-                            const int tok1 = (row + 1) / a.G, g1 = row + 1 - tok1 * a.G;
-                            float* d1 = a.scores + (((size_t)(t.row + tok1) * a.Hkv + w.kvh) * a.slots_max + s0 + g) * a.G + g1;
+                            float* d1 = score_at(t.row, row + 1) + (size_t)(s0 + g) * a.G;
                             d1[0] = s[n][1];
                             d1[8 * a.G] = s[n][3];
                         }
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x = few_max(s[n][e], s[n][2 + e]);
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) x = few_max(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    top[n][e] = x;
-                    grow |= !(x <= m[n][e]);  // also for NaN
-                }
+                // (also for NaN)
+                grow |= !(few_max(s[n][0], s[n][2]) - m[n][0] <= kFewTop) || !(few_max(s[n][1], s[n][3]) - m[n][1] <= kFewTop);
             }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -455,10 +461,19 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
                     float f[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float now = few_max(m[n][e], top[n][e]);
-                        f[e] = m[n][e] == now || m[n][e] == -INFINITY ? 1.f : exp2f(m[n][e] - now);
-                        m[n][e] = now;
-                        l[n][e] *= f[e];
+                        float top = few_max(s[n][e], s[n][2 + e]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = few_max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        f[e] = 1.f;
+                        if (!(top - m[n][e] <= kFewTop)) {
+                            // a NaN or infinite maximum makes every weight, and so the row, NaN; far from 0 the 11 would
+                            // be lost in rounding
+                            const float now = top < INFINITY ? (fabsf(top) < 0x1p20f ? top - kFewLift : top)
+                                                             : __int_as_float(0x7FC00000);
+                            f[e] = m[n][e] == kFewNone ? 0.f : exp2f(m[n][e] - now);
+                            m[n][e] = now;
+                            l[n][e] *= f[e];
+                        }
                     }
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
@@ -466,16 +481,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
                         for (int e = 0; e < 4; ++e) o[k][n][e] *= f[e & 1];
                 }
             }
+            uint32_t pb[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // a NaN or infinite maximum makes every weight, and so the row, NaN
-                    const float mm = m[n][e & 1];
-                    const float sub = mm == -INFINITY ? 0.f : (mm < INFINITY ? mm : __int_as_float(0x7FC00000));
-                    y[e] = few_exp2((s[n][e] - sub) + kFewLift);
-                }
+                for (int e = 0; e < 4; ++e) y[e] = few_exp2(s[n][e] - m[n][e & 1]);
                 l[n][0] += y[0] + y[2];
                 l[n][1] += y[1] + y[3];
                 const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
@@ -581,26 +592,27 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
 
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in their
 // order: a warp for each row and head of up to 8 pieces, else the CTA's four warps
-// take every fourth piece and are joined in their order.
-template <int HD>
+// take every fourth piece and are joined in their order.  ROWS: rows of a CTA, 1
+// where there are few (148 pieces of each of 32 rows: 115 us a call with four rows
+// of a CTA one after the other).  Where the row belongs is looked up while the
+// kernel before still runs.
+template <int HD, int ROWS>
 __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
     constexpr int W = HD / 32;
     __shared__ float sm[4], sl[4], so[4][HD];
     __shared__ int sbad[4];
     pdl_trigger();
-    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long total = a.pre[a.B], per = few_per(a, total);
-    const long long rows = (long long)a.T * a.Hq, first = 4LL * blockIdx.x;
+    const long long rows = (long long)a.T * a.Hq, first = (long long)ROWS * blockIdx.x;
     struct Row {
-        int n, b, p, kvh, row;
+        int n, b, p, kvh, row, np, tile;
         long long r0, u0;
         __half* dst;
         size_t at;
     };
     auto find = [&](long long idx) {
         Row x;
-        x.n = 0;
+        x.n = x.np = 0;
         if (idx >= rows) return x;
         const int r = (int)(idx / a.Hq), head = (int)(idx - (long long)r * a.Hq);
         int lo = 0, hi = a.B;  // first sequence whose end is past the row
@@ -613,19 +625,26 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
         const FewSeq s = few_seq(a, lo);
         const int i = r - s.lo;
         if (i < 0 || i >= s.n) return x;
-        const int tile = i / a.tpt;
-        const FewTile t = few_tile(a, s, tile);
+        x.tile = i / a.tpt;
+        x.np = few_tile(a, s, x.tile).np;
         x.b = lo;
         x.p = s.ctx + i;
         x.kvh = head / a.G;
-        x.row = (i - tile * a.tpt) * a.G + head - x.kvh * a.G;
-        x.u0 = a.pre[lo] + ((long long)tile * a.Hkv + x.kvh) * a.np[lo];
-        x.r0 = x.u0 / per;
-        x.n = t.np > 0 ? (int)((x.u0 + t.np - 1) / per - x.r0) + 1 : 0;
+        x.row = (i - x.tile * a.tpt) * a.G + head - x.kvh * a.G;
         x.dst = a.out + (size_t)r * a.ldo + (size_t)head * HD;
         x.at = (size_t)r * a.Hq + head;
         return x;
     };
+    Row mine = find(first + (ROWS == 1 ? 0 : warp));
+    pdl_wait();
+    const long long total = a.pre[a.B], per = few_per(a, total);
+    auto count = [&](Row& x) {  // its pieces
+        if (x.np <= 0) return;
+        x.u0 = a.pre[x.b] + ((long long)x.tile * a.Hkv + x.kvh) * a.np[x.b];
+        x.r0 = x.u0 / per;
+        x.n = (int)((x.u0 + x.np - 1) / per - x.r0) + 1;
+    };
+    count(mine);
     float m, l, o[W];
     bool bad;
     auto join = [&](const Row& x, int k0, int step) {  // pieces k0, k0 + step, ..
@@ -634,18 +653,18 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
         bad = false;
 #pragma unroll
         for (int e = 0; e < W; ++e) o[e] = 0.f;
-        constexpr int P = 4;
+        constexpr int P = 8;
         for (int k = k0; k < x.n; k += P * step) {
             float2 ml[P];
             float v[P][W];
 #pragma unroll
             for (int u = 0; u < P; ++u) {
-                const long long range = x.r0 + min(x.n - 1, k + u * step);
-                const size_t at = (size_t)(2 * range + (x.u0 > range * per ? 1 : 0)) * tile_rows + x.row;
-                ml[u] = a.pml[at];
+                const bool real = k + u * step < x.n;
+                const long long range = x.r0 + k + u * step;
+                const size_t at = real ? (size_t)(2 * range + (x.u0 > range * per ? 1 : 0)) * tile_rows + x.row : 0;
+                ml[u] = real ? a.pml[at] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int e = 0; e < W; ++e) v[u][e] = a.po[at * HD + lane * W + e];
-                if (k + u * step >= x.n) ml[u] = make_float2(-INFINITY, 0.f);
+                for (int e = 0; e < W; ++e) v[u][e] = real ? a.po[at * HD + lane * W + e] : 0.f;
             }
             float top = m;
 #pragma unroll
@@ -680,14 +699,17 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
         if (a.ml && lane == 0) a.ml[x.at] = make_float2(m, inv);
         if (__any_sync(0xffffffffu, bad) && l == l) few_nonfinite<HD>(a, x.b, x.p, x.kvh, x.dst);
     };
-    const Row mine = find(first + warp);
-    if (mine.n > 1 && mine.n <= 8) {
+    if (mine.n > 1 && mine.n <= 8 && (ROWS > 1 || warp == 0)) {
         join(mine, 0, 1);
         finish(mine);
     }
     if (!__syncthreads_or(mine.n > 8)) return;
-    for (int k = 0; k < 4; ++k) {
-        const Row x = find(first + k);
+    for (int k = 0; k < ROWS; ++k) {
+        Row x = mine;
+        if constexpr (ROWS > 1) {
+            x = find(first + k);
+            count(x);
+        }
         if (x.n <= 8) continue;  // (the same for all)
         join(x, warp, 4);
         if (lane == 0) {
@@ -723,7 +745,8 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
 
 // weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
 // of 2^(x - m) / l, from the scores that few_rows_kernel left.  A warp for 128
-// slots of a head, four a lane.
+// slots of a head, four a lane; V heads' scores in one load.
+template <int V>
 __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant__ FewArgs a) {
     extern __shared__ int chunks[];
     pdl_wait();
@@ -741,27 +764,47 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
         const int per_head = (chunks[lo + 1] - chunks[lo]) / a.Hkv, local = c - chunks[lo];
         const int kvh = local / per_head, j0 = 128 * (local - kvh * per_head);
         const int end = min(min(s.ctx + s.n, a.slots_max), j0 + 128);
-        float sum[4] = {};
+        float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
+        float sum[4] = {}, was[4] = {};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (j0 + 32 * u + lane < end) was[u] = dst[j0 + 32 * u + lane];
+#pragma unroll 2
         for (int i = max(0, j0 - s.ctx); i < s.n; ++i) {
-            const int r = s.lo + i, p = s.ctx + i;
+            const int r = s.lo + i, p = min(s.ctx + i, end - 1);
             const float* src = a.scores + ((size_t)r * a.Hkv + kvh) * a.slots_max * a.G;
             const float2* ml = a.ml + (size_t)r * a.Hq + kvh * a.G;
-            for (int g = 0; g < a.G; ++g) {
-                const float2 y = ml[g];
-                const float sub = y.x == -INFINITY ? 0.f : y.x;
+            for (int g = 0; g < a.G; g += V) {
+                float x[4][V];
+                float2 y[V];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int j = j0 + 32 * u + lane;
-                    if (j < end && j <= p) sum[u] += few_exp2((src[(size_t)j * a.G + g] - sub) + kFewLift) * y.y;
+                    const float* at = src + (size_t)j * a.G + g;
+                    if (j <= p) {
+                        if constexpr (V == 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(at);
+                            x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
+                        } else if constexpr (V == 2) {
+                            const float2 f = *reinterpret_cast<const float2*>(at);
+                            x[u][0] = f.x, x[u][1] = f.y;
+                        } else {
+                            x[u][0] = *at;
+                        }
+                    }
                 }
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = ml[g + v];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (j0 + 32 * u + lane <= p)
+#pragma unroll
+                        for (int v = 0; v < V; ++v) sum[u] += few_exp2(x[u][v] - y[v].x) * y[v].y;
             }
         }
-        float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = j0 + 32 * u + lane;
-            if (j < end) dst[j] += sum[u];
-        }
+        for (int u = 0; u < 4; ++u)
+            if (j0 + 32 * u + lane < end) dst[j0 + 32 * u + lane] = was[u] + sum[u];
     }
 }
 
@@ -862,16 +905,20 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)(((long long)a.T * a.Hq + 3) / 4));
+    const long long rows = (long long)a.T * a.Hq;
+    const bool single = rows <= 2048;
+    cfg.gridDim = dim3((unsigned)(single ? rows : (rows + 3) / 4));
     cfg.blockDim = dim3(128);
-    if (HD == 128) SD_CUDA(cudaLaunchKernelEx(&cfg, few_merge_kernel<128>, a, 8 * NT));
-    else SD_CUDA(cudaLaunchKernelEx(&cfg, few_merge_kernel<64>, a, 8 * NT));
+    const auto merge = HD == 128 ? (single ? few_merge_kernel<128, 1> : few_merge_kernel<128, 4>)
+                                 : (single ? few_merge_kernel<64, 1> : few_merge_kernel<64, 4>);
+    SD_CUDA(cudaLaunchKernelEx(&cfg, merge, a, 8 * NT));
     if (acc) {
         const long long chunks = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
         cfg.gridDim = dim3((unsigned)std::min<long long>((chunks + 7) / 8, 8LL * sms));
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = (size_t)(a.B + 1) * 4;
-        SD_CUDA(cudaLaunchKernelEx(&cfg, few_weights_kernel, a));
+        const auto weigh = a.G % 4 == 0 ? few_weights_kernel<4> : (a.G % 2 == 0 ? few_weights_kernel<2> : few_weights_kernel<1>);
+        SD_CUDA(cudaLaunchKernelEx(&cfg, weigh, a));
     }
     return SPECDEC_OK;
 }
