@@ -24,9 +24,12 @@ constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a ca
 // A warp works for itself: it streams pages (16 tokens of one KV head, K and V
 // together, one TMA request) through a ring of its own, so no barrier of the CTA
 // stands between its loads and its arithmetic.  The call's pages, in the order
-// (sequence, tile of rows, KV head, page), are cut into equal ranges, one for
-// each warp of the grid: ragged lengths balance by themselves.  A tile is as many
-// whole tokens as fit into 8 * NT rows (row = token * G + g).  For a page
+// (sequence, tile of rows, KV head, page), are cut into ranges, one for each warp,
+// so ragged lengths balance by themselves.  SMs do not get equal shares of the
+// memory's rate (with one equal range for each warp the CTAs of 64 single tokens
+// on 4096 ended between 124 and 166 us), so a fifth of the pages is left for a
+// second wave of CTAs, which start where the first ones end early.  A tile is as
+// many whole tokens as fit into 8 * NT rows (row = token * G + g).  For a page
 //   S^T [16 keys][rows] = K Q^T,  P = 2^(S' - m),  O^T [hd][rows] += V^T P
 // in mma.sync of 16 x 8 x 16: 16 keys of 8 rows are 4 FLOP for each byte of the
 // cache, far from what the tensor cores of either kind can do, and the fragments
@@ -39,9 +42,13 @@ constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a ca
 //
 // Ranges that a warp shares with others leave unnormalised O with (m, l); they
 // are joined in their order.
-constexpr int kFewWarps = 8;
-constexpr int kFewMaxCtas = 148;   // ranges: at most so many CTAs of warps
+constexpr int kFewWarps = 4;       // of a CTA
+constexpr int kFewMaxSms = 148;    // SMs for which there are ranges
 constexpr int kFewMaxRows = 32;    // rows of a tile
+// CTAs of an SM, and waves of them.  Registers allow three of one tile of 8 rows; the pieces of many rows cost as
+// much as the wave gains.
+__host__ __device__ constexpr int few_resident(int NT) { return NT == 1 ? 3 : 2; }
+__host__ __device__ constexpr int few_waves(int NT) { return NT <= 2 ? 2 : 1; }
 constexpr int kFewMinPages = 4;    // of a range
 constexpr float kFewLift = 11.0f, kFewTop = 15.0f;
 constexpr float kFewNone = -3e38f;  // m of a row that has seen no slot: below all scores
@@ -62,13 +69,13 @@ struct FewArgs {
     __half* out;
     int ldo;
     float scale_log2;
-    int ranges;
+    int ctas, waves;    // CTAs of a wave
     // workspace
-    long long* pre;     // [B + 1] pages before sequence b, then the pages of a range
+    long long* pre;     // [B + 1] pages before sequence b
     int32_t* np;        // [B] pages of each (tile, head) of sequence b
     int32_t* chunks;    // [B + 1] chunks of slots before sequence b (weights)
-    float2* pml;        // [2 * ranges][rows] m, l of a piece (l < 0: it met an infinity or NaN of V)
-    float* po;          // [2 * ranges][rows][hd]
+    float2* pml;        // [ranges][2][rows] m, l of a piece (l < 0: it met an infinity or NaN of V): of the range's
+    float* po;          // [ranges][2][rows][hd]  first pages, or of later ones
     float2* ml;         // [T][Hq] m, 1 / l (weights)
     float* scores;      // [T][Hkv][slots_max][G] (weights)
     DeviceStatus* status;
@@ -205,15 +212,17 @@ __device__ __noinline__ void few_nonfinite(const FewArgs& a, int b, int p, int k
             if (bad[e] != 0.f) dst[lane * W + e] = __float2half_rn(bad[e]);
 }
 
-template <int HD>
+template <int HD, int NT>
 struct FewCfg {
     static constexpr int PAGE = 64 * HD;                 // bytes of a page's K and V of a head
-    static constexpr int RING = HD == 128 ? 3 : 6;       // pages in flight of a warp
+    // Pages in flight of a warp: no more than the rate needs.  With 192 KB of an SM in flight 64 single tokens on 4096
+    // took 185 us, with 128 KB 182; the SMs' shares of the rate are further apart.
+    static constexpr int RING = (HD == 128 ? 1 : 2) * (NT == 1 ? 2 : 3);
     static constexpr size_t smem(int B) {
         return 1024 + (size_t)kFewWarps * RING * PAGE + kFewWarps * RING * 8 + (size_t)(B + 1) * 8 + (size_t)B * sizeof(FewSeq) + 16;
     }
 };
-static_assert(FewCfg<128>::smem(kBoundMaxSeqs) <= 232448 && FewCfg<64>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a CTA");
+static_assert(FewCfg<64, 2>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a CTA");
 
 // Pages before each sequence, by every CTA for itself from the lengths in device
 // memory (so a captured call serves other lengths); CTA 0 leaves them for the
@@ -286,15 +295,34 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     __syncthreads();
     return total;
 }
-// Pages of a range.
-__device__ __forceinline__ long long few_per(const FewArgs& a, long long total) {
-    return max((long long)kFewMinPages, (total + a.ranges - 1) / a.ranges);
-}
+// How the pages are cut: the first wave's ranges of per0 pages, then those of the second wave of per1.
+struct FewCut {
+    long long total, from1;
+    int warps, per0, per1;  // warps of a wave
+    __device__ __forceinline__ FewCut(const FewArgs& a, long long n) : total(n), warps(a.ctas * kFewWarps) {
+        // Few pages for each warp: their pieces would cost more than the wave gains (in us, with one wave and with two:
+        // one token on 65,536, 18 pages a warp, 57 and 91; 64 tokens on up to 8192, 33 pages, 100 and 93).
+        const bool both = a.waves > 1 && n >= 24LL * a.tpt * a.G / 8 * warps;
+        const long long given = both ? n - n / 5 : n;
+        per0 = (int)max((long long)kFewMinPages, (given + warps - 1) / warps);
+        from1 = min(n, (long long)warps * per0);
+        per1 = (int)max((long long)kFewMinPages, (n - from1 + warps - 1) / warps);
+    }
+    __device__ __forceinline__ long long begin(int r) const {
+        return r < warps ? (long long)r * per0 : from1 + (long long)(r - warps) * per1;
+    }
+    __device__ __forceinline__ long long end(int r) const {
+        return r < warps ? min(begin(r) + per0, from1) : min(begin(r) + per1, total);
+    }
+    __device__ __forceinline__ int of(long long u) const {
+        return u < from1 ? (int)(u / per0) : warps + (int)((u - from1) / per1);
+    }
+};
 
 template <int HD, int NT, bool ACC>
-__global__ void __launch_bounds__(32 * kFewWarps, 1)
+__global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
     few_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
-    using C = FewCfg<HD>;
+    using C = FewCfg<HD, NT>;
     constexpr int KS = HD / 16, NH = HD / 64, RING = C::RING;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
@@ -311,10 +339,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const long long total = few_plan(a, pre, seqs, ACC);  // ends with a CTA-wide barrier
-    const long long per = few_per(a, total);
+    const FewCut cut(a, total);
     // neighbouring ranges on different SMs: a call of few ranges has them to itself
-    const int range = warp * gridDim.x + blockIdx.x;
-    const long long u0 = min(total, range * per), u1 = min(total, u0 + per);
+    const int wave = blockIdx.x / a.ctas, range = (wave * kFewWarps + warp) * a.ctas + (blockIdx.x - wave * a.ctas);
+    const long long u0 = cut.begin(range), u1 = cut.end(range);
     if (u0 >= u1) return;
 
     // ---- loads: as many pages ahead as the ring holds
@@ -591,22 +619,23 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1)
 }
 
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in their
-// order: a warp for each row and head of up to 8 pieces, else the CTA's four warps
-// take every fourth piece and are joined in their order.  ROWS: rows of a CTA, 1
-// where there are few (148 pieces of each of 32 rows: 115 us a call with four rows
-// of a CTA one after the other).  Where the row belongs is looked up while the
-// kernel before still runs.
-template <int HD, int ROWS>
-__global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
+// order: a warp for each row and head of up to 8 pieces, else the CTA's WARPS warps
+// take pieces in turn and are joined in their order.  ROWS: rows of a CTA, 1 where
+// there are few (148 pieces of each of 32 rows: 115 us a call with four rows of a
+// CTA one after the other, 57 with one).  Where the row belongs is looked up while
+// the kernel before still runs.
+template <int HD, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
     constexpr int W = HD / 32;
-    __shared__ float sm[4], sl[4], so[4][HD];
-    __shared__ int sbad[4];
+    static_assert(ROWS == 1 || ROWS == WARPS, "rows of a CTA");
+    __shared__ float sm[WARPS], sl[WARPS], so[WARPS][HD];
+    __shared__ int sbad[WARPS];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long rows = (long long)a.T * a.Hq, first = (long long)ROWS * blockIdx.x;
     struct Row {
-        int n, b, p, kvh, row, np, tile;
-        long long r0, u0;
+        int n, b, p, kvh, row, np, tile, r0;
+        long long u0;
         __half* dst;
         size_t at;
     };
@@ -637,12 +666,12 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
     };
     Row mine = find(first + (ROWS == 1 ? 0 : warp));
     pdl_wait();
-    const long long total = a.pre[a.B], per = few_per(a, total);
+    const FewCut cut(a, a.pre[a.B]);
     auto count = [&](Row& x) {  // its pieces
         if (x.np <= 0) return;
         x.u0 = a.pre[x.b] + ((long long)x.tile * a.Hkv + x.kvh) * a.np[x.b];
-        x.r0 = x.u0 / per;
-        x.n = (int)((x.u0 + x.np - 1) / per - x.r0) + 1;
+        x.r0 = cut.of(x.u0);
+        x.n = cut.of(x.u0 + x.np - 1) - x.r0 + 1;
     };
     count(mine);
     float m, l, o[W];
@@ -660,8 +689,8 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
 #pragma unroll
             for (int u = 0; u < P; ++u) {
                 const bool real = k + u * step < x.n;
-                const long long range = x.r0 + k + u * step;
-                const size_t at = real ? (size_t)(2 * range + (x.u0 > range * per ? 1 : 0)) * tile_rows + x.row : 0;
+                const int range = x.r0 + k + u * step;
+                const size_t at = real ? (size_t)(2 * range + (x.u0 > cut.begin(range) ? 1 : 0)) * tile_rows + x.row : 0;
                 ml[u] = real ? a.pml[at] : make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[u][e] = real ? a.po[at * HD + lane * W + e] : 0.f;
@@ -711,7 +740,7 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
             count(x);
         }
         if (x.n <= 8) continue;  // (the same for all)
-        join(x, warp, 4);
+        join(x, warp, WARPS);
         if (lane == 0) {
             sm[warp] = m;
             sl[warp] = l;
@@ -722,14 +751,14 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
         __syncthreads();
         if (warp == 0) {
             float top = sm[0];
-            for (int q = 1; q < 4; ++q) top = few_max(top, sm[q]);
+            for (int q = 1; q < WARPS; ++q) top = few_max(top, sm[q]);
             const float sub = top == -INFINITY ? 0.f : top;
             m = top;
             l = 0.f;
             bad = false;
 #pragma unroll
             for (int e = 0; e < W; ++e) o[e] = 0.f;
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < WARPS; ++q) {
                 const float w = exp2f(sm[q] - sub);
                 bad |= sbad[q] != 0;
                 if (w == 0.f) continue;
@@ -811,17 +840,23 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
 // ------------------------------------------------------------------ host side
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// CTAs of a wave: no more than there can be ranges.
+static int few_ctas(int sms, int NT, int T, int Hkv, int max_blocks) {
+    const long long ranges = ((long long)T * Hkv * max_blocks + kFewMinPages - 1) / kFewMinPages;
+    return (int)std::min<long long>(few_resident(NT) * std::min(sms, kFewMaxSms), ranges);
+}
 // Sizes that do not fall where B, T or max_blocks grows.
 struct FewSpace {
-    int ctas, rows;
     size_t pre, np, chunks, pml, po, ml, scores, bytes;  // offsets, and all
 };
 static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks, bool acc) {
     FewSpace s = {};
-    const long long rows = (long long)T * (Hq / Hkv);
-    s.rows = (int)std::min<long long>(kFewMaxRows, (rows + 7) / 8 * 8);
-    s.ctas = (int)std::min<long long>(kFewMaxCtas, ((long long)T * Hkv * max_blocks + kFewMinPages - 1) / kFewMinPages);
-    const size_t pieces = (size_t)2 * kFewWarps * s.ctas * s.rows;
+    // rows of all pieces: two for each range, of the kernel that has most
+    const long long rows = std::min<long long>(kFewMaxRows, ((long long)T * (Hq / Hkv) + 7) / 8 * 8);
+    long long most = 0;
+    for (int nt = 1; nt <= 4; ++nt)
+        most = std::max(most, 2LL * few_waves(nt) * few_ctas(kFewMaxSms, nt, T, Hkv, max_blocks) * kFewWarps * std::min<long long>(8 * nt, rows));
+    const size_t pieces = (size_t)most;
     size_t at = 0;
     auto room = [&](size_t n) {
         const size_t here = at;
@@ -860,9 +895,9 @@ static int few_sms(int* out) {  // SMs of the current device; sets the kernels' 
         for (int nt = 1; nt <= 4; ++nt)
             for (int acc = 0; acc < 2; ++acc) {
                 SD_CUDA(cudaFuncSetAttribute(few_fn(128, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)FewCfg<128>::smem(kBoundMaxSeqs)));
+                                             (int)FewCfg<128, 2>::smem(kBoundMaxSeqs)));
                 SD_CUDA(cudaFuncSetAttribute(few_fn(64, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)FewCfg<64>::smem(kBoundMaxSeqs)));
+                                             (int)FewCfg<64, 2>::smem(kBoundMaxSeqs)));
             }
         SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         facts[dev].store(n);
@@ -891,13 +926,14 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     const long long want = std::min<long long>(kFewMaxRows, (((long long)a.T + a.B - 1) / a.B) * a.G);
     const int NT = (int)((want + 7) / 8);
     a.tpt = 8 * NT / a.G;
-    const int ctas = std::min(sp.ctas, sms);
-    a.ranges = ctas * kFewWarps;
+    a.ctas = few_ctas(sms, NT, a.T, a.Hkv, a.max_blocks);
+    a.waves = few_waves(NT);
     CUtensorMap map;
     if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 2))) return rc;
-    const size_t smem = HD == 128 ? FewCfg<128>::smem(a.B) : FewCfg<64>::smem(a.B);
+    const size_t smem = HD == 128 ? (NT == 1 ? FewCfg<128, 1>::smem(a.B) : FewCfg<128, 2>::smem(a.B))
+                                  : (NT == 1 ? FewCfg<64, 1>::smem(a.B) : FewCfg<64, 2>::smem(a.B));
     void* args[] = {&map, &a};
-    SD_CUDA(cudaLaunchKernel(few_fn(HD, NT, acc), dim3((unsigned)ctas), dim3(32 * kFewWarps), args, smem, s));
+    SD_CUDA(cudaLaunchKernel(few_fn(HD, NT, acc), dim3((unsigned)(a.ctas * a.waves)), dim3(32 * kFewWarps), args, smem, s));
     cudaLaunchConfig_t cfg = {};
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -906,11 +942,12 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     const long long rows = (long long)a.T * a.Hq;
-    const bool single = rows <= 2048;
-    cfg.gridDim = dim3((unsigned)(single ? rows : (rows + 3) / 4));
-    cfg.blockDim = dim3(128);
-    const auto merge = HD == 128 ? (single ? few_merge_kernel<128, 1> : few_merge_kernel<128, 4>)
-                                 : (single ? few_merge_kernel<64, 1> : few_merge_kernel<64, 4>);
+    const int kind = rows <= 256 ? 0 : rows <= 2048 ? 1 : 2;
+    cfg.gridDim = dim3((unsigned)(kind < 2 ? rows : (rows + 3) / 4));
+    cfg.blockDim = dim3(kind == 0 ? 512 : 128);
+    const auto merge =
+        HD == 128 ? (kind == 0 ? few_merge_kernel<128, 1, 16> : kind == 1 ? few_merge_kernel<128, 1, 4> : few_merge_kernel<128, 4, 4>)
+                  : (kind == 0 ? few_merge_kernel<64, 1, 16> : kind == 1 ? few_merge_kernel<64, 1, 4> : few_merge_kernel<64, 4, 4>);
     SD_CUDA(cudaLaunchKernelEx(&cfg, merge, a, 8 * NT));
     if (acc) {
         const long long chunks = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
