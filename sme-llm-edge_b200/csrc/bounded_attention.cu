@@ -227,6 +227,7 @@ static_assert(FewCfg<64, 2>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a 
 // Pages before each sequence, by every CTA for itself from the lengths in device
 // memory (so a captured call serves other lengths); CTA 0 leaves them for the
 // kernels that follow.
+template <bool LEAVE = true>
 __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, FewSeq* seqs, bool acc) {
     __shared__ long long wsum[kFewWarps];
     __shared__ int csum[kFewWarps];
@@ -275,7 +276,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     for (int b = b0; b < b1; ++b) {
         const long long all = pre[b];
         pre[b] = before;
-        if (blockIdx.x == 0) {
+        if (LEAVE && blockIdx.x == 0) {
             a.pre[b] = before;
             a.np[b] = seqs[b].np;
             if (acc) {
@@ -287,7 +288,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     }
     if (tid == 0) {
         pre[a.B] = total;
-        if (blockIdx.x == 0) {
+        if (LEAVE && blockIdx.x == 0) {
             a.pre[a.B] = total;
             if (acc) a.chunks[a.B] = ctotal;
         }
@@ -837,6 +838,183 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
     }
 }
 
+// ------------------------------------------------------------------ many rows
+//
+// weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
+// of 2^(x - m) / l, where the rows' (m, 1 / l) are known (the tensor-core kernel's):
+// the scores are computed again rather than kept, a read of K (256 bytes of a slot
+// and head of 128) against one write and one read of 4 bytes for each row.  A warp
+// streams K pages of its range past 64 rows at a time,
+//   S^T [16 keys][64 rows] = K Q^T in mma.sync, whose lanes hold a slot's scores of
+// 16 rows: the sum over rows is theirs and two shuffles'.
+constexpr int kWeighRows = 64, kWeighRing = 8192;  // bytes: 2 or 4 pages of a warp, twice
+
+template <int HD>
+struct WeighCfg {
+    static constexpr int PAGE = 32 * HD;  // bytes of a page's K of a head
+    static constexpr int RING = 4 * kWeighRing / PAGE;
+    static constexpr size_t smem(int B) {
+        return 1024 + (size_t)kFewWarps * RING * (PAGE + 8) + (size_t)(B + 1) * 8 + (size_t)B * sizeof(FewSeq) + 16;
+    }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(32 * kFewWarps, 2)
+    weigh_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ FewArgs a) {
+    using C = WeighCfg<HD>;
+    constexpr int KS = HD / 16, RING = C::RING, NT = kWeighRows / 8;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + kFewWarps * RING * C::PAGE);
+    long long* pre = reinterpret_cast<long long*>(bars + kFewWarps * RING);
+    FewSeq* seqs = reinterpret_cast<FewSeq*>(pre + a.B + 1);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring = s_addr(base + warp * RING * C::PAGE), bar = s_addr(bars + warp * RING);
+    if (lane == 0) {
+        for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const long long total = few_plan<false>(a, pre, seqs, false);  // ends with a CTA-wide barrier
+    const FewCut cut(a, total);
+    const int range = warp * a.ctas + blockIdx.x;
+    const long long u0 = cut.begin(range), u1 = cut.end(range);
+    if (u0 >= u1) return;
+    auto groups_of = [&](const FewWalk& w) { return (w.t.tokens * a.G + kWeighRows - 1) / kWeighRows; };
+
+    // ---- loads: a segment's pages once for each 64 of its rows
+    FewWalk ld = {};
+    ld.u = u0;
+    ld.hi = u1;
+    int asked = 0, tb = 0, ent = 0, ent_next = 0, v = 0, left = 0;  // left: groups of the segment still to load
+    bool more = true;
+    auto entry = [&](int i) -> int {
+        if (i >= ld.ve) return 0;
+        const int x = a.tables[(size_t)ld.b * a.max_blocks + i];
+        return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
+    };
+    auto load = [&]() {
+        while (more && v >= ld.ve) {
+            if (--left <= 0) {
+                more = few_next(a, pre, seqs, ld);
+                if (!more) return;
+                left = ld.v < ld.ve ? groups_of(ld) : 0;
+            }
+            v = tb = left > 0 ? ld.v : ld.ve;
+            ent = entry(tb + lane);
+            ent_next = entry(tb + 32 + lane);
+        }
+        if (!more) return;
+        if (v - tb >= 32) {
+            tb += 32;
+            ent = ent_next;
+            ent_next = entry(tb + 32 + lane);
+        }
+        const int page = __shfl_sync(0xffffffffu, ent, v - tb);
+        if (lane == 0) {
+            const uint32_t b = bar + 8 * (asked % RING);
+            mbar_expect_tx(b, C::PAGE);
+            tma_load_5d(ring + (asked % RING) * C::PAGE, &kmap, 0, ld.kvh * 16, 0, 0, page, b);
+        }
+        ++asked;
+        ++v;
+    };
+    for (int i = 0; i < RING; ++i) load();
+    pdl_wait();  // m and l of the rows
+
+    const uint32_t k_row = (uint32_t)(lane & 15), k_chunk = (uint32_t)(lane >> 4);
+    FewWalk w = {};
+    w.u = u0;
+    w.hi = u1;
+    int done = 0;
+    bool ok = true;
+    while (ok && few_next(a, pre, seqs, w)) {
+        if (w.v >= w.ve) continue;
+        const FewTile& t = w.t;
+        const int rows = t.tokens * a.G, groups = groups_of(w);
+        float* dst = a.weights + ((size_t)w.b * a.Hkv + w.kvh) * a.ldw;
+        for (int k0 = 0; ok && k0 < groups; ++k0) {
+            const int row0 = k0 * kWeighRows;
+            uint32_t qf[NT][KS][2];
+            float m[NT][2], inv[NT][2];
+            int slot_of[NT][2];  // -1: no row
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int row = row0 + 8 * n + g;
+                const bool real = row < rows;
+                const int tok = real ? row / a.G : 0;
+                const __half* src = a.q + (size_t)(t.row + tok) * a.ldq + (size_t)(w.kvh * a.G + (real ? row - tok * a.G : 0)) * HD + 2 * t4;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    qf[n][k][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+                    qf[n][k][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = row0 + 8 * n + 2 * t4 + e, ct = c / a.G;
+                    slot_of[n][e] = c < rows ? t.p0 + ct : -1;
+                    const float2 y = c < rows ? __ldcg(a.ml + (size_t)(t.row + ct) * a.Hq + w.kvh * a.G + c - ct * a.G) : make_float2(0.f, 0.f);
+                    m[n][e] = y.x == -INFINITY ? 0.f : y.x;
+                    inv[n][e] = y.y;
+                }
+            }
+            const int first = t.p0 + row0 / a.G, last = t.p0 + (min(rows, row0 + kWeighRows) - 1) / a.G;  // slots of the group's rows
+            for (int i = w.v; i < w.ve; ++i) {
+                const int at = done % RING;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
+                const uint32_t sk = ring + at * C::PAGE;
+                const int s0 = 16 * i;
+                // lanes t4 = 0, 1 keep slots g, g + 8 of the page
+                const int mine = s0 + g + 8 * t4;
+                const bool keeps = t4 < 2 && mine <= last && mine < a.slots_max;
+                const float was = keeps ? dst[mine] : 0.f;
+                float s[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t x[4];
+                    few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) few_mma(s[n], x, qf[n][k][0], qf[n][k][1]);
+                }
+                ++done;
+                __syncwarp();  // the page has been read
+                load();
+                float sum[2] = {0.f, 0.f};
+                if (s0 + 15 <= first) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sum[e >> 1] = fmaf(few_exp2(s[n][e] * a.scale_log2 - m[n][e & 1]), inv[n][e & 1], sum[e >> 1]);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (s0 + g + 8 * (e >> 1) <= slot_of[n][e & 1])
+                                sum[e >> 1] = fmaf(few_exp2(s[n][e] * a.scale_log2 - m[n][e & 1]), inv[n][e & 1], sum[e >> 1]);
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], d);
+                    sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], d);
+                }
+                if (keeps) dst[mine] = was + (t4 ? sum[1] : sum[0]);
+            }
+        }
+    }
+    if (!ok) {
+        if (lane == 0) record_timeout(a.status, 41);
+        // the copies in flight land before the CTA leaves
+        for (int c = done; c < asked; ++c) (void)mbar_wait(bar + 8 * (c % RING), (uint32_t)(c / RING) & 1u);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -899,10 +1077,46 @@ static int few_sms(int* out) {  // SMs of the current device; sets the kernels' 
                 SD_CUDA(cudaFuncSetAttribute(few_fn(64, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)FewCfg<64, 2>::smem(kBoundMaxSeqs)));
             }
+        SD_CUDA(cudaFuncSetAttribute(weigh_rows_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)WeighCfg<128>::smem(kBoundMaxSeqs)));
+        SD_CUDA(cudaFuncSetAttribute(weigh_rows_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)WeighCfg<64>::smem(kBoundMaxSeqs)));
         SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         facts[dev].store(n);
     }
     *out = n;
+    return SPECDEC_OK;
+}
+
+// Rows past kFewMaxRows a sequence with weights: the attention on the tensor cores, which leaves (m, 1 / l), then the weights.
+static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
+    int sms = 0;
+    int rc = few_sms(&sms);
+    if (rc) return rc;
+    a.ml = static_cast<float2*>(ws);
+    a.status = device_status_ptr();
+    a.slots_max = a.max_blocks * 16;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)HD));
+    rc = rows_packed_launch(a.q, a.ldq, a.kv, a.num_blocks, a.Hkv, HD, a.tables, a.max_blocks, a.ctx_len, a.row_off, a.B,
+                            a.T, a.Hq, a.window, 0, a.ml, a.out, a.ldo,
+                            static_cast<char*>(ws) + up256((size_t)a.T * a.Hq * sizeof(float2)), s);
+    if (rc) return rc;
+    a.tpt = 1 << 24;  // a sequence is one tile
+    a.waves = 1;
+    a.ctas = (int)std::min<long long>(2 * std::min(sms, kFewMaxSms), ((long long)a.B * a.Hkv * a.max_blocks + kFewMinPages - 1) / kFewMinPages);
+    CUtensorMap map;
+    if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 1))) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.ctas);
+    cfg.blockDim = dim3(32 * kFewWarps);
+    cfg.dynamicSmemBytes = HD == 128 ? WeighCfg<128>::smem(a.B) : WeighCfg<64>::smem(a.B);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    SD_CUDA(cudaLaunchKernelEx(&cfg, HD == 128 ? weigh_rows_kernel<128> : weigh_rows_kernel<64>, map, a));
     return SPECDEC_OK;
 }
 
@@ -994,6 +1208,12 @@ static int check_bound_memory(const char* who, const void* q, const void* kv, co
 
 using namespace specdec;
 
+// Calls of few rows keep their scores; the room for that ends where the others begin.
+static size_t accumulate_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks) {
+    const int most = (int)std::min<long long>(T, (long long)B * (kFewMaxRows / std::max(1, std::min(kFewMaxRows, Hq / Hkv))));
+    return std::max(few_space(B, most, Hq, Hkv, HD, max_blocks, true).bytes,
+                    up256((size_t)T * Hq * sizeof(float2)) + rows_packed_workspace(B, T, Hq, HD, max_blocks));
+}
 static bool few_rows(int B, int T, int G) { return G <= kFewMaxRows && T <= (long long)B * (kFewMaxRows / G); }
 static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
                         const int32_t* tables, int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B,
@@ -1053,13 +1273,13 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
     }
     return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
                               num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads,
-                              window, sinks, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
+                              window, sinks, nullptr, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads,
                                                                int head_dim, int max_blocks) {
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_blocks <= 0) return 0;
-    return few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, true).bytes;
+    return accumulate_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks);
 }
 
 extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1088,5 +1308,6 @@ extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const ui
                          out, ldo);
     f.weights = weights;
     f.ldw = ldw;
-    return launch_few(f, head_dim, true, workspace, as_stream(stream));
+    return few_rows(B, T, n_q_heads / n_kv_heads) ? launch_few(f, head_dim, true, workspace, as_stream(stream))
+                                                  : launch_many(f, head_dim, workspace, as_stream(stream));
 }

@@ -88,6 +88,7 @@ constexpr int kRowsTmemCols = 512;
 constexpr float kHalfMax = 65504.0f, kHalfOver = 65520.0f;  // fp16's largest; from here on it rounds to infinity
 constexpr float kRowsLag = 8.0f;     // what a row's maximum may grow by before m follows
 constexpr float kRowsLift = 7.0f;    // P is 2^7 times the weight: at most 2^(8 + 7) < 65504
+constexpr float kRowsUnlift = 128.0f;
 // From this maximum on (in units of x) score * scale - m is not one fused
 // operation: that leaves the rounding of m = score * scale in x, 32 at 2^29, and
 // P would be 2^(x + 7).  Product and difference apart, the largest gives 0.  Below
@@ -127,6 +128,7 @@ struct RowsArgs {
     int n_groups, B, T, R;
     int tq_small;  // tokens of the small query box
     int window, sinks;  // kModeWindow
+    float2* ml;         // kModeWindow, may be null: [T][Hq] each row's m and 2^7 / l (l is that of the lifted weights)
     RowsDiv by_item, by_hkv;  // 2 * tpt tokens of an item; KV heads
     int slots_max;  // max_blocks * 16
     __half* out;
@@ -1170,6 +1172,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                         l = -l;
                 }
                 if (it.prow >= 0 && real) a.pml[prow] = make_float2(m, l);
+                if constexpr (WIN)
+                    if (a.ml && it.prow < 0 && real) a.ml[(size_t)tok * a.Hq + head] = make_float2(m, inv * kRowsUnlift);
             }
             tc_fence_before();  // O was read before the slot's next P is announced
             done_item(k);
@@ -1372,6 +1376,7 @@ __device__ __noinline__ void rows_merge_nonfinite(const RowsArgs& a, const RowsM
         l += exp2f(ml.x - sub) * fabsf(ml.y);
     }
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    if (a.ml && (threadIdx.x & 7) == 0) a.ml[(size_t)tok * a.Hq + head] = make_float2(top, inv * kRowsUnlift);
     for (int e = threadIdx.x & 7; e < HD; e += 8) {
         float sum = 0.f, bad = 0.f;
         for (int p = 0; p < n; ++p) {
@@ -1472,6 +1477,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
         return;
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
+    if (a.ml && lane == 0) a.ml[(size_t)tok * a.Hq + head] = make_float2(M, inv * kRowsUnlift);
     __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + 4 * lane;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -1484,6 +1490,7 @@ __device__ __forceinline__ void rows_merge_row(const RowsArgs& a, int tok, int h
 
 template <int HD>
 __global__ void __launch_bounds__(256) rows_merge_kernel(const __grid_constant__ RowsArgs a) {
+    if (a.ml) pdl_trigger();  // what weighs the slots may load its first keys
     pdl_wait();
     if (*a.any_parts == 0) return;
     const int rows = a.T * a.Hq;
@@ -1653,7 +1660,7 @@ size_t rows_packed_workspace(int B, int T, int Hq, int HD, int max_blocks) {
 }
 int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_blocks, int Hkv, int HD, const int32_t* tables,
                        int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B, int T, int Hq, int window,
-                       int sinks, __half* out, int ldo, void* ws, cudaStream_t s) {
+                       int sinks, float2* ml, __half* out, int ldo, void* ws, cudaStream_t s) {
     size_t prows = prompt_partial_rows(T, max_blocks);
     if ((long long)T * Hq >= 1 << 30) prows = 0;  // the merge counts rows and heads in 32 bits
     RowsArgs a = {};
@@ -1670,6 +1677,7 @@ int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_block
     a.tq_small = 1;
     a.window = window;
     a.sinks = sinks;
+    a.ml = ml;
     a.out = out;
     a.ldo = ldo;
     const int tpt2 = 2 * (128 / (Hq / Hkv));
@@ -1706,7 +1714,7 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
         return rc;
     return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
                               num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads, 0,
-                              0, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
+                              0, nullptr, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads,
