@@ -74,15 +74,28 @@ __device__ __forceinline__ void norm_load8(const float* src, float (&x)[8]) {
     x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
 }
 
-template <int HD, typename In>
+// U: head groups that a warp has in flight at a time (their loads go out together, before the row's place is looked up).
+template <int HD, typename In, int U>
 __global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
-    constexpr int LPH = HD / 8, HS = 32 / LPH;  // lanes of a head, heads of a warp at a time
+    constexpr int LPH = HD / 8, HS = 32 / LPH;  // lanes of a head, heads of a group
     const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH, d0 = 8 * l;
     const long long w = (long long)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
-    const int r = (int)(w / a.parts), part = (int)(w % a.parts);
+    const int r = a.parts == 1 ? (int)w : (int)(w / a.parts), part = (int)(w - (long long)r * a.parts);
     if (r >= a.T) return;
     const int heads = a.Hq + 2 * a.Hkv;
-    const In* row = static_cast<const In*>(a.qkv) + (size_t)r * a.ld;
+    const In* row = static_cast<const In*>(a.qkv) + (size_t)r * a.ld + d0;
+    float x[U][8];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * a.parts * HS + sub;
+            if (h < heads) norm_load(row + (size_t)h * HD, x[u]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+        }
+    };
+    fetch(part * HS);
     const int b = norm_sequence(a, r);
     if (b < 0) return;
     const int slot = max(0, min(a.ctx_len[b], 1 << 30)) + (r - max(0, a.row_off[b]));
@@ -98,44 +111,52 @@ __global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rope_kernel(const __g
         const size_t at = (size_t)p * a.half + (upper ? d0 - a.half : d0);
         norm_load8(a.cos_t + at, c);
         norm_load8(a.sin_t + at, s);
+        if (!upper)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = -s[e];
     }
-    float qw[8], kw[8];
-    if (a.qw) norm_load8(a.qw + d0, qw);
-    if (a.kw) norm_load8(a.kw + d0, kw);
-    for (int h0 = part * HS; h0 < heads; h0 += a.parts * HS) {
-        const int h = h0 + sub;
-        const bool real = h < heads, is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-        float x[8] = {};
-        if (real) norm_load(row + (size_t)h * HD + d0, x);
-        float sum = 0.f;
+    const int other = turns ? sub * LPH + (upper ? l - away : l + away) : lane;
+    __half* kv = a.kv + ((size_t)max(page, 0) * 2 * a.Hkv * 16 + (slot & 15)) * HD + d0;
+    for (int h0 = part * HS; h0 < heads; h0 += U * a.parts * HS) {
+        if (h0 > part * HS) fetch(h0);
+        float sum[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+        for (int u = 0; u < U; ++u) {
+            sum[u] = 0.f;
 #pragma unroll
-        for (int o = LPH / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if ((is_q && a.qw) || (is_k && a.kw)) {
-            const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (is_q ? qw[e] : kw[e]);
+            for (int e = 0; e < 8; ++e) sum[u] = fmaf(x[u][e], x[u][e], sum[u]);
         }
-        const int other = sub * LPH + (upper ? l - away : l + away);
-        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], turns ? other : lane);
-        if (turns && (is_q || is_k)) {
+        for (int o = LPH / 2; o; o >>= 1)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = upper ? x[e] * c[e] + y[e] * s[e] : x[e] * c[e] - y[e] * s[e];
-        }
-        uint4 out;
-        __half2* o2 = reinterpret_cast<__half2*>(&out);
+            for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o2[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-        if (!real) continue;
-        if (is_q) {
-            *reinterpret_cast<uint4*>(a.q_out + (size_t)r * a.ldq + (size_t)h * HD + d0) = out;
-        } else if (paged) {
-            const int kvh = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
-            __half* dst = a.kv + ((((size_t)page * 2 + (is_k ? 0 : 1)) * a.Hkv + kvh) * 16 + (slot & 15)) * HD + d0;
-            *reinterpret_cast<uint4*>(dst) = out;
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * a.parts * HS + sub;
+            const bool real = h < heads, is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
+            const float* norm = is_q ? a.qw : is_k ? a.kw : nullptr;
+            if (norm) {
+                float g[8];
+                norm_load8(norm + d0, g);
+                const float inv = rsqrtf(sum[u] * (1.0f / HD) + a.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * inv * g[e];
+            }
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[u][e], other);
+            if (turns && (is_q || is_k)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * c[e] + y[e] * s[e];
+            }
+            uint4 out;
+            __half2* o2 = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o2[e] = __floats2half2_rn(x[u][2 * e], x[u][2 * e + 1]);
+            if (real && is_q)
+                *reinterpret_cast<uint4*>(a.q_out + (size_t)r * a.ldq + (size_t)h * HD + d0) = out;
+            else if (real && paged)  // [K|V][kv head][16][HD]: K's heads, then V's
+                *reinterpret_cast<uint4*>(kv + (size_t)(h - a.Hq) * 16 * HD) = out;
         }
     }
 }
@@ -216,17 +237,26 @@ extern "C" int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, 
     a.T = T;
     a.q_out = reinterpret_cast<__half*>(q_out);
     a.ldq = ldq;
-    a.parts = 1;
+    // Few rows: a warp for each head group, so that a row's chain of look-ups is all there is; many: PARTS_NOTE
+    const int groups = ((n_q_heads + 2 * n_kv_heads) * head_dim + 255) / 256;
+    const bool many = (long long)T * groups > 148LL * 64 * 4;
+    a.parts = many ? (groups + 7) / 8 : groups;
     const long long warps = (long long)T * a.parts;
-    const unsigned grid = (unsigned)((warps + kNormWarps - 1) / kNormWarps);
+    const dim3 grid((unsigned)((warps + kNormWarps - 1) / kNormWarps)), block(32 * kNormWarps);
     cudaStream_t s = as_stream(stream);
+#define NORM_LAUNCH(hd, type)                                          \
+    do {                                                               \
+        if (many) qk_norm_rope_kernel<hd, type, 4><<<grid, block, 0, s>>>(a); \
+        else qk_norm_rope_kernel<hd, type, 1><<<grid, block, 0, s>>>(a);      \
+    } while (0)
     if (head_dim == 128) {
-        if (qkv_f16) qk_norm_rope_kernel<128, __half><<<grid, 32 * kNormWarps, 0, s>>>(a);
-        else qk_norm_rope_kernel<128, float><<<grid, 32 * kNormWarps, 0, s>>>(a);
+        if (qkv_f16) NORM_LAUNCH(128, __half);
+        else NORM_LAUNCH(128, float);
     } else {
-        if (qkv_f16) qk_norm_rope_kernel<64, __half><<<grid, 32 * kNormWarps, 0, s>>>(a);
-        else qk_norm_rope_kernel<64, float><<<grid, 32 * kNormWarps, 0, s>>>(a);
+        if (qkv_f16) NORM_LAUNCH(64, __half);
+        else NORM_LAUNCH(64, float);
     }
+#undef NORM_LAUNCH
     SD_LAUNCH_CHECK("qk_norm_rope_kernel");
     return SPECDEC_OK;
 }
