@@ -8,10 +8,9 @@
 // A row's values are read once and written once; HBM bounds many rows, the chain
 // bounds -> sequence -> page number -> store a few.
 //
-// head_dim / 8 lanes hold a head, 8 values each, so that an fp16 head is loaded
-// and stored in 16-byte pieces, and 2 (head_dim 128) or 4 heads are in a warp.
-// The sum of squares and the pair's other half come by shuffles (r / 16 lanes
-// away).
+// head_dim / 8 lanes hold a head, and 2 (head_dim 128) or 4 heads are in a warp.  A
+// lane holds four values and the other halves of their pairs (8 of the rest where
+// a head turns in part): only the sum of squares crosses lanes.
 #include "common.cuh"
 #include "internal.h"
 #include "ptx.cuh"
@@ -19,7 +18,7 @@
 namespace specdec {
 
 constexpr int kNormMaxSeqs = 1024;
-constexpr int kNormWarps = 8;
+constexpr int kNormWarps = 4;
 
 struct NormArgs {
     const void* qkv;
@@ -52,48 +51,61 @@ __device__ __forceinline__ int norm_sequence(const NormArgs& a, int r) {
     return b < a.B && a.row_off[b] <= r ? b : -1;
 }
 
+// Four values at lo and four at hi, as they lie in memory.
 template <typename In>
-__device__ __forceinline__ void norm_load(const In* src, float (&x)[8]) {
-    if constexpr (sizeof(In) == 4) {
-        const float4 u = __ldcs(reinterpret_cast<const float4*>(src)), v = __ldcs(reinterpret_cast<const float4*>(src) + 1);
+struct NormRaw;
+template <>
+struct NormRaw<float> {
+    float4 u, v;
+    __device__ __forceinline__ void load(const float* src, int lo, int hi) {
+        u = __ldcs(reinterpret_cast<const float4*>(src + lo));
+        v = __ldcs(reinterpret_cast<const float4*>(src + hi));
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
         x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
         x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-    } else {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(src));
-        const __half2* h = reinterpret_cast<const __half2*>(&u);
+    }
+};
+template <>
+struct NormRaw<__half> {
+    uint2 u, v;
+    __device__ __forceinline__ void load(const __half* src, int lo, int hi) {
+        u = __ldcs(reinterpret_cast<const uint2*>(src + lo));
+        v = __ldcs(reinterpret_cast<const uint2*>(src + hi));
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t h[4] = {u.x, u.y, v.x, v.y};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float2 f = __half22float2(h[e]);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
             x[2 * e] = f.x, x[2 * e + 1] = f.y;
         }
     }
-}
-__device__ __forceinline__ void norm_load8(const float* src, float (&x)[8]) {
-    const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 4);
+};
+__device__ __forceinline__ void norm_load4(const float* src, float* x) {
+    const float4 u = *reinterpret_cast<const float4*>(src);
     x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
 }
 
 // U: head groups that a warp has in flight at a time (their loads go out together, before the row's place is looked up).
-template <int HD, typename In, int U>
-__global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
+template <int HD, typename In, int U, int MINB>
+__global__ void __launch_bounds__(32 * kNormWarps, MINB) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
     constexpr int LPH = HD / 8, HS = 32 / LPH;  // lanes of a head, heads of a group
-    const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH, d0 = 8 * l;
+    const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH;
+    // this lane's values: d .. d + 3 and their pairs, or 8 of those that do not turn
+    const int pairs = a.half / 4;  // lanes that turn
+    const bool turns = l < pairs;
+    const int lo = turns ? 4 * l : 2 * a.half + 8 * (l - pairs), hi = turns ? lo + a.half : lo + 4;
     const long long w = (long long)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
     const int r = a.parts == 1 ? (int)w : (int)(w / a.parts), part = (int)(w - (long long)r * a.parts);
     if (r >= a.T) return;
     const int heads = a.Hq + 2 * a.Hkv;
-    const In* row = static_cast<const In*>(a.qkv) + (size_t)r * a.ld + d0;
-    float x[U][8];
+    const In* row = static_cast<const In*>(a.qkv) + (size_t)r * a.ld;
+    NormRaw<In> raw[U];
     auto fetch = [&](int h0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + u * a.parts * HS + sub;
-            if (h < heads) norm_load(row + (size_t)h * HD, x[u]);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-        }
+        for (int u = 0; u < U; ++u)  // (behind the last head: the last one again)
+            raw[u].load(row + (size_t)min(h0 + u * a.parts * HS + sub, heads - 1) * HD, lo, hi);
     };
     fetch(part * HS);
     const int b = norm_sequence(a, r);
@@ -101,62 +113,52 @@ __global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rope_kernel(const __g
     const int slot = max(0, min(a.ctx_len[b], 1 << 30)) + (r - max(0, a.row_off[b]));
     const int page = slot < a.max_blocks * 16 ? a.tables[(size_t)b * a.max_blocks + (slot >> 4)] : -1;
     const bool paged = page >= 0 && page < a.num_blocks;
-    // what this lane's values turn by: its pairs are pair0 .. pair0 + 7 of the head
-    const bool turns = d0 < 2 * a.half;
-    const bool upper = d0 >= a.half;
-    const int away = a.half / 8;  // lanes to the pair's other half
-    float c[8], s[8];
+    float c[4], s[4];
     if (turns) {
         const int p = max(0, min(a.pos ? a.pos[r] : slot, a.max_pos - 1));
-        const size_t at = (size_t)p * a.half + (upper ? d0 - a.half : d0);
-        norm_load8(a.cos_t + at, c);
-        norm_load8(a.sin_t + at, s);
-        if (!upper)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = -s[e];
+        norm_load4(a.cos_t + (size_t)p * a.half + lo, c);
+        norm_load4(a.sin_t + (size_t)p * a.half + lo, s);
     }
-    const int other = turns ? sub * LPH + (upper ? l - away : l + away) : lane;
-    __half* kv = a.kv + ((size_t)max(page, 0) * 2 * a.Hkv * 16 + (slot & 15)) * HD + d0;
+    __half* kv = a.kv + ((size_t)max(page, 0) * 2 * a.Hkv * 16 + (slot & 15)) * HD;
     for (int h0 = part * HS; h0 < heads; h0 += U * a.parts * HS) {
         if (h0 > part * HS) fetch(h0);
-        float sum[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            sum[u] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[u] = fmaf(x[u][e], x[u][e], sum[u]);
-        }
-#pragma unroll
-        for (int o = LPH / 2; o; o >>= 1)
-#pragma unroll
-            for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = h0 + u * a.parts * HS + sub;
             const bool real = h < heads, is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
+            float x[8], sum = 0.f;
+            raw[u].get(x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+            for (int o = LPH / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float* norm = is_q ? a.qw : is_k ? a.kw : nullptr;
             if (norm) {
                 float g[8];
-                norm_load8(norm + d0, g);
-                const float inv = rsqrtf(sum[u] * (1.0f / HD) + a.eps);
+                norm_load4(norm + lo, g);
+                norm_load4(norm + hi, g + 4);
+                const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * inv * g[e];
+                for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * g[e];
             }
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[u][e], other);
             if (turns && (is_q || is_k)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * c[e] + y[e] * s[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float y = x[e], z = x[e + 4];
+                    x[e] = y * c[e] - z * s[e];
+                    x[e + 4] = z * c[e] + y * s[e];
+                }
             }
-            uint4 out;
-            __half2* o2 = reinterpret_cast<__half2*>(&out);
+            uint2 out[2];
+            __half2* o2 = reinterpret_cast<__half2*>(out);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o2[e] = __floats2half2_rn(x[u][2 * e], x[u][2 * e + 1]);
-            if (real && is_q)
-                *reinterpret_cast<uint4*>(a.q_out + (size_t)r * a.ldq + (size_t)h * HD + d0) = out;
-            else if (real && paged)  // [K|V][kv head][16][HD]: K's heads, then V's
-                *reinterpret_cast<uint4*>(kv + (size_t)(h - a.Hq) * 16 * HD) = out;
+            for (int e = 0; e < 4; ++e) o2[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+            // a query head; or in [K|V][kv head][16][HD], K's heads and then V's
+            __half* dst = is_q ? a.q_out + (size_t)r * a.ldq + (size_t)h * HD : kv + (size_t)(h - a.Hq) * 16 * HD;
+            if (real && (is_q || paged)) {
+                *reinterpret_cast<uint2*>(dst + lo) = out[0];
+                *reinterpret_cast<uint2*>(dst + hi) = out[1];
+            }
         }
     }
 }
@@ -237,17 +239,19 @@ extern "C" int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, 
     a.T = T;
     a.q_out = reinterpret_cast<__half*>(q_out);
     a.ldq = ldq;
-    // Few rows: a warp for each head group, so that a row's chain of look-ups is all there is; many: PARTS_NOTE
+    // Few rows: a warp for each head group, so that a row's chain of look-ups is all there is (160 rows of 32/8 heads of
+    // 128, fp32: 3.7 us, a warp for the whole row 16.6).  Many: four groups in flight, four times, at 28 warps of an SM
+    // (8 x 2501 such rows 117 us, 0.97 of the copy rate; 16 groups in flight or more warps of fewer registers 120 to 148).
     const int groups = ((n_q_heads + 2 * n_kv_heads) * head_dim + 255) / 256;
     const bool many = (long long)T * groups > 148LL * 64 * 4;
-    a.parts = many ? (groups + 7) / 8 : groups;
+    a.parts = many ? (groups + 15) / 16 : groups;
     const long long warps = (long long)T * a.parts;
     const dim3 grid((unsigned)((warps + kNormWarps - 1) / kNormWarps)), block(32 * kNormWarps);
     cudaStream_t s = as_stream(stream);
 #define NORM_LAUNCH(hd, type)                                          \
-    do {                                                               \
-        if (many) qk_norm_rope_kernel<hd, type, 4><<<grid, block, 0, s>>>(a); \
-        else qk_norm_rope_kernel<hd, type, 1><<<grid, block, 0, s>>>(a);      \
+    do {                                                                         \
+        if (many) qk_norm_rope_kernel<hd, type, 4, 7><<<grid, block, 0, s>>>(a); \
+        else qk_norm_rope_kernel<hd, type, 1, 8><<<grid, block, 0, s>>>(a);      \
     } while (0)
     if (head_dim == 128) {
         if (qkv_f16) NORM_LAUNCH(128, __half);
