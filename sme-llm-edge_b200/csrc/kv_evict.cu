@@ -1,16 +1,18 @@
 // kv_evict.cu -- requests of the paged cache that keep their first, their last
 // and their heaviest tokens (specdec_kv_evict_pages).
 //
-// Three launches:
+// Three steps:
 //   select  a CTA for each request: the request is checked, the `keep` tokens
-//           that stay are found (a radix select over the weights' 32-bit keys,
-//           ties to the lower slot) and listed in order, with the first slot
-//           that another token moves into and the pages that have to be replaced
-//           because others hold them;
+//           that stay are found (the smallest of their weights' 32-bit keys, bits
+//           from the top; ties to the lower slot) and listed in order, with the
+//           first slot that another token moves into and the pages that have to be
+//           replaced because others hold them;
 //   tables  one CTA: all requests' errors, free pages for those replaced, then
 //           tables, lengths and reference counts;
 //   move    a CTA for each (request, layer, K or V of a head), and for each head
 //           of the weights: rows move up in place.
+// Up to 8 requests are selected by the CTAs of one cluster, whose first goes on
+// with the tables: two launches.
 //
 // In place: token j of those that stay comes from slot kept[j] >= j, so what a
 // chunk of tokens is written over has been read once the chunk itself is in
@@ -22,7 +24,7 @@
 
 namespace specdec {
 
-constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32;  // of a CTA at most
 constexpr int kMoveThreads = 256;
 
 struct EvictReq {
@@ -57,7 +59,8 @@ struct EvictArgs {
 };
 
 // Exclusive sum over the CTA; every thread gets the total.
-__device__ int evict_scan(int v, int* sh, int* total) {
+template <int THREADS>
+__device__ __forceinline__ int evict_scan(int v, int* sh, int* total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     int x = v;
 #pragma unroll
@@ -68,13 +71,13 @@ __device__ int evict_scan(int v, int* sh, int* total) {
     __syncthreads();
     if (lane == 31) sh[w] = x;
     __syncthreads();
-    int s = sh[lane];
+    int s = lane < THREADS / 32 ? sh[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < THREADS / 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += y;
     }
-    *total = __shfl_sync(0xffffffffu, s, 31);
+    *total = __shfl_sync(0xffffffffu, s, THREADS / 32 - 1);
     const int before = __shfl_sync(0xffffffffu, s, max(0, w - 1));
     return (w ? before : 0) + x - v;
 }
@@ -82,16 +85,67 @@ __device__ int evict_scan(int v, int* sh, int* total) {
 // Order-preserving key of a token's weight: the heads' sum in 64 bits, rounded
 // once (so that its order does not hang on the order of the sum), -0 as 0, NaN
 // above all.
-__device__ __forceinline__ uint32_t evict_key(const float* w, int heads, size_t ldw) {
-    double s = 0.0;
-    for (int h = 0; h < heads; ++h) s += (double)w[h * ldw];
-    const float f = (float)s + 0.0f;
+__device__ __forceinline__ uint32_t evict_key(double sum) {
+    const float f = (float)sum + 0.0f;
     return f != f ? 0xFFFFFFFFu : logit_key(f);
 }
 
-__global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const __grid_constant__ EvictArgs a) {
-    __shared__ int sh[kEvictWarps], hist[256], pick[2], hole_s, need_s;
-    const int i = blockIdx.x, tid = threadIdx.x;
+constexpr int kEvictKeys = 8;  // of a thread, where a request's stay in registers
+constexpr int kEvictCluster = 8;
+
+struct EvictShared {
+    int scan[kEvictWarps], hist[256], pick[2], hole, need;
+    uint32_t count[2][kEvictWarps];
+};
+
+// The smallest key that stays, and how many of it: `want` of the keys, the largest
+// first; 0 is no key.  From registers, two bits at a time: one barrier a round (a
+// histogram of 256 digits has most of a request's keys in a few bins).
+template <int THREADS>
+__device__ __forceinline__ uint32_t evict_threshold(EvictShared& sh, const uint32_t (&k)[kEvictKeys], int want, int* ties) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint32_t tau = 0;
+    int left = want;
+    for (int shift = 30; shift >= 0; shift -= 2) {
+        // keys with digits 3, 2, 1 under the bits known: 10 bits each (256 of a warp at most)
+        uint32_t c = 0;
+        const uint32_t known = tau >> shift;
+#pragma unroll
+        for (int u = 0; u < kEvictKeys; ++u) {
+            const uint32_t d = min((k[u] >> shift) - known, 4u);
+            uint32_t one;  // (shl gives 0 from 32 on; digit 0 counts into the two bits above)
+            asm("shl.b32 %0, 1, %1;" : "=r"(one) : "r"(30u - 10u * d));
+            c += one;
+        }
+        c = __reduce_add_sync(0xffffffffu, c);
+        uint32_t* row = sh.count[(shift >> 1) & 1];
+        if (lane == 0) row[w] = c;
+        __syncthreads();
+        const uint32_t x = lane < THREADS / 32 ? row[lane] : 0;
+        const uint32_t hi = __reduce_add_sync(0xffffffffu, (x & 1023u) | ((x >> 10) & 1023u) << 16);
+        const int c3 = (int)(hi & 0xFFFFu), c2 = (int)(hi >> 16), c1 = (int)__reduce_add_sync(0xffffffffu, (x >> 20) & 1023u);
+        uint32_t digit = 3;
+        if (left > c3) {
+            left -= c3;
+            digit = 2;
+            if (left > c2) {
+                left -= c2;
+                digit = 1;
+                if (left > c1) {
+                    left -= c1;
+                    digit = 0;
+                }
+            }
+        }
+        tau |= digit << shift;
+    }
+    *ties = left;
+    return tau;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void evict_select(const EvictArgs& a, EvictShared& sh, int i) {
+    const int tid = threadIdx.x;
     const int r = a.reqs[i];
     bool bad = r < 0 || r >= a.max_reqs;
     int nb = -1, L = 0;
@@ -100,123 +154,187 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const __
         L = a.len[r];
         bad = nb < 0 || nb > a.max_bpr || L < 0 || L > (long long)nb * a.bs || L > a.ldw;
     }
-    for (int j = tid; j < a.n; j += kEvictThreads) bad |= j != i && a.reqs[j] == r;
-    bad = __syncthreads_or(bad);
-    if (!bad) {
-        for (int d = tid; d < nb; d += kEvictThreads) {
+    const bool sound = !bad;
+    for (int j = tid; j < a.n; j += THREADS) bad |= j != i && a.reqs[j] == r;
+    if (sound)
+        for (int d = tid; d < nb; d += THREADS) {
             const int p = a.tables[(size_t)r * a.max_bpr + d];
             bad |= p < 0 || p >= a.num_blocks;
         }
-        bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        sh.hole = a.keep;
+        sh.need = 0;
     }
+    // (the weights are on their way before all checks are known)
+    const int lo = a.first, hi = L - a.last, want = a.keep - a.first - a.last;  // the others: slots lo .. hi - 1
+    const float* w = a.w + (size_t)(sound ? r : 0) * a.wheads * a.ldw;
+    const bool small = L <= kEvictKeys * THREADS;
+    const int j0 = kEvictKeys * tid;
+    uint32_t k[kEvictKeys], real = 0;
+    if (sound && L > a.keep && small && want > 0) {
+        double sum[kEvictKeys];
+#pragma unroll
+        for (int u = 0; u < kEvictKeys; ++u) {
+            sum[u] = 0.0;
+            if (j0 + u >= lo && j0 + u < hi) real |= 1u << u;
+        }
+        if (real) {
+            // whole 32-byte runs where they are aligned, so that all heads' loads go out together
+            const bool wide = (a.ldw & 3) == 0 && (reinterpret_cast<uintptr_t>(a.w) & 15) == 0 && j0 + kEvictKeys <= a.ldw;
+            if (wide) {
+#pragma unroll 4
+                for (int h = 0; h < a.wheads; ++h) {
+                    const float4* src = reinterpret_cast<const float4*>(w + (size_t)h * a.ldw + j0);
+                    const float4 x = src[0], y = src[1];
+                    sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
+                    sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
+                }
+            } else {
+                for (int h = 0; h < a.wheads; ++h)
+#pragma unroll
+                    for (int u = 0; u < kEvictKeys; ++u) sum[u] += w[(size_t)h * a.ldw + min(j0 + u, a.ldw - 1)];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kEvictKeys; ++u) k[u] = (real >> u) & 1u ? evict_key(sum[u]) : 0u;
+    }
+    bad = __syncthreads_or(bad);
     const bool gone = !bad && L > a.keep;
     int32_t* user = a.kept ? a.kept + (size_t)i * a.keep : nullptr;
     if (!gone) {
         if (user)
-            for (int j = tid; j < a.keep; j += kEvictThreads) user[j] = !bad && j < L ? j : -1;
+            for (int j = tid; j < a.keep; j += THREADS) user[j] = !bad && j < L ? j : -1;
         if (tid == 0) a.req[i] = {bad, 0, a.keep, 0, a.keep};
         return;
     }
     int32_t* list = a.list + (size_t)i * a.list_len;
-    uint32_t* keys = a.keys + (size_t)i * a.slots;
-    const int lo = a.first, hi = L - a.last, want = a.keep - a.first - a.last;  // the others: slots lo .. hi - 1
-    for (int j = lo + tid; j < hi; j += kEvictThreads)
-        keys[j] = evict_key(a.w + (size_t)r * a.wheads * a.ldw + j, a.wheads, a.ldw);
-    // the smallest key that stays, and how many of it
-    uint32_t tau = 0;
-    int ties = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = lo + tid; j < hi; j += kEvictThreads) {
-            const uint32_t k = keys[j];
-            if (shift == 24 || (k >> (shift + 8)) == (tau >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        int tot;
-        const int c = tid < 256 ? hist[255 - tid] : 0;
-        const int above = evict_scan(c, sh, &tot);
-        if (c && above < ties && above + c >= ties) {
-            pick[0] = 255 - tid;
-            pick[1] = above;
-        }
-        __syncthreads();
-        if (want > 0) {
-            tau |= (uint32_t)pick[0] << shift;
-            ties -= pick[1];
-        }
-        __syncthreads();
-    }
-    if (tid == 0) {
-        hole_s = a.keep;
-        need_s = 0;
-    }
-    __syncthreads();
-    // the list: the thread's slots are neighbours, tile by tile
-    int out = 0, taken = 0, hole = a.keep;
-    for (int t0 = 0; t0 < L; t0 += 4 * kEvictThreads) {
-        int stay[4], tie[4], nt = 0, ns = 0;
+    int hole = a.keep, tot;
+    if (small) {
+        uint32_t tau = 0xFFFFFFFFu;
+        int ties = 0;
+        if (want > 0) tau = evict_threshold<THREADS>(sh, k, want, &ties);
+        uint32_t stay = 0, tie = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = t0 + 4 * tid + u;
+        for (int u = 0; u < kEvictKeys; ++u) {
+            const int j = j0 + u;
             const bool other = j >= lo && j < hi;
-            const uint32_t k = other && want > 0 ? keys[j] : 0;
-            tie[u] = other && want > 0 && k == tau;
-            stay[u] = j < L && (!other || (want > 0 && k > tau));
-            nt += tie[u];
+            if (j < L && !other) stay |= 1u << u;
+            if (other && want > 0) {
+                if (k[u] > tau) stay |= 1u << u;
+                if (k[u] == tau) tie |= 1u << u;
+            }
         }
-        int tot;
-        int before = taken + evict_scan(nt, sh, &tot);
-        taken += tot;
+        // both sums in one, 16 bits each (8192 slots at most)
+        const int before = evict_scan<THREADS>(__popc(stay) | __popc(tie) << 16, sh.scan, &tot);
+        int ahead = before & 0xFFFF, tied = before >> 16;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (tie[u] && before++ < ties) stay[u] = 1;
-            ns += stay[u];
+        for (int u = 0; u < kEvictKeys; ++u) {
+            const int place = ahead + min(tied, ties), j = j0 + u;
+            const bool is_tie = (tie >> u) & 1u, is_in = ((stay >> u) & 1u) || (is_tie && tied < ties);
+            if (is_in) {
+                list[place] = j;
+                if (user) user[place] = j;
+                if (j != place) hole = min(hole, place);
+            }
+            ahead += (stay >> u) & 1u;
+            tied += is_tie;
         }
-        int place = out + evict_scan(ns, sh, &tot);
-        out += tot;
+    } else {
+        uint32_t* keys = a.keys + (size_t)i * a.slots;
+        for (int j = lo + tid; j < hi; j += THREADS) {
+            double sum = 0.0;
+#pragma unroll 4
+            for (int h = 0; h < a.wheads; ++h) sum += w[(size_t)h * a.ldw + j];
+            keys[j] = evict_key(sum);
+        }
+        uint32_t tau = 0;
+        int ties = want;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            if (tid < 256) sh.hist[tid] = 0;
+            __syncthreads();
+            for (int j = lo + tid; j < hi; j += THREADS) {
+                const uint32_t x = keys[j];
+                if (shift == 24 || (x >> (shift + 8)) == (tau >> (shift + 8))) atomicAdd(&sh.hist[(x >> shift) & 255], 1);
+            }
+            __syncthreads();
+            const int c = tid < 256 ? sh.hist[255 - tid] : 0;
+            const int above = evict_scan<THREADS>(c, sh.scan, &tot);
+            if (c && above < ties && above + c >= ties) {
+                sh.pick[0] = 255 - tid;
+                sh.pick[1] = above;
+            }
+            __syncthreads();
+            if (want > 0) {
+                tau |= (uint32_t)sh.pick[0] << shift;
+                ties -= sh.pick[1];
+            }
+            __syncthreads();
+        }
+        // the list: the thread's slots are neighbours, tile by tile
+        int out = 0, taken = 0;
+        for (int t0 = 0; t0 < L; t0 += 4 * THREADS) {
+            int stay[4], tie[4], nt = 0, ns = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (!stay[u]) continue;
-            const int j = t0 + 4 * tid + u;
-            list[place] = j;
-            if (user) user[place] = j;
-            if (j != place) hole = min(hole, place);
-            ++place;
+            for (int u = 0; u < 4; ++u) {
+                const int j = t0 + 4 * tid + u;
+                const bool other = j >= lo && j < hi;
+                const uint32_t x = other && want > 0 ? keys[j] : 0;
+                tie[u] = other && want > 0 && x == tau;
+                stay[u] = j < L && (!other || (want > 0 && x > tau));
+                nt += tie[u];
+            }
+            int before = taken + evict_scan<THREADS>(nt, sh.scan, &tot);
+            taken += tot;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (tie[u] && before++ < ties) stay[u] = 1;
+                ns += stay[u];
+            }
+            int place = out + evict_scan<THREADS>(ns, sh.scan, &tot);
+            out += tot;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (!stay[u]) continue;
+                const int j = t0 + 4 * tid + u;
+                list[place] = j;
+                if (user) user[place] = j;
+                if (j != place) hole = min(hole, place);
+                ++place;
+            }
         }
     }
-    if (hole < a.keep) atomicMin(&hole_s, hole);
+    if (hole < a.keep) atomicMin(&sh.hole, hole);
     __syncthreads();
-    hole = hole_s;
+    hole = sh.hole;
     const int d0 = hole / a.bs, d1 = (a.keep + a.bs - 1) / a.bs;
     int need = 0;
     int32_t* old = a.old + (size_t)i * a.max_bpr;
-    for (int d = tid; d < nb; d += kEvictThreads) {
+    for (int d = tid; d < nb; d += THREADS) {
         const int p = a.tables[(size_t)r * a.max_bpr + d];
         const bool swap = hole < a.keep && d >= d0 && d < d1 && a.ref[p] > 1;
         old[d] = swap ? ~p : p;
         need += swap;
     }
-    if (need) atomicAdd(&need_s, need);
+    if (need) atomicAdd(&sh.need, need);
     __syncthreads();
     if (tid == 0) {
         const bool first_page = hole < a.keep && old[d0] < 0;  // (written by some thread before the barrier)
-        a.req[i] = {0, 1, hole, need_s, first_page ? d0 * a.bs : hole};
+        a.req[i] = {0, 1, hole, sh.need, first_page ? d0 * a.bs : hole};
     }
 }
 
-__global__ void __launch_bounds__(kEvictThreads) kv_evict_tables_kernel(const __grid_constant__ EvictArgs a) {
-    __shared__ int sh[kEvictWarps];
+template <int THREADS>
+__device__ __forceinline__ void evict_tables(const EvictArgs& a, int* sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     bool bad = false;
     int need = 0;
-    for (int i = tid; i < a.n; i += kEvictThreads) {
+    for (int i = tid; i < a.n; i += THREADS) {
         bad |= a.req[i].bad != 0;
         need += a.req[i].need;
     }
     bad = __syncthreads_or(bad);
     int total;
-    (void)evict_scan(need, sh, &total);
+    (void)evict_scan<THREADS>(need, sh, &total);
     if (bad) {
         if (tid == 0) {
             *a.go = 0;
@@ -226,11 +344,11 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_tables_kernel(const __
     }
     if (total > 0) {  // the lowest free pages, in order
         int got = 0;
-        for (int b0 = 0; b0 < a.num_blocks && got < total; b0 += kEvictThreads) {
+        for (int b0 = 0; b0 < a.num_blocks && got < total; b0 += THREADS) {
             const int b = b0 + tid;
             const int is_free = b < a.num_blocks && a.ref[b] == 0;
             int tot;
-            const int before = got + evict_scan(is_free, sh, &tot);
+            const int before = got + evict_scan<THREADS>(is_free, sh, &tot);
             if (is_free && before < total) a.fresh[before] = b;
             got += tot;
         }
@@ -245,7 +363,7 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_tables_kernel(const __
     __syncthreads();
     // a warp for each request
     const int pages = (a.keep + a.bs - 1) / a.bs;
-    for (int i = warp; i < a.n; i += kEvictWarps) {
+    for (int i = warp; i < a.n; i += THREADS / 32) {
         if (!a.req[i].gone) continue;
         const int r = a.reqs[i], nb = a.nblk[r];
         int at = 0;  // fresh pages of the requests before
@@ -280,10 +398,26 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_tables_kernel(const __
     }
 }
 
+// PHASE 0: both steps of up to kEvictCluster requests, by a cluster (CTAS > 1) or a CTA; 1 and 2: one of them.
+template <int PHASE, int CTAS, int THREADS>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS)
+    kv_evict_plan_kernel(const __grid_constant__ EvictArgs a) {
+    __shared__ EvictShared sh;
+    pdl_trigger();
+    if constexpr (PHASE == 2) pdl_wait();
+    if (PHASE < 2 && (int)blockIdx.x < a.n) evict_select<THREADS>(a, sh, blockIdx.x);
+    if constexpr (PHASE == 0) {
+        if constexpr (CTAS > 1) cluster_sync_all();
+        else __syncthreads();
+    }
+    if (PHASE != 1 && blockIdx.x == 0) evict_tables<THREADS>(a, sh.scan);
+}
+
 // x < 2 * Hkv: K or V of a head of layer y; above: a head of the weights.
 __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const __grid_constant__ EvictArgs a, __half* kv,
                                                                      size_t layer_stride, int Hkv, int hd, int planes) {
     const int i = blockIdx.z, x = blockIdx.x, tid = threadIdx.x;
+    pdl_wait();
     if (!*a.go) return;
     const EvictReq q = a.req[i];
     if (!q.gone) return;
@@ -380,14 +514,32 @@ int kv_evict_launch(const KVState& st, const int32_t* reqs, int n, int keep, int
     a.old = reinterpret_cast<int32_t*>(w);
     w += up256((size_t)n * st.max_bpr * 4);
     a.fresh = reinterpret_cast<int32_t*>(w);
-    kv_evict_select_kernel<<<n, kEvictThreads, 0, s>>>(a);
-    SD_LAUNCH_CHECK("kv_evict_select_kernel");
-    kv_evict_tables_kernel<<<1, kEvictThreads, 0, s>>>(a);
-    SD_LAUNCH_CHECK("kv_evict_tables_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    // No more threads than the tables' slots need: a barrier of 32 warps takes twice one of 8.
+    const int threads = a.slots <= 256 * kEvictKeys ? 256 : a.slots <= 512 * kEvictKeys ? 512 : kEvictThreads;
+    const int kind = n == 1 ? 0 : n <= kEvictCluster ? 1 : 2;
+#define EVICT_PLAN(t)                                                                    \
+    (kind == 0 ? kv_evict_plan_kernel<0, 1, t>                                           \
+               : kind == 1 ? kv_evict_plan_kernel<0, kEvictCluster, t> : kv_evict_plan_kernel<1, 1, t>)
+    const auto plan = threads == 256 ? EVICT_PLAN(256) : threads == 512 ? EVICT_PLAN(512) : EVICT_PLAN(kEvictThreads);
+#undef EVICT_PLAN
+    plan<<<kind == 1 ? kEvictCluster : n, threads, 0, s>>>(a);
+    SD_LAUNCH_CHECK("kv_evict_plan_kernel");
+    if (kind == 2) {
+        cfg.gridDim = dim3(1);
+        cfg.blockDim = dim3(kEvictThreads);
+        SD_CUDA(cudaLaunchKernelEx(&cfg, kv_evict_plan_kernel<2, 1, kEvictThreads>, a));
+    }
     const int planes = layers > 0 ? 2 * Hkv : 0;
-    const dim3 grid((unsigned)(planes + wheads), (unsigned)std::max(1, layers), (unsigned)n);
-    kv_evict_move_kernel<<<grid, kMoveThreads, 0, s>>>(a, kv, layer_stride, Hkv, hd, planes);
-    SD_LAUNCH_CHECK("kv_evict_move_kernel");
+    cfg.gridDim = dim3((unsigned)(planes + wheads), (unsigned)std::max(1, layers), (unsigned)n);
+    cfg.blockDim = dim3(kMoveThreads);
+    SD_CUDA(cudaLaunchKernelEx(&cfg, kv_evict_move_kernel, a, kv, layer_stride, Hkv, hd, planes));
     return SPECDEC_OK;
 }
 
