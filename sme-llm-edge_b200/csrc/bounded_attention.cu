@@ -320,11 +320,191 @@ struct FewCut {
     }
 };
 
+// What a warp holds of a tile: its queries as MMA fragments (lane 4 g + t4: row g), each row's m and partial sums, O.
+template <int HD, int NT, bool ACC>
+struct FewWork {
+    static constexpr int KS = HD / 16, NH = HD / 64;
+    uint32_t qf[NT][KS][2];
+    int slot_of[NT][2];  // slots of this lane's rows 2 t4, 2 t4 + 1 (of those behind the tile: the last one's)
+    float m[NT][2], l[NT][2], o[KS][NT][4];
+    float* score[NT];  // of this lane's rows at its slot of a page
+    FewTile t;
+    int kvh, rows, p1;
+    bool bad;  // an infinity or a NaN of V was left out
+
+    __device__ __forceinline__ float* score_at(const FewArgs& a, int row) const {
+        const int tok = row / a.G;
+        return a.scores + ((size_t)(t.row + tok) * a.Hkv + kvh) * a.slots_max * a.G + (row - tok * a.G);
+    }
+    __device__ __forceinline__ void begin(const FewArgs& a, const FewTile& tile, int head) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+        t = tile;
+        kvh = head;
+        rows = t.tokens * a.G;
+        p1 = t.p0 + t.tokens - 1;
+        bad = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = 8 * n + g;
+            const bool real = row < rows;
+            const int tok = real ? row / a.G : 0;
+            const __half* src = a.q + (size_t)(t.row + tok) * a.ldq + (size_t)(kvh * a.G + (real ? row - tok * a.G : 0)) * HD + 2 * t4;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                qf[n][k][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+                qf[n][k][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                slot_of[n][e] = t.p0 + min(t.tokens - 1, (8 * n + 2 * t4 + e) / a.G);
+                m[n][e] = kFewNone;
+                l[n][e] = 0.f;
+            }
+            if constexpr (ACC) score[n] = score_at(a, 8 * n + 2 * t4) + (size_t)g * a.G;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
+    }
+    // The page in shared memory at sk, whose first slot is s0.
+    __device__ __forceinline__ void page(const FewArgs& a, uint32_t sk, int s0) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+        const uint32_t k_row = (uint32_t)(lane & 15), k_chunk = (uint32_t)(lane >> 4);
+        const uint32_t v_row = (uint32_t)((lane & 7) + ((lane >> 4) & 1) * 8), v_chunk = (uint32_t)((lane >> 3) & 1);
+        const uint32_t sv = sk + NH * 2048;
+        // every row sees every slot of the page
+        const bool clear = s0 + 15 <= t.p0 && (s0 + 15 < a.sinks || s0 > p1 - a.window);
+        float s[NT][4], s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile of rows: two chains
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t x[4];
+            few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) few_mma(NT == 1 && (k & 1) ? s2 : s[n], x, qf[n][k][0], qf[n][k][1]);
+        }
+        if constexpr (NT == 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0][e] += s2[e];
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] *= a.scale_log2;
+                if (!clear) {
+                    const int slot = s0 + g + 8 * (e >> 1), p = slot_of[n][e & 1];
+                    if (!(slot <= p && (slot < a.sinks || slot > p - a.window))) s[n][e] = -INFINITY;
+                }
+            }
+            if constexpr (ACC) {  // the rows' scores, for their weights once the rows' sums are known
+                const int row = 8 * n + 2 * t4;
+                float* dst = score[n] + (size_t)s0 * a.G;
+                if ((a.G & 1) == 0) {
+                    if (row < rows) {
+                        *reinterpret_cast<float2*>(dst) = make_float2(s[n][0], s[n][1]);
+                        *reinterpret_cast<float2*>(dst + 8 * a.G) = make_float2(s[n][2], s[n][3]);
+                    }
+                } else {
+                    if (row < rows) {
+                        dst[0] = s[n][0];
+                        dst[8 * a.G] = s[n][2];
+                    }
+                    if (row + 1 < rows) {
+                        float* d1 = score_at(a, row + 1) + (size_t)(s0 + g) * a.G;
+                        d1[0] = s[n][1];
+                        d1[8 * a.G] = s[n][3];
+                    }
+                }
+            }
+            // (also for NaN)
+            grow |= !(few_max(s[n][0], s[n][2]) - m[n][0] <= kFewTop) || !(few_max(s[n][1], s[n][3]) - m[n][1] <= kFewTop);
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = few_max(s[n][e], s[n][2 + e]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = few_max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    f[e] = 1.f;
+                    if (!(top - m[n][e] <= kFewTop)) {
+                        // a NaN or infinite maximum makes every weight, and so the row, NaN; far from 0 the 11 would
+                        // be lost in rounding
+                        const float now = top < INFINITY ? (fabsf(top) < 0x1p20f ? top - kFewLift : top)
+                                                         : __int_as_float(0x7FC00000);
+                        f[e] = m[n][e] == kFewNone ? 0.f : exp2f(m[n][e] - now);
+                        m[n][e] = now;
+                        l[n][e] *= f[e];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[k][n][e] *= f[e & 1];
+            }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = few_exp2(s[n][e] - m[n][e & 1]);
+            l[n][0] += y[0] + y[2];
+            l[n][1] += y[1] + y[3];
+            const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
+            pb[n][0] = few_turn(*reinterpret_cast<const uint32_t*>(&h0));
+            pb[n][1] = few_turn(*reinterpret_cast<const uint32_t*>(&h1));
+        }
+        // V: slots that no row sees may hold anything and become 0; infinities and NaN of slots that some rows see
+        // too (0 * NaN would reach the others), and the rows look them up at the end
+        uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, some[2] = {0u, 0u};
+        if (!clear) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int slot = s0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
+                const bool any = slot <= p1 && (slot < a.sinks || slot > t.p0 - a.window);
+                const bool all = slot <= t.p0 && (slot < a.sinks || slot > p1 - a.window);
+                const uint32_t half = e & 1 ? 0xFFFF0000u : 0xFFFFu;
+                if (!any) keep[e >> 1] &= ~half;
+                else if (!all) some[e >> 1] |= half;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t x[4];
+            few_ldm<true>(x, sv + (k >> 2) * 2048 + v_row * 128 + (((2 * (k & 3) + v_chunk) ^ (v_row & 7)) << 4));
+            if (!clear) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] &= keep[e >> 1];
+                    uint32_t wild = 0;
+                    if ((x[e] & 0x7C00u) == 0x7C00u) wild |= 0xFFFFu;
+                    if ((x[e] & 0x7C000000u) == 0x7C000000u) wild |= 0xFFFF0000u;
+                    wild &= some[e >> 1];
+                    bad |= wild != 0;
+                    x[e] &= ~wild;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) few_mma(o[k][n], x, pb[n][0], pb[n][1]);
+        }
+    }
+};
+
 template <int HD, int NT, bool ACC>
 __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
     few_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
     using C = FewCfg<HD, NT>;
-    constexpr int KS = HD / 16, NH = HD / 64, RING = C::RING;
+    constexpr int KS = HD / 16, RING = C::RING;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -384,8 +564,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
     for (int i = 0; i < RING; ++i) load();
 
     // ---- arithmetic
-    const uint32_t k_row = (uint32_t)(lane & 15), k_chunk = (uint32_t)(lane >> 4);
-    const uint32_t v_row = (uint32_t)((lane & 7) + ((lane >> 4) & 1) * 8), v_chunk = (uint32_t)((lane >> 3) & 1);
     FewWalk w = {};
     w.u = u0;
     w.hi = u1;
@@ -393,182 +571,29 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
     bool ok = true;
     while (ok && few_next(a, pre, seqs, w)) {
         const FewTile& t = w.t;
-        const int rows = t.tokens * a.G, p1 = t.p0 + t.tokens - 1;
-        uint32_t qf[NT][KS][2];
-        int slot_of[NT][2];  // slots of this lane's rows 2 t4, 2 t4 + 1 (of those behind the tile: the last one's)
-        float m[NT][2], l[NT][2], o[KS][NT][4];
-        float* score[NT];  // of this lane's rows at its slot of a page
-        auto score_at = [&](int row0, int row) {
-            const int tok = row / a.G;
-            return a.scores + ((size_t)(row0 + tok) * a.Hkv + w.kvh) * a.slots_max * a.G + (row - tok * a.G);
-        };
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = 8 * n + g;
-            const bool real = row < rows;
-            const int tok = real ? row / a.G : 0;
-            const __half* src = a.q + (size_t)(t.row + tok) * a.ldq + (size_t)(w.kvh * a.G + (real ? row - tok * a.G : 0)) * HD + 2 * t4;
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                qf[n][k][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-                qf[n][k][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                slot_of[n][e] = t.p0 + min(t.tokens - 1, (8 * n + 2 * t4 + e) / a.G);
-                m[n][e] = kFewNone;
-                l[n][e] = 0.f;
-            }
-            if constexpr (ACC) score[n] = score_at(t.row, 8 * n + 2 * t4) + (size_t)g * a.G;
-        }
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
-        bool bad = false;
+        const int rows = t.tokens * a.G;
+        FewWork<HD, NT, ACC> f;
+        f.begin(a, t, w.kvh);
         for (int v = w.v; v < w.ve; ++v) {
             const int at = done % RING;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
-            const uint32_t sk = ring + at * C::PAGE, sv = sk + NH * 2048;
+            const uint32_t sk = ring + at * C::PAGE;
             const int s0 = 16 * (v < t.sinkp ? v : v + t.gap);
-            // every row sees every slot of the page
-            const bool clear = s0 + 15 <= t.p0 && (s0 + 15 < a.sinks || s0 > p1 - a.window);
-            float s[NT][4], s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile of rows: two chains
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t x[4];
-                few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) few_mma(NT == 1 && (k & 1) ? s2 : s[n], x, qf[n][k][0], qf[n][k][1]);
-            }
-            if constexpr (NT == 1)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[0][e] += s2[e];
-            bool grow = false;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[n][e] *= a.scale_log2;
-                    if (!clear) {
-                        const int slot = s0 + g + 8 * (e >> 1), p = slot_of[n][e & 1];
-                        if (!(slot <= p && (slot < a.sinks || slot > p - a.window))) s[n][e] = -INFINITY;
-                    }
-                }
-                if constexpr (ACC) {  // the rows' scores, for their weights once the rows' sums are known
-                    const int row = 8 * n + 2 * t4;
-                    float* dst = score[n] + (size_t)s0 * a.G;
-                    if ((a.G & 1) == 0) {
-                        if (row < rows) {
-                            *reinterpret_cast<float2*>(dst) = make_float2(s[n][0], s[n][1]);
-                            *reinterpret_cast<float2*>(dst + 8 * a.G) = make_float2(s[n][2], s[n][3]);
-                        }
-                    } else {
-                        if (row < rows) {
-                            dst[0] = s[n][0];
-                            dst[8 * a.G] = s[n][2];
-                        }
-                        if (row + 1 < rows) {
-                            float* d1 = score_at(t.row, row + 1) + (size_t)(s0 + g) * a.G;
-                            d1[0] = s[n][1];
-                            d1[8 * a.G] = s[n][3];
-                        }
-                    }
-                }
-                // (also for NaN)
-                grow |= !(few_max(s[n][0], s[n][2]) - m[n][0] <= kFewTop) || !(few_max(s[n][1], s[n][3]) - m[n][1] <= kFewTop);
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float f[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = few_max(s[n][e], s[n][2 + e]);
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) top = few_max(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        f[e] = 1.f;
-                        if (!(top - m[n][e] <= kFewTop)) {
-                            // a NaN or infinite maximum makes every weight, and so the row, NaN; far from 0 the 11 would
-                            // be lost in rounding
-                            const float now = top < INFINITY ? (fabsf(top) < 0x1p20f ? top - kFewLift : top)
-                                                             : __int_as_float(0x7FC00000);
-                            f[e] = m[n][e] == kFewNone ? 0.f : exp2f(m[n][e] - now);
-                            m[n][e] = now;
-                            l[n][e] *= f[e];
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < KS; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[k][n][e] *= f[e & 1];
-                }
-            }
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = few_exp2(s[n][e] - m[n][e & 1]);
-                l[n][0] += y[0] + y[2];
-                l[n][1] += y[1] + y[3];
-                const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
-                pb[n][0] = few_turn(*reinterpret_cast<const uint32_t*>(&h0));
-                pb[n][1] = few_turn(*reinterpret_cast<const uint32_t*>(&h1));
-            }
-            // V: slots that no row sees may hold anything and become 0; infinities and NaN of slots that some rows see
-            // too (0 * NaN would reach the others), and the rows look them up at the end
-            uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, some[2] = {0u, 0u};
-            if (!clear) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int slot = s0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
-                    const bool any = slot <= p1 && (slot < a.sinks || slot > t.p0 - a.window);
-                    const bool all = slot <= t.p0 && (slot < a.sinks || slot > p1 - a.window);
-                    const uint32_t half = e & 1 ? 0xFFFF0000u : 0xFFFFu;
-                    if (!any) keep[e >> 1] &= ~half;
-                    else if (!all) some[e >> 1] |= half;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t x[4];
-                few_ldm<true>(x, sv + (k >> 2) * 2048 + v_row * 128 + (((2 * (k & 3) + v_chunk) ^ (v_row & 7)) << 4));
-                if (!clear) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] &= keep[e >> 1];
-                        uint32_t wild = 0;
-                        if ((x[e] & 0x7C00u) == 0x7C00u) wild |= 0xFFFFu;
-                        if ((x[e] & 0x7C000000u) == 0x7C000000u) wild |= 0xFFFF0000u;
-                        wild &= some[e >> 1];
-                        bad |= wild != 0;
-                        x[e] &= ~wild;
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) few_mma(o[k][n], x, pb[n][0], pb[n][1]);
-            }
+            f.page(a, sk, s0);
             ++done;
             __syncwarp();  // the page has been read
             load();
         }
         if (!ok) break;
         // ---- the segment's rows
-        bad = __any_sync(0xffffffffu, bad);
+        const bool bad = __any_sync(0xffffffffu, f.bad);
         const int piece = 2 * range + (w.begun == u0 ? 0 : 1);
         if (w.v >= w.ve && !w.whole) continue;  // behind the tile's pages
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float sum = l[n][e];
+                float sum = f.l[n][e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 const int row = 8 * n + 2 * t4 + e;
@@ -582,12 +607,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float y = o[k][n][e + 2 * h] * inv;
+                            const float y = f.o[k][n][e + 2 * h] * inv;
                             wild |= !(fabsf(y) < INFINITY);
                             // (a finite mean that rounding took past fp16's largest)
                             if (real) dst[16 * k + 8 * h + g] = __float2half_rn(y == y ? fminf(fmaxf(y, -kFewMax), kFewMax) : y);
                         }
-                    if (ACC && real && g == 0) a.ml[(size_t)r * a.Hq + head] = make_float2(m[n][e], inv);
+                    if (ACC && real && g == 0) a.ml[(size_t)r * a.Hq + head] = make_float2(f.m[n][e], inv);
                     const uint32_t look = __ballot_sync(0xffffffffu, real && wild && sum == sum);
                     for (int q = 0; q < 4; ++q) {  // rows that met an infinity or a NaN
                         if (!(look & (0x11111111u << q))) continue;
@@ -602,12 +627,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float y = o[k][n][e + 2 * h];
+                            const float y = f.o[k][n][e + 2 * h];
                             wild |= !(fabsf(y) < INFINITY);
                             if (real) dst[16 * k + 8 * h + g] = y;
                         }
                     wild = (__ballot_sync(0xffffffffu, wild) & (0x11111111u << t4)) != 0;
-                    if (real && g == 0) a.pml[(size_t)piece * (8 * NT) + row] = make_float2(m[n][e], wild ? -sum : sum);
+                    if (real && g == 0) a.pml[(size_t)piece * (8 * NT) + row] = make_float2(f.m[n][e], wild ? -sum : sum);
                 }
             }
         }
@@ -616,6 +641,151 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
         if (lane == 0) record_timeout(a.status, 40);
         // the copies in flight land before the CTA leaves
         for (int c = done; c < asked; ++c) (void)mbar_wait(bar + 8 * (c % RING), (uint32_t)(c / RING) & 1u);
+    }
+}
+
+// Short tables: a CTA for each sequence and KV head, whose eight warps take its pages
+// in turn and join what they have in shared memory: one launch, where latency is all
+// there is.  With weights, the CTA adds them up from the scores that its warps left.
+constexpr int kShortWarps = 8, kShortPages = 32;  // table entries at most
+
+template <int HD, int NT>
+struct ShortCfg {
+    static constexpr int PAGE = 64 * HD, RING = HD == 128 ? 2 : 4;  // a warp's ring holds its rows' O afterwards
+    static constexpr size_t smem = 1024 + (size_t)kShortWarps * RING * (PAGE + 8) + (size_t)kShortWarps * 8 * NT * 8 + 8 * NT * 8;
+    static_assert(RING * PAGE >= 8 * NT * HD * 4, "a warp's O");
+};
+
+template <int HD, int NT, bool ACC>
+__global__ void __launch_bounds__(32 * kShortWarps, 1)
+    short_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
+    using C = ShortCfg<HD, NT>;
+    constexpr int KS = HD / 16, RING = C::RING, W = HD / 32;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + kShortWarps * RING * C::PAGE);
+    float2* pml = reinterpret_cast<float2*>(bars + kShortWarps * RING);  // [warp][row] m, l (l < 0: look V up again)
+    float2* lse = pml + kShortWarps * 8 * NT;                            // [row] m, 1 / l
+    pdl_trigger();
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int g = lane >> 2, t4 = lane & 3;
+    const int b = blockIdx.y, kvh = blockIdx.x;
+    const uint32_t ring = s_addr(base + warp * RING * C::PAGE), bar = s_addr(bars + warp * RING);
+    const float* own_o = reinterpret_cast<const float*>(base);
+    const int ent = a.max_blocks > lane ? a.tables[(size_t)b * a.max_blocks + lane] : 0;  // (32 entries at most)
+    const FewSeq s = few_seq(a, b);
+    if (lane == 0) {
+        for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    int asked = 0, done = 0;
+    bool ok = true;
+    const int tiles = (s.n + a.tpt - 1) / a.tpt;
+    for (int tile = 0; tile < tiles; ++tile) {
+        const FewTile t = few_tile(a, s, tile);
+        const int rows = t.tokens * a.G;
+        int next = warp;  // page to ask for
+        auto load = [&]() {
+            if (next >= t.np) return;
+            int page = __shfl_sync(0xffffffffu, ent, next < t.sinkp ? next : next + t.gap);
+            if (page < 0 || page >= a.num_blocks) page = 0;  // a malformed table reads block 0, never out of range
+            if (lane == 0) {
+                const uint32_t at = bar + 8 * (asked % RING);
+                mbar_expect_tx(at, C::PAGE);
+                tma_load_5d(ring + (asked % RING) * C::PAGE, &kvmap, 0, kvh * 16, 0, 0, page, at);
+            }
+            ++asked;
+            next += kShortWarps;
+        };
+        for (int i = 0; i < RING; ++i) load();
+        FewWork<HD, NT, ACC> f;
+        f.begin(a, t, kvh);
+        for (int v = warp; v < t.np && ok; v += kShortWarps) {
+            const int at = done % RING;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
+            f.page(a, ring + at * C::PAGE, 16 * (v < t.sinkp ? v : v + t.gap));
+            ++done;
+            __syncwarp();  // the page has been read
+            load();
+        }
+        if (!ok) {
+            if (lane == 0) record_timeout(a.status, 42);
+            // the copies in flight land before anything else is done with their places
+            for (int c = done; c < asked; ++c) (void)mbar_wait(bar + 8 * (c % RING), (uint32_t)(c / RING) & 1u);
+            done = asked;
+        }
+        // this warp's part, over its ring
+        const bool bad = __any_sync(0xffffffffu, f.bad);
+        float* mine = reinterpret_cast<float*>(base + warp * RING * C::PAGE);
+        bool wild = bad;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = f.l[n][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int row = 8 * n + 2 * t4 + e;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float y = f.o[k][n][e + 2 * h];
+                        wild |= !(fabsf(y) < INFINITY);
+                        mine[row * HD + 16 * k + 8 * h + g] = y;
+                    }
+                wild = __any_sync(0xffffffffu, wild);
+                if (g == 0) pml[warp * 8 * NT + row] = make_float2(f.m[n][e], wild ? -sum : sum);
+            }
+        __syncthreads();
+        // rows of the tile, a warp for each in turn
+        for (int row = warp; row < rows; row += kShortWarps) {
+            const int tok = row / a.G, head = kvh * a.G + row - tok * a.G, r = t.row + tok;
+            float M = -INFINITY, l = 0.f, y[W] = {};
+            bool look = false;
+#pragma unroll
+            for (int q = 0; q < kShortWarps; ++q) M = few_max(M, pml[q * 8 * NT + row].x);
+#pragma unroll
+            for (int q = 0; q < kShortWarps; ++q) {
+                const float2 ml = pml[q * 8 * NT + row];
+                look |= !(ml.y >= 0.f);
+                const float w = exp2f(ml.x - M);
+                if (w == 0.f) continue;  // a part without weight may hold anything
+                l += w * fabsf(ml.y);
+                const float* src = own_o + q * (RING * C::PAGE / 4) + row * HD + lane * W;
+#pragma unroll
+                for (int e = 0; e < W; ++e) y[e] += w * src[e];
+            }
+            const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+            __half* dst = a.out + (size_t)r * a.ldo + (size_t)head * HD;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const float x = y[e] * inv;
+                look |= !(fabsf(x) < INFINITY);
+                dst[lane * W + e] = __float2half_rn(x == x ? fminf(fmaxf(x, -kFewMax), kFewMax) : x);
+            }
+            if (ACC && lane == 0) lse[row] = make_float2(M, inv);
+            if (__any_sync(0xffffffffu, look) && l == l) {
+                __syncwarp();
+                few_nonfinite<HD>(a, b, t.p0 + tok, kvh, dst);
+            }
+        }
+        fence_async_smem();  // the rings were written and read here: the next tile's loads come behind it
+        __syncthreads();
+        if constexpr (ACC) {
+            float* weights = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
+            const int end = min(t.p0 + t.tokens, a.slots_max);
+            for (int j = threadIdx.x; j < end; j += 32 * kShortWarps) {
+                float sum = 0.f;
+                for (int row = max(0, j - t.p0) * a.G; row < rows; ++row) {
+                    const float2 y = lse[row];
+                    sum += few_exp2(f.score_at(a, row)[(size_t)j * a.G] - y.x) * y.y;
+                }
+                weights[j] += sum;
+            }
+        }
     }
 }
 
@@ -1063,6 +1233,16 @@ static const void* few_fn(int HD, int NT, bool acc) {
     return acc ? FEW_NT(64, true) : FEW_NT(64, false);
 #undef FEW_NT
 }
+static const void* short_fn(int HD, int NT, bool acc) {
+#define SHORT_NT(hd, ac) (NT == 1 ? (const void*)short_rows_kernel<hd, 1, ac> : (const void*)short_rows_kernel<hd, 2, ac>)
+    if (HD == 128) return acc ? SHORT_NT(128, true) : SHORT_NT(128, false);
+    return acc ? SHORT_NT(64, true) : SHORT_NT(64, false);
+#undef SHORT_NT
+}
+static size_t short_smem(int HD, int NT) {
+    return HD == 128 ? (NT == 1 ? ShortCfg<128, 1>::smem : ShortCfg<128, 2>::smem)
+                     : (NT == 1 ? ShortCfg<64, 1>::smem : ShortCfg<64, 2>::smem);
+}
 static int few_sms(int* out) {  // SMs of the current device; sets the kernels' shared memory on it once
     static std::atomic<int> facts[64];
     int dev = 0;
@@ -1070,6 +1250,11 @@ static int few_sms(int* out) {  // SMs of the current device; sets the kernels' 
     SD_CHECK(dev >= 0 && dev < 64, SPECDEC_ENOTSUP, "attention: device index above 63");
     int n = facts[dev].load();
     if (!n) {
+        for (int nt = 1; nt <= 2; ++nt)
+            for (int acc = 0; acc < 2; ++acc)
+                for (int hd = 64; hd <= 128; hd += 64)
+                    SD_CUDA(cudaFuncSetAttribute(short_fn(hd, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)short_smem(hd, nt)));
         for (int nt = 1; nt <= 4; ++nt)
             for (int acc = 0; acc < 2; ++acc) {
                 SD_CUDA(cudaFuncSetAttribute(few_fn(128, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1144,6 +1329,12 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     a.waves = few_waves(NT);
     CUtensorMap map;
     if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 2))) return rc;
+    if (NT <= 2 && a.max_blocks <= kShortPages && a.Hkv <= 65535) {
+        void* args[] = {&map, &a};
+        SD_CUDA(cudaLaunchKernel(short_fn(HD, NT, acc), dim3((unsigned)a.Hkv, (unsigned)a.B), dim3(32 * kShortWarps), args,
+                                 short_smem(HD, NT), s));
+        return SPECDEC_OK;
+    }
     const size_t smem = HD == 128 ? (NT == 1 ? FewCfg<128, 1>::smem(a.B) : FewCfg<128, 2>::smem(a.B))
                                   : (NT == 1 ? FewCfg<64, 1>::smem(a.B) : FewCfg<64, 2>::smem(a.B));
     void* args[] = {&map, &a};
