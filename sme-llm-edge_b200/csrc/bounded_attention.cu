@@ -69,11 +69,13 @@ struct FewArgs {
     __half* out;
     int ldo;
     float scale_log2;
-    int ctas, waves;    // CTAs of a wave
+    int ctas, waves;    // CTAs of a wave (ranges)
+    int chunk, chunks;  // pages of a piece, pieces of a table at most (chunk 0: ranges)
     // workspace
     long long* pre;     // [B + 1] pages before sequence b
     int32_t* np;        // [B] pages of each (tile, head) of sequence b
-    int32_t* chunks;    // [B + 1] chunks of slots before sequence b (weights)
+    int32_t* runs;      // [B + 1] runs of 128 slots before sequence b (weights)
+    // ranges; or [T][Hq][chunks] and [T][Hq][chunks][hd]
     float2* pml;        // [ranges][2][rows] m, l of a piece (l < 0: it met an infinity or NaN of V): of the range's
     float* po;          // [ranges][2][rows][hd]  first pages, or of later ones
     float2* ml;         // [T][Hq] m, 1 / l (weights)
@@ -280,7 +282,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
             a.pre[b] = before;
             a.np[b] = seqs[b].np;
             if (acc) {
-                a.chunks[b] = cbefore;
+                a.runs[b] = cbefore;
                 if (all > 0) cbefore += a.Hkv * ((seqs[b].np + 7) / 8);
             }
         }
@@ -290,7 +292,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
         pre[a.B] = total;
         if (LEAVE && blockIdx.x == 0) {
             a.pre[a.B] = total;
-            if (acc) a.chunks[a.B] = ctotal;
+            if (acc) a.runs[a.B] = ctotal;
         }
     }
     __syncthreads();
@@ -644,37 +646,44 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
     }
 }
 
-// Short tables: a CTA for each sequence and KV head, whose eight warps take its pages
-// in turn and join what they have in shared memory: one launch, where latency is all
-// there is.  With weights, the CTA adds them up from the scores that its warps left.
-constexpr int kShortWarps = 8, kShortPages = 32;  // table entries at most
+// Chunks: a CTA for each sequence, KV head and run of `chunk` pages, whose warps take
+// the pages in turn and join what they have in shared memory.  Where the run is all
+// there is the result is final, and the CTA adds up its slots' weights too: one
+// launch for short tables.  CTAs come to the SMs as these are free, which evens out
+// both ragged lengths and the SMs' shares of the memory's rate (64 single tokens on
+// 2000: 88 us, ranges 101).
+constexpr int kChunkMost = 128, kChunkLeast = 64;  // pages (four table entries of a lane)
+constexpr int kChunkCtas = 4096;                   // of a call at most
 
-template <int HD, int NT>
-struct ShortCfg {
+template <int HD, int WARPS>
+struct ChunkCfg {
     static constexpr int PAGE = 64 * HD, RING = HD == 128 ? 2 : 4;  // a warp's ring holds its rows' O afterwards
-    static constexpr size_t smem = 1024 + (size_t)kShortWarps * RING * (PAGE + 8) + (size_t)kShortWarps * 8 * NT * 8 + 8 * NT * 8;
-    static_assert(RING * PAGE >= 8 * NT * HD * 4, "a warp's O");
+    static constexpr size_t smem(int NT) {
+        return 1024 + (size_t)WARPS * RING * (PAGE + 8) + (size_t)WARPS * 8 * NT * 8 + 8 * NT * 8;
+    }
+    static_assert(RING * PAGE >= kFewMaxRows * HD * 4, "a warp's O");
 };
 
-template <int HD, int NT, bool ACC>
-__global__ void __launch_bounds__(32 * kShortWarps, 1)
-    short_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
-    using C = ShortCfg<HD, NT>;
+template <int HD, int NT, bool ACC, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : NT == 1 ? 3 : 2)
+    chunk_rows_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ FewArgs a) {
+    using C = ChunkCfg<HD, WARPS>;
     constexpr int KS = HD / 16, RING = C::RING, W = HD / 32;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + kShortWarps * RING * C::PAGE);
-    float2* pml = reinterpret_cast<float2*>(bars + kShortWarps * RING);  // [warp][row] m, l (l < 0: look V up again)
-    float2* lse = pml + kShortWarps * 8 * NT;                            // [row] m, 1 / l
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + WARPS * RING * C::PAGE);
+    float2* pml = reinterpret_cast<float2*>(bars + WARPS * RING);  // [warp][row] m, l (l < 0: look V up again)
+    float2* lse = pml + WARPS * 8 * NT;                            // [row] m, 1 / l
     pdl_trigger();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int g = lane >> 2, t4 = lane & 3;
-    const int b = blockIdx.y, kvh = blockIdx.x;
+    const int kvh = blockIdx.x, b = blockIdx.y, v0 = blockIdx.z * a.chunk;
     const uint32_t ring = s_addr(base + warp * RING * C::PAGE), bar = s_addr(bars + warp * RING);
     const float* own_o = reinterpret_cast<const float*>(base);
-    const int ent = a.max_blocks > lane ? a.tables[(size_t)b * a.max_blocks + lane] : 0;  // (32 entries at most)
     const FewSeq s = few_seq(a, b);
+    if (s.n == 0 || (v0 > 0 && v0 >= few_pages(a, s))) return;
+    const bool all = (min(s.ctx + s.n, a.slots_max) + 15) >> 4 <= a.chunk;  // no tile of the sequence has another piece
     if (lane == 0) {
         for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -685,11 +694,22 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
     const int tiles = (s.n + a.tpt - 1) / a.tpt;
     for (int tile = 0; tile < tiles; ++tile) {
         const FewTile t = few_tile(a, s, tile);
-        const int rows = t.tokens * a.G;
-        int next = warp;  // page to ask for
+        if (v0 > 0 && v0 >= t.np) continue;  // (the same for all)
+        const int rows = t.tokens * a.G, ve = min(t.np, v0 + a.chunk);
+        const bool whole = v0 == 0 && t.np <= a.chunk;
+        int ent[kChunkMost / 32];
+#pragma unroll
+        for (int i = 0; i < kChunkMost / 32; ++i) {
+            const int v = v0 + 32 * i + lane;
+            ent[i] = v < ve ? a.tables[(size_t)b * a.max_blocks + (v < t.sinkp ? v : v + t.gap)] : 0;
+        }
+        int next = v0 + warp;  // page to ask for
         auto load = [&]() {
-            if (next >= t.np) return;
-            int page = __shfl_sync(0xffffffffu, ent, next < t.sinkp ? next : next + t.gap);
+            if (next >= ve) return;
+            int page = ent[0];
+#pragma unroll
+            for (int i = 1; i < kChunkMost / 32; ++i) page = (next - v0) >> 5 == i ? ent[i] : page;
+            page = __shfl_sync(0xffffffffu, page, (next - v0) & 31);
             if (page < 0 || page >= a.num_blocks) page = 0;  // a malformed table reads block 0, never out of range
             if (lane == 0) {
                 const uint32_t at = bar + 8 * (asked % RING);
@@ -697,12 +717,12 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
                 tma_load_5d(ring + (asked % RING) * C::PAGE, &kvmap, 0, kvh * 16, 0, 0, page, at);
             }
             ++asked;
-            next += kShortWarps;
+            next += WARPS;
         };
         for (int i = 0; i < RING; ++i) load();
         FewWork<HD, NT, ACC> f;
         f.begin(a, t, kvh);
-        for (int v = warp; v < t.np && ok; v += kShortWarps) {
+        for (int v = v0 + warp; v < ve && ok; v += WARPS) {
             const int at = done % RING;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
             f.page(a, ring + at * C::PAGE, 16 * (v < t.sinkp ? v : v + t.gap));
@@ -717,9 +737,8 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
             done = asked;
         }
         // this warp's part, over its ring
-        const bool bad = __any_sync(0xffffffffu, f.bad);
         float* mine = reinterpret_cast<float*>(base + warp * RING * C::PAGE);
-        bool wild = bad;
+        bool wild = f.bad;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -741,14 +760,14 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
             }
         __syncthreads();
         // rows of the tile, a warp for each in turn
-        for (int row = warp; row < rows; row += kShortWarps) {
+        for (int row = warp; row < rows; row += WARPS) {
             const int tok = row / a.G, head = kvh * a.G + row - tok * a.G, r = t.row + tok;
             float M = -INFINITY, l = 0.f, y[W] = {};
             bool look = false;
 #pragma unroll
-            for (int q = 0; q < kShortWarps; ++q) M = few_max(M, pml[q * 8 * NT + row].x);
+            for (int q = 0; q < WARPS; ++q) M = few_max(M, pml[q * 8 * NT + row].x);
 #pragma unroll
-            for (int q = 0; q < kShortWarps; ++q) {
+            for (int q = 0; q < WARPS; ++q) {
                 const float2 ml = pml[q * 8 * NT + row];
                 look |= !(ml.y >= 0.f);
                 const float w = exp2f(ml.x - M);
@@ -758,6 +777,13 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
 #pragma unroll
                 for (int e = 0; e < W; ++e) y[e] += w * src[e];
             }
+            if (!whole) {
+                const size_t at = ((size_t)r * a.Hq + head) * a.chunks + blockIdx.z;
+#pragma unroll
+                for (int e = 0; e < W; ++e) a.po[at * HD + lane * W + e] = y[e];
+                if (lane == 0) a.pml[at] = make_float2(M, look ? -l : l);
+                continue;
+            }
             const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
             __half* dst = a.out + (size_t)r * a.ldo + (size_t)head * HD;
 #pragma unroll
@@ -766,7 +792,10 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
                 look |= !(fabsf(x) < INFINITY);
                 dst[lane * W + e] = __float2half_rn(x == x ? fminf(fmaxf(x, -kFewMax), kFewMax) : x);
             }
-            if (ACC && lane == 0) lse[row] = make_float2(M, inv);
+            if (ACC && lane == 0) {
+                lse[row] = make_float2(M, inv);
+                if (!all) a.ml[(size_t)r * a.Hq + head] = make_float2(M, inv);
+            }
             if (__any_sync(0xffffffffu, look) && l == l) {
                 __syncwarp();
                 few_nonfinite<HD>(a, b, t.p0 + tok, kvh, dst);
@@ -775,15 +804,18 @@ __global__ void __launch_bounds__(32 * kShortWarps, 1)
         fence_async_smem();  // the rings were written and read here: the next tile's loads come behind it
         __syncthreads();
         if constexpr (ACC) {
-            float* weights = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
-            const int end = min(t.p0 + t.tokens, a.slots_max);
-            for (int j = threadIdx.x; j < end; j += 32 * kShortWarps) {
-                float sum = 0.f;
-                for (int row = max(0, j - t.p0) * a.G; row < rows; ++row) {
-                    const float2 y = lse[row];
-                    sum += few_exp2(f.score_at(a, row)[(size_t)j * a.G] - y.x) * y.y;
+            if (all) {
+                float* weights = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
+                const int end = min(t.p0 + t.tokens, a.slots_max);
+                for (int j = threadIdx.x; j < end; j += 32 * WARPS) {
+                    float sum = 0.f;
+                    const float was = weights[j];
+                    for (int row = max(0, j - t.p0) * a.G; row < rows; ++row) {
+                        const float2 y = lse[row];
+                        sum += few_exp2(f.score_at(a, row)[(size_t)j * a.G] - y.x) * y.y;
+                    }
+                    weights[j] = was + sum;
                 }
-                weights[j] += sum;
             }
         }
     }
@@ -812,7 +844,8 @@ __global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_cons
     };
     auto find = [&](long long idx) {
         Row x;
-        x.n = x.np = 0;
+        x.n = x.np = x.r0 = 0;
+        x.u0 = 0;
         if (idx >= rows) return x;
         const int r = (int)(idx / a.Hq), head = (int)(idx - (long long)r * a.Hq);
         int lo = 0, hi = a.B;  // first sequence whose end is past the row
@@ -837,9 +870,13 @@ __global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_cons
     };
     Row mine = find(first + (ROWS == 1 ? 0 : warp));
     pdl_wait();
-    const FewCut cut(a, a.pre[a.B]);
+    const FewCut cut(a, a.chunk ? 0 : a.pre[a.B]);
     auto count = [&](Row& x) {  // its pieces
         if (x.np <= 0) return;
+        if (a.chunk) {
+            x.n = (x.np + a.chunk - 1) / a.chunk;
+            return;
+        }
         x.u0 = a.pre[x.b] + ((long long)x.tile * a.Hkv + x.kvh) * a.np[x.b];
         x.r0 = cut.of(x.u0);
         x.n = cut.of(x.u0 + x.np - 1) - x.r0 + 1;
@@ -861,7 +898,9 @@ __global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_cons
             for (int u = 0; u < P; ++u) {
                 const bool real = k + u * step < x.n;
                 const int range = x.r0 + k + u * step;
-                const size_t at = real ? (size_t)(2 * range + (x.u0 > cut.begin(range) ? 1 : 0)) * tile_rows + x.row : 0;
+                size_t at = 0;
+                if (real) at = a.chunk ? x.at * a.chunks + k + u * step
+                                       : (size_t)(2 * range + (x.u0 > cut.begin(range) ? 1 : 0)) * tile_rows + x.row;
                 ml[u] = real ? a.pml[at] : make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[u][e] = real ? a.po[at * HD + lane * W + e] : 0.f;
@@ -948,21 +987,33 @@ __global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_cons
 // slots of a head, four a lane; V heads' scores in one load.
 template <int V>
 __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant__ FewArgs a) {
-    extern __shared__ int chunks[];
+    extern __shared__ int runs[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (a.chunk) {  // blocks (1024 slots, KV head, sequence)
+        const FewSeq s = few_seq(a, blockIdx.z);
+        const int end = min(s.ctx + s.n, a.slots_max);
+        if (s.n == 0 || (end + 15) >> 4 <= a.chunk || 1024 * (int)blockIdx.x >= end) return;  // (a CTA has added up its own)
+    }
     pdl_wait();
-    for (int b = threadIdx.x; b <= a.B; b += 256) chunks[b] = a.chunks[b];
-    __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, total = chunks[a.B];
+    if (!a.chunk) {
+        for (int b = threadIdx.x; b <= a.B; b += 256) runs[b] = a.runs[b];
+        __syncthreads();
+    }
+    const int total = a.chunk ? 8 * (int)(blockIdx.x + 1) : runs[a.B];
     for (int c = blockIdx.x * 8 + warp; c < total; c += gridDim.x * 8) {
-        int lo = 0, hi = a.B;
+        int lo = a.chunk ? (int)blockIdx.z : 0, hi = a.chunk ? lo : a.B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (chunks[mid] <= c) lo = mid;
+            if (runs[mid] <= c) lo = mid;
             else hi = mid;
         }
         const FewSeq s = few_seq(a, lo);
-        const int per_head = (chunks[lo + 1] - chunks[lo]) / a.Hkv, local = c - chunks[lo];
-        const int kvh = local / per_head, j0 = 128 * (local - kvh * per_head);
+        int kvh = blockIdx.y, j0 = 128 * c;
+        if (!a.chunk) {
+            const int per_head = (runs[lo + 1] - runs[lo]) / a.Hkv, local = c - runs[lo];
+            kvh = local / per_head;
+            j0 = 128 * (local - kvh * per_head);
+        }
         const int end = min(min(s.ctx + s.n, a.slots_max), j0 + 128);
         float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
         float sum[4] = {}, was[4] = {};
@@ -1188,6 +1239,20 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
 // ------------------------------------------------------------------ host side
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Pages of a run and runs of a table where every run has a CTA; 0 pages where too
+// many of them might be empty (tables far wider than most sequences): ranges, which
+// are cut by the lengths in device memory.
+struct FewChunks {
+    int pages, count;
+};
+static FewChunks few_chunks(int B, int Hkv, int max_blocks) {
+    const long long pairs = (long long)B * Hkv, all = pairs * max_blocks;
+    // whole tables where they are short; else runs for two CTAs of each SM
+    const int pages = (int)std::min<long long>(kChunkMost, std::max<long long>(kChunkLeast, (all + 2 * kFewMaxSms - 1) / (2 * kFewMaxSms)));
+    const int count = (max_blocks + pages - 1) / pages;
+    if (pairs * count > kChunkCtas || B > 65535 || count > 65535) return {0, 0};
+    return {pages, count};
+}
 // CTAs of a wave: no more than there can be ranges.
 static int few_ctas(int sms, int NT, int T, int Hkv, int max_blocks) {
     const long long ranges = ((long long)T * Hkv * max_blocks + kFewMinPages - 1) / kFewMinPages;
@@ -1195,7 +1260,7 @@ static int few_ctas(int sms, int NT, int T, int Hkv, int max_blocks) {
 }
 // Sizes that do not fall where B, T or max_blocks grows.
 struct FewSpace {
-    size_t pre, np, chunks, pml, po, ml, scores, bytes;  // offsets, and all
+    size_t pre, np, runs, pml, po, ml, scores, bytes;  // offsets, and all
 };
 static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks, bool acc) {
     FewSpace s = {};
@@ -1204,7 +1269,9 @@ static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks,
     long long most = 0;
     for (int nt = 1; nt <= 4; ++nt)
         most = std::max(most, 2LL * few_waves(nt) * few_ctas(kFewMaxSms, nt, T, Hkv, max_blocks) * kFewWarps * std::min<long long>(8 * nt, rows));
-    const size_t pieces = (size_t)most;
+    // or one for each run of a row and head: calls of few rows have at most kFewMaxRows rows for each of a sequence's heads' runs
+    const long long runs = std::min<long long>((long long)T * Hq * ((max_blocks + kChunkLeast - 1) / kChunkLeast), (long long)kFewMaxRows * kChunkCtas);
+    const size_t pieces = (size_t)std::max(most, runs);
     size_t at = 0;
     auto room = [&](size_t n) {
         const size_t here = at;
@@ -1213,7 +1280,7 @@ static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks,
     };
     s.pre = room((size_t)(B + 1) * 8);
     s.np = room((size_t)B * 4);
-    s.chunks = room((size_t)(B + 1) * 4);
+    s.runs = room((size_t)(B + 1) * 4);
     s.pml = room(pieces * sizeof(float2));
     s.po = room(pieces * HD * sizeof(float));
     if (acc) {
@@ -1233,15 +1300,21 @@ static const void* few_fn(int HD, int NT, bool acc) {
     return acc ? FEW_NT(64, true) : FEW_NT(64, false);
 #undef FEW_NT
 }
-static const void* short_fn(int HD, int NT, bool acc) {
-#define SHORT_NT(hd, ac) (NT == 1 ? (const void*)short_rows_kernel<hd, 1, ac> : (const void*)short_rows_kernel<hd, 2, ac>)
-    if (HD == 128) return acc ? SHORT_NT(128, true) : SHORT_NT(128, false);
-    return acc ? SHORT_NT(64, true) : SHORT_NT(64, false);
-#undef SHORT_NT
+template <int HD, bool ACC, int WARPS>
+static const void* chunk_nt(int NT) {
+    return NT == 1 ? (const void*)chunk_rows_kernel<HD, 1, ACC, WARPS>
+           : NT == 2 ? (const void*)chunk_rows_kernel<HD, 2, ACC, WARPS>
+           : NT == 3 ? (const void*)chunk_rows_kernel<HD, 3, ACC, WARPS> : (const void*)chunk_rows_kernel<HD, 4, ACC, WARPS>;
 }
-static size_t short_smem(int HD, int NT) {
-    return HD == 128 ? (NT == 1 ? ShortCfg<128, 1>::smem : ShortCfg<128, 2>::smem)
-                     : (NT == 1 ? ShortCfg<64, 1>::smem : ShortCfg<64, 2>::smem);
+static const void* chunk_fn(int HD, int NT, bool acc, int warps) {
+    if (HD == 128) return warps == 8 ? (acc ? chunk_nt<128, true, 8>(NT) : chunk_nt<128, false, 8>(NT))
+                                     : (acc ? chunk_nt<128, true, 4>(NT) : chunk_nt<128, false, 4>(NT));
+    return warps == 8 ? (acc ? chunk_nt<64, true, 8>(NT) : chunk_nt<64, false, 8>(NT))
+                      : (acc ? chunk_nt<64, true, 4>(NT) : chunk_nt<64, false, 4>(NT));
+}
+static size_t chunk_smem(int HD, int NT, int warps) {
+    return HD == 128 ? (warps == 8 ? ChunkCfg<128, 8>::smem(NT) : ChunkCfg<128, 4>::smem(NT))
+                     : (warps == 8 ? ChunkCfg<64, 8>::smem(NT) : ChunkCfg<64, 4>::smem(NT));
 }
 static int few_sms(int* out) {  // SMs of the current device; sets the kernels' shared memory on it once
     static std::atomic<int> facts[64];
@@ -1250,11 +1323,11 @@ static int few_sms(int* out) {  // SMs of the current device; sets the kernels' 
     SD_CHECK(dev >= 0 && dev < 64, SPECDEC_ENOTSUP, "attention: device index above 63");
     int n = facts[dev].load();
     if (!n) {
-        for (int nt = 1; nt <= 2; ++nt)
-            for (int acc = 0; acc < 2; ++acc)
-                for (int hd = 64; hd <= 128; hd += 64)
-                    SD_CUDA(cudaFuncSetAttribute(short_fn(hd, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)short_smem(hd, nt)));
+        for (int i = 0; i < 32; ++i) {
+            const int hd = i & 1 ? 128 : 64, warps = i & 2 ? 8 : 4, acc = i >> 2 & 1, nt = (i >> 3) + 1;
+            SD_CUDA(cudaFuncSetAttribute(chunk_fn(hd, nt, acc, warps), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)chunk_smem(hd, nt, warps)));
+        }
         for (int nt = 1; nt <= 4; ++nt)
             for (int acc = 0; acc < 2; ++acc) {
                 SD_CUDA(cudaFuncSetAttribute(few_fn(128, nt, acc), cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1313,7 +1386,7 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     char* w = static_cast<char*>(ws);
     a.pre = reinterpret_cast<long long*>(w + sp.pre);
     a.np = reinterpret_cast<int32_t*>(w + sp.np);
-    a.chunks = reinterpret_cast<int32_t*>(w + sp.chunks);
+    a.runs = reinterpret_cast<int32_t*>(w + sp.runs);
     a.pml = reinterpret_cast<float2*>(w + sp.pml);
     a.po = reinterpret_cast<float*>(w + sp.po);
     a.ml = acc ? reinterpret_cast<float2*>(w + sp.ml) : nullptr;
@@ -1329,16 +1402,21 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     a.waves = few_waves(NT);
     CUtensorMap map;
     if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 2))) return rc;
-    if (NT <= 2 && a.max_blocks <= kShortPages && a.Hkv <= 65535) {
-        void* args[] = {&map, &a};
-        SD_CUDA(cudaLaunchKernel(short_fn(HD, NT, acc), dim3((unsigned)a.Hkv, (unsigned)a.B), dim3(32 * kShortWarps), args,
-                                 short_smem(HD, NT), s));
-        return SPECDEC_OK;
-    }
-    const size_t smem = HD == 128 ? (NT == 1 ? FewCfg<128, 1>::smem(a.B) : FewCfg<128, 2>::smem(a.B))
+    const size_t few_smem = HD == 128 ? (NT == 1 ? FewCfg<128, 1>::smem(a.B) : FewCfg<128, 2>::smem(a.B))
                                   : (NT == 1 ? FewCfg<64, 1>::smem(a.B) : FewCfg<64, 2>::smem(a.B));
+    const FewChunks ch = few_chunks(a.B, a.Hkv, a.max_blocks);
+    a.chunk = ch.pages;
+    a.chunks = ch.count;
     void* args[] = {&map, &a};
-    SD_CUDA(cudaLaunchKernel(few_fn(HD, NT, acc), dim3((unsigned)(a.ctas * a.waves)), dim3(32 * kFewWarps), args, smem, s));
+    if (a.chunk) {
+        // (eight warps on a run where CTAs are few)
+        const int warps = (long long)a.B * a.Hkv * a.chunks <= sms ? 8 : 4;
+        SD_CUDA(cudaLaunchKernel(chunk_fn(HD, NT, acc, warps), dim3((unsigned)a.Hkv, (unsigned)a.B, (unsigned)a.chunks),
+                                 dim3(32 * warps), args, chunk_smem(HD, NT, warps), s));
+        if (a.chunks == 1) return SPECDEC_OK;
+    } else {
+        SD_CUDA(cudaLaunchKernel(few_fn(HD, NT, acc), dim3((unsigned)(a.ctas * a.waves)), dim3(32 * kFewWarps), args, few_smem, s));
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -1355,10 +1433,11 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
                   : (kind == 0 ? few_merge_kernel<64, 1, 16> : kind == 1 ? few_merge_kernel<64, 1, 4> : few_merge_kernel<64, 4, 4>);
     SD_CUDA(cudaLaunchKernelEx(&cfg, merge, a, 8 * NT));
     if (acc) {
-        const long long chunks = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
-        cfg.gridDim = dim3((unsigned)std::min<long long>((chunks + 7) / 8, 8LL * sms));
+        const long long runs = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
+        cfg.gridDim = a.chunk ? dim3((unsigned)((a.max_blocks + 63) / 64), (unsigned)a.Hkv, (unsigned)a.B)
+                              : dim3((unsigned)std::min<long long>((runs + 7) / 8, 8LL * sms));
         cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = (size_t)(a.B + 1) * 4;
+        cfg.dynamicSmemBytes = a.chunk ? 0 : (size_t)(a.B + 1) * 4;
         const auto weigh = a.G % 4 == 0 ? few_weights_kernel<4> : (a.G % 2 == 0 ? few_weights_kernel<2> : few_weights_kernel<1>);
         SD_CUDA(cudaLaunchKernelEx(&cfg, weigh, a));
     }
