@@ -807,14 +807,44 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : NT == 1 ? 3 : 2)
             if (all) {
                 float* weights = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
                 const int end = min(t.p0 + t.tokens, a.slots_max);
-                for (int j = threadIdx.x; j < end; j += 32 * WARPS) {
-                    float sum = 0.f;
-                    const float was = weights[j];
-                    for (int row = max(0, j - t.p0) * a.G; row < rows; ++row) {
-                        const float2 y = lse[row];
-                        sum += few_exp2(f.score_at(a, row)[(size_t)j * a.G] - y.x) * y.y;
+                // four slots of a thread at a time, so that their loads are out together
+                for (int j0 = threadIdx.x; j0 < end; j0 += 4 * 32 * WARPS) {
+                    float sum[4] = {}, was[4] = {};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j0 + 32 * WARPS * u < end) was[u] = weights[j0 + 32 * WARPS * u];
+                    for (int tok = max(0, j0 - t.p0); tok < t.tokens; ++tok) {
+                        const float* src = f.score_at(a, tok * a.G);
+                        const float2* y = lse + tok * a.G;
+                        const int last = min(t.p0 + tok, end - 1);
+                        if ((a.G & 3) == 0) {
+                            for (int h = 0; h < a.G; h += 4) {
+                                float4 x[4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (j0 + 32 * WARPS * u <= last)
+                                        x[u] = *reinterpret_cast<const float4*>(src + (size_t)(j0 + 32 * WARPS * u) * a.G + h);
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (j0 + 32 * WARPS * u <= last)
+                                        sum[u] += few_exp2(x[u].x - y[h].x) * y[h].y + few_exp2(x[u].y - y[h + 1].x) * y[h + 1].y +
+                                                  few_exp2(x[u].z - y[h + 2].x) * y[h + 2].y + few_exp2(x[u].w - y[h + 3].x) * y[h + 3].y;
+                            }
+                        } else {
+                            for (int h = 0; h < a.G; ++h) {
+                                float x[4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (j0 + 32 * WARPS * u <= last) x[u] = src[(size_t)(j0 + 32 * WARPS * u) * a.G + h];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (j0 + 32 * WARPS * u <= last) sum[u] += few_exp2(x[u] - y[h].x) * y[h].y;
+                            }
+                        }
                     }
-                    weights[j] = was + sum;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j0 + 32 * WARPS * u < end) weights[j0 + 32 * WARPS * u] = was[u] + sum[u];
                 }
             }
         }
