@@ -13,6 +13,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace specdec {
 
@@ -229,7 +230,6 @@ static_assert(FewCfg<64, 2>::smem(kBoundMaxSeqs) <= 232448, "shared memory of a 
 // Pages before each sequence, by every CTA for itself from the lengths in device
 // memory (so a captured call serves other lengths); CTA 0 leaves them for the
 // kernels that follow.
-template <bool LEAVE = true>
 __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, FewSeq* seqs, bool acc) {
     __shared__ long long wsum[kFewWarps];
     __shared__ int csum[kFewWarps];
@@ -278,7 +278,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     for (int b = b0; b < b1; ++b) {
         const long long all = pre[b];
         pre[b] = before;
-        if (LEAVE && blockIdx.x == 0) {
+        if (blockIdx.x == 0) {
             a.pre[b] = before;
             a.np[b] = seqs[b].np;
             if (acc) {
@@ -290,7 +290,7 @@ __device__ __forceinline__ long long few_plan(const FewArgs& a, long long* pre, 
     }
     if (tid == 0) {
         pre[a.B] = total;
-        if (LEAVE && blockIdx.x == 0) {
+        if (blockIdx.x == 0) {
             a.pre[a.B] = total;
             if (acc) a.runs[a.B] = ctotal;
         }
@@ -399,7 +399,7 @@ struct FewWork {
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] *= a.scale_log2;
+                s[n][e] = __fmul_rn(s[n][e], a.scale_log2);  // (rounded by itself: the largest less m is exact)
                 if (!clear) {
                     const int slot = s0 + g + 8 * (e >> 1), p = slot_of[n][e & 1];
                     if (!(slot <= p && (slot < a.sinks || slot > p - a.window))) s[n][e] = -INFINITY;
@@ -1092,177 +1092,207 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
 // ------------------------------------------------------------------ many rows
 //
 // weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
-// of 2^(x - m) / l, where the rows' (m, 1 / l) are known (the tensor-core kernel's):
+// of 2^(x - m) / l, where the rows' (m, 1 / l) are known (the packed-row kernel's):
 // the scores are computed again rather than kept, a read of K (256 bytes of a slot
-// and head of 128) against one write and one read of 4 bytes for each row.  A warp
-// streams K pages of its range past 64 rows at a time,
-//   S^T [16 keys][64 rows] = K Q^T in mma.sync, whose lanes hold a slot's scores of
-// 16 rows: the sum over rows is theirs and two shuffles'.
-constexpr int kWeighRows = 64, kWeighRing = 8192;  // bytes: 2 or 4 pages of a warp, twice
+// and head of 128) against one write and one read of 4 bytes for each row.
+//   S^T [128 slots][rows] = K Q^T by tcgen05.mma into tensor memory: a lane is a
+// slot, so a thread sums its slot's weights over up to 128 rows by itself.  That is
+// three instructions a score, half of what the memory takes for K at 64 rows
+// (mma.sync fragments, 16 slots a warp, took twice the instructions and 42 us where
+// this takes NOTE).  One CTA for a KV head and run of 1024 slots; warps:
+//   0-3  sums, 4  MMA issuer, 5  loads (a group's queries, 128-slot tiles of K)
+constexpr int kWeighTiles = 8, kWeighThreads = 192, kWeighTmem = 256;
 
 template <int HD>
 struct WeighCfg {
-    static constexpr int PAGE = 32 * HD;  // bytes of a page's K of a head
-    static constexpr int RING = 4 * kWeighRing / PAGE;
-    static constexpr size_t smem(int B) {
-        return 1024 + (size_t)kFewWarps * RING * (PAGE + 8) + (size_t)(B + 1) * 8 + (size_t)B * sizeof(FewSeq) + 16;
-    }
+    static constexpr int NH = HD / 64, TILE = NH * 16384, RING = HD == 128 ? 2 : 4;
+    static constexpr size_t smem = 1024 + (size_t)(1 + RING) * TILE + 128 * 8 + (2 * RING + 6) * 8 + 16;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(32 * kFewWarps, 2)
-    weigh_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kWeighThreads, 2)
+    weigh_rows_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ FewArgs a) {
     using C = WeighCfg<HD>;
-    constexpr int KS = HD / 16, RING = C::RING, NT = kWeighRows / 8;
+    constexpr int NH = C::NH, RING = C::RING;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + kFewWarps * RING * C::PAGE);
-    long long* pre = reinterpret_cast<long long*>(bars + kFewWarps * RING);
-    FewSeq* seqs = reinterpret_cast<FewSeq*>(pre + a.B + 1);
+    unsigned char* sQ = base;              // [NH][128 rows][128 B]
+    unsigned char* sK = base + C::TILE;    // [RING][NH][128 slots][128 B]
+    float2* lse = reinterpret_cast<float2*>(sK + RING * C::TILE);  // [row] m, 1 / l
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(lse + 128);
+    uint64_t* k_empty = k_full + RING;
+    uint64_t* q_full = k_empty + RING;
+    uint64_t* q_empty = q_full + 1;
+    uint64_t* s_full = q_empty + 1;  // [2] scores landed
+    uint64_t* s_free = s_full + 2;   // [2] scores read (4 warps)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_free + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const int g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring = s_addr(base + warp * RING * C::PAGE), bar = s_addr(bars + warp * RING);
-    if (lane == 0) {
-        for (int i = 0; i < RING; ++i) mbar_init(bar + 8 * i, 1);
+    const int kvh = blockIdx.x, b = blockIdx.y;
+    const FewSeq s = few_seq(a, b);
+    const int end = min(s.ctx + s.n, a.slots_max), tiles = (end + 127) >> 7, step = gridDim.z * kWeighTiles;
+    const int first_tile = blockIdx.z * kWeighTiles;
+    if (s.n == 0 || first_tile >= tiles) return;
+    const int tpt = 128 / a.G, groups = (s.n + tpt - 1) / tpt;  // tokens of a group of rows
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(s_addr(&k_full[i]), 1);
+            mbar_init(s_addr(&k_empty[i]), 1);
+        }
+        mbar_init(s_addr(q_full), 1);
+        mbar_init(s_addr(q_empty), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_addr(&s_full[i]), 1);
+            mbar_init(s_addr(&s_free[i]), 4);
+        }
+        *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const long long total = few_plan<false>(a, pre, seqs, false);  // ends with a CTA-wide barrier
-    const FewCut cut(a, total);
-    const int range = warp * a.ctas + blockIdx.x;
-    const long long u0 = cut.begin(range), u1 = cut.end(range);
-    if (u0 >= u1) return;
-    auto groups_of = [&](const FewWalk& w) { return (w.t.tokens * a.G + kWeighRows - 1) / kWeighRows; };
-
-    // ---- loads: a segment's pages once for each 64 of its rows
-    FewWalk ld = {};
-    ld.u = u0;
-    ld.hi = u1;
-    int asked = 0, tb = 0, ent = 0, ent_next = 0, v = 0, left = 0;  // left: groups of the segment still to load
-    bool more = true;
-    auto entry = [&](int i) -> int {
-        if (i >= ld.ve) return 0;
-        const int x = a.tables[(size_t)ld.b * a.max_blocks + i];
-        return x < 0 || x >= a.num_blocks ? 0 : x;  // a malformed table reads block 0, never out of range
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)),
+                     "r"(kWeighTmem));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    auto wait = [&](uint64_t* bar, int turn) -> bool {  // false: it ran out, here or in another role
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(s_addr(bar), (uint32_t)turn & 1u)) != 0;
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_timeout(a.status, 41);
+        }
+        return ok && !__any_sync(0xffffffffu, *abort_flag != 0);
     };
-    auto load = [&]() {
-        while (more && v >= ld.ve) {
-            if (--left <= 0) {
-                more = few_next(a, pre, seqs, ld);
-                if (!more) return;
-                left = ld.v < ld.ve ? groups_of(ld) : 0;
-            }
-            v = tb = left > 0 ? ld.v : ld.ve;
-            ent = entry(tb + lane);
-            ent_next = entry(tb + 32 + lane);
+    // every role goes through the groups, and in each through the CTA's tiles
+    if (warp == 5) {
+        int kc = 0, qc = 0;
+        bool ok = true;
+        for (int k = 0; ok && k < groups; ++k) {
+            for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
+                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile) {
+                    const int pages = min(8, ((end + 15) >> 4) - 8 * tile), at = kc % RING, turn = kc / RING;
+                    int page = 0;
+                    if (lane < pages * NH) page = a.tables[(size_t)b * a.max_blocks + 8 * tile + lane / NH];
+                    if (page < 0 || page >= a.num_blocks) page = 0;  // a malformed table reads block 0, never out of range
+                    if (turn && !(ok = wait(&k_empty[at], turn - 1))) break;
+                    if (lane == 0) mbar_expect_tx(s_addr(&k_full[at]), (uint32_t)(pages * NH * 2048));
+                    __syncwarp();
+                    if (lane < pages * NH)
+                        tma_load_5d(s_addr(sK + at * C::TILE + (lane % NH) * 16384 + (lane / NH) * 2048), &kmap, 0, kvh * 16,
+                                    lane % NH, 0, page, s_addr(&k_full[at]));
+                    ++kc;
+                    if (tile == first_tile) {  // the group's queries, behind its first keys
+                        if (k && !(ok = wait(q_empty, k - 1))) break;
+                        if (lane == 0) {
+                            mbar_expect_tx(s_addr(q_full), (uint32_t)(tpt * a.G * 128 * NH));
+                            for (int h = 0; h < NH; ++h)
+                                tma_load_4d(s_addr(sQ + h * 16384), &qmap, 0, h, kvh * a.G, s.lo + k * tpt, s_addr(q_full));
+                        }
+                        __syncwarp();
+                        ++qc;
+                    }
+                }
         }
-        if (!more) return;
-        if (v - tb >= 32) {
-            tb += 32;
-            ent = ent_next;
-            ent_next = entry(tb + 32 + lane);
+        // the copies in flight land before the CTA leaves
+        if (qc) (void)mbar_wait(s_addr(q_full), (uint32_t)(qc - 1) & 1u);
+        for (int c = max(0, kc - RING); c < kc; ++c) (void)mbar_wait(s_addr(&k_full[c % RING]), (uint32_t)(c / RING) & 1u);
+    } else if (warp == 4) {
+        const uint64_t qd = sw128_desc(s_addr(sQ)), kd0 = sw128_desc(s_addr(sK));
+        int kc = 0;
+        bool ok = true;
+        for (int k = 0; ok && k < groups; ++k) {
+            const int rows = min(tpt, s.n - k * tpt) * a.G;
+            const uint32_t idesc = idesc_f16(128, (rows + 15) & ~15);
+            ok = wait(q_full, k);
+            for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
+                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile, ++kc) {
+                    const int at = kc % RING, buf = kc & 1;
+                    if (!(ok = wait(&k_full[at], kc / RING))) break;
+                    if (kc >= 2 && !(ok = wait(&s_free[buf], (kc >> 1) - 1))) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint64_t kd = kd0 + (uint64_t)(at * (C::TILE >> 4));
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk)
+                            tc_mma_f16_ss(tmem + buf * 128, kd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                                          qd + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
+                        tc_commit(s_addr(&s_full[buf]));
+                        tc_commit(s_addr(&k_empty[at]));
+                        // (the group's last tile: commits cover all MMAs before them)
+                        if (tile + 1 >= min(tiles, t0 + kWeighTiles) && t0 + step >= tiles) tc_commit(s_addr(q_empty));
+                    }
+                    __syncwarp();
+                }
         }
-        const int page = __shfl_sync(0xffffffffu, ent, v - tb);
-        if (lane == 0) {
-            const uint32_t b = bar + 8 * (asked % RING);
-            mbar_expect_tx(b, C::PAGE);
-            tma_load_5d(ring + (asked % RING) * C::PAGE, &kmap, 0, ld.kvh * 16, 0, 0, page, b);
-        }
-        ++asked;
-        ++v;
-    };
-    for (int i = 0; i < RING; ++i) load();
-    pdl_wait();  // m and l of the rows
-
-    const uint32_t k_row = (uint32_t)(lane & 15), k_chunk = (uint32_t)(lane >> 4);
-    FewWalk w = {};
-    w.u = u0;
-    w.hi = u1;
-    int done = 0;
-    bool ok = true;
-    while (ok && few_next(a, pre, seqs, w)) {
-        if (w.v >= w.ve) continue;
-        const FewTile& t = w.t;
-        const int rows = t.tokens * a.G, groups = groups_of(w);
-        float* dst = a.weights + ((size_t)w.b * a.Hkv + w.kvh) * a.ldw;
-        for (int k0 = 0; ok && k0 < groups; ++k0) {
-            const int row0 = k0 * kWeighRows;
-            uint32_t qf[NT][KS][2];
-            float m[NT][2], inv[NT][2];
-            int slot_of[NT][2];  // -1: no row
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int row = row0 + 8 * n + g;
-                const bool real = row < rows;
-                const int tok = real ? row / a.G : 0;
-                const __half* src = a.q + (size_t)(t.row + tok) * a.ldq + (size_t)(w.kvh * a.G + (real ? row - tok * a.G : 0)) * HD + 2 * t4;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    qf[n][k][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-                    qf[n][k][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c = row0 + 8 * n + 2 * t4 + e, ct = c / a.G;
-                    slot_of[n][e] = c < rows ? t.p0 + ct : -1;
-                    const float2 y = c < rows ? __ldcg(a.ml + (size_t)(t.row + ct) * a.Hq + w.kvh * a.G + c - ct * a.G) : make_float2(0.f, 0.f);
-                    m[n][e] = y.x == -INFINITY ? 0.f : y.x;
-                    inv[n][e] = y.y;
-                }
+        // every MMA has finished with shared and tensor memory before the CTA leaves
+        if (kc > 0) (void)mbar_wait(s_addr(&s_full[(kc - 1) & 1]), (uint32_t)((kc - 1) >> 1) & 1u);
+        __syncwarp();
+    } else {
+        pdl_wait();  // m and l of the rows
+        const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+        float* weights = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
+        int kc = 0;
+        bool ok = true;
+        for (int k = 0; k < groups; ++k) {  // (all of them: the four warps meet at the barriers also where one gave up)
+            const int tokens = min(tpt, s.n - k * tpt), rows = tokens * a.G, p0 = s.ctx + k * tpt, p1 = p0 + tokens - 1;
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // the rows before have been read
+            {
+                const int c = threadIdx.x, tok = c / a.G;
+                float2 y = make_float2(0.f, 0.f);
+                if (c < rows) y = __ldcg(a.ml + (size_t)(s.lo + k * tpt + tok) * a.Hq + kvh * a.G + c - tok * a.G);
+                if (y.x == -INFINITY) y.x = 0.f;
+                lse[c] = y;
             }
-            const int first = t.p0 + row0 / a.G, last = t.p0 + (min(rows, row0 + kWeighRows) - 1) / a.G;  // slots of the group's rows
-            for (int i = w.v; i < w.ve; ++i) {
-                const int at = done % RING;
-                if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * at, (uint32_t)(done / RING) & 1u)))) break;
-                const uint32_t sk = ring + at * C::PAGE;
-                const int s0 = 16 * i;
-                // lanes t4 = 0, 1 keep slots g, g + 8 of the page
-                const int mine = s0 + g + 8 * t4;
-                const bool keeps = t4 < 2 && mine <= last && mine < a.slots_max;
-                const float was = keeps ? dst[mine] : 0.f;
-                float s[NT][4];
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
+                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile, ++kc) {
+                    const int buf = kc & 1, j = 128 * tile + threadIdx.x;
+                    const bool keeps = j <= p1 && j < end;
+                    const float was = keeps ? weights[j] : 0.f;
+                    const int from = max(0, j - p0) * a.G;  // the first row that sees this slot
+                    const bool clear = 128 * tile + 127 <= p0;
+                    if (!(ok = wait(&s_full[buf], kc >> 1))) break;
+                    tc_fence_after();
+                    float sum[4] = {};
+                    const bool here = 128 * tile + 32 * warp <= p1;  // some row sees a slot of this warp
+                    if (here) {
+                        for (int c0 = 0; c0 < rows; c0 += 32) {
+                            uint32_t v[32];
+                            __syncwarp();
+                            tc_ld_x32(t_lane + buf * 128 + c0, v);
+                            tc_wait_ld();
+                            if (clear && c0 + 32 <= rows) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                                for (int e = 0; e < 32; ++e) {
+                                    const float2 y = lse[c0 + e];
+                                    sum[e & 3] = fmaf(few_exp2(__fmul_rn(__uint_as_float(v[e]), a.scale_log2) - y.x), y.y, sum[e & 3]);
+                                }
+                            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    uint32_t x[4];
-                    few_ldm<false>(x, sk + (k >> 2) * 2048 + k_row * 128 + (((2 * (k & 3) + k_chunk) ^ (k_row & 7)) << 4));
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) few_mma(s[n], x, qf[n][k][0], qf[n][k][1]);
+                                for (int e = 0; e < 32; ++e) {
+                                    const float2 y = lse[c0 + e];
+                                    const float w = few_exp2(__fmul_rn(__uint_as_float(v[e]), a.scale_log2) - y.x) * y.y;
+                                    if (c0 + e >= from && c0 + e < rows) sum[e & 3] += w;
+                                }
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_addr(&s_free[buf]));
+                    if (keeps) weights[j] = was + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
                 }
-                ++done;
-                __syncwarp();  // the page has been read
-                load();
-                float sum[2] = {0.f, 0.f};
-                if (s0 + 15 <= first) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sum[e >> 1] = fmaf(few_exp2(s[n][e] * a.scale_log2 - m[n][e & 1]), inv[n][e & 1], sum[e >> 1]);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (s0 + g + 8 * (e >> 1) <= slot_of[n][e & 1])
-                                sum[e >> 1] = fmaf(few_exp2(s[n][e] * a.scale_log2 - m[n][e & 1]), inv[n][e & 1], sum[e >> 1]);
-                }
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], d);
-                    sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], d);
-                }
-                if (keeps) dst[mine] = was + (t4 ? sum[1] : sum[0]);
-            }
         }
     }
-    if (!ok) {
-        if (lane == 0) record_timeout(a.status, 41);
-        // the copies in flight land before the CTA leaves
-        for (int c = done; c < asked; ++c) (void)mbar_wait(bar + 8 * (c % RING), (uint32_t)(c / RING) & 1u);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kWeighTmem));
     }
 }
 
@@ -1366,9 +1396,9 @@ static int few_sms(int* out) {  // SMs of the current device; sets the kernels' 
                                              (int)FewCfg<64, 2>::smem(kBoundMaxSeqs)));
             }
         SD_CUDA(cudaFuncSetAttribute(weigh_rows_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)WeighCfg<128>::smem(kBoundMaxSeqs)));
+                                     (int)WeighCfg<128>::smem));
         SD_CUDA(cudaFuncSetAttribute(weigh_rows_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)WeighCfg<64>::smem(kBoundMaxSeqs)));
+                                     (int)WeighCfg<64>::smem));
         SD_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         facts[dev].store(n);
     }
@@ -1389,22 +1419,22 @@ static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
                             a.T, a.Hq, a.window, 0, a.ml, a.out, a.ldo,
                             static_cast<char*>(ws) + up256((size_t)a.T * a.Hq * sizeof(float2)), s);
     if (rc) return rc;
-    a.tpt = 1 << 24;  // a sequence is one tile
-    a.waves = 1;
-    a.ctas = (int)std::min<long long>(2 * std::min(sms, kFewMaxSms), ((long long)a.B * a.Hkv * a.max_blocks + kFewMinPages - 1) / kFewMinPages);
-    CUtensorMap map;
-    if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 1))) return rc;
+    CUtensorMap qmap, kmap;
+    if ((rc = make_q_tmap(&qmap, a.q, a.ldq, a.T, a.Hq, HD, a.G, 128 / a.G))) return rc;
+    if ((rc = make_kv_tmap(&kmap, a.kv, a.num_blocks, a.Hkv, HD, 1, 1))) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.ctas);
-    cfg.blockDim = dim3(32 * kFewWarps);
-    cfg.dynamicSmemBytes = HD == 128 ? WeighCfg<128>::smem(a.B) : WeighCfg<64>::smem(a.B);
+    // a CTA for each run of slots, or (tables far wider than most sequences) for several
+    const int runs = (a.max_blocks + 8 * kWeighTiles - 1) / (8 * kWeighTiles);
+    cfg.gridDim = dim3((unsigned)a.Hkv, (unsigned)a.B, (unsigned)std::min(runs, std::max(1, kChunkCtas / (a.B * a.Hkv))));
+    cfg.blockDim = dim3(kWeighThreads);
+    cfg.dynamicSmemBytes = HD == 128 ? WeighCfg<128>::smem : WeighCfg<64>::smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    SD_CUDA(cudaLaunchKernelEx(&cfg, HD == 128 ? weigh_rows_kernel<128> : weigh_rows_kernel<64>, map, a));
+    SD_CUDA(cudaLaunchKernelEx(&cfg, HD == 128 ? weigh_rows_kernel<128> : weigh_rows_kernel<64>, qmap, kmap, a));
     return SPECDEC_OK;
 }
 

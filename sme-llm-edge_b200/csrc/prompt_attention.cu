@@ -1503,7 +1503,7 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const __grid_constant__
 // ------------------------------------------------------------------ host side
 // The queries as [T][Hq][HD / 64][64]: one box is `tokens` tokens of one group
 // and column half, rows token * G + g of 128 bytes.
-static int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq, int HD, int G, int tokens) {
+int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq, int HD, int G, int tokens) {
     auto enc = attn_encode();
     SD_CHECK(enc, SPECDEC_ENOTSUP, "cuTensorMapEncodeTiled unavailable");
     cuuint64_t dims[4] = {64, (cuuint64_t)(HD / 64), (cuuint64_t)Hq, (cuuint64_t)T};
