@@ -1099,7 +1099,7 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
 // slot, so a thread sums its slot's weights over up to 128 rows by itself.  That is
 // three instructions a score, half of what the memory takes for K at 64 rows
 // (mma.sync fragments, 16 slots a warp, took twice the instructions and 42 us where
-// this takes NOTE).  One CTA for a KV head and run of 1024 slots; warps:
+// this takes NOTE).  One CTA for a KV head and run of up to 1024 slots; warps:
 //   0-3  sums, 4  MMA issuer, 5  loads (a group's queries, 128-slot tiles of K)
 constexpr int kWeighTiles = 8, kWeighThreads = 192, kWeighTmem = 256;
 
@@ -1132,8 +1132,8 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int kvh = blockIdx.x, b = blockIdx.y;
     const FewSeq s = few_seq(a, b);
-    const int end = min(s.ctx + s.n, a.slots_max), tiles = (end + 127) >> 7, step = gridDim.z * kWeighTiles;
-    const int first_tile = blockIdx.z * kWeighTiles;
+    const int end = min(s.ctx + s.n, a.slots_max), tiles = (end + 127) >> 7, run = a.chunk, step = gridDim.z * run;
+    const int first_tile = blockIdx.z * run;
     if (s.n == 0 || first_tile >= tiles) return;
     const int tpt = 128 / a.G, groups = (s.n + tpt - 1) / tpt;  // tokens of a group of rows
     if (threadIdx.x == 0) {
@@ -1173,7 +1173,7 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
         bool ok = true;
         for (int k = 0; ok && k < groups; ++k) {
             for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
-                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile) {
+                for (int tile = t0; tile < min(tiles, t0 + run); ++tile) {
                     const int pages = min(8, ((end + 15) >> 4) - 8 * tile), at = kc % RING, turn = kc / RING;
                     int page = 0;
                     if (lane < pages * NH) page = a.tables[(size_t)b * a.max_blocks + 8 * tile + lane / NH];
@@ -1209,7 +1209,7 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
             const uint32_t idesc = idesc_f16(128, (rows + 15) & ~15);
             ok = wait(q_full, k);
             for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
-                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile, ++kc) {
+                for (int tile = t0; tile < min(tiles, t0 + run); ++tile, ++kc) {
                     const int at = kc % RING, buf = kc & 1;
                     if (!(ok = wait(&k_full[at], kc / RING))) break;
                     if (kc >= 2 && !(ok = wait(&s_free[buf], (kc >> 1) - 1))) break;
@@ -1223,7 +1223,7 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
                         tc_commit(s_addr(&s_full[buf]));
                         tc_commit(s_addr(&k_empty[at]));
                         // (the group's last tile: commits cover all MMAs before them)
-                        if (tile + 1 >= min(tiles, t0 + kWeighTiles) && t0 + step >= tiles) tc_commit(s_addr(q_empty));
+                        if (tile + 1 >= min(tiles, t0 + run) && t0 + step >= tiles) tc_commit(s_addr(q_empty));
                     }
                     __syncwarp();
                 }
@@ -1249,7 +1249,7 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int t0 = first_tile; ok && t0 < tiles; t0 += step)
-                for (int tile = t0; tile < min(tiles, t0 + kWeighTiles); ++tile, ++kc) {
+                for (int tile = t0; tile < min(tiles, t0 + run); ++tile, ++kc) {
                     const int buf = kc & 1, j = 128 * tile + threadIdx.x;
                     const bool keeps = j <= p1 && j < end;
                     const float was = keeps ? weights[j] : 0.f;
@@ -1423,8 +1423,11 @@ static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
     if ((rc = make_q_tmap(&qmap, a.q, a.ldq, a.T, a.Hq, HD, a.G, 128 / a.G))) return rc;
     if ((rc = make_kv_tmap(&kmap, a.kv, a.num_blocks, a.Hkv, HD, 1, 1))) return rc;
     cudaLaunchConfig_t cfg = {};
-    // a CTA for each run of slots, or (tables far wider than most sequences) for several
-    const int runs = (a.max_blocks + 8 * kWeighTiles - 1) / (8 * kWeighTiles);
+    // a CTA for each run of slots (two for each SM, in tables that are full), or for several where tables are far wider
+    // than most sequences
+    const int tiles = (a.max_blocks + 7) / 8;
+    a.chunk = (int)std::min<long long>(kWeighTiles, std::max<long long>(1, (long long)a.B * a.Hkv * tiles / (2 * kFewMaxSms)));
+    const int runs = (tiles + a.chunk - 1) / a.chunk;
     cfg.gridDim = dim3((unsigned)a.Hkv, (unsigned)a.B, (unsigned)std::min(runs, std::max(1, kChunkCtas / (a.B * a.Hkv))));
     cfg.blockDim = dim3(kWeighThreads);
     cfg.dynamicSmemBytes = HD == 128 ? WeighCfg<128>::smem : WeighCfg<64>::smem;

@@ -244,12 +244,13 @@ struct RowsCut {
     float per_fine, per_coarse;  // reciprocals
     int whole;
     int dual;  // key tiles from which a segment of one tile is worked on as duals
+    int few;   // tokens of a segment of few rows
 };
 __device__ __forceinline__ bool rows_dual(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
     return s.n <= a.tpt && s.kt >= cut.dual;
 }
 __device__ __forceinline__ int rows_splits(const RowsArgs& a, const RowsSeg& s, const RowsCut& cut) {
-    const int S = s.n <= 64 / a.G ? (int)ceilf((float)s.kt * cut.per_fine)
+    const int S = s.n <= cut.few ? (int)ceilf((float)s.kt * cut.per_fine)
                                   : (s.kt <= cut.whole ? 1 : (int)rintf((float)s.kt * cut.per_coarse));
     const int most = rows_dual(a, s, cut) ? min(kRowsMaxSplits, s.kt) / 2 : min(kRowsMaxSplits, s.kt);
     return rows_clamp(S, 1, max(1, most));
@@ -385,7 +386,7 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
     const float mean = work / (float)gridDim.x;
     const float none = 1e-9f;  // of 2^23 key tiles at most: one piece
     RowsCut cut = {a.prows ? 1.f / fmaxf(4.f, 0.25f * mean) : none, a.prows ? 1.f / fmaxf(8.f, 0.5f * mean) : none,
-                   (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows ? 2 : 1 << 30};
+                   (int)fminf(1.1f * mean, (float)(1 << 26)), a.prows ? 2 : 1 << 30, (WIN ? 16 : 64) / a.G};
     int item0 = 0, prow0 = 0, tot_items = 0, tot_prows = 0;
 #pragma unroll 1
     for (int round = 0;; ++round) {
