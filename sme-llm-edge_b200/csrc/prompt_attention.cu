@@ -1019,7 +1019,32 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                             mx[1] = rows_max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
                         }
                     };
-                    if (masked) {  // what the row does not see: -infinity
+                    // What the row does not see: -infinity.  With a window a fifth of the tiles
+                    // or more are masked: there it is done on the way through the maximum.
+                    auto hide = [&](uint32_t(&v)[32], int q) {
+                        const uint32_t w = (uint32_t)((q & 2 ? seen_hi : seen_lo) >> (32 * (q & 1)));
+                        if (__all_sync(0xffffffffu, w == 0xFFFFFFFFu)) return;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((w >> e) & 1u)) v[e] = 0xFF800000u;
+                        tc_st_x32(t_s + 32 * q, v);
+                    };
+                    if (WIN && masked) {
+                        tc_ld_x32(t_s, va);
+                        tc_wait_ld();
+#pragma unroll 1
+                        for (int q = 0; q < 4; q += 2) {
+                            tc_ld_x32(t_s + 32 * (q + 1), vb);
+                            hide(va, q);
+                            largest(va, q);
+                            tc_wait_ld();
+                            if (q == 0) tc_ld_x32(t_s + 64, va);
+                            hide(vb, q + 1);
+                            largest(vb, q + 1);
+                            tc_wait_ld();
+                        }
+                        tc_wait_st();
+                    } else if (masked) {
 #pragma unroll 1
                         for (int q = 0; q < 8; ++q) {
                             const uint32_t w = (uint32_t)((q & 4 ? seen_hi : seen_lo) >> (16 * (q & 3)));
@@ -1034,16 +1059,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                         }
                         tc_wait_st();
                     }
-                    tc_ld_x32(t_s, va);
-                    tc_wait_ld();
+                    if (!(WIN && masked)) {
+                        tc_ld_x32(t_s, va);
+                        tc_wait_ld();
 #pragma unroll 1
-                    for (int q = 0; q < 4; q += 2) {
-                        tc_ld_x32(t_s + 32 * (q + 1), vb);
-                        largest(va, q);
-                        tc_wait_ld();
-                        if (q == 0) tc_ld_x32(t_s + 64, va);
-                        largest(vb, q + 1);
-                        tc_wait_ld();
+                        for (int q = 0; q < 4; q += 2) {
+                            tc_ld_x32(t_s + 32 * (q + 1), vb);
+                            largest(va, q);
+                            tc_wait_ld();
+                            if (q == 0) tc_ld_x32(t_s + 64, va);
+                            largest(vb, q + 1);
+                            tc_wait_ld();
+                        }
                     }
                     tc_ld_x32(t_s, va);
                     const float top = rows_max3(mx[0], mx[1], mx[1]) * a.scale_log2;
