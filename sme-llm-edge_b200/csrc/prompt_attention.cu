@@ -970,6 +970,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const int ti = row / a.G, g = row % a.G;       // token of the tile, head of the group
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_s = t_lane + ws * 128, t_o = t_lane + 256 + ws * HD;
+        // rows begin at 32-byte sectors: each is written by one store
+        const bool sectors = WIN && ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.ldo * 2) & 31) == 0;
         int c = 0, ended = 0;   // operations and items done on this slot
         int op = 0, tile = 0;   // operations (on both slots) and key tiles of the items before
         bool ok = true;
@@ -1167,17 +1169,33 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                         far = rows_max3(far, fabsf(__uint_as_float(ov[e])), fabsf(__uint_as_float(ov[e + 1])));
                     if (real && it.prow < 0) {
                         __half* dst = a.out + (size_t)tok * a.ldo + (size_t)head * HD + c0;
+                        if (WIN && sectors) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 w;
-                            uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+                            for (int e = 0; e < 32; e += 16) {
+                                uint32_t w[8];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const __half2 h = __floats2half2_rn(__uint_as_float(ov[e + 2 * q]) * inv,
-                                                                    __uint_as_float(ov[e + 2 * q + 1]) * inv);
-                                wp[q] = *reinterpret_cast<const uint32_t*>(&h);
+                                for (int q = 0; q < 8; ++q) {
+                                    const __half2 h = __floats2half2_rn(__uint_as_float(ov[e + 2 * q]) * inv,
+                                                                        __uint_as_float(ov[e + 2 * q + 1]) * inv);
+                                    w[q] = *reinterpret_cast<const uint32_t*>(&h);
+                                }
+                                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + e),
+                                             "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                             : "memory");
                             }
-                            *reinterpret_cast<uint4*>(dst + e) = w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint4 w;
+                                uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const __half2 h = __floats2half2_rn(__uint_as_float(ov[e + 2 * q]) * inv,
+                                                                        __uint_as_float(ov[e + 2 * q + 1]) * inv);
+                                    wp[q] = *reinterpret_cast<const uint32_t*>(&h);
+                                }
+                                *reinterpret_cast<uint4*>(dst + e) = w;
+                            }
                         }
                     } else if (real) {
                         // whole 32-byte sectors: a lane's row is far from the next lane's
@@ -1342,23 +1360,34 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     touched = true;
                 }
                 bool found = false;
+                auto place = [&](int i) {  // the i-th 16 bytes
+                    const int row = i / (NH * 8), h = i / 8 % NH;
+                    return reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 + (i & 7) * 16);
+                };
+                // the top bit of a half: its exponent is all ones
+                auto wild = [](uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; };
+                auto clean = [&](uint32_t w) {
+                    const uint32_t t = wild(w);
+                    return w & ~((t & 0x8000u ? 0xFFFFu : 0u) | (t & 0x80000000u ? 0xFFFF0000u : 0u));
+                };
+                // U pieces of a lane at a time.  With a window P.V of two tiles of each item and slot waits for this warp
+                // (one piece at a time took 1.5 us of a tile); without one, one at a time is the smaller code.
+                constexpr int U = WIN ? 4 : 1;
                 auto look = [&](int from, int to) {
-                    for (int i = from * NH * 8 + lane; i < to * NH * 8; i += 32) {
-                        const int row = i / (NH * 8), h = i / 8 % NH;
-                        uint4* at = reinterpret_cast<uint4*>(v + ((row >> 4) * NH + h) * kBlockHalf + (row & 15) * 128 +
-                                                             (i & 7) * 16);
-                        uint4 x = *at;
-                        uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
-                        bool mine = false;
-    #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool l16 = (xs[e] & 0x7C00u) == 0x7C00u, h16 = (xs[e] & 0x7C000000u) == 0x7C000000u;
-                            if (l16) xs[e] &= 0xFFFF0000u;
-                            if (h16) xs[e] &= 0x0000FFFFu;
-                            mine |= l16 || h16;
-                        }
-                        if (mine) *at = x;
-                        found |= mine;
+                    const int i1 = to * NH * 8;
+                    for (int i0 = from * NH * 8 + lane; i0 < i1; i0 += 32 * U) {
+                        uint4 x[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) x[u] = i0 + 32 * u < i1 ? *place(i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int u = 0; u < U; ++u) any |= wild(x[u].x) | wild(x[u].y) | wild(x[u].z) | wild(x[u].w);
+                        if (any == 0) continue;
+                        found = true;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (i0 + 32 * u < i1)
+                                *place(i0 + 32 * u) = make_uint4(clean(x[u].x), clean(x[u].y), clean(x[u].z), clean(x[u].w));
                     }
                 };
                 look(lo, n);
