@@ -1318,6 +1318,9 @@ static int few_ctas(int sms, int NT, int T, int Hkv, int max_blocks) {
     const long long ranges = ((long long)T * Hkv * max_blocks + kFewMinPages - 1) / kFewMinPages;
     return (int)std::min<long long>(few_resident(NT) * std::min(sms, kFewMaxSms), ranges);
 }
+// Weights of few rows keep their scores, up to 1 GiB of them; other calls compute them again.
+constexpr size_t kFewScores = (size_t)1 << 30;
+static size_t few_scores(int T, int Hq, int max_blocks) { return (size_t)T * Hq * max_blocks * 16 * sizeof(float); }
 // Sizes that do not fall where B, T or max_blocks grows.
 struct FewSpace {
     size_t pre, np, runs, pml, po, ml, scores, bytes;  // offsets, and all
@@ -1345,7 +1348,7 @@ static FewSpace few_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks,
     s.po = room(pieces * HD * sizeof(float));
     if (acc) {
         s.ml = room((size_t)T * Hq * sizeof(float2));
-        s.scores = room((size_t)T * Hq * max_blocks * 16 * sizeof(float));
+        s.scores = room(std::min(kFewScores, few_scores(T, Hq, max_blocks)));  // (calls with more keep none)
     }
     s.bytes = at;
     return s;
@@ -1525,15 +1528,18 @@ static int check_bound(const char* who, const void* q, int ldq, const void* kv, 
 }
 static int check_bound_memory(const char* who, const void* q, const void* kv, const void* out, const void* tables,
                               const void* ctx_len, const void* row_off, const void* ws) {
-    const std::string w(who);
     const struct {
         const void* p;
         const char* what;
-    } given[] = {{q, ": q"}, {kv, ": the KV pool"}, {out, ": out"}, {tables, ": tables"}, {ctx_len, ": ctx_len"},
-                 {row_off, ": row_off"}, {ws, ": the workspace"}};
-    int rc;
-    for (const auto& g : given)
-        if ((rc = check_on_device(g.p, (w + g.what).c_str()))) return rc;
+    } given[] = {{q, "q"}, {kv, "the KV pool"}, {out, "out"}, {tables, "tables"}, {ctx_len, "ctx_len"},
+                 {row_off, "row_off"}, {ws, "the workspace"}};
+    for (const auto& g : given) {
+        const int rc = check_on_device(g.p, g.what);
+        if (rc) {
+            set_error(std::string(who) + ": " + specdec_last_error());
+            return rc;
+        }
+    }
     return SPECDEC_OK;
 }
 
@@ -1541,7 +1547,6 @@ static int check_bound_memory(const char* who, const void* q, const void* kv, co
 
 using namespace specdec;
 
-// Calls of few rows keep their scores; the room for that ends where the others begin.
 static size_t accumulate_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks) {
     const int most = (int)std::min<long long>(T, (long long)B * (kFewMaxRows / std::max(1, std::min(kFewMaxRows, Hq / Hkv))));
     return std::max(few_space(B, most, Hq, Hkv, HD, max_blocks, true).bytes,
@@ -1641,6 +1646,7 @@ extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const ui
                          out, ldo);
     f.weights = weights;
     f.ldw = ldw;
-    return few_rows(B, T, n_q_heads / n_kv_heads) ? launch_few(f, head_dim, true, workspace, as_stream(stream))
-                                                  : launch_many(f, head_dim, workspace, as_stream(stream));
+    const bool few = few_rows(B, T, n_q_heads / n_kv_heads) && few_scores(T, n_q_heads, max_blocks) <= kFewScores;
+    return few ? launch_few(f, head_dim, true, workspace, as_stream(stream))
+               : launch_many(f, head_dim, workspace, as_stream(stream));
 }

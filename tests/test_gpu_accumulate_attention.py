@@ -248,3 +248,39 @@ def test_host_and_foreign_memory_is_refused(cuda_device):
     with pytest.raises(S.SpecdecError, match="workspace"):
         call(s, ws.cpu())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("wide", [1100, 90000])
+def test_tables_far_wider_than_the_sequences(cuda_device, wide):
+    heads = (32, 8, 128) if wide == 1100 else (8, 2, 64)
+    lens = [(1 + (i % 9 == 0), (37 * i) % 700) for i in range(64)] if wide == 1100 else [(1, 5000), (3, 40), (0, 7), (2, 999)]
+    s = make(lens, *heads, seed=wide % 91, wide=wide)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_scores_past_what_is_kept(cuda_device):
+    """Tables so wide that the rows' scores would take more than 1 GiB: they are computed again."""
+    s = make([(1, 300), (2, 50)], 8, 2, 64, seed=3, wide=800000)
+    ws = call(s)
+    assert ws.numel() < 3 << 30
+    verify(s)
+    del ws
+
+
+def test_many_rows_beside_many_sequences(cuda_device):
+    """One CTA goes through several runs of a sequence's slots."""
+    s = make([(0, 3)] * 1000 + [(4200, 0)] + [(0, 0)] * 23, 32, 4, 64, seed=5)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+@pytest.mark.parametrize("G", [1, 3, 5, 7, 8, 12, 16, 31, 32])
+@pytest.mark.parametrize("lens", [[(1, 700), (2, 130)], [(40, 300), (3, 90)]])
+def test_head_groups(cuda_device, G, lens):
+    s = make(lens, 2 * G, 2, 64 if G % 2 else 128, seed=G)
+    ws = call(s)
+    verify(s)
+    del ws

@@ -169,6 +169,30 @@ def test_against_the_definition(cuda_device, state, reqs, keep, first, last):
     assert status == (S.ENOMEM if state["spare"] == 1 and "shared" in state else S.OK)
 
 
+@pytest.mark.parametrize("n", [8, 9, 40])
+def test_many_requests(cuda_device, n):
+    """Up to 8 requests are selected and given their tables in one launch, more in two."""
+    r = random.Random(n)
+    lens = [r.randrange(1, 300) for _ in range(n + 3)]
+    shared = [(i, i - 1, min(lens[i], lens[i - 1]) // 16) for i in range(1, n + 3, 5)]
+    st = State(lens, 20, 10 * n, seed=n, shared=shared, layers=1)
+    reqs = list(range(n + 3))
+    r.shuffle(reqs)
+    assert st.check(reqs[:n], 60, 3, 7) == S.OK
+    st.lens[reqs[0]] += 16 * 30  # one request out of order among the others
+    assert st.check(reqs[:n], 20, 3, 7) == S.EINVAL
+
+
+@pytest.mark.parametrize("slots", [2047, 2048, 2049, 4096, 4100, 8192, 8193])
+def test_sizes_at_which_the_selection_changes(cuda_device, slots):
+    """Threads by the table's width, keys in registers by the request's length; weights that are not aligned to 16 bytes."""
+    wide = (slots + 15) // 16
+    for ldw in (wide * 16, wide * 16 + 5):
+        st = State([slots], wide, 0, heads=2, layers=1, Hkv=1, ldw=ldw, seed=slots)
+        assert st.check([0], slots - 700, 11, 200) == S.OK
+        assert st.check([0], 77, 0, 0) == S.OK
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_random_rounds(cuda_device, seed):
     """Rounds of growth and eviction on the same tables."""

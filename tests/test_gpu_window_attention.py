@@ -338,3 +338,28 @@ def test_host_and_foreign_memory_is_refused(cuda_device):
     with pytest.raises(S.SpecdecError, match="workspace"):
         call(s, ws.cpu())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("wide", [1100, 90000])
+def test_tables_far_wider_than_the_sequences(cuda_device, wide):
+    """Where a CTA for every run of the table would find nothing, the pages are cut by the lengths in device memory."""
+    heads = (32, 8, 128) if wide == 1100 else (8, 2, 64)
+    lens = [(1 + (i % 9 == 0), (37 * i) % 700) for i in range(64)] if wide == 1100 else [(1, 5000), (3, 40), (0, 7), (2, 999)]
+    for window, sinks in ((1 << 20, 0), (300, 20)):
+        s = make(lens, *heads, window, sinks, seed=wide % 91, wide=wide)
+        ws = call(s)
+        verify(s)
+        first = s["out"].clone()
+        ws.fill_(0xFF)
+        call(s, ws)
+        torch.cuda.synchronize()
+        assert torch.equal(first, s["out"])
+        del ws
+
+
+def test_long_calls_under_wide_tables(cuda_device):
+    """Pages enough for a second wave of ranges."""
+    s = make([(1, 1500 + 7 * i) for i in range(64)], 8, 8, 64, 1 << 20, 0, seed=3, wide=1100, gone=False)
+    ws = call(s)
+    verify(s)
+    del ws
