@@ -244,7 +244,9 @@ extern "C" int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, 
     // (8 x 2501 such rows 117 us, 0.97 of the copy rate; 16 groups in flight or more warps of fewer registers 120 to 148).
     const int groups = ((n_q_heads + 2 * n_kv_heads) * head_dim + 255) / 256;
     const bool many = (long long)T * groups > 148LL * 64 * 4;
-    a.parts = many ? (groups + 15) / 16 : groups;
+    // (eight times where that still fills the SMs: a row's look-ups are made by fewer warps)
+    const int groups_of_warp = (long long)T * groups >= 148LL * 28 * 32 ? 32 : 16;
+    a.parts = many ? (groups + groups_of_warp - 1) / groups_of_warp : groups;
     const long long warps = (long long)T * a.parts;
     const dim3 grid((unsigned)((warps + kNormWarps - 1) / kNormWarps)), block(32 * kNormWarps);
     cudaStream_t s = as_stream(stream);
