@@ -858,14 +858,13 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : NT == 1 ? 3 : 2)
 // CTA one after the other, 57 with one).  Where the row belongs is looked up while
 // the kernel before still runs.
 template <int HD, int ROWS, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
+__device__ __forceinline__ void few_merge(const FewArgs& a, int tile_rows, unsigned block) {
     constexpr int W = HD / 32;
     static_assert(ROWS == 1 || ROWS == WARPS, "rows of a CTA");
     __shared__ float sm[WARPS], sl[WARPS], so[WARPS][HD];
     __shared__ int sbad[WARPS];
-    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long rows = (long long)a.T * a.Hq, first = (long long)ROWS * blockIdx.x;
+    const long long rows = (long long)a.T * a.Hq, first = (long long)ROWS * block;
     struct Row {
         int n, b, p, kvh, row, np, tile, r0;
         long long u0;
@@ -1012,6 +1011,43 @@ __global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_cons
     }
 }
 
+template <int HD, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) few_merge_kernel(const __grid_constant__ FewArgs a, int tile_rows) {
+    pdl_trigger();
+    few_merge<HD, ROWS, WARPS>(a, tile_rows, blockIdx.x);
+}
+
+// A row's weights of up to four slots j + STEP u <= last, added to sum: src its scores [slot][G], ml its heads' (m, 1 / l).
+template <int V, int STEP>
+__device__ __forceinline__ void few_weigh(const float* src, const float2* ml, int G, int j, int last, float (&sum)[4]) {
+    for (int g = 0; g < G; g += V) {
+        float x[4][V];
+        float2 y[V];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float* at = src + (size_t)(j + STEP * u) * G + g;
+            if (j + STEP * u <= last) {
+                if constexpr (V == 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(at);
+                    x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
+                } else if constexpr (V == 2) {
+                    const float2 f = *reinterpret_cast<const float2*>(at);
+                    x[u][0] = f.x, x[u][1] = f.y;
+                } else {
+                    x[u][0] = *at;
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = ml[g + v];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (j + STEP * u <= last)
+#pragma unroll
+                for (int v = 0; v < V; ++v) sum[u] += few_exp2(x[u][v] - y[v].x) * y[v].y;
+    }
+}
+
 // weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
 // of 2^(x - m) / l, from the scores that few_rows_kernel left.  A warp for 128
 // slots of a head, four a lane; V heads' scores in one load.
@@ -1019,74 +1055,88 @@ template <int V>
 __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant__ FewArgs a) {
     extern __shared__ int runs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.chunk) {  // blocks (1024 slots, KV head, sequence)
-        const FewSeq s = few_seq(a, blockIdx.z);
-        const int end = min(s.ctx + s.n, a.slots_max);
-        if (s.n == 0 || (end + 15) >> 4 <= a.chunk || 1024 * (int)blockIdx.x >= end) return;  // (a CTA has added up its own)
-    }
     pdl_wait();
-    if (!a.chunk) {
-        for (int b = threadIdx.x; b <= a.B; b += 256) runs[b] = a.runs[b];
-        __syncthreads();
-    }
-    const int total = a.chunk ? 8 * (int)(blockIdx.x + 1) : runs[a.B];
+    for (int b = threadIdx.x; b <= a.B; b += 256) runs[b] = a.runs[b];
+    __syncthreads();
+    const int total = runs[a.B];
     for (int c = blockIdx.x * 8 + warp; c < total; c += gridDim.x * 8) {
-        int lo = a.chunk ? (int)blockIdx.z : 0, hi = a.chunk ? lo : a.B;
+        int lo = 0, hi = a.B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (runs[mid] <= c) lo = mid;
             else hi = mid;
         }
         const FewSeq s = few_seq(a, lo);
-        int kvh = blockIdx.y, j0 = 128 * c;
-        if (!a.chunk) {
-            const int per_head = (runs[lo + 1] - runs[lo]) / a.Hkv, local = c - runs[lo];
-            kvh = local / per_head;
-            j0 = 128 * (local - kvh * per_head);
-        }
+        const int per_head = (runs[lo + 1] - runs[lo]) / a.Hkv, local = c - runs[lo];
+        const int kvh = local / per_head, j0 = 128 * (local - kvh * per_head);
         const int end = min(min(s.ctx + s.n, a.slots_max), j0 + 128);
         float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
         float sum[4] = {}, was[4] = {};
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (j0 + 32 * u + lane < end) was[u] = dst[j0 + 32 * u + lane];
-#pragma unroll 2
         for (int i = max(0, j0 - s.ctx); i < s.n; ++i) {
             const int r = s.lo + i, p = min(s.ctx + i, end - 1);
             const float* src = a.scores + ((size_t)r * a.Hkv + kvh) * a.slots_max * a.G;
             const float2* ml = a.ml + (size_t)r * a.Hq + kvh * a.G;
-            for (int g = 0; g < a.G; g += V) {
-                float x[4][V];
-                float2 y[V];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int j = j0 + 32 * u + lane;
-                    const float* at = src + (size_t)j * a.G + g;
-                    if (j <= p) {
-                        if constexpr (V == 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(at);
-                            x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
-                        } else if constexpr (V == 2) {
-                            const float2 f = *reinterpret_cast<const float2*>(at);
-                            x[u][0] = f.x, x[u][1] = f.y;
-                        } else {
-                            x[u][0] = *at;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int v = 0; v < V; ++v) y[v] = ml[g + v];
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (j0 + 32 * u + lane <= p)
-#pragma unroll
-                        for (int v = 0; v < V; ++v) sum[u] += few_exp2(x[u][v] - y[v].x) * y[v].y;
-            }
+            few_weigh<V, 32>(src, ml, a.G, j0 + lane, p, sum);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (j0 + 32 * u + lane < end) dst[j0 + 32 * u + lane] = was[u] + sum[u];
     }
+}
+
+// Behind chunks: the rows' pieces joined by the first `merges` CTAs, and what the
+// slots of sequences of more than one chunk received by the others, 512 slots of a KV
+// head each, which join the rows' (m, l) for themselves: neither waits for the other.
+template <int HD, int ROWS, int V>
+__global__ void __launch_bounds__(128) few_join_kernel(const __grid_constant__ FewArgs a, int tile_rows, unsigned merges,
+                                                       unsigned runs) {
+    if (blockIdx.x < merges) {
+        few_merge<HD, ROWS, 4>(a, tile_rows, blockIdx.x);
+        return;
+    }
+    __shared__ float2 lse[64];
+    const unsigned w = blockIdx.x - merges;
+    const int b = (int)(w / runs / a.Hkv), kvh = (int)(w / runs % a.Hkv), j0 = 512 * (int)(w % runs);
+    const FewSeq s = few_seq(a, b);
+    const int end = min(s.ctx + s.n, a.slots_max);
+    if (s.n == 0 || (end + 15) >> 4 <= a.chunk || j0 >= end) return;  // (one chunk: its CTA has added up its own)
+    pdl_wait();
+    const int j = j0 + (int)threadIdx.x, tokens = 64 / a.G;
+    float* dst = a.weights + ((size_t)b * a.Hkv + kvh) * a.ldw;
+    float sum[4] = {}, was[4] = {};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (j + 128 * u < end) was[u] = dst[j + 128 * u];
+    for (int i0 = max(0, j0 - s.ctx); i0 < s.n; i0 += tokens) {
+        const int n = min(tokens, s.n - i0);
+        __syncthreads();
+        if ((int)threadIdx.x < n * a.G) {
+            const int tok = i0 + (int)threadIdx.x / a.G, head = kvh * a.G + (int)threadIdx.x % a.G;
+            const size_t at = (size_t)(s.lo + tok) * a.Hq + head;
+            const int pieces = (few_tile(a, s, tok / a.tpt).np + a.chunk - 1) / a.chunk;
+            if (pieces <= 1) {
+                lse[threadIdx.x] = a.ml[at];
+            } else {
+                float m = -INFINITY, l = 0.f;
+                for (int k = 0; k < pieces; ++k) m = few_max(m, a.pml[at * a.chunks + k].x);
+                for (int k = 0; k < pieces; ++k) {
+                    const float2 y = a.pml[at * a.chunks + k];
+                    l += exp2f(y.x - m) * fabsf(y.y);
+                }
+                lse[threadIdx.x] = make_float2(m, l > 0.f || l != l ? 1.0f / l : 0.f);
+            }
+        }
+        __syncthreads();
+        for (int i = 0; i < n; ++i)
+            few_weigh<V, 128>(a.scores + ((size_t)(s.lo + i0 + i) * a.Hkv + kvh) * a.slots_max * a.G, lse + i * a.G, a.G, j,
+                              min(s.ctx + i0 + i, end - 1), sum);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (j + 128 * u < end) dst[j + 128 * u] = was[u] + sum[u];
 }
 
 // ------------------------------------------------------------------ many rows
@@ -1444,6 +1494,16 @@ static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
     return SPECDEC_OK;
 }
 
+using FewJoin = void (*)(const FewArgs, int, unsigned, unsigned);
+template <int HD, int ROWS>
+static FewJoin join_v(int G) {
+    return G % 4 == 0 ? few_join_kernel<HD, ROWS, 4> : G % 2 == 0 ? few_join_kernel<HD, ROWS, 2> : few_join_kernel<HD, ROWS, 1>;
+}
+static FewJoin join_fn(int HD, bool single, int G) {
+    if (HD == 128) return single ? join_v<128, 1>(G) : join_v<128, 4>(G);
+    return single ? join_v<64, 1>(G) : join_v<64, 4>(G);
+}
+
 static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     int sms = 0;
     int rc = few_sms(&sms);
@@ -1492,6 +1552,13 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     cfg.numAttrs = 1;
     const long long rows = (long long)a.T * a.Hq;
     const int kind = rows <= 256 ? 0 : rows <= 2048 ? 1 : 2;
+    if (acc && a.chunk) {
+        const unsigned merges = (unsigned)(kind < 2 ? rows : (rows + 3) / 4), runs = (unsigned)((a.max_blocks + 31) / 32);
+        cfg.gridDim = dim3(merges + runs * (unsigned)(a.B * a.Hkv));
+        cfg.blockDim = dim3(128);
+        SD_CUDA(cudaLaunchKernelEx(&cfg, join_fn(HD, kind < 2, a.G), a, 8 * NT, merges, runs));
+        return SPECDEC_OK;
+    }
     cfg.gridDim = dim3((unsigned)(kind < 2 ? rows : (rows + 3) / 4));
     cfg.blockDim = dim3(kind == 0 ? 512 : 128);
     const auto merge =
@@ -1500,10 +1567,9 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     SD_CUDA(cudaLaunchKernelEx(&cfg, merge, a, 8 * NT));
     if (acc) {
         const long long runs = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
-        cfg.gridDim = a.chunk ? dim3((unsigned)((a.max_blocks + 63) / 64), (unsigned)a.Hkv, (unsigned)a.B)
-                              : dim3((unsigned)std::min<long long>((runs + 7) / 8, 8LL * sms));
+        cfg.gridDim = dim3((unsigned)std::min<long long>((runs + 7) / 8, 8LL * sms));
         cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = a.chunk ? 0 : (size_t)(a.B + 1) * 4;
+        cfg.dynamicSmemBytes = (size_t)(a.B + 1) * 4;
         const auto weigh = a.G % 4 == 0 ? few_weights_kernel<4> : (a.G % 2 == 0 ? few_weights_kernel<2> : few_weights_kernel<1>);
         SD_CUDA(cudaLaunchKernelEx(&cfg, weigh, a));
     }
