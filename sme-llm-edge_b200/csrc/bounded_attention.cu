@@ -1049,26 +1049,37 @@ __device__ __forceinline__ void few_weigh(const float* src, const float2* ml, in
 }
 
 // weights[b][kvh][j] += sum over the rows that see slot j, and the group's heads,
-// of 2^(x - m) / l, from the scores that few_rows_kernel left.  A warp for 128
-// slots of a head, four a lane; V heads' scores in one load.
+// of 2^(x - m) / l, from the scores that the attention left.  A warp for 128 slots of
+// a head, four a lane; V heads' scores in one load.
 template <int V>
 __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant__ FewArgs a) {
     extern __shared__ int runs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (a.chunk) {  // blocks (1024 slots, KV head, sequence)
+        const FewSeq s = few_seq(a, blockIdx.z);
+        const int end = min(s.ctx + s.n, a.slots_max);
+        if (s.n == 0 || (end + 15) >> 4 <= a.chunk || 1024 * (int)blockIdx.x >= end) return;  // (a CTA has added up its own)
+    }
     pdl_wait();
-    for (int b = threadIdx.x; b <= a.B; b += 256) runs[b] = a.runs[b];
-    __syncthreads();
-    const int total = runs[a.B];
+    if (!a.chunk) {
+        for (int b = threadIdx.x; b <= a.B; b += 256) runs[b] = a.runs[b];
+        __syncthreads();
+    }
+    const int total = a.chunk ? 8 * (int)(blockIdx.x + 1) : runs[a.B];
     for (int c = blockIdx.x * 8 + warp; c < total; c += gridDim.x * 8) {
-        int lo = 0, hi = a.B;
+        int lo = a.chunk ? (int)blockIdx.z : 0, hi = a.chunk ? lo : a.B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (runs[mid] <= c) lo = mid;
             else hi = mid;
         }
         const FewSeq s = few_seq(a, lo);
-        const int per_head = (runs[lo + 1] - runs[lo]) / a.Hkv, local = c - runs[lo];
-        const int kvh = local / per_head, j0 = 128 * (local - kvh * per_head);
+        int kvh = blockIdx.y, j0 = 128 * c;
+        if (!a.chunk) {
+            const int per_head = (runs[lo + 1] - runs[lo]) / a.Hkv, local = c - runs[lo];
+            kvh = local / per_head;
+            j0 = 128 * (local - kvh * per_head);
+        }
         const int end = min(min(s.ctx + s.n, a.slots_max), j0 + 128);
         float* dst = a.weights + ((size_t)lo * a.Hkv + kvh) * a.ldw;
         float sum[4] = {}, was[4] = {};
@@ -1087,14 +1098,19 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
     }
 }
 
-// Behind chunks: the rows' pieces joined by the first `merges` CTAs, and what the
-// slots of sequences of more than one chunk received by the others, 512 slots of a KV
-// head each, which join the rows' (m, l) for themselves: neither waits for the other.
-template <int HD, int ROWS, int V>
+// Behind chunks of up to kFewJoin rows and heads, both in one launch: the rows' pieces
+// joined by the first `merges` CTAs, and what the slots of sequences of more than one
+// chunk received by the others, 512 slots of a KV head each, which join the rows'
+// (m, l) for themselves, so neither waits for the other.  In place of two launches: one
+// token of each of 4 sequences on 3000 17.4 -> 15.3 us a call, of 8 on 8192 57.9 -> 54.6.
+// The merge's registers leave the weights fewer warps, which costs more where rows are
+// many: of 64 on 4096 198.7 -> 200.4, of 148 419.7 -> 439.3, four of each of 64 251 -> 263.
+constexpr long long kFewJoin = 1024;
+template <int HD, int V>
 __global__ void __launch_bounds__(128) few_join_kernel(const __grid_constant__ FewArgs a, int tile_rows, unsigned merges,
                                                        unsigned runs) {
     if (blockIdx.x < merges) {
-        few_merge<HD, ROWS, 4>(a, tile_rows, blockIdx.x);
+        few_merge<HD, 1, 4>(a, tile_rows, blockIdx.x);
         return;
     }
     __shared__ float2 lse[64];
@@ -1149,7 +1165,7 @@ __global__ void __launch_bounds__(128) few_join_kernel(const __grid_constant__ F
 // slot, so a thread sums its slot's weights over up to 128 rows by itself.  That is
 // three instructions a score, half of what the memory takes for K at 64 rows
 // (mma.sync fragments, 16 slots a warp, took twice the instructions and 42 us where
-// this takes NOTE).  One CTA for a KV head and run of up to 1024 slots; warps:
+// this takes 17).  One CTA for a KV head and run of up to 1024 slots; warps:
 //   0-3  sums, 4  MMA issuer, 5  loads (a group's queries, 128-slot tiles of K)
 constexpr int kWeighTiles = 8, kWeighThreads = 192, kWeighTmem = 256;
 
@@ -1495,13 +1511,10 @@ static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
 }
 
 using FewJoin = void (*)(const FewArgs, int, unsigned, unsigned);
-template <int HD, int ROWS>
-static FewJoin join_v(int G) {
-    return G % 4 == 0 ? few_join_kernel<HD, ROWS, 4> : G % 2 == 0 ? few_join_kernel<HD, ROWS, 2> : few_join_kernel<HD, ROWS, 1>;
-}
-static FewJoin join_fn(int HD, bool single, int G) {
-    if (HD == 128) return single ? join_v<128, 1>(G) : join_v<128, 4>(G);
-    return single ? join_v<64, 1>(G) : join_v<64, 4>(G);
+static FewJoin join_fn(int HD, int G) {
+    const int v = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+    if (HD == 128) return v == 4 ? few_join_kernel<128, 4> : v == 2 ? few_join_kernel<128, 2> : few_join_kernel<128, 1>;
+    return v == 4 ? few_join_kernel<64, 4> : v == 2 ? few_join_kernel<64, 2> : few_join_kernel<64, 1>;
 }
 
 static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
@@ -1552,11 +1565,11 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     cfg.numAttrs = 1;
     const long long rows = (long long)a.T * a.Hq;
     const int kind = rows <= 256 ? 0 : rows <= 2048 ? 1 : 2;
-    if (acc && a.chunk) {
-        const unsigned merges = (unsigned)(kind < 2 ? rows : (rows + 3) / 4), runs = (unsigned)((a.max_blocks + 31) / 32);
+    if (acc && a.chunk && rows <= kFewJoin) {
+        const unsigned merges = (unsigned)rows, runs = (unsigned)((a.max_blocks + 31) / 32);
         cfg.gridDim = dim3(merges + runs * (unsigned)(a.B * a.Hkv));
         cfg.blockDim = dim3(128);
-        SD_CUDA(cudaLaunchKernelEx(&cfg, join_fn(HD, kind < 2, a.G), a, 8 * NT, merges, runs));
+        SD_CUDA(cudaLaunchKernelEx(&cfg, join_fn(HD, a.G), a, 8 * NT, merges, runs));
         return SPECDEC_OK;
     }
     cfg.gridDim = dim3((unsigned)(kind < 2 ? rows : (rows + 3) / 4));
@@ -1567,9 +1580,10 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     SD_CUDA(cudaLaunchKernelEx(&cfg, merge, a, 8 * NT));
     if (acc) {
         const long long runs = (long long)a.B * a.Hkv * ((a.max_blocks + 7) / 8);
-        cfg.gridDim = dim3((unsigned)std::min<long long>((runs + 7) / 8, 8LL * sms));
+        cfg.gridDim = a.chunk ? dim3((unsigned)((a.max_blocks + 63) / 64), (unsigned)a.Hkv, (unsigned)a.B)
+                              : dim3((unsigned)std::min<long long>((runs + 7) / 8, 8LL * sms));
         cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = (size_t)(a.B + 1) * 4;
+        cfg.dynamicSmemBytes = a.chunk ? 0 : (size_t)(a.B + 1) * 4;
         const auto weigh = a.G % 4 == 0 ? few_weights_kernel<4> : (a.G % 2 == 0 ? few_weights_kernel<2> : few_weights_kernel<1>);
         SD_CUDA(cudaLaunchKernelEx(&cfg, weigh, a));
     }
