@@ -1058,7 +1058,11 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const __grid_constant_
     if (a.chunk) {  // blocks (1024 slots, KV head, sequence)
         const FewSeq s = few_seq(a, blockIdx.z);
         const int end = min(s.ctx + s.n, a.slots_max);
-        if (s.n == 0 || (end + 15) >> 4 <= a.chunk || 1024 * (int)blockIdx.x >= end) return;  // (a CTA has added up its own)
+        // (short sequences: a CTA of the attention has added up its own)
+        if (s.n == 0 || (end + 15) >> 4 <= a.chunk || 1024 * (int)blockIdx.x >= end) {
+            if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0) pdl_wait();  // who waits for this kernel waits for those before it
+            return;
+        }
     }
     pdl_wait();
     if (!a.chunk) {
@@ -1200,7 +1204,10 @@ __global__ void __launch_bounds__(kWeighThreads, 2)
     const FewSeq s = few_seq(a, b);
     const int end = min(s.ctx + s.n, a.slots_max), tiles = (end + 127) >> 7, run = a.chunk, step = gridDim.z * run;
     const int first_tile = blockIdx.z * run;
-    if (s.n == 0 || first_tile >= tiles) return;
+    if (s.n == 0 || first_tile >= tiles) {
+        if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0) pdl_wait();  // who waits for this kernel waits for those before it
+        return;
+    }
     const int tpt = 128 / a.G, groups = (s.n + tpt - 1) / tpt;  // tokens of a group of rows
     if (threadIdx.x == 0) {
         for (int i = 0; i < RING; ++i) {

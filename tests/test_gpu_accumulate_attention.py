@@ -284,3 +284,27 @@ def test_head_groups(cuda_device, G, lens):
     ws = call(s)
     verify(s)
     del ws
+
+
+@pytest.mark.parametrize("lens,heads", [([(1, 5)] * 40, (32, 8, 128)), ([(4, 20)] * 12, (40, 8, 128)),
+                                        ([(0, 30)] * 3 + [(200, 0)], (8, 2, 64))])
+def test_what_follows_a_captured_call_sees_its_results(cuda_device, lens, heads):
+    # tables of several runs, sequences of one: nothing is left for the last kernel of the call to do
+    s = make(lens, *heads, seed=8, wide=1 << 8)
+    ws = call(s)
+    torch.cuda.synchronize()
+    kept, gained = torch.empty_like(s["out"]), torch.empty_like(s["weights"])
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        s["out"].fill_(7.0)
+        s["weights"].copy_(s["before"])
+        call(s, ws, torch.cuda.current_stream())
+        kept.copy_(s["out"])
+        gained.copy_(s["weights"])
+    for _ in range(5):
+        kept.zero_()
+        gained.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        s["weights"].copy_(gained)
+        verify(s, out=kept)
