@@ -389,9 +389,11 @@ int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_laye
  * single tokens keep a running sum; the last rows of a prompt (ctx_len the
  * tokens before them) weigh the whole prompt.  Layers may add into the same
  * weights one after another.  The sums run in a fixed order: the result is
- * deterministic.  Up to 32 query heads for each KV head, and 16 rows a
- * sequence are what it is made for; T <= 65536.  The rest as for
- * specdec_attention_prompt. */
+ * deterministic.  Up to 32 query heads for each KV head; T <= 65536.  out and
+ * weights overlap neither q nor each other.  Calls of up to 32 / (query heads
+ * of a KV head) rows a sequence on average keep their scores in the workspace
+ * (T * n_q_heads * max_blocks * 64 bytes, 1 GiB at most); others compute them
+ * twice.  The rest as for specdec_attention_prompt. */
 size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                     int max_blocks);
 int specdec_attention_accumulate(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,

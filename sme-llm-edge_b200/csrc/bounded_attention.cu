@@ -1723,6 +1723,8 @@ extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const ui
                  (reinterpret_cast<uintptr_t>(weights) & 15) == 0,
              SPECDEC_EINVAL, "attention_accumulate: weights 16-byte aligned, ldw a multiple of 4 that holds max_blocks * 16 slots");
     if (B == 0 || T == 0) return SPECDEC_OK;
+    // (the weights of many rows read the queries again when the outputs are written)
+    SD_CHECK(q != out, SPECDEC_EINVAL, "attention_accumulate: out must not be q");
     SD_CHECK(workspace && (reinterpret_cast<uintptr_t>(workspace) & 31) == 0 &&
                  workspace_bytes >=
                      specdec_attention_accumulate_workspace_bytes(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks),

@@ -40,6 +40,11 @@ def test_accumulate_refuses(bad):
     assert "attention_accumulate" in S.last_error()
 
 
+def test_accumulate_refuses_its_queries_as_its_output():
+    assert attend(True, ws_bytes=1 << 50) == S.EINVAL
+    assert "out must not be q" in S.last_error()
+
+
 def write(**kw):
     a = dict(qkv=PTR, half=0, ld=768, qn=PTR, kn=PTR, eps=1e-5, cos=PTR, sin=PTR, max_pos=9, rot=64, pos=PTR, kv=PTR,
              num_blocks=4, Hkv=2, hd=64, tables=PTR, max_blocks=4, ctx=PTR, off=PTR, B=2, T=8, Hq=8, q=PTR, ldq=512)
