@@ -373,7 +373,8 @@ int specdec_attention_shared_prefix(const uint16_t* q, const uint16_t* kv_layer,
  * not see are specdec_attention_prompt's; pages of which no row of a sequence
  * sees a slot are not read, so their table entries may be anything (-1 where
  * they were given back).  Rows keep their slots: a slot is a position here.
- * Single tokens and prompts are both served by this call. */
+ * Single tokens and prompts are both served by this call, also together: where
+ * B < T, long sequences and short ones go through kernels of their own. */
 size_t specdec_attention_window_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                 int max_blocks);
 int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,

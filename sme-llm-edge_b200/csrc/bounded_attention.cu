@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -65,6 +66,7 @@ struct FewArgs {
     const int32_t* ctx_len;
     const int32_t* row_off;
     int B, T, window, sinks;
+    int least, most;  // sequences of up to `least` and of more than `most` rows are left out
     float* weights;
     int ldw;
     __half* out;
@@ -93,6 +95,7 @@ __device__ __forceinline__ FewSeq few_seq(const FewArgs& a, int b) {
     s.np = 0;
     s.lo = max(0, min(a.row_off[b], a.T));
     s.n = max(s.lo, min(a.row_off[b + 1], a.T)) - s.lo;
+    if (s.n <= a.least || s.n > a.most) s.n = 0;
     s.ctx = max(0, min(a.ctx_len[b], 1 << 30));
     return s;
 }
@@ -1492,7 +1495,7 @@ static int launch_many(FewArgs a, int HD, void* ws, cudaStream_t s) {
     a.slots_max = a.max_blocks * 16;
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)HD));
     rc = rows_packed_launch(a.q, a.ldq, a.kv, a.num_blocks, a.Hkv, HD, a.tables, a.max_blocks, a.ctx_len, a.row_off, a.B,
-                            a.T, a.Hq, a.window, 0, a.ml, a.out, a.ldo,
+                            a.T, a.Hq, a.window, 0, a.least, a.ml, a.out, a.ldo,
                             static_cast<char*>(ws) + up256((size_t)a.T * a.Hq * sizeof(float2)), s);
     if (rc) return rc;
     CUtensorMap qmap, kmap;
@@ -1636,10 +1639,20 @@ using namespace specdec;
 
 static size_t accumulate_space(int B, int T, int Hq, int Hkv, int HD, int max_blocks) {
     const int most = (int)std::min<long long>(T, (long long)B * (kFewMaxRows / std::max(1, std::min(kFewMaxRows, Hq / Hkv))));
-    return std::max(few_space(B, most, Hq, Hkv, HD, max_blocks, true).bytes,
-                    up256((size_t)T * Hq * sizeof(float2)) + rows_packed_workspace(B, T, Hq, HD, max_blocks));
+    return few_space(B, most, Hq, Hkv, HD, max_blocks, true).bytes + up256((size_t)T * Hq * sizeof(float2)) +
+           rows_packed_workspace(B, T, Hq, HD, max_blocks);
 }
 static bool few_rows(int B, int T, int G) { return G <= kFewMaxRows && T <= (long long)B * (kFewMaxRows / G); }
+// Rows that a sequence of a few-row call may have at most, else it is left to the packed rows' kernels; 0: there is no
+// such bound.  A call's average says nothing of its longest sequence, whose tiles would go one after the other through
+// the CTAs of its heads, each reading K and V again: 63 single tokens on 4096 beside a chunk of 190 on 8000 1633 us, with
+// weights 2043; divided 257 and 413.  Where no sequence is long the other launches find nothing to do, for 6 to 17 us
+// (32 x 5 on 4096 115 -> 124, with weights 154 -> 171), so calls of up to one row a sequence, which are single tokens
+// unless others are empty, are not divided.
+static int few_most(int B, int T, int G) {
+    const int most = kFewMaxRows / G;
+    return T > B && T > most ? most : 0;
+}
 static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
                         const int32_t* tables, int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B,
                         int T, int n_q_heads, uint16_t* out, int ldo) {
@@ -1658,6 +1671,7 @@ static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, in
     a.B = B;
     a.T = T;
     a.window = kBoundSlots;
+    a.most = INT_MAX;
     a.out = reinterpret_cast<__half*>(out);
     a.ldo = ldo;
     return a;
@@ -1666,8 +1680,8 @@ static FewArgs few_args(const uint16_t* q, int ldq, const uint16_t* kv_layer, in
 extern "C" size_t specdec_attention_window_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                            int max_blocks) {
     if (B <= 0 || T <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_blocks <= 0) return 0;
-    return std::max(few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes,
-                    rows_packed_workspace(B, T, n_q_heads, head_dim, max_blocks));
+    return few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes +
+           rows_packed_workspace(B, T, n_q_heads, head_dim, max_blocks);
 }
 
 extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks,
@@ -1689,16 +1703,21 @@ extern "C" int specdec_attention_window(const uint16_t* q, int ldq, const uint16
     // past the last slot that a row could have both change nothing (and sums with them stay in 32 bits)
     window = std::min(window, kBoundSlots);
     sinks = std::min(sinks, 16 * max_blocks);
+    char* rest = static_cast<char*>(workspace);
+    int least = 0;
     if (few_rows(B, T, n_q_heads / n_kv_heads)) {
         FewArgs f = few_args(q, ldq, kv_layer, num_blocks, n_kv_heads, tables, max_blocks, ctx_len, row_off, B, T,
                              n_q_heads, out, ldo);
         f.window = window;
         f.sinks = sinks;
-        return launch_few(f, head_dim, false, workspace, as_stream(stream));
+        least = few_most(B, T, f.G);
+        if (least) f.most = least;
+        if ((rc = launch_few(f, head_dim, false, workspace, as_stream(stream))) || !least) return rc;
+        rest += few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, false).bytes;
     }
     return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
                               num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads,
-                              window, sinks, nullptr, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
+                              window, sinks, least, nullptr, reinterpret_cast<__half*>(out), ldo, rest, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads,
@@ -1736,6 +1755,14 @@ extern "C" int specdec_attention_accumulate(const uint16_t* q, int ldq, const ui
     f.weights = weights;
     f.ldw = ldw;
     const bool few = few_rows(B, T, n_q_heads / n_kv_heads) && few_scores(T, n_q_heads, max_blocks) <= kFewScores;
-    return few ? launch_few(f, head_dim, true, workspace, as_stream(stream))
-               : launch_many(f, head_dim, workspace, as_stream(stream));
+    char* rest = static_cast<char*>(workspace);
+    if (few) {
+        const int most = few_most(B, T, f.G);
+        if (most) f.most = most;
+        if ((rc = launch_few(f, head_dim, true, workspace, as_stream(stream))) || !most) return rc;
+        rest += few_space(B, T, n_q_heads, n_kv_heads, head_dim, max_blocks, true).bytes;
+        f.least = most;
+        f.most = INT_MAX;
+    }
+    return launch_many(f, head_dim, rest, as_stream(stream));
 }

@@ -90,13 +90,13 @@ int launch_attention(const __half* q, const __half* kv_layer, int num_blocks, in
                      void* ws, size_t ws_bytes, int max_ctx, cudaStream_t s);
 
 // Packed rows on the tensor cores (prompt_attention.cu): causal, or (window > 0)
-// within a window and behind the first `sinks` tokens, where ml (may be null)
-// receives each row's (m, 1 / l): a slot's weight is 2^(score log2(e) / sqrt(HD) - m) / l.
+// within a window and behind the first `sinks` tokens, of the sequences of more
+// than `least` rows (others' stay as they are), where ml (may be null) receives each row's (m, 1 / l): a slot's weight is 2^(score log2(e) / sqrt(HD) - m) / l.
 int make_q_tmap(CUtensorMap* map, const __half* q, int ldq, int T, int Hq, int HD, int G, int tokens);
 size_t rows_packed_workspace(int B, int T, int Hq, int HD, int max_blocks);
 int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_blocks, int Hkv, int HD, const int32_t* tables,
                        int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B, int T, int Hq, int window,
-                       int sinks, float2* ml, __half* out, int ldo, void* ws, cudaStream_t s);
+                       int sinks, int least, float2* ml, __half* out, int ldo, void* ws, cudaStream_t s);
 
 // ---------------------------------------------------------------- sampling / acceptance
 constexpr size_t kAcceptStatsBytes = 32;  // one logits row's statistics in the acceptance scratch

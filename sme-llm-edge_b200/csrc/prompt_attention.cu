@@ -128,6 +128,7 @@ struct RowsArgs {
     int n_groups, B, T, R;
     int tq_small;  // tokens of the small query box
     int window, sinks;  // kModeWindow
+    int least;          // kModeWindow: sequences of up to so many rows are left out
     float2* ml;         // kModeWindow, may be null: [T][Hq] each row's m and 2^7 / l (l is that of the lifted weights)
     RowsDiv by_item, by_hkv;  // 2 * tpt tokens of an item; KV heads
     int slots_max;  // max_blocks * 16
@@ -182,6 +183,7 @@ __device__ __forceinline__ RowsSeg rows_seg(const RowsArgs& a, int i, const int*
     if (a.row_off) {
         s.lo = rows_clamp(off[i], 0, a.T);
         s.n = rows_clamp(off[i + 1], s.lo, a.T) - s.lo;
+        if (WIN && s.n <= a.least) s.n = 0;
         s.ctx = rows_clamp(ctx_len[i], 0, 1 << 30);
         s.base = 0;
         s.end = min(s.ctx + s.n, a.slots_max);
@@ -429,7 +431,8 @@ __device__ void rows_plan(const RowsArgs& a, RowsPlan& p) {
                 }
             } else {
                 RowsMeta& m = a.meta[s.trow];
-                m.n_own = rows_fit(a, s, parts, prow0) ? parts : 0;
+                // (a sequence that is left out has rows, which are not this kernel's)
+                m.n_own = (!WIN || s.n > 0) && rows_fit(a, s, parts, prow0) ? parts : 0;
                 m.base_own = prow0;
                 m.stride_own = s.n;
             }
@@ -900,6 +903,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar.i_want + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+    if constexpr (WIN) {
+        if (a.least > 0) {  // nothing but sequences that are left out
+            bool some = false;
+            for (int b = threadIdx.x; b < a.B; b += kRowsThreads) {
+                const int lo = rows_clamp(a.row_off[b], 0, a.T);
+                some |= rows_clamp(a.row_off[b + 1], lo, a.T) - lo > a.least;
+            }
+            if (!__syncthreads_or(some)) {
+                if (blockIdx.x == 0 && threadIdx.x == 0) *a.any_parts = 0;
+                return;
+            }
+        }
+    }
     pdl_trigger();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -1717,7 +1733,7 @@ size_t rows_packed_workspace(int B, int T, int Hq, int HD, int max_blocks) {
 }
 int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_blocks, int Hkv, int HD, const int32_t* tables,
                        int max_blocks, const int32_t* ctx_len, const int32_t* row_off, int B, int T, int Hq, int window,
-                       int sinks, float2* ml, __half* out, int ldo, void* ws, cudaStream_t s) {
+                       int sinks, int least, float2* ml, __half* out, int ldo, void* ws, cudaStream_t s) {
     size_t prows = prompt_partial_rows(T, max_blocks);
     if ((long long)T * Hq >= 1 << 30) prows = 0;  // the merge counts rows and heads in 32 bits
     RowsArgs a = {};
@@ -1734,6 +1750,7 @@ int rows_packed_launch(const __half* q, int ldq, const __half* kv, int num_block
     a.tq_small = 1;
     a.window = window;
     a.sinks = sinks;
+    a.least = least;
     a.ml = ml;
     a.out = out;
     a.ldo = ldo;
@@ -1771,7 +1788,7 @@ extern "C" int specdec_attention_prompt(const uint16_t* q, int ldq, const uint16
         return rc;
     return rows_packed_launch(reinterpret_cast<const __half*>(q), ldq, reinterpret_cast<const __half*>(kv_layer),
                               num_blocks, n_kv_heads, head_dim, tables, max_blocks, ctx_len, row_off, B, T, n_q_heads, 0,
-                              0, nullptr, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
+                              0, 0, nullptr, reinterpret_cast<__half*>(out), ldo, workspace, as_stream(stream));
 }
 
 extern "C" size_t specdec_attention_shared_prefix_workspace_bytes(int B, int R, int n_groups, int n_q_heads,

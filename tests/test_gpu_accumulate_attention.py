@@ -13,7 +13,7 @@ import torch
 
 import specdec as S
 from attn_plain import close, rows_plain
-from test_gpu_window_attention import NAN, make as make_window
+from test_gpu_window_attention import MIXED, NAN, make as make_window
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -308,3 +308,14 @@ def test_what_follows_a_captured_call_sees_its_results(cuda_device, lens, heads)
         torch.cuda.synchronize()
         s["weights"].copy_(gained)
         verify(s, out=kept)
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(8, 2, 64), (32, 8, 128), (5, 1, 128), (3, 3, 64), (16, 1, 64)])
+@pytest.mark.parametrize("lens", MIXED)
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_a_long_sequence_among_short_ones(cuda_device, Hq, Hkv, hd, lens, wide):
+    s = make(lens, Hq, Hkv, hd, seed=Hq, wide=wide, tail_rows=3)
+    ws = workspace(s)
+    for _ in range(2):
+        call(s, ws)
+    verify(s, times=2)

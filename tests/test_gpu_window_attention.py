@@ -363,3 +363,41 @@ def test_long_calls_under_wide_tables(cuda_device):
     ws = call(s)
     verify(s)
     del ws
+
+
+# few rows on average, most of them in one or two sequences
+MIXED = [[(1, 300)] * 30 + [(33, 500)], [(0, 40)] * 12 + [(90, 100)], [(1, 90)] * 6 + [(8, 300), (9, 300)] + [(1, 5)] * 6 + [(20, 0)]]
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(8, 2, 64), (32, 8, 128), (5, 1, 128), (3, 3, 64), (16, 1, 64)])
+@pytest.mark.parametrize("lens", MIXED)
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_a_long_sequence_among_short_ones(cuda_device, Hq, Hkv, hd, lens, wide):
+    s = make(lens, Hq, Hkv, hd, 120, 5, seed=Hq, wide=wide, tail_rows=3)
+    ws = call(s)
+    verify(s)
+    del ws
+
+
+def test_rows_that_move_between_sequences_of_a_captured_call(cuda_device):
+    lens = [[(4, 300)] * 20, [(1, 300)] * 19 + [(61, 300)], [(0, 300)] * 10 + [(8, 300)] * 10, [(80, 300)] + [(0, 300)] * 19]
+    s = make([(80, 300)] * 20, 32, 8, 128, 100, 4, gone=False)
+    s["kv"] = torch.nan_to_num(s["kv"], nan=0.5)
+    s["T"], s["lens"] = 80, lens[0]
+    s["q"], s["out"] = s["q"][:80].contiguous(), s["out"][:80].contiguous()
+
+    def bounds(x):
+        s["off"].copy_(torch.tensor([sum(n for n, _ in x[:i]) for i in range(21)], dtype=torch.int32))
+    bounds(lens[0])
+    ws = call(s)
+    torch.cuda.synchronize()
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        call(s, ws, torch.cuda.current_stream())
+    for x in lens[1:] + lens:
+        bounds(x)
+        s["lens"] = x
+        s["out"].fill_(7.0)
+        ws.fill_(0xFF)
+        graph.replay()
+        verify(s, what=str(x[-1]))
