@@ -472,7 +472,9 @@ int specdec_kv_fork_pages(int32_t* tables, int32_t* n_blocks, int32_t* lens, int
  * 64 bits and rounded to 32; of equal weights the lower slot stays; NaN is
  * above all numbers.  The tokens that stay keep their order and move up to
  * slots 0 .. keep-1, in all `layers` layers of the pool (as for
- * specdec_kv_fork; 0: tables and weights only) and in the weights, whose
+ * specdec_kv_fork; 0: tables and weights only, and the caller moves its K/V
+ * itself, by `kept` and a copy of the tables from before the call, ahead of
+ * the next block that is handed out) and in the weights, whose
  * entries from slot `keep` on become 0.  Pages behind are released; a page
  * that a token moves into and that others hold too is replaced by a free one
  * (the lowest, in the order of the call; pages that this call releases are not

@@ -403,14 +403,23 @@ class PagedKVCache:
         check(_lib.specdec_kv_fork(self._h, _p(src), _p(new), src.size, None, 0, 0, 0, 0, None))
 
     def evict_by_weight(self, request_ids, keep: int, first: int, last: int, weights, weight_heads: int, ldw: int,
-                        kept=None):
+                        kept=None, pool=None, layers: int = 0, layer_stride: int = 0, n_kv_heads: int = 0,
+                        head_dim: int = 0, stream=None):
         """Each request keeps its first `first`, its last `last` and its
-        heaviest other tokens, `keep` in all (tables and weights only; the K/V
-        payload lives in the engine's pool).  weights: device pointer of fp32
-        [max_requests, weight_heads, ldw]; kept: of int32 [n, keep], or None."""
+        heaviest other tokens, `keep` in all; they move up in the tables, in
+        the weights and in `layers` layers of the K/V pool.  weights: device
+        pointer of fp32 [max_requests, weight_heads, ldw]; kept: of int32
+        [n, keep], or None; pool: of fp16 [num_blocks, 2, n_kv_heads, 16,
+        head_dim] for each layer, layer_stride halves apart; stream: the one
+        that they were written on.
+
+        Without a pool the K/V stay where they are, under slots that no longer
+        are theirs: copy the tables (`read`) and pass `kept` before, and then
+        move the rows before the next block is handed out (slot j is the former
+        slot kept[i][j], in the page that the copied table names)."""
         reqs = np.ascontiguousarray(request_ids, dtype=np.int32).reshape(-1)
-        check(_lib.specdec_kv_evict(self._h, _p(reqs), reqs.size, keep, first, last, weights, weight_heads, ldw, None,
-                                    0, 0, 0, 0, kept, None))
+        check(_lib.specdec_kv_evict(self._h, _p(reqs), reqs.size, keep, first, last, weights, weight_heads, ldw, pool,
+                                    layers, layer_stride, n_kv_heads, head_dim, kept, stream))
 
     def free_merged_blocks(self, request_id: int, num_blocks_to_free: int):
         check(_lib.specdec_kv_free_merged_blocks(self._h, request_id, num_blocks_to_free, None))
