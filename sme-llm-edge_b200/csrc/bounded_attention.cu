@@ -28,10 +28,9 @@ constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a ca
 // stands between its loads and its arithmetic.  The call's pages, in the order
 // (sequence, tile of rows, KV head, page), are cut into ranges, one for each warp,
 // so ragged lengths balance by themselves.  SMs do not get equal shares of the
-// memory's rate (with one equal range for each warp the CTAs of 64 single tokens
-// on 4096 ended between 124 and 166 us), so a fifth of the pages is left for a
-// second wave of CTAs, which start where the first ones end early.  A tile is as
-// many whole tokens as fit into 8 * NT rows (row = token * G + g).  For a page
+// memory's rate, so in long calls a fifth of the pages is left for a second wave
+// of CTAs, which start where the first ones end early.  A tile is as many whole
+// tokens as fit into 8 * NT rows (row = token * G + g).  For a page
 //   S^T [16 keys][rows] = K Q^T,  P = 2^(S' - m),  O^T [hd][rows] += V^T P
 // in mma.sync of 16 x 8 x 16: 16 keys of 8 rows are 4 FLOP for each byte of the
 // cache, far from what the tensor cores of either kind can do, and the fragments
@@ -47,8 +46,8 @@ constexpr int kBoundSlots = (1 << 30) + (1 << 24);  // contexts and rows of a ca
 constexpr int kFewWarps = 4;       // of a CTA
 constexpr int kFewMaxSms = 148;    // SMs for which there are ranges
 constexpr int kFewMaxRows = 32;    // rows of a tile
-// CTAs of an SM, and waves of them.  Registers allow three of one tile of 8 rows; the pieces of many rows cost as
-// much as the wave gains.
+// CTAs of an SM, and waves of them at most.  Registers allow three of one tile of 8 rows; pieces of more than 16 rows cost
+// more than the wave gains.
 __host__ __device__ constexpr int few_resident(int NT) { return NT == 1 ? 3 : 2; }
 __host__ __device__ constexpr int few_waves(int NT) { return NT <= 2 ? 2 : 1; }
 constexpr int kFewMinPages = 4;    // of a range
@@ -73,6 +72,7 @@ struct FewArgs {
     int ldo;
     float scale_log2;
     int ctas, waves;    // CTAs of a wave (ranges)
+    int wave_pages;     // pages of a warp from which there is a second wave
     int chunk, chunks;  // pages of a piece, pieces of a table at most (chunk 0: ranges)
     // workspace
     long long* pre;     // [B + 1] pages before sequence b
@@ -221,8 +221,8 @@ __device__ __noinline__ void few_nonfinite(const FewArgs& a, int b, int p, int k
 template <int HD, int NT>
 struct FewCfg {
     static constexpr int PAGE = 64 * HD;                 // bytes of a page's K and V of a head
-    // Pages in flight of a warp: no more than the rate needs.  With 192 KB of an SM in flight 64 single tokens on 4096
-    // took 185 us, with 128 KB 182; the SMs' shares of the rate are further apart.
+    // Pages in flight of a warp: 64 single tokens on 4096 (8 heads of 128, tables of 2048 pages) take 181 us with two in
+    // each warp of three CTAs of an SM, 184 with three in each of two CTAs, 186 with two.
     static constexpr int RING = (HD == 128 ? 1 : 2) * (NT == 1 ? 2 : 3);
     static constexpr size_t smem(int B) {
         return 1024 + (size_t)kFewWarps * RING * PAGE + kFewWarps * RING * 8 + (size_t)(B + 1) * 8 + (size_t)B * sizeof(FewSeq) + 16;
@@ -306,9 +306,7 @@ struct FewCut {
     long long total, from1;
     int warps, per0, per1;  // warps of a wave
     __device__ __forceinline__ FewCut(const FewArgs& a, long long n) : total(n), warps(a.ctas * kFewWarps) {
-        // Few pages for each warp: their pieces would cost more than the wave gains (in us, with one wave and with two:
-        // one token on 65,536, 18 pages a warp, 57 and 91; 64 tokens on up to 8192, 33 pages, 100 and 93).
-        const bool both = a.waves > 1 && n >= 24LL * a.tpt * a.G / 8 * warps;
+        const bool both = a.waves > 1 && n >= (long long)a.wave_pages * warps;
         const long long given = both ? n - n / 5 : n;
         per0 = (int)max((long long)kFewMinPages, (given + warps - 1) / warps);
         from1 = min(n, (long long)warps * per0);
@@ -654,7 +652,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, few_resident(NT))
 // there is the result is final, and the CTA adds up its slots' weights too: one
 // launch for short tables.  CTAs come to the SMs as these are free, which evens out
 // both ragged lengths and the SMs' shares of the memory's rate (64 single tokens on
-// 2000: 88 us, ranges 101).
+// 2000, 8 heads of 128: 96 us, ranges 108).
 constexpr int kChunkMost = 128, kChunkLeast = 64;  // pages (four table entries of a lane)
 constexpr int kChunkCtas = 4096;                   // of a call at most
 
@@ -857,9 +855,9 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : NT == 1 ? 3 : 2)
 // out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over a row's pieces, in their
 // order: a warp for each row and head of up to 8 pieces, else the CTA's WARPS warps
 // take pieces in turn and are joined in their order.  ROWS: rows of a CTA, 1 where
-// there are few (148 pieces of each of 32 rows: 115 us a call with four rows of a
-// CTA one after the other, 57 with one).  Where the row belongs is looked up while
-// the kernel before still runs.
+// there are few (one token on 65,520: 57 us a call with four rows of a CTA one
+// after the other, 48 with one; 91 and 56 in ranges, under a wider table).  Where
+// the row belongs is looked up while the kernel before still runs.
 template <int HD, int ROWS, int WARPS>
 __device__ __forceinline__ void few_merge(const FewArgs& a, int tile_rows, unsigned block) {
     constexpr int W = HD / 32;
@@ -1549,6 +1547,12 @@ static int launch_few(FewArgs a, int HD, bool acc, void* ws, cudaStream_t s) {
     a.tpt = 8 * NT / a.G;
     a.ctas = few_ctas(sms, NT, a.T, a.Hkv, a.max_blocks);
     a.waves = few_waves(NT);
+    // With few pages for each warp the wave's pieces cost more than it gains, the sooner the more rows they have.  In us,
+    // with one wave and with two, of 64 sequences under tables of 2048 pages, 8 heads of 128, L tokens (L * 32 / 1776
+    // pages a warp at 3 CTAs of an SM): one row a piece on 1536 / 4096 / 12,288 73.6, 73.6 / 171, 168 / 487, 474; four
+    // 89.7, 91.0 / 185, 180 / 493, 485; five 82.3, 97.5 / 180, 187 / 489, 489; eight 82.8, 96.9 / 181, 188 / 493, 494,
+    // on 16,384 667, 663; sixteen on 2048 / 8192 / 16,384 125, 139 / 375, 381 / 718, 709.
+    a.wave_pages = want <= 4 ? 24 : 200;
     CUtensorMap map;
     if ((rc = make_kv_tmap(&map, a.kv, a.num_blocks, a.Hkv, HD, HD / 64, 2))) return rc;
     const size_t few_smem = HD == 128 ? (NT == 1 ? FewCfg<128, 1>::smem(a.B) : FewCfg<128, 2>::smem(a.B))

@@ -241,7 +241,7 @@ extern "C" int specdec_qk_norm_rope_kv(const void* qkv, int qkv_f16, int ldqkv, 
     a.ldq = ldq;
     // Few rows: a warp for each head group, so that a row's chain of look-ups is all there is (160 rows of 32/8 heads of
     // 128, fp32: 3.7 us, a warp for the whole row 16.6).  Many: four groups in flight, four times, at 28 warps of an SM
-    // (8 x 2501 such rows 117 us, 0.97 of the copy rate; 16 groups in flight or more warps of fewer registers 120 to 148).
+    // (8 x 2501 such rows 117 us, 0.96 of the copy rate; 16 groups in flight or more warps of fewer registers 120 to 148).
     const int groups = ((n_q_heads + 2 * n_kv_heads) * head_dim + 255) / 256;
     const bool many = (long long)T * groups > 148LL * 64 * 4;
     // (eight times where that still fills the SMs: a row's look-ups are made by fewer warps)
