@@ -394,7 +394,15 @@ int specdec_attention_window(const uint16_t* q, int ldq, const uint16_t* kv_laye
  * weights overlap neither q nor each other.  Calls of up to 32 / (query heads
  * of a KV head) rows a sequence on average keep their scores in the workspace
  * (T * n_q_heads * max_blocks * 64 bytes, 1 GiB at most); others compute them
- * twice.  The rest as for specdec_attention_prompt. */
+ * twice.  The weights that are added up are fp32, the outputs and the time of a
+ * long sequence among empty ones are specdec_attention_window's (922 us, alone
+ * 52).  Every row counts, drafts that are rejected later too: verify with
+ * specdec_attention_window (a window that reaches the first slot) and add up
+ * the accepted rows alone, their queries gathered and ctx_len as before.  Where
+ * drafts were added up nevertheless, set the entries behind the new length to
+ * 0: specdec_kv_truncate does not know the weights, and what is written into
+ * those slots next would start with them.  The rest as for
+ * specdec_attention_prompt. */
 size_t specdec_attention_accumulate_workspace_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim,
                                                     int max_blocks);
 int specdec_attention_accumulate(const uint16_t* q, int ldq, const uint16_t* kv_layer, int num_blocks, int n_kv_heads,
