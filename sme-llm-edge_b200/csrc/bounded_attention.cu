@@ -1649,10 +1649,17 @@ static size_t accumulate_space(int B, int T, int Hq, int Hkv, int HD, int max_bl
 static bool few_rows(int B, int T, int G) { return G <= kFewMaxRows && T <= (long long)B * (kFewMaxRows / G); }
 // Rows that a sequence of a few-row call may have at most, else it is left to the packed rows' kernels; 0: there is no
 // such bound.  A call's average says nothing of its longest sequence, whose tiles would go one after the other through
-// the CTAs of its heads, each reading K and V again: 63 single tokens on 4096 beside a chunk of 190 on 8000 1633 us, with
-// weights 2043; divided 257 and 413.  Where no sequence is long the other launches find nothing to do, for 6 to 17 us
-// (32 x 5 on 4096 115 -> 124, with weights 154 -> 171), so calls of up to one row a sequence, which are single tokens
-// unless others are empty, are not divided.
+// the CTAs of its heads, each reading K and V again.  In us, 32/8 heads of 128, undivided / divided (with weights), and
+// all by the packed rows' kernels without a window:
+//   63 single tokens on 4096 beside 190 rows on 8000   1613 / 249 (2032 / 402), 212
+//   31 beside 90                                        773 / 138 (982 / 211), 157
+//   50, 10 rows on 8000, 10 empty sequences             253 / 174 (295 / 211), 165
+// Where no sequence is long the other launches find nothing to do, for 8 to 18:
+//   32 x 5 rows on 4096                                 105 / 114 (144 / 160), 123
+//   32 x 5 on 512                                      22.4 / 30.4 (29.1 / 41.2), 39.6
+//   64 x 2 on 2048                                      100 / 109 (120 / 138), 118
+// So calls of up to one row a sequence, which are single tokens unless others are empty, are not divided.  If others are,
+// a long one takes its time: 64 rows on 8000 among 63 empty sequences 787 (922), alone 36 (52).
 static int few_most(int B, int T, int G) {
     const int most = kFewMaxRows / G;
     return T > B && T > most ? most : 0;
