@@ -411,13 +411,16 @@ class PagedKVCache:
         pointer of fp32 [max_requests, weight_heads, ldw]; kept: of int32
         [n, keep], or None; pool: of fp16 [num_blocks, 2, n_kv_heads, 16,
         head_dim] for each layer, layer_stride halves apart; stream: the one
-        that they were written on.
+        that they were written on (the manager's own earlier calls, which are
+        on the default stream, come first).
 
         Without a pool the K/V stay where they are, under slots that no longer
         are theirs: copy the tables (`read`) and pass `kept` before, and then
         move the rows before the next block is handed out (slot j is the former
         slot kept[i][j], in the page that the copied table names)."""
         reqs = np.ascontiguousarray(request_ids, dtype=np.int32).reshape(-1)
+        if stream is not None:
+            check(_lib.specdec_kv_read(self._h, None, None, None, None))  # waits for the default stream
         check(_lib.specdec_kv_evict(self._h, _p(reqs), reqs.size, keep, first, last, weights, weight_heads, ldw, pool,
                                     layers, layer_stride, n_kv_heads, head_dim, kept, stream))
 

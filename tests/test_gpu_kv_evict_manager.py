@@ -92,3 +92,21 @@ def test_a_pool_that_does_not_fit_is_refused(cuda_device):
         other.evict_by_weight([0], 20, 1, 1, w.data_ptr(), HKV, w.shape[2], **good)
     torch.cuda.synchronize()
     assert torch.equal(whole, before)
+
+
+def test_what_the_manager_did_before_is_seen_on_another_stream(cuda_device):
+    """free_request does not wait: the blocks that it gives back are the only ones that the eviction can take."""
+    for _ in range(20):
+        kv = S.PagedKVCache(33, PAGE, max_requests=4, max_blocks_per_request=16)
+        kv.append_batch([0, 1], [250, 256])
+        kv.fork([0], [3])
+        w = torch.rand((4, HKV, 256), device=DEV)
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        with pytest.raises(S.SpecdecError) as e:
+            kv.evict_by_weight([3], 64, 4, 16, w.data_ptr(), HKV, 256, stream=stream.cuda_stream)
+        assert e.value.code == S.ENOMEM
+        torch.cuda._sleep(2_000_000)  # keeps the default stream busy for a millisecond
+        kv.free_request(1)
+        kv.evict_by_weight([3], 64, 4, 16, w.data_ptr(), HKV, 256, stream=stream.cuda_stream)
+        assert int(kv.read()[1][3]) == 64
